@@ -52,7 +52,26 @@ _SIGS = {
     "fuma_coef_to_node_blocked": [_P, _P, _P, _I32, _I64, _I32, _P, _P],
     "fuma_rmsnorm_sh_fwd": [_P, _P, _P, _P, _F32, _I64, _I32, _P, _P, _P],
     "fuma_rmsnorm_sh_bwd": [_P, _P, _P, _P, _P, _I64, _I32, _P, _P],
+    "fuma_grouped_linear": [_P, _I64, _P, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
+    "fuma_grouped_linear_dgrad": [_P, _I64, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
+    "fuma_grouped_linear_wgrad": [_P, _I64, _P, _I64, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I64, _P, _P],
+    "fuma_grouped_bias_grad": [_P, _I64, _P, _I32, _I32, _I64, _I32, _I32, _P, _P, _I64, _P],
+    "fuma_split_bf16x3": [_P, _I64, _I64, _I32, _P, _P],
+    "fuma_quantize_rows_fp8": [_P, _I64, _I64, _I32, _I32, _P, _I64, _P, _P],
+    "fuma_quantize_weight_fp8": [_P, _I32, _I32, _I32, _P, _I64, _P, _P, _I64, _P, _P],
+    "fuma_grouped_linear_fp8": [_P, _P, _P, _P, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
+    "fuma_mix_experts": [_P, _I64, _I64, _P, _I32, _I32, _I64, _I32, _P, _P],
+    "fuma_mix_experts_dcoeff": [_P, _P, _I32, _I32, _I64, _I32, _P, _P, _I64, _P],
     "fuma_morton_reorder_noalloc": [_P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+}
+
+# scratch sizes (name -> argument types, return type int64)
+_SIZE_SIGS = {
+    "fuma_morton_scratch_bytes": [_I64],
+    "fuma_neighbor_scratch_bytes": [_I64, _P],
+    "fuma_grouped_wgrad_work_bytes": [_I64, _I32, _I32],
+    "fuma_grouped_bias_grad_work_bytes": [_I64, _I32, _I32],
+    "fuma_mix_experts_work_bytes": [_I32, _I32, _I64],
 }
 
 _lib = None
@@ -82,18 +101,17 @@ def load(allow_build: bool = False) -> ctypes.CDLL:
             fn.argtypes = args
             fn.restype = ctypes.c_int
         lib.fuma_version.restype = ctypes.c_int
-        lib.fuma_morton_scratch_bytes.argtypes = [_I64]
-        lib.fuma_morton_scratch_bytes.restype = ctypes.c_int64
-        lib.fuma_neighbor_scratch_bytes.argtypes = [_I64, _P]
-        lib.fuma_neighbor_scratch_bytes.restype = ctypes.c_int64
+        for name, args in _SIZE_SIGS.items():
+            fn = getattr(lib, name)
+            fn.argtypes = args
+            fn.restype = ctypes.c_int64
         lib.fuma_last_error.restype = ctypes.c_char_p
         _lib = lib
         return lib
 
 
 def exported_symbols():
-    return ["fuma_version", "fuma_last_error", "fuma_morton_scratch_bytes", "fuma_neighbor_scratch_bytes",
-            *_SIGS.keys()]
+    return ["fuma_version", "fuma_last_error", *_SIZE_SIGS.keys(), *_SIGS.keys()]
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -117,6 +135,9 @@ _SIGS["fuma_rotate_scatter_fwd_f16x3"] = _SIGS["fuma_rotate_scatter_fwd"][:-1] +
 
 KERNELS_PER_CALL = {name: 1 for name in _SIGS}
 KERNELS_PER_CALL["fuma_gather_bwd"] = 3
+KERNELS_PER_CALL["fuma_grouped_linear_wgrad"] = 2
+KERNELS_PER_CALL["fuma_grouped_bias_grad"] = 2
+KERNELS_PER_CALL["fuma_mix_experts_dcoeff"] = 2
 KERNELS_PER_CALL["fuma_gather_fwd"] = 2
 KERNELS_PER_CALL["fuma_csr_permute"] = 2
 KERNELS_PER_CALL["fuma_neighbor_list"] = 4

@@ -5,6 +5,7 @@
 
 #include "../../include/flash_uma_b200.h"
 #include "common.cuh"
+#include "grouped.cuh"
 #include "kernels.h"
 
 using namespace fuma;
@@ -694,6 +695,214 @@ int fuma_split_f16(const float* x, int64_t n, float scale, void* hi, void* lo, v
   BIND(x);
   launch_split_f16(x, hi, lo, scale, n, (cudaStream_t)stream);
   return launched("split_f16");
+}
+
+// ---- mixture of linear experts -----------------------------------------------------------------
+
+int64_t fuma_grouped_wgrad_work_bytes(int64_t T, int32_t N, int32_t K) {
+  return T > 0 && N > 0 && K > 0 ? grouped_wgrad_work_bytes(T, N, K) : 0;
+}
+
+int64_t fuma_grouped_bias_grad_work_bytes(int64_t T, int32_t N, int32_t groups) {
+  return T > 0 && N > 0 && groups > 0 ? grouped_colsum_work_bytes(T, N, groups) : 0;
+}
+
+int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P) {
+  return S > 0 && E > 0 && P > 0 ? mix_dcoeff_work_bytes(S, E, P) : 0;
+}
+
+namespace {
+
+int check_grouped(const char* what, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype) {
+  REQUIRE(G >= 1 && G <= kMaxGroups, "%s: G=%d must be from 1 to %d", what, G, kMaxGroups);
+  REQUIRE(T >= 0 && T < (int64_t(1) << 31) - 256, "%s: T=%lld out of range", what, (long long)T);
+  REQUIRE(N > 0 && N % 8 == 0 && K > 0 && K % 8 == 0, "%s: N=%d and K=%d must be positive multiples of 8", what, N, K);
+  REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "%s: dtype=%d must be 0 (fp32), 1 (bf16) or 2 (fp16)", what, dtype);
+  REQUIRE((int64_t)G * (N > K ? N : K) < (int64_t(1) << 31), "%s: G * max(N, K) too large", what);
+  REQUIRE((T / 128 + G) * (int64_t)((N > K ? N : K) / 32 + 1) < (int64_t(1) << 31), "%s: too many output tiles", what);
+  return FUMA_OK;
+}
+
+int grouped_done(const char* what, int r) {
+  if (r == -1) return fail(FUMA_E_INVALID, "%s: could not encode the TMA tensor maps: %s", what, gemm_map_error());
+  if (r != 0) return fail(r, "%s: launch failed: %s", what, cudaGetErrorString((cudaError_t)r));
+  return launched(what);
+}
+
+#define CHECK(call)             \
+  do {                          \
+    if (int rc_ = (call)) return rc_; \
+  } while (0)
+
+}  // namespace
+
+int fuma_grouped_linear(const void* x, int64_t ldx, const void* W, const int64_t* offsets, int32_t G,
+                        const void* bias, int32_t bias_rows, int64_t T, int32_t N, int32_t K, int32_t dtype, void* y,
+                        int* err_flag, void* stream) {
+  CHECK(check_grouped("grouped_linear", G, T, N, K, dtype));
+  REQUIRE(ldx >= K && ldx % 8 == 0, "grouped_linear: ldx=%lld must be >= K and a multiple of 8", (long long)ldx);
+  REQUIRE(!bias || bias_rows == 1 || bias_rows == G, "grouped_linear: bias_rows=%d must be 1 or G", bias_rows);
+  if (T == 0) return FUMA_OK;
+  REQUIRE(x && W && y, "grouped_linear: null pointer");
+  REQUIRE(offsets || G == 1, "grouped_linear: offsets may be NULL for one group only");
+  REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(W, "W"); REQUIRE_ALIGNED(y, "y");
+  BIND(x);
+  GroupedOperands o{x, W, ldx, K, dtype == kDtypeF32 ? 1 : 0, dtype};
+  GroupedArgs p{};
+  p.offsets = offsets; p.G = G; p.T = T; p.N = N; p.K = K;
+  p.C = y; p.ldc = N; p.out_dtype = dtype;
+  p.bias = bias; p.bias_rows = bias_rows; p.bias_dtype = dtype;
+  return grouped_done("grouped_linear", launch_grouped_rows(o, p, false, err_flag, (cudaStream_t)stream));
+}
+
+int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const void* W, const int64_t* offsets, int32_t G,
+                              int64_t T, int32_t N, int32_t K, int32_t dtype, void* dx, int* err_flag, void* stream) {
+  CHECK(check_grouped("grouped_linear_dgrad", G, T, N, K, dtype));
+  REQUIRE(lddy >= N && lddy % 8 == 0, "grouped_linear_dgrad: lddy=%lld must be >= N and a multiple of 8",
+          (long long)lddy);
+  if (T == 0) return FUMA_OK;
+  REQUIRE(dy && W && dx, "grouped_linear_dgrad: null pointer");
+  REQUIRE(offsets || G == 1, "grouped_linear_dgrad: offsets may be NULL for one group only");
+  REQUIRE_ALIGNED(dy, "dy"); REQUIRE_ALIGNED(W, "W"); REQUIRE_ALIGNED(dx, "dx");
+  BIND(dy);
+  GroupedOperands o{dy, W, lddy, K, dtype == kDtypeF32 ? 1 : 0, dtype};
+  GroupedArgs p{};
+  p.offsets = offsets; p.G = G; p.T = T; p.N = K; p.K = N;
+  p.C = dx; p.ldc = K; p.out_dtype = dtype;
+  return grouped_done("grouped_linear_dgrad", launch_grouped_rows(o, p, true, err_flag, (cudaStream_t)stream));
+}
+
+int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int64_t* offsets,
+                              int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dW, void* work,
+                              int64_t work_bytes, int* err_flag, void* stream) {
+  CHECK(check_grouped("grouped_linear_wgrad", G, T, N, K, dtype));
+  REQUIRE(lddy >= N && lddy % 8 == 0 && ldx >= K && ldx % 8 == 0, "grouped_linear_wgrad: bad leading dimensions");
+  REQUIRE(dW, "grouped_linear_wgrad: null pointer");
+  REQUIRE_ALIGNED(dW, "dW");
+  BIND(dW);
+  if (T == 0) {   // no rows: zeros
+    const cudaError_t st =
+        cudaMemsetAsync(dW, 0, (size_t)G * N * K * (dtype == kDtypeF32 ? 4 : 2), (cudaStream_t)stream);
+    return st == cudaSuccess ? FUMA_OK : fail((int)st, "grouped_linear_wgrad: %s", cudaGetErrorString(st));
+  }
+  REQUIRE(dy && x, "grouped_linear_wgrad: null pointer");
+  REQUIRE(offsets || G == 1, "grouped_linear_wgrad: offsets may be NULL for one group only");
+  const int64_t need = grouped_wgrad_work_bytes(T, N, K);
+  REQUIRE(work_bytes >= need && (need == 0 || work), "grouped_linear_wgrad: needs %lld bytes of work space, got %lld",
+          (long long)need, (long long)work_bytes);
+  REQUIRE_ALIGNED(dy, "dy"); REQUIRE_ALIGNED(x, "x");
+  if (work) REQUIRE_ALIGNED(work, "work");
+  GroupedOperands o{dy, x, lddy, ldx, dtype == kDtypeF32 ? 1 : 0, dtype};
+  GroupedArgs p{};
+  p.offsets = offsets; p.G = G; p.T = T; p.M = N; p.N = K;
+  p.C = dW; p.out_dtype = dtype; p.work = work;
+  return grouped_done("grouped_linear_wgrad", launch_grouped_wgrad(o, p, err_flag, (cudaStream_t)stream));
+}
+
+int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets, int32_t G, int32_t shared, int64_t T,
+                           int32_t N, int32_t dtype, void* db, void* work, int64_t work_bytes, void* stream) {
+  CHECK(check_grouped("grouped_bias_grad", G, T, N, N, dtype));
+  REQUIRE(lddy >= N && lddy % 8 == 0, "grouped_bias_grad: lddy=%lld must be >= N and a multiple of 8", (long long)lddy);
+  REQUIRE(db && (T == 0 || dy), "grouped_bias_grad: null pointer");
+  REQUIRE(offsets || G == 1, "grouped_bias_grad: offsets may be NULL for one group only");
+  const int64_t need = T > 0 ? grouped_colsum_work_bytes(T, N, shared ? 1 : G) : 0;
+  REQUIRE(work_bytes >= need && (need == 0 || work), "grouped_bias_grad: needs %lld bytes of work space, got %lld",
+          (long long)need, (long long)work_bytes);
+  if (T > 0) REQUIRE_ALIGNED(dy, "dy");
+  BIND(db);
+  const cudaError_t st = launch_grouped_colsum(dy, lddy, dtype, offsets, G, shared != 0, T, N,
+                                               static_cast<float*>(work), db, (cudaStream_t)stream);
+  return grouped_done("grouped_bias_grad", (int)st);
+}
+
+int fuma_split_bf16x3(const float* x, int64_t ldx, int64_t rows, int32_t cols, void* out, void* stream) {
+  REQUIRE(rows >= 0 && cols > 0 && cols % 4 == 0, "split_bf16x3: bad shape rows=%lld cols=%d", (long long)rows, cols);
+  REQUIRE(ldx >= cols && ldx % 4 == 0, "split_bf16x3: ldx=%lld must be >= cols and a multiple of 4", (long long)ldx);
+  if (rows == 0) return FUMA_OK;
+  REQUIRE(x && out, "split_bf16x3: null pointer");
+  REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(out, "out");
+  BIND(x);
+  launch_split_bf16x3(x, ldx, rows, cols, out, (cudaStream_t)stream);
+  return launched("split_bf16x3");
+}
+
+int fuma_quantize_rows_fp8(const void* x, int64_t ldx, int64_t T, int32_t K, int32_t dtype, void* codes, int64_t ldq,
+                           float* scales, void* stream) {
+  REQUIRE(T >= 0 && T < (int64_t(1) << 31) && K > 0 && K % 8 == 0, "quantize_rows_fp8: bad shape T=%lld K=%d",
+          (long long)T, K);
+  REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "quantize_rows_fp8: dtype=%d must be 0, 1 or 2", dtype);
+  REQUIRE(ldx >= K && ldx % 8 == 0, "quantize_rows_fp8: ldx=%lld must be >= K and a multiple of 8", (long long)ldx);
+  REQUIRE(ldq == (K + 15) / 16 * 16, "quantize_rows_fp8: ldq=%lld must be K rounded up to 16", (long long)ldq);
+  if (T == 0) return FUMA_OK;
+  REQUIRE(x && codes && scales, "quantize_rows_fp8: null pointer");
+  REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(codes, "codes");
+  BIND(x);
+  launch_quantize_rows(x, ldx, dtype, T, K, codes, ldq, scales, (cudaStream_t)stream);
+  return launched("quantize_rows_fp8");
+}
+
+int fuma_quantize_weight_fp8(const float* w, int32_t G, int32_t N, int32_t K, void* codes, int64_t ldq, float* scales,
+                             void* codes_t, int64_t ldt, float* scales_t, void* stream) {
+  REQUIRE(G >= 1 && G <= kMaxGroups && N > 0 && K > 0 && N <= (1 << 22) && K <= (1 << 22),
+          "quantize_weight_fp8: bad shape G=%d N=%d K=%d", G, N, K);
+  REQUIRE(ldq == (K + 15) / 16 * 16 && ldt == (N + 15) / 16 * 16,
+          "quantize_weight_fp8: ldq and ldt must be K and N rounded up to 16");
+  REQUIRE(w && codes && scales && codes_t && scales_t, "quantize_weight_fp8: null pointer");
+  REQUIRE_ALIGNED(codes, "codes"); REQUIRE_ALIGNED(codes_t, "codes_t");
+  BIND(w);
+  launch_quantize_weight(w, G, N, K, codes, ldq, scales, codes_t, ldt, scales_t, (cudaStream_t)stream);
+  return launched("quantize_weight_fp8");
+}
+
+int fuma_grouped_linear_fp8(const void* x_codes, const float* x_scales, const void* w_codes, const float* w_scales,
+                            const int64_t* offsets, int32_t G, const float* bias, int32_t bias_rows, int64_t T,
+                            int32_t N, int32_t K, int32_t out_dtype, void* y, int* err_flag, void* stream) {
+  CHECK(check_grouped("grouped_linear_fp8", G, T, N, K, out_dtype));
+  REQUIRE(!bias || bias_rows == 1 || bias_rows == G, "grouped_linear_fp8: bias_rows=%d must be 1 or G", bias_rows);
+  if (T == 0) return FUMA_OK;
+  REQUIRE(x_codes && x_scales && w_codes && w_scales && y, "grouped_linear_fp8: null pointer");
+  REQUIRE(offsets || G == 1, "grouped_linear_fp8: offsets may be NULL for one group only");
+  REQUIRE_ALIGNED(x_codes, "x_codes"); REQUIRE_ALIGNED(w_codes, "w_codes"); REQUIRE_ALIGNED(y, "y");
+  BIND(x_codes);
+  const int64_t ld = (K + 15) / 16 * 16;
+  GroupedOperands o{x_codes, w_codes, ld, ld, 2, 0};
+  GroupedArgs p{};
+  p.offsets = offsets; p.G = G; p.T = T; p.N = N; p.K = K;
+  p.C = y; p.ldc = N; p.out_dtype = out_dtype;
+  p.bias = bias; p.bias_rows = bias_rows; p.bias_dtype = kDtypeF32;
+  p.scale_a = x_scales; p.scale_b = w_scales; p.blocks_n = (N + 127) / 128;
+  return grouped_done("grouped_linear_fp8", launch_grouped_rows(o, p, false, err_flag, (cudaStream_t)stream));
+}
+
+int fuma_mix_experts(const float* coeff, int64_t stride_s, int64_t stride_e, const void* experts, int32_t S, int32_t E,
+                     int64_t P, int32_t dtype, void* out, void* stream) {
+  REQUIRE(S >= 0 && E > 0 && P >= 0 && P <= (int64_t(1) << 38), "mix_experts: bad sizes S=%d E=%d P=%lld", S, E,
+          (long long)P);
+  REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "mix_experts: dtype=%d must be 0, 1 or 2", dtype);
+  if (S == 0 || P == 0) return FUMA_OK;
+  REQUIRE(coeff && experts && out, "mix_experts: null pointer");
+  REQUIRE_ALIGNED(experts, "experts"); REQUIRE_ALIGNED(out, "out");
+  BIND(experts);
+  return grouped_done("mix_experts", (int)launch_mix(coeff, stride_s, stride_e, experts, S, E, P, dtype, out,
+                                                     (cudaStream_t)stream));
+}
+
+int fuma_mix_experts_dcoeff(const void* grad, const void* experts, int32_t S, int32_t E, int64_t P, int32_t dtype,
+                            float* dcoeff, void* work, int64_t work_bytes, void* stream) {
+  REQUIRE(S >= 0 && E > 0 && P > 0 && P <= (int64_t(1) << 38), "mix_experts_dcoeff: bad sizes S=%d E=%d P=%lld", S, E,
+          (long long)P);
+  REQUIRE(S <= 64 * 65535 && E <= 64 * 65535, "mix_experts_dcoeff: S=%d or E=%d too large", S, E);
+  REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "mix_experts_dcoeff: dtype=%d must be 0, 1 or 2", dtype);
+  if (S == 0) return FUMA_OK;
+  const int64_t need = mix_dcoeff_work_bytes(S, E, P);
+  REQUIRE(grad && experts && dcoeff && work, "mix_experts_dcoeff: null pointer");
+  REQUIRE(work_bytes >= need, "mix_experts_dcoeff: needs %lld bytes of work space, got %lld", (long long)need,
+          (long long)work_bytes);
+  REQUIRE_ALIGNED(grad, "grad"); REQUIRE_ALIGNED(experts, "experts"); REQUIRE_ALIGNED(work, "work");
+  BIND(grad);
+  return grouped_done("mix_experts_dcoeff", (int)launch_mix_dcoeff(grad, experts, S, E, P, dtype,
+                                                                   static_cast<float*>(work), dcoeff,
+                                                                   (cudaStream_t)stream));
 }
 
 }  // extern "C"

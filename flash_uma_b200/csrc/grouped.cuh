@@ -1,0 +1,68 @@
+// Arguments shared by the grouped dense maps (grouped.cu), the fp8 quantisation (fp8.cu), the
+// expert mix (mix.cu) and the C ABI.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace fuma {
+
+constexpr int kMaxGroups = 4096;   // their work prefix sits in shared memory
+constexpr int kDtypeF32 = 0, kDtypeBf16 = 1, kDtypeF16 = 2;
+constexpr int kErrOffsets = 64;    // group offsets that decrease or leave [0, T]
+
+// kind: 0 bf16 / fp16 (dtype), 1 three bf16 planes of fp32, 2 e4m3. Leading dimensions in elements.
+struct GroupedOperands {
+  const void* A;
+  const void* B;
+  int64_t lda, ldb;
+  int kind, dtype;
+};
+
+struct GroupedArgs {
+  const int64_t* offsets;   // [G + 1], device
+  int G;
+  int64_t T;                // rows of the ragged operand(s)
+  int M, N, K;              // row maps: N output columns, contraction K. Weight gradient: dW is [G, M, N].
+  void* C;
+  int64_t ldc;
+  int out_dtype;
+  const void* bias;         // [N] or [G, N] or null
+  int bias_rows, bias_dtype;
+  const float* scale_a;     // fp8: [ceil(K / 128)][T]
+  const float* scale_b;     // fp8: [G][blocks_n][ceil(K / 128)]
+  int blocks_n;
+  // Weight gradient: fp32 partial matrices of groups longer than `chunk` rows. Such a group starts
+  // at row a; its chunk 0 takes slot a / chunk, its chunk c >= 1 slot `slots` + a / chunk + c. Two such
+  // groups never meet: a group of more than `chunk` rows moves a / chunk on by at least
+  // floor(len / chunk) >= 1 for the next one, whose later chunks then start at least
+  // floor(len / chunk) + 1 > ceil(len / chunk) - 1 slots further on. Both ranges end at or before
+  // T / chunk + 1 = `slots`.
+  void* work;
+  int64_t slots;
+  int* err;
+  // set by the launcher
+  int bn, tiles_m, tiles_n, chunk;
+  uint32_t mma_format;
+};
+
+int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed, int* err, cudaStream_t s);
+int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cudaStream_t s);
+int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N);
+int64_t grouped_colsum_work_bytes(int64_t T, int N, int groups);
+cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const int64_t* off, int G, bool shared,
+                                  int64_t T, int N, float* part, void* out, cudaStream_t s);
+void launch_split_bf16x3(const float* x, int64_t ldx, int64_t rows, int cols, void* out, cudaStream_t s);
+
+void launch_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t T, int K, void* codes, int64_t ldq,
+                          float* scales, cudaStream_t s);
+void launch_quantize_weight(const float* w, int G, int N, int K, void* codes, int64_t ldq, float* scales,
+                            void* codes_t, int64_t ldt, float* scales_t, cudaStream_t s);
+
+// out[s, p] = sum_e c[s * cs + e * ce] X[e, p]
+cudaError_t launch_mix(const float* c, int64_t cs, int64_t ce, const void* X, int S, int E, int64_t P, int dtype,
+                       void* out, cudaStream_t s);
+int64_t mix_dcoeff_work_bytes(int S, int E, int64_t P);
+cudaError_t launch_mix_dcoeff(const void* dW, const void* X, int S, int E, int64_t P, int dtype, float* part,
+                              float* out, cudaStream_t s);
+
+}  // namespace fuma

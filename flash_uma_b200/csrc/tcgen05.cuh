@@ -89,5 +89,10 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 // On failure returns false and leaves a message for gemm_map_error().
 bool make_map_t(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, int64_t rows, int64_t cols,
                 int64_t ld_bytes, int box_cols, int box_rows, CUtensorMapSwizzle swz);
+// 4-D tensor map (cols contiguous, rows, matrices, planes; strides in bytes), boxes of one matrix and
+// box_planes planes, zero fill out of range.
+bool make_map_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, int64_t cols, int64_t rows,
+                 int64_t mats, int64_t planes, int64_t row_bytes, int64_t mat_bytes, int64_t plane_bytes, int box_cols,
+                 int box_rows, int box_planes, CUtensorMapSwizzle swz);
 
 }  // namespace fuma

@@ -1,0 +1,139 @@
+"""Dense maps on block-scaled 8-bit operands (e4m3, one scale for each block of 128).
+
+The step below the ``"f16"`` mode of :mod:`flash_uma_b200.linear`: frozen weights at one byte per
+value, products on the fp8 tensor cores, fp32 sums; about 4 significant bits per operand, for
+screening and other uses that bear errors of a few percent per product. :class:`Fp8Weight` holds
+a frozen matrix (or one per system) in 128 x 128 blocks, laid out once; :func:`fp8_linear` rounds the
+activations in blocks of 128 along each row and multiplies. A scale is the smallest power of two
+(at least 2^-126) that brings its block's largest magnitude to 448 or below, so a value is rounded
+once, to nearest even.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+from ._native import ptr, stream_of
+from .grouped import MAX_GROUPS, _ceil8, _check_dtype, _rows, _same_device, check_groups, guard_capture
+from .linear import error_flag
+
+_BLOCK = 128
+
+
+def _ceil16(n: int) -> int:
+    return (n + 15) // 16 * 16
+
+
+def _blocks(n: int) -> int:
+    return (n + _BLOCK - 1) // _BLOCK
+
+
+class Fp8Weight:
+    """Frozen weights [N, K] or [G, N, K] (any floating type, on a GPU) as e4m3 codes and scales, and
+    the same of the transposed matrices for the input gradient: two bytes per weight in all."""
+
+    def __init__(self, weight: torch.Tensor):
+        nat.require_cuda(weight)
+        if weight.dim() not in (2, 3):
+            raise ValueError(f"weight must be [N, K] or [groups, N, K] (got {tuple(weight.shape)})")
+        _check_dtype("weight", weight)
+        w = weight.detach()
+        w = w[None] if w.dim() == 2 else w
+        self.G, self.N, self.K = w.shape
+        if not 1 <= self.G <= MAX_GROUPS:
+            raise ValueError(f"the number of groups must be from 1 to {MAX_GROUPS} (got {self.G})")
+        if self.N < 1 or self.K < 1:
+            raise ValueError(f"weight needs N >= 1 and K >= 1 (got {tuple(weight.shape)})")
+        self.Np, self.Kp = _ceil8(self.N), _ceil8(self.K)
+        w = torch.nn.functional.pad(w.float(), (0, self.Kp - self.K, 0, self.Np - self.N)).contiguous()
+        dev, G, Np, Kp = w.device, self.G, self.Np, self.Kp
+        self.device = dev
+        self.codes = torch.empty(G, Np, _ceil16(Kp), device=dev, dtype=torch.uint8)
+        self.scales = torch.empty(G, _blocks(Np), _blocks(Kp), device=dev)
+        self.codes_t = torch.empty(G, Kp, _ceil16(Np), device=dev, dtype=torch.uint8)
+        self.scales_t = torch.empty(G, _blocks(Kp), _blocks(Np), device=dev)
+        nat.call("fuma_quantize_weight_fp8", ptr(w), G, Np, Kp, ptr(self.codes), _ceil16(Kp), ptr(self.scales),
+                 ptr(self.codes_t), _ceil16(Np), ptr(self.scales_t), stream_of(w))
+
+    def dequantize(self) -> torch.Tensor:
+        """The values that the codes stand for, fp32 [G, N, K]."""
+        v = self.codes.view(torch.float8_e4m3fn).float()[:, : self.N, : self.K]
+        s = self.scales.repeat_interleave(_BLOCK, 1).repeat_interleave(_BLOCK, 2)
+        return v * s[:, : self.N, : self.K]
+
+
+def quantize_rows(x: torch.Tensor):
+    """x [T, K] -> (codes uint8 [T, K rounded up to 16], scales float32 [ceil(K / 128), T]): e4m3 in
+    blocks of 128 along each row (``fuma_quantize_rows_fp8``)."""
+    nat.require_cuda(x)
+    code = _check_dtype("x", x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be [rows, K] with K >= 1 (got {tuple(x.shape)})")
+    T, Kp = x.shape[0], _ceil8(x.shape[1])
+    x = _rows(x, Kp)
+    codes = torch.empty(T, _ceil16(Kp), device=x.device, dtype=torch.uint8)
+    scales = torch.empty(_blocks(Kp), T, device=x.device)
+    if T:
+        nat.call("fuma_quantize_rows_fp8", ptr(x), x.stride(0), T, Kp, code, ptr(codes), _ceil16(Kp), ptr(scales),
+                 stream_of(x))
+    return codes, scales
+
+
+def _product(x, w_codes, w_scales, offsets, bias, N, K):
+    T = x.shape[0]
+    y = torch.empty(T, N, device=x.device, dtype=x.dtype)
+    if T:
+        codes, scales = quantize_rows(x)
+        nat.call("fuma_grouped_linear_fp8", ptr(codes), ptr(scales), ptr(w_codes), ptr(w_scales), ptr(offsets),
+                 w_codes.shape[0], ptr(bias), 0 if bias is None else (1 if bias.dim() == 1 else w_codes.shape[0]), T, N,
+                 K, _check_dtype("x", x), ptr(y), ptr(error_flag(x.device)), stream_of(x))
+    return y
+
+
+class _Fp8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets, bias):
+        ctx.weight = weight
+        ctx.save_for_backward(*(() if offsets is None else (offsets,)))
+        b = bias
+        if b is not None:
+            b = torch.nn.functional.pad(b, (0, weight.Np - weight.N)) if weight.Np != weight.N else b.contiguous()
+        y = _product(x, weight.codes, weight.scales, offsets, b, weight.Np, weight.Kp)
+        return y if weight.Np == weight.N else y[:, : weight.N]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        weight = ctx.weight
+        offsets = ctx.saved_tensors[0] if ctx.saved_tensors else None
+        dx = _product(g, weight.codes_t, weight.scales_t, offsets, None, weight.Kp, weight.Np)
+        return (dx if weight.Kp == weight.K else dx[:, : weight.K]), None, None, None
+
+
+@torch.compiler.disable
+def fp8_linear(x: torch.Tensor, weight: Fp8Weight, offsets: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``y = x_q W_q^T (+ bias)`` with x rounded to e4m3 in row blocks of 128; y has x's type
+    (float32, bfloat16 or float16), sums are fp32.
+
+    ``offsets`` [G + 1] int64 gives the rows of each of the weight's G matrices, as in
+    :func:`flash_uma_b200.grouped.grouped_linear`; None: all rows through the one matrix. ``bias``
+    float32 [N] or [G, N]. Weights and bias are frozen (a bias that requires a gradient is refused);
+    the gradient of x is ``g_q W_q`` with the output's gradient rounded the same way (for forces). A block
+    with a value that is not finite makes the results that depend on it NaN."""
+    nat.require_cuda(x, offsets, bias)
+    if not isinstance(weight, Fp8Weight):
+        raise TypeError(f"weight must be an Fp8Weight (got {type(weight).__name__})")
+    _check_dtype("x", x)
+    if bias is not None and bias.dtype != torch.float32:
+        raise TypeError(f"bias must be float32 (got {bias.dtype})")
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise ValueError("fp8_linear has frozen weights: the bias must not require a gradient")
+    if offsets is None and weight.G != 1:
+        raise ValueError(f"offsets are needed for the weight's {weight.G} matrices")
+    check_groups(x, weight.G, weight.N, weight.K, offsets, bias)
+    _same_device(x, weight=weight, offsets=offsets, bias=bias)
+    edges = guard_capture(x)
+    out = _Fp8LinearFn.apply(x, weight, None if offsets is None else offsets.contiguous(), bias)
+    del edges
+    return out

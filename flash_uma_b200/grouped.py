@@ -1,0 +1,300 @@
+"""Dense layers of a mixture of linear experts: per-system weights and the grouped dense map.
+
+FAIRChem's UMA models keep E expert matrices per dense layer and give a system the mean of them
+under its own coefficients. The reference (and :class:`~flash_uma_b200.wrapper.ZeroAllocBackbone`)
+takes a model whose experts were merged for one composition (``readme.md:35-72``). For a batch of
+unlike systems, and for training, every system keeps its own matrix:
+
+* :func:`mix_experts`: ``W[s] = sum_e coeff[s, e] experts[e]``, with both gradients;
+* :func:`grouped_linear`: ``y[t] = W[g(t)] x[t] + b`` for rows grouped by system, with the
+  gradients of ``x``, ``W`` and ``b``;
+* :class:`MoleLinear`: the two together, a layer.
+
+Counterpart of :class:`~flash_uma_b200.linear.FrozenLinear` (one frozen matrix for all rows) on
+the same tensor cores. Types: fp32 (three bf16 planes per operand, six products: 24 bits and the
+whole fp32 range, no range error), bf16 and fp16 (fp32 sums, one rounding at the end).
+:func:`flash_uma_b200.fp8.fp8_linear` is the map on frozen 8-bit weights.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+
+from . import _native as nat
+from ._native import ptr, stream_of
+from .linear import error_flag
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_GROUPS = 4096
+
+
+def _check_dtype(name: str, t: torch.Tensor) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})")
+    return code
+
+
+def _same_device(first: torch.Tensor, **others) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {first.device}")
+
+
+_EAGER = "flash_uma_b200.eager"
+
+
+def guard_capture(*inputs) -> list:
+    """Refuse to put a call on leaf tensors into a CUDA graph capture while an eager graph of the same leaves
+    is alive: autograd keeps one gradient node per leaf, bound to the stream it was made on, and a
+    captured backward pass that meets a node of an uncaptured stream invalidates the capture or ends the
+    process. The node carries a mark from the first eager call, and goes with the eager graph; the
+    caller holds the returned list until its own graph holds the nodes."""
+    if not torch.is_grad_enabled():
+        return []
+    leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
+    if not leaves:
+        return []
+    capturing = torch.cuda.is_current_stream_capturing()
+    edges = [torch.autograd.graph.get_gradient_edge(t) for t in leaves]
+    for e in edges:
+        marks = e.node.metadata
+        if not capturing:
+            marks[_EAGER] = True
+        elif marks.get(_EAGER):
+            raise RuntimeError("a CUDA graph capture of this call needs the results of earlier eager calls on the "
+                               "same leaf tensors to be released or detached first (their autograd graph is alive)")
+    return edges
+
+
+def _rows(x: torch.Tensor, cols: int) -> torch.Tensor:
+    """``x`` [T, >= width] as an operand: ``cols`` (a multiple of 8) columns, rows a multiple of 8
+    elements apart, 16-byte aligned. A copy only where ``x`` is not that already."""
+    if x.shape[1] != cols:
+        x = torch.nn.functional.pad(x, (0, cols - x.shape[1]))
+    if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < cols or x.data_ptr() % 16 != 0:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _matrices(w: torch.Tensor, N: int, K: int) -> torch.Tensor:
+    """``w`` [G, n, k] contiguous, 16-byte aligned, zero-padded to [G, N, K]."""
+    if w.shape[1] != N or w.shape[2] != K:
+        w = torch.nn.functional.pad(w, (0, K - w.shape[2], 0, N - w.shape[1]))
+    w = w.contiguous()
+    return w.clone() if w.data_ptr() % 16 else w
+
+
+def _ceil8(n: int) -> int:
+    return (n + 7) // 8 * 8
+
+
+def _planes(x: torch.Tensor) -> torch.Tensor:
+    """[3, rows, cols] bf16 planes of an fp32 operand [rows, cols] (``fuma_split_bf16x3``)."""
+    rows, cols = x.shape
+    out = torch.empty(3, rows, cols, device=x.device, dtype=torch.bfloat16)
+    nat.call("fuma_split_bf16x3", ptr(x), x.stride(0), rows, cols, ptr(out), stream_of(x))
+    return out
+
+
+def _operand(x: torch.Tensor, cols: int):
+    """(tensor, leading dimension) of a row operand for the C ABI."""
+    x = _rows(x, cols)
+    if x.dtype == torch.float32:
+        return _planes(x), cols
+    return x, x.stride(0)
+
+
+def _weight_operand(w: torch.Tensor) -> torch.Tensor:
+    G, N, K = w.shape
+    return _planes(w.view(G * N, K)) if w.dtype == torch.float32 else w
+
+
+class _GroupedLinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets, bias):
+        T = x.shape[0]
+        G, N, K = weight.shape
+        Np, Kp = _ceil8(N), _ceil8(K)
+        code = _DTYPES[x.dtype]
+        ctx.save_for_backward(x, weight, offsets)
+        ctx.bias_shape = None if bias is None else bias.shape
+        y = torch.empty(T, Np, device=x.device, dtype=x.dtype)
+        if T:
+            b = bias
+            if b is not None:
+                b = torch.nn.functional.pad(b, (0, Np - N)) if Np != N else b.contiguous()
+            a, lda = _operand(x, Kp)
+            w = _weight_operand(_matrices(weight, Np, Kp))
+            nat.call("fuma_grouped_linear", ptr(a), lda, ptr(w), ptr(offsets), G, ptr(b),
+                     0 if b is None else (1 if b.dim() == 1 else G), T, Np, Kp, code, ptr(y),
+                     ptr(error_flag(x.device)), stream_of(x))
+        return y if Np == N else y[:, :N]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, weight, offsets = ctx.saved_tensors
+        T = x.shape[0]
+        G, N, K = weight.shape
+        Np, Kp = _ceil8(N), _ceil8(K)
+        code = _DTYPES[x.dtype]
+        want_x, want_w, _, want_b = ctx.needs_input_grad
+        dx = dw = db = None
+        s, err = stream_of(x), ptr(error_flag(x.device))
+        g = _rows(g, Np)
+        a, lda = _operand(g, Np) if T and (want_x or want_w) else (g, Np)
+        if want_x:
+            dx = torch.empty(T, Kp, device=x.device, dtype=x.dtype)
+            if T:
+                w = _weight_operand(_matrices(weight, Np, Kp))
+                nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, ptr(w), ptr(offsets), G, T, Np, Kp, code, ptr(dx),
+                         err, s)
+            dx = dx if Kp == K else dx[:, :K]
+        if want_w:
+            dw = torch.empty(G, Np, Kp, device=x.device, dtype=x.dtype)
+            b, ldb = _operand(x, Kp) if T else (x, Kp)
+            nbytes = int(nat.load().fuma_grouped_wgrad_work_bytes(T, Np, Kp))
+            work = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+            nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, ptr(b), ldb, ptr(offsets), G, T, Np, Kp, code, ptr(dw),
+                     ptr(work), nbytes, err, s)
+            dw = dw if (Np, Kp) == (N, K) else dw[:, :N, :K]
+        if want_b:
+            shared = len(ctx.bias_shape) == 1
+            db = torch.empty(*ctx.bias_shape[:-1], Np, device=x.device, dtype=x.dtype)
+            nbytes = int(nat.load().fuma_grouped_bias_grad_work_bytes(T, Np, 1 if shared else G))
+            work = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+            nat.call("fuma_grouped_bias_grad", ptr(g), g.stride(0) if T else Np, ptr(offsets), G, 1 if shared else 0, T,
+                     Np, code, ptr(db), ptr(work), nbytes, s)
+            db = db if Np == N else db[..., :N]
+        return dx, dw, None, db
+
+
+def check_groups(x: torch.Tensor, G: int, N: int, K: int, offsets: torch.Tensor | None, bias: torch.Tensor | None):
+    """The argument checks that the grouped dense maps share."""
+    if x.dim() != 2 or x.shape[1] != K:
+        raise ValueError(f"x must be [rows, {K}] (got {tuple(x.shape)})")
+    if not 1 <= G <= MAX_GROUPS:
+        raise ValueError(f"the number of groups must be from 1 to {MAX_GROUPS} (got {G})")
+    if offsets is not None:
+        if offsets.dtype != torch.int64:
+            raise TypeError(f"offsets must be int64 (got {offsets.dtype})")
+        if offsets.shape != (G + 1,):
+            raise ValueError(f"offsets must be [{G + 1}] for {G} groups (got {tuple(offsets.shape)})")
+    if bias is not None and bias.shape not in ((N,), (G, N)):
+        raise ValueError(f"bias must be [{N}] or [{G}, {N}] (got {tuple(bias.shape)})")
+
+
+@torch.compiler.disable
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
+                   bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``y[t] = weight[g] @ x[t] (+ bias)`` for the rows ``offsets[g] <= t < offsets[g + 1]``.
+
+    x [T, K]; weight [G, N, K]; offsets [G + 1] int64 on the same GPU, not decreasing, within
+    [0, T] (groups may be empty; the values are read on the device, so the call does not
+    synchronise); bias [N] (one for all groups) or [G, N]. All of one type: float32, bfloat16 or
+    float16. Returns [T, N]; rows outside [offsets[0], offsets[G]) come back as zeros and get zero
+    gradients. Differentiable in x, weight and bias (once); repeated calls give the same bits.
+
+    K and N that are not multiples of 8 run on zero-padded copies, rows that are not contiguous
+    or 16-byte aligned on a copy. Bad offset values are recorded in the device error flag
+    (:func:`flash_uma_b200.linear.check_errors`); an infinite fp32 input may give NaN where fp32
+    arithmetic gives an infinity."""
+    nat.require_cuda(x, weight, offsets, bias)
+    if weight.dim() != 3:
+        raise ValueError(f"weight must be [groups, N, K] (got {tuple(weight.shape)})")
+    G, N, K = weight.shape
+    _check_dtype("x", x)
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise TypeError("x, weight and bias must have the same dtype")
+    if N < 1 or K < 1:
+        raise ValueError(f"weight needs N >= 1 and K >= 1 (got {tuple(weight.shape)})")
+    check_groups(x, G, N, K, offsets, bias)
+    _same_device(x, weight=weight, offsets=offsets, bias=bias)
+    edges = guard_capture(x, weight, bias)
+    out = _GroupedLinearFn.apply(x, weight, offsets.contiguous(), bias)
+    del edges
+    return out
+
+
+class _MixFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, coeff, experts):
+        S, E = coeff.shape
+        P = experts[0].numel()
+        x = _flat(experts)
+        out = torch.empty(S, *experts.shape[1:], device=experts.device, dtype=experts.dtype)
+        nat.call("fuma_mix_experts", ptr(coeff), coeff.stride(0), coeff.stride(1), ptr(x), S, E, P,
+                 _DTYPES[experts.dtype], ptr(out), stream_of(experts))
+        ctx.save_for_backward(coeff, experts)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        coeff, experts = ctx.saved_tensors
+        S, E = coeff.shape
+        P = experts[0].numel()
+        code, s = _DTYPES[experts.dtype], stream_of(experts)
+        g = _flat(g)
+        dc = de = None
+        if ctx.needs_input_grad[0]:
+            dc = torch.zeros(S, E, device=coeff.device) if P == 0 else torch.empty(S, E, device=coeff.device)
+            nbytes = int(nat.load().fuma_mix_experts_work_bytes(S, E, P))
+            if nbytes:
+                work = torch.empty(nbytes, device=coeff.device, dtype=torch.uint8)
+                nat.call("fuma_mix_experts_dcoeff", ptr(g), ptr(_flat(experts)), S, E, P, code, ptr(dc), ptr(work),
+                         nbytes, s)
+        if ctx.needs_input_grad[1]:
+            de = torch.empty(experts.shape, device=experts.device, dtype=experts.dtype)
+            if S == 0:
+                de.zero_()
+            else:
+                nat.call("fuma_mix_experts", ptr(coeff), coeff.stride(1), coeff.stride(0), ptr(g), E, S, P, code,
+                         ptr(de), s)
+        return dc, de
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+@torch.compiler.disable
+def mix_experts(coeff: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
+    """``W[s] = sum_e coeff[s, e] experts[e]``: coeff [S, E] float32 (any strides), experts [E, ...]
+    float32, bfloat16 or float16 -> [S, ...] of the experts' type, summed in fp32. Differentiable
+    (once) in both; the gradient of coeff is float32, its sum over a matrix joined in fp64."""
+    nat.require_cuda(coeff, experts)
+    _check_dtype("experts", experts)
+    if coeff.dtype != torch.float32:
+        raise TypeError(f"coeff must be float32 (got {coeff.dtype})")
+    if experts.dim() < 1 or coeff.dim() != 2 or coeff.shape[1] != experts.shape[0] or experts.shape[0] < 1:
+        raise ValueError(f"coeff must be [systems, experts] for experts [experts, ...] (got {tuple(coeff.shape)} and "
+                         f"{tuple(experts.shape)})")
+    _same_device(experts, coeff=coeff)
+    edges = guard_capture(coeff, experts)
+    out = _MixFn.apply(coeff, experts)
+    del edges
+    return out
+
+
+class MoleLinear(nn.Module):
+    """Mixture-of-linear-experts layer: experts [E, N, K] and one bias [N], trainable;
+    ``forward(x, coeff, offsets)`` maps the rows of system s (``offsets[s] <= t < offsets[s + 1]``)
+    with ``sum_e coeff[s, e] experts[e]``. ``coeff`` [systems, E] float32 comes from the model's
+    router (a softmax over the system embedding, say) and gets its gradient."""
+
+    def __init__(self, experts: torch.Tensor, bias: torch.Tensor | None = None):
+        super().__init__()
+        if experts.dim() != 3:
+            raise ValueError(f"experts must be [experts, N, K] (got {tuple(experts.shape)})")
+        self.experts = nn.Parameter(experts.detach().clone())
+        self.bias = None if bias is None else nn.Parameter(bias.detach().clone())
+
+    def forward(self, x: torch.Tensor, coeff: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+        return grouped_linear(x, mix_experts(coeff, self.experts), offsets, self.bias)
+
+    def extra_repr(self) -> str:
+        E, N, K = self.experts.shape
+        return f"experts={E}, N={N}, K={K}, bias={self.bias is not None}"

@@ -36,6 +36,7 @@ _err_host: dict[int, torch.Tensor] = {}     # pinned mirrors, filled asynchronou
 
 _ERR_RANGE = 16
 _ERR_INDEX = 32   # fuma_morton_reorder: an edge index outside [0, N)
+_ERR_OFFSETS = 64   # grouped dense maps: group offsets that decrease or leave [0, T]
 
 
 def default_mode() -> str:
@@ -47,8 +48,9 @@ def default_mode() -> str:
 
 def error_flag(device: torch.device) -> torch.Tensor:
     """Per-device int32 flag (the first error recorded is kept): a GEMM pipeline wait timed out
-    (codes 1-5), an f16x3 input is out of the fp16 range (code 16), or the Morton reorder met an
-    edge index outside [0, N) (code 32)."""
+    (codes 1-5), an f16x3 input is out of the fp16 range (code 16), the Morton reorder met an
+    edge index outside [0, N) (code 32), or a grouped dense map got offsets that decrease or leave
+    [0, T] (code 64)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _err_flags.get(idx)
     if t is None:
@@ -61,6 +63,9 @@ def _raise(idx: int, code: int):
     if code == _ERR_INDEX:
         raise RuntimeError(f"fuma_morton_reorder: an edge index on cuda:{idx} is outside [0, num_atoms); the edge "
                            "was renumbered to atom 0 and the results are invalid")
+    if code == _ERR_OFFSETS:
+        raise RuntimeError(f"grouped_linear: the group offsets of a call on cuda:{idx} decrease or leave [0, rows]; "
+                           "its results are invalid")
     if code == _ERR_RANGE:
         raise RuntimeError(f"fuma_linear_f16x3: an input value on cuda:{idx} is beyond the fp16 range of the f16x3 "
                            "split (|x| >= 65520); construct the model with gemm='tf32x3' for such data")

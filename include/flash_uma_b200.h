@@ -322,6 +322,65 @@ int fuma_morton_reorder_noalloc(const float* pos, const int64_t* Z, const int64_
                                 float* pos_s, int64_t* Z_s, int64_t* batch_s, int64_t* ii, int64_t* jj, int* err_flag,
                                 void* stream);
 
+/* ---- mixture of linear experts: mixed weights, grouped dense maps, fp8 dense maps ------------
+ * The reference takes a model whose experts FAIRChem has merged for ONE composition; these entry
+ * points are the dense layers of a batch of unlike systems, where every system has its own
+ * weighted mean of the experts. No counterpart in the reference.
+ *
+ * dtype: 0 fp32, 1 bf16, 2 fp16 (the arrays declared void*). Groups: rows [offsets[g],
+ * offsets[g + 1]) of the T rows go through matrix g; offsets [G + 1] is a device array, so the
+ * launch needs no host copy of it; empty groups are allowed, rows outside [offsets[0],
+ * offsets[G]) are written as zeros, and offsets may be NULL for one group of all rows. Offsets that
+ * decrease or leave [0, T] put 64 into err_flag (the results are then undefined, all accesses stay in
+ * bounds). 1 <= G <= 4096; N and K multiples of 8; leading dimensions (elements) multiples of 8;
+ * arrays 16-byte aligned. Work space: see the *_work_bytes functions (0: may be NULL).
+ *
+ * fp32 operands come as three bf16 planes (fuma_split_bf16x3 of x, dy and W viewed as rows): plane
+ * i starts i * rows * ld elements after plane 0. Results and biases are fp32.
+ *
+ * y[t, n] = sum_k x[t, k] W[g, n, k] + bias (bias_rows 1: bias[n], G: bias[g, n]; may be NULL) */
+int fuma_grouped_linear(const void* x, int64_t ldx, const void* W, const int64_t* offsets, int32_t G,
+                        const void* bias, int32_t bias_rows, int64_t T, int32_t N, int32_t K, int32_t dtype, void* y,
+                        int* err_flag, void* stream);
+/* dx[t, k] = sum_n dy[t, n] W[g, n, k] */
+int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const void* W, const int64_t* offsets, int32_t G,
+                              int64_t T, int32_t N, int32_t K, int32_t dtype, void* dx, int* err_flag, void* stream);
+/* dW[g, n, k] = sum over the rows of g of dy[t, n] x[t, k]; zeros for a group without rows. No
+ * atomics: the same call gives the same bits. */
+int64_t fuma_grouped_wgrad_work_bytes(int64_t T, int32_t N, int32_t K);
+int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int64_t* offsets,
+                              int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dW, void* work,
+                              int64_t work_bytes, int* err_flag, void* stream);
+/* db[g, n] = sum over the rows of g of dy[t, n] (shared: one sum [n] over all groups' rows); dy itself, no planes. */
+int64_t fuma_grouped_bias_grad_work_bytes(int64_t T, int32_t N, int32_t groups);
+int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets, int32_t G, int32_t shared, int64_t T,
+                           int32_t N, int32_t dtype, void* db, void* work, int64_t work_bytes, void* stream);
+/* out [3][rows][cols] bf16: x = p0 + p1 + p2 to 24 bits over the whole fp32 range (rows ldx floats apart). */
+int fuma_split_bf16x3(const float* x, int64_t ldx, int64_t rows, int32_t cols, void* out, void* stream);
+/* Block-scaled e4m3 operands: a block of 128 values is stored as codes times the smallest power of two
+ * (at least 2^-126) that brings its largest magnitude to 448 or below, rounded to nearest even; a block
+ * with a value that is not finite gets the scale NaN.
+ * Rows x [T, K] -> codes [T, ldq] (ldq: K rounded up to 16), scales [ceil(K / 128)][T]. */
+int fuma_quantize_rows_fp8(const void* x, int64_t ldx, int64_t T, int32_t K, int32_t dtype, void* codes, int64_t ldq,
+                           float* scales, void* stream);
+/* Weights w [G, N, K] in 128 x 128 blocks -> codes [G, N, ldq], scales [G][ceil(N/128)][ceil(K/128)] and the
+ * transposed codes_t [G, K, ldt], scales_t [G][ceil(K/128)][ceil(N/128)] (the input gradient's operand). */
+int fuma_quantize_weight_fp8(const float* w, int32_t G, int32_t N, int32_t K, void* codes, int64_t ldq, float* scales,
+                             void* codes_t, int64_t ldt, float* scales_t, void* stream);
+/* fuma_grouped_linear on such operands (codes [T, ceil16(K)] and [G, N, ceil16(K)]); y of type out_dtype,
+ * bias fp32. The input gradient is the same call on the quantised gradient and the transposed weights. */
+int fuma_grouped_linear_fp8(const void* x_codes, const float* x_scales, const void* w_codes, const float* w_scales,
+                            const int64_t* offsets, int32_t G, const float* bias, int32_t bias_rows, int64_t T,
+                            int32_t N, int32_t K, int32_t out_dtype, void* y, int* err_flag, void* stream);
+/* out[s, p] = sum_e coeff[s * stride_s + e * stride_e] experts[e, p], p < P; coeff fp32. With the
+ * strides and S, E exchanged, the experts' gradient from the mixed weights' gradient. */
+int fuma_mix_experts(const float* coeff, int64_t stride_s, int64_t stride_e, const void* experts, int32_t S, int32_t E,
+                     int64_t P, int32_t dtype, void* out, void* stream);
+/* dcoeff[s, e] = sum_p grad[s, p] experts[e, p], fp32 [S, E], joined in fp64 without atomics. */
+int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P);
+int fuma_mix_experts_dcoeff(const void* grad, const void* experts, int32_t S, int32_t E, int64_t P, int32_t dtype,
+                            float* dcoeff, void* work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,91 @@
+"""Refusals of the expert-mixture entry points, on the host and without a GPU: the C ABI checks its
+arguments before any launch, the Python calls refuse CPU tensors."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flash_uma_b200 import _native, build
+    build.build()
+    return _native.load()
+
+
+P = 4096   # a 16-byte aligned non-null address that no check reads
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(G=0), b"G=0"), (dict(G=4097), b"G=4097"), (dict(T=-1), b"T=-1"), (dict(T=2 ** 31), b"out of range"),
+    (dict(N=12), b"multiples of 8"), (dict(K=0), b"multiples of 8"), (dict(dtype=3), b"dtype=3"),
+    (dict(ldx=8), b"ldx=8"), (dict(ldx=20), b"ldx=20"), (dict(bias=P, bias_rows=2), b"bias_rows=2"),
+    (dict(x=None), b"null pointer"), (dict(offsets=None), b"one group only"),
+    (dict(T=2 ** 31 - 512, N=2 ** 20, G=1), b"too many output tiles"), (dict(G=4096, N=2 ** 20), b"too large"),
+])
+def test_grouped_linear_refusals(lib, change, message):
+    a = dict(x=P, ldx=16, W=P, offsets=P, G=3, bias=None, bias_rows=0, T=10, N=24, K=16, dtype=1, y=P)
+    a.update(change)
+    assert lib.fuma_grouped_linear(*a.values(), None, None) == -1
+    assert message in lib.fuma_last_error()
+
+
+def test_alignment_refused(lib):
+    assert lib.fuma_grouped_linear(P + 8, 16, P, P, 3, None, 0, 10, 24, 16, 1, P, None, None) == -2
+    assert lib.fuma_grouped_linear_dgrad(P, 24, P + 2, P, 3, 10, 24, 16, 1, P, None, None) == -2
+    assert lib.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P + 4, 16, P, None) == -2
+    assert lib.fuma_mix_experts(P, 4, 1, P + 4, 2, 4, 64, 0, P, None) == -2
+
+
+def test_other_refusals(lib):
+    f = lib
+    assert f.fuma_grouped_linear_dgrad(P, 16, P, P, 3, 10, 24, 16, 1, P, None, None) == -1        # lddy < N
+    assert f.fuma_split_bf16x3(P, 6, 4, 6, P, None) == -1
+    assert f.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P, 24, P, None) == -1                        # ldq
+    assert f.fuma_quantize_weight_fp8(P, 1, 24, 16, P, 16, P, P, 24, P, None) == -1               # ldt
+    assert f.fuma_grouped_linear_fp8(P, P, P, P, None, 2, None, 0, 10, 24, 16, 1, P, None, None) == -1
+    assert f.fuma_mix_experts(P, 4, 1, P, 2, 0, 64, 0, P, None) == -1
+    assert f.fuma_mix_experts_dcoeff(P, P, 2, 4, 64, 5, P, P, 1 << 20, None) == -1
+    assert f.fuma_mix_experts_dcoeff(P, P, 2, 4, 64, 0, P, P, 4, None) == -1                      # work space
+    # nothing to do: no launch, no device needed
+    assert f.fuma_grouped_linear(None, 16, None, None, 3, None, 0, 0, 24, 16, 1, None, None, None) == 0
+    assert f.fuma_mix_experts(None, 4, 1, None, 0, 4, 64, 0, None, None) == 0
+
+
+def test_work_sizes(lib):
+    """The weight gradient's work space holds two slots per chunk bound of the rows; none for short batches."""
+    n = lib.fuma_grouped_wgrad_work_bytes
+    assert n(0, 64, 64) == 0 and n(2048, 64, 64) == 0
+    assert n(2049, 64, 64) >= 2 * 2 * 64 * 64 * 4
+    assert lib.fuma_grouped_bias_grad_work_bytes(1000, 64, 5) >= (2 + 5) * 64 * 4
+    assert lib.fuma_mix_experts_work_bytes(3, 4, 1000) >= 3 * 4 * 4
+
+
+def test_partial_slots_never_meet():
+    """The slot rule of the weight gradient's partial matrices, restated: over random group lengths no two
+    chunks share a slot and all stay inside the work space."""
+    g = torch.Generator().manual_seed(0)
+    chunk = 64
+    for _ in range(300):
+        lens = (torch.rand(12, generator=g) ** 3 * 400).long().tolist()
+        T, a, used = sum(lens), 0, set()
+        slots = T // chunk + 1
+        for n in lens:
+            if n > chunk:
+                for c in range(-(-n // chunk)):
+                    s = a // chunk if c == 0 else slots + a // chunk + c
+                    assert s not in used and 0 <= s < 2 * slots
+                    assert c == 0 or s >= slots
+                    used.add(s)
+            a += n
+
+
+def test_cpu_tensors_refused():
+    from flash_uma_b200.fp8 import Fp8Weight, quantize_rows
+    from flash_uma_b200.grouped import grouped_linear, mix_experts
+    x = torch.zeros(4, 8)
+    for call in (lambda: grouped_linear(x, torch.zeros(1, 8, 8), torch.tensor([0, 4])),
+                 lambda: mix_experts(torch.zeros(2, 3), torch.zeros(3, 8)),
+                 lambda: quantize_rows(x), lambda: Fp8Weight(x)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
