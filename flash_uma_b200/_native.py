@@ -59,9 +59,9 @@ _SIGS = {
     "fuma_split_bf16x3": [_P, _I64, _I64, _I32, _P, _P],
     "fuma_quantize_rows_fp8": [_P, _I64, _I64, _I32, _I32, _P, _I64, _P, _P],
     "fuma_quantize_weight_fp8": [_P, _I32, _I32, _I32, _P, _I64, _P, _P, _I64, _P, _P],
-    "fuma_grouped_linear_fp8": [_P, _P, _P, _P, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
-    "fuma_mix_experts": [_P, _I64, _I64, _P, _I32, _I32, _I64, _I32, _P, _P],
-    "fuma_mix_experts_dcoeff": [_P, _P, _I32, _I32, _I64, _I32, _P, _P, _I64, _P],
+    "fuma_grouped_linear_fp8": [_P, _I64, _P, _P, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I64, _P, _P],
+    "fuma_mix_experts": [_P, _I64, _I64, _P, _I32, _I32, _I64, _I32, _P, _P, _P],
+    "fuma_mix_experts_bwd": [_P, _P, _I64, _I64, _P, _I32, _I32, _I64, _I32, _P, _P, _P, _I64, _P, _P],
     "fuma_morton_reorder_noalloc": [_P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P],
 }
 
@@ -71,7 +71,8 @@ _SIZE_SIGS = {
     "fuma_neighbor_scratch_bytes": [_I64, _P],
     "fuma_grouped_wgrad_work_bytes": [_I64, _I32, _I32],
     "fuma_grouped_bias_grad_work_bytes": [_I64, _I32, _I32],
-    "fuma_mix_experts_work_bytes": [_I32, _I32, _I64],
+    "fuma_fp8_work_bytes": [_I64, _I32],
+    "fuma_mix_experts_work_bytes": [_I32, _I32, _I64, _I32],
 }
 
 _lib = None
@@ -119,7 +120,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """The current stream of ``t``'s device as a cudaStream_t (the raw handle: a Stream object costs 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 # kernels each entry point launches (used by launch accounting)
@@ -137,7 +139,8 @@ KERNELS_PER_CALL = {name: 1 for name in _SIGS}
 KERNELS_PER_CALL["fuma_gather_bwd"] = 3
 KERNELS_PER_CALL["fuma_grouped_linear_wgrad"] = 2
 KERNELS_PER_CALL["fuma_grouped_bias_grad"] = 2
-KERNELS_PER_CALL["fuma_mix_experts_dcoeff"] = 2
+KERNELS_PER_CALL["fuma_grouped_linear_fp8"] = 2
+KERNELS_PER_CALL["fuma_mix_experts_bwd"] = 2
 KERNELS_PER_CALL["fuma_gather_fwd"] = 2
 KERNELS_PER_CALL["fuma_csr_permute"] = 2
 KERNELS_PER_CALL["fuma_neighbor_list"] = 4

@@ -707,8 +707,8 @@ int64_t fuma_grouped_bias_grad_work_bytes(int64_t T, int32_t N, int32_t groups) 
   return T > 0 && N > 0 && groups > 0 ? grouped_colsum_work_bytes(T, N, groups) : 0;
 }
 
-int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P) {
-  return S > 0 && E > 0 && P > 0 ? mix_dcoeff_work_bytes(S, E, P) : 0;
+int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P, int32_t dtype) {
+  return S > 0 && E > 0 && P > 0 ? mix_bwd_work_bytes(S, E, P, dtype) : 0;
 }
 
 namespace {
@@ -854,55 +854,71 @@ int fuma_quantize_weight_fp8(const float* w, int32_t G, int32_t N, int32_t K, vo
   return launched("quantize_weight_fp8");
 }
 
-int fuma_grouped_linear_fp8(const void* x_codes, const float* x_scales, const void* w_codes, const float* w_scales,
+int64_t fuma_fp8_work_bytes(int64_t T, int32_t K) {
+  if (T <= 0 || K <= 0) return 0;
+  return (T * ((K + 15) / 16 * 16) + 255) / 256 * 256 + (K + 127) / 128 * T * 4;
+}
+
+int fuma_grouped_linear_fp8(const void* x, int64_t ldx, const void* w_codes, const float* w_scales,
                             const int64_t* offsets, int32_t G, const float* bias, int32_t bias_rows, int64_t T,
-                            int32_t N, int32_t K, int32_t out_dtype, void* y, int* err_flag, void* stream) {
-  CHECK(check_grouped("grouped_linear_fp8", G, T, N, K, out_dtype));
+                            int32_t N, int32_t K, int32_t dtype, void* y, void* work, int64_t work_bytes, int* err_flag,
+                            void* stream) {
+  CHECK(check_grouped("grouped_linear_fp8", G, T, N, K, dtype));
+  REQUIRE(ldx >= K && ldx % 8 == 0, "grouped_linear_fp8: ldx=%lld must be >= K and a multiple of 8", (long long)ldx);
   REQUIRE(!bias || bias_rows == 1 || bias_rows == G, "grouped_linear_fp8: bias_rows=%d must be 1 or G", bias_rows);
   if (T == 0) return FUMA_OK;
-  REQUIRE(x_codes && x_scales && w_codes && w_scales && y, "grouped_linear_fp8: null pointer");
+  REQUIRE(x && w_codes && w_scales && y && work, "grouped_linear_fp8: null pointer");
   REQUIRE(offsets || G == 1, "grouped_linear_fp8: offsets may be NULL for one group only");
-  REQUIRE_ALIGNED(x_codes, "x_codes"); REQUIRE_ALIGNED(w_codes, "w_codes"); REQUIRE_ALIGNED(y, "y");
-  BIND(x_codes);
+  REQUIRE(work_bytes >= fuma_fp8_work_bytes(T, K), "grouped_linear_fp8: needs %lld bytes of work space, got %lld",
+          (long long)fuma_fp8_work_bytes(T, K), (long long)work_bytes);
+  REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(w_codes, "w_codes"); REQUIRE_ALIGNED(y, "y"); REQUIRE_ALIGNED(work, "work");
+  BIND(x);
   const int64_t ld = (K + 15) / 16 * 16;
-  GroupedOperands o{x_codes, w_codes, ld, ld, 2, 0};
+  uint8_t* codes = static_cast<uint8_t*>(work);
+  float* scales = reinterpret_cast<float*>(codes + (T * ld + 255) / 256 * 256);
+  launch_quantize_rows(x, ldx, dtype, T, K, codes, ld, scales, (cudaStream_t)stream);
+  CHECK(launched("grouped_linear_fp8"));
+  GroupedOperands o{codes, w_codes, ld, ld, 2, 0};
   GroupedArgs p{};
   p.offsets = offsets; p.G = G; p.T = T; p.N = N; p.K = K;
-  p.C = y; p.ldc = N; p.out_dtype = out_dtype;
+  p.C = y; p.ldc = N; p.out_dtype = dtype;
   p.bias = bias; p.bias_rows = bias_rows; p.bias_dtype = kDtypeF32;
-  p.scale_a = x_scales; p.scale_b = w_scales; p.blocks_n = (N + 127) / 128;
+  p.scale_a = scales; p.scale_b = w_scales; p.blocks_n = (N + 127) / 128;
   return grouped_done("grouped_linear_fp8", launch_grouped_rows(o, p, false, err_flag, (cudaStream_t)stream));
 }
 
 int fuma_mix_experts(const float* coeff, int64_t stride_s, int64_t stride_e, const void* experts, int32_t S, int32_t E,
-                     int64_t P, int32_t dtype, void* out, void* stream) {
+                     int64_t P, int32_t dtype, void* out, int* err_flag, void* stream) {
   REQUIRE(S >= 0 && E > 0 && P >= 0 && P <= (int64_t(1) << 38), "mix_experts: bad sizes S=%d E=%d P=%lld", S, E,
           (long long)P);
+  REQUIRE(S <= 64 * 65535, "mix_experts: S=%d too large", S);
   REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "mix_experts: dtype=%d must be 0, 1 or 2", dtype);
   if (S == 0 || P == 0) return FUMA_OK;
   REQUIRE(coeff && experts && out, "mix_experts: null pointer");
   REQUIRE_ALIGNED(experts, "experts"); REQUIRE_ALIGNED(out, "out");
   BIND(experts);
-  return grouped_done("mix_experts", (int)launch_mix(coeff, stride_s, stride_e, experts, S, E, P, dtype, out,
+  return grouped_done("mix_experts", (int)launch_mix(coeff, stride_s, stride_e, experts, S, E, P, dtype, out, err_flag,
                                                      (cudaStream_t)stream));
 }
 
-int fuma_mix_experts_dcoeff(const void* grad, const void* experts, int32_t S, int32_t E, int64_t P, int32_t dtype,
-                            float* dcoeff, void* work, int64_t work_bytes, void* stream) {
-  REQUIRE(S >= 0 && E > 0 && P > 0 && P <= (int64_t(1) << 38), "mix_experts_dcoeff: bad sizes S=%d E=%d P=%lld", S, E,
+int fuma_mix_experts_bwd(const void* grad, const float* coeff, int64_t stride_s, int64_t stride_e, const void* experts,
+                         int32_t S, int32_t E, int64_t P, int32_t dtype, float* dcoeff, void* dexperts, void* work,
+                         int64_t work_bytes, int* err_flag, void* stream) {
+  REQUIRE(S > 0 && E > 0 && P > 0 && P <= (int64_t(1) << 38), "mix_experts_bwd: bad sizes S=%d E=%d P=%lld", S, E,
           (long long)P);
-  REQUIRE(S <= 64 * 65535 && E <= 64 * 65535, "mix_experts_dcoeff: S=%d or E=%d too large", S, E);
-  REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "mix_experts_dcoeff: dtype=%d must be 0, 1 or 2", dtype);
-  if (S == 0) return FUMA_OK;
-  const int64_t need = mix_dcoeff_work_bytes(S, E, P);
-  REQUIRE(grad && experts && dcoeff && work, "mix_experts_dcoeff: null pointer");
-  REQUIRE(work_bytes >= need, "mix_experts_dcoeff: needs %lld bytes of work space, got %lld", (long long)need,
-          (long long)work_bytes);
-  REQUIRE_ALIGNED(grad, "grad"); REQUIRE_ALIGNED(experts, "experts"); REQUIRE_ALIGNED(work, "work");
+  REQUIRE(S <= 64 * 65535 && E <= 64 * 65535, "mix_experts_bwd: S=%d or E=%d too large", S, E);
+  REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "mix_experts_bwd: dtype=%d must be 0, 1 or 2", dtype);
+  REQUIRE(grad && coeff && experts && (dcoeff || dexperts), "mix_experts_bwd: null pointer");
+  const int64_t need = dcoeff ? mix_bwd_work_bytes(S, E, P, dtype) : 0;
+  REQUIRE(work_bytes >= need && (need == 0 || work), "mix_experts_bwd: needs %lld bytes of work space, got %lld",
+          (long long)need, (long long)work_bytes);
+  REQUIRE_ALIGNED(grad, "grad"); REQUIRE_ALIGNED(experts, "experts");
+  if (work) REQUIRE_ALIGNED(work, "work");
+  if (dexperts) REQUIRE_ALIGNED(dexperts, "dexperts");
   BIND(grad);
-  return grouped_done("mix_experts_dcoeff", (int)launch_mix_dcoeff(grad, experts, S, E, P, dtype,
-                                                                   static_cast<float*>(work), dcoeff,
-                                                                   (cudaStream_t)stream));
+  return grouped_done("mix_experts_bwd", (int)launch_mix_bwd(coeff, stride_s, stride_e, grad, experts, S, E, P, dtype,
+                                                             dcoeff, dexperts, static_cast<float*>(work), err_flag,
+                                                             (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -463,26 +463,29 @@ __global__ void __launch_bounds__(kGThreads, 1)
       for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
       const float* sa = nullptr;
       const float* sb = nullptr;
-      float s_next = 1.0f;
+      float a_next = 1.0f, b_next = 1.0f;
       if constexpr (kKind == kFp8) {
         // the scales of one segment ahead, so their latency hides behind the wait for its MMAs
         const int64_t r = min(t.row0 + q * 32 + lane, p.T - 1);
         sa = p.scale_a + r;
         sb = p.scale_b + ((int64_t)t.g * p.blocks_n + min(n0 / 128, p.blocks_n - 1)) * t.kblocks;
-        s_next = sa[0] * sb[0];
+        a_next = sa[0];
+        b_next = sb[0];
       }
       bool ok = true;
       for (int sg = 0; sg < segs; ++sg, ++seg) {
         const int buf = seg % L::kBufs;
-        const float s = s_next;
+        const float s_a = a_next, s_b = b_next;   // multiplied after the wait: the loads stay in flight
         if constexpr (kKind == kFp8) {
           const int kb = sg + 1 < segs ? sg + 1 : sg;
-          s_next = sa[(int64_t)kb * p.T] * sb[kb];
+          a_next = sa[(int64_t)kb * p.T];
+          b_next = sb[kb];
         }
         ok = mbar_wait(&bar_acc_full[buf], (seg / L::kBufs) & 1, abort_flag, p.err, kErrWaitAcc);
         ok = __all_sync(kFull, ok && !*abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const float s = s_a * s_b;
         const uint32_t taddr = tmem + (uint32_t)(buf * L::kAccCols + col0) + ((uint32_t)(q * 32) << 16);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {

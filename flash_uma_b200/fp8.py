@@ -14,7 +14,7 @@ import torch
 
 from . import _native as nat
 from ._native import ptr, stream_of
-from .grouped import MAX_GROUPS, _ceil8, _check_dtype, _rows, _same_device, check_groups, guard_capture
+from .grouped import _DTYPES, MAX_GROUPS, _apply, _ceil8, _check_dtype, _rows, _same_device, check_groups, guard_capture
 from .linear import error_flag
 
 _BLOCK = 128
@@ -80,26 +80,32 @@ def quantize_rows(x: torch.Tensor):
 
 
 def _product(x, w_codes, w_scales, offsets, bias, N, K):
-    T = x.shape[0]
-    y = torch.empty(T, N, device=x.device, dtype=x.dtype)
+    T, G = x.shape[0], w_codes.shape[0]
+    y = torch.empty((T, N), device=x.device, dtype=x.dtype)
     if T:
-        codes, scales = quantize_rows(x)
-        nat.call("fuma_grouped_linear_fp8", ptr(codes), ptr(scales), ptr(w_codes), ptr(w_scales), ptr(offsets),
-                 w_codes.shape[0], ptr(bias), 0 if bias is None else (1 if bias.dim() == 1 else w_codes.shape[0]), T, N,
-                 K, _check_dtype("x", x), ptr(y), ptr(error_flag(x.device)), stream_of(x))
+        x = _rows(x, K)
+        nbytes = nat.load().fuma_fp8_work_bytes(T, K)   # the quantised rows and their scales
+        work = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+        nat.call("fuma_grouped_linear_fp8", ptr(x), x.stride(0), ptr(w_codes), ptr(w_scales), ptr(offsets), G, ptr(bias),
+                 0 if bias is None else (1 if bias.dim() == 1 else G), T, N, K, _DTYPES[x.dtype], ptr(y), ptr(work),
+                 nbytes, ptr(error_flag(x.device)), stream_of(x))
     return y
 
 
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
+    def compute(x, weight, offsets, bias):
+        if bias is not None:
+            pad = weight.Np - weight.N
+            bias = torch.nn.functional.pad(bias, (0, pad)) if pad else bias.contiguous()
+        y = _product(x, weight.codes, weight.scales, offsets, bias, weight.Np, weight.Kp)
+        return y if weight.Np == weight.N else y[:, : weight.N]
+
+    @staticmethod
     def forward(ctx, x, weight, offsets, bias):
         ctx.weight = weight
         ctx.save_for_backward(*(() if offsets is None else (offsets,)))
-        b = bias
-        if b is not None:
-            b = torch.nn.functional.pad(b, (0, weight.Np - weight.N)) if weight.Np != weight.N else b.contiguous()
-        y = _product(x, weight.codes, weight.scales, offsets, b, weight.Np, weight.Kp)
-        return y if weight.Np == weight.N else y[:, : weight.N]
+        return _Fp8LinearFn.compute(x, weight, offsets, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -133,7 +139,4 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Weight, offsets: torch.Tensor | None 
         raise ValueError(f"offsets are needed for the weight's {weight.G} matrices")
     check_groups(x, weight.G, weight.N, weight.K, offsets, bias)
     _same_device(x, weight=weight, offsets=offsets, bias=bias)
-    edges = guard_capture(x)
-    out = _Fp8LinearFn.apply(x, weight, None if offsets is None else offsets.contiguous(), bias)
-    del edges
-    return out
+    return _apply(_Fp8LinearFn, guard_capture(x), x, weight, None if offsets is None else offsets.contiguous(), bias)

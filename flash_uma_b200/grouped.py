@@ -17,6 +17,8 @@ whole fp32 range, no range error), bf16 and fp16 (fp32 sums, one rounding at the
 """
 from __future__ import annotations
 
+import weakref
+
 import torch
 import torch.nn as nn
 
@@ -41,30 +43,37 @@ def _same_device(first: torch.Tensor, **others) -> None:
             raise ValueError(f"{name} is on {t.device}, the call's other tensors on {first.device}")
 
 
-_EAGER = "flash_uma_b200.eager"
+# autograd nodes of eager calls, while their graph is alive
+_live_nodes: "weakref.WeakSet" = weakref.WeakSet()
 
 
-def guard_capture(*inputs) -> list:
-    """Refuse to put a call on leaf tensors into a CUDA graph capture while an eager graph of the same leaves
-    is alive: autograd keeps one gradient node per leaf, bound to the stream it was made on, and a
-    captured backward pass that meets a node of an uncaptured stream invalidates the capture or ends the
-    process. The node carries a mark from the first eager call, and goes with the eager graph; the
-    caller holds the returned list until its own graph holds the nodes."""
-    if not torch.is_grad_enabled():
-        return []
-    leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
-    if not leaves:
-        return []
-    capturing = torch.cuda.is_current_stream_capturing()
-    edges = [torch.autograd.graph.get_gradient_edge(t) for t in leaves]
-    for e in edges:
-        marks = e.node.metadata
-        if not capturing:
-            marks[_EAGER] = True
-        elif marks.get(_EAGER):
-            raise RuntimeError("a CUDA graph capture of this call needs the results of earlier eager calls on the "
-                               "same leaf tensors to be released or detached first (their autograd graph is alive)")
-    return edges
+def guard_capture(*inputs) -> bool:
+    """True if the current stream is capturing. Refuses to put a call on leaf tensors into a CUDA graph capture
+    while an eager graph of the same leaves is alive: autograd keeps one gradient node per leaf, bound to the
+    stream it was made on, and a captured backward pass that meets a node of an uncaptured stream
+    invalidates the capture or ends the process. Seen are the eager calls of this module and of fp8."""
+    if not torch.cuda.is_current_stream_capturing():
+        return False
+    if torch.is_grad_enabled():
+        leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
+        for node in list(_live_nodes):
+            for edge, _ in node.next_functions:
+                held = getattr(edge, "variable", None)
+                if held is not None and any(held is t for t in leaves):
+                    raise RuntimeError("a CUDA graph capture of this call needs the results of earlier eager calls on "
+                                       "the same leaf tensors to be released or detached first (their autograd graph "
+                                       "is alive)")
+    return True
+
+
+def _apply(fn, capturing: bool, *args):
+    """``fn.apply`` where a gradient may be asked for, else its forward alone."""
+    if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
+        return fn.compute(*args)
+    out = fn.apply(*args)
+    if not capturing:
+        _live_nodes.add(out.grad_fn)
+    return out
 
 
 def _rows(x: torch.Tensor, cols: int) -> torch.Tensor:
@@ -112,24 +121,27 @@ def _weight_operand(w: torch.Tensor) -> torch.Tensor:
 
 class _GroupedLinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, offsets, bias):
+    def compute(x, weight, offsets, bias):
         T = x.shape[0]
         G, N, K = weight.shape
         Np, Kp = _ceil8(N), _ceil8(K)
-        code = _DTYPES[x.dtype]
-        ctx.save_for_backward(x, weight, offsets)
-        ctx.bias_shape = None if bias is None else bias.shape
-        y = torch.empty(T, Np, device=x.device, dtype=x.dtype)
+        y = torch.empty((T, Np), device=x.device, dtype=x.dtype)
         if T:
-            b = bias
-            if b is not None:
-                b = torch.nn.functional.pad(b, (0, Np - N)) if Np != N else b.contiguous()
+            bias_rows = 0
+            if bias is not None:
+                bias_rows = 1 if bias.dim() == 1 else G
+                bias = torch.nn.functional.pad(bias, (0, Np - N)) if Np != N else bias.contiguous()
             a, lda = _operand(x, Kp)
             w = _weight_operand(_matrices(weight, Np, Kp))
-            nat.call("fuma_grouped_linear", ptr(a), lda, ptr(w), ptr(offsets), G, ptr(b),
-                     0 if b is None else (1 if b.dim() == 1 else G), T, Np, Kp, code, ptr(y),
-                     ptr(error_flag(x.device)), stream_of(x))
+            nat.call("fuma_grouped_linear", ptr(a), lda, ptr(w), ptr(offsets), G, ptr(bias), bias_rows, T, Np, Kp,
+                     _DTYPES[x.dtype], ptr(y), ptr(error_flag(x.device)), stream_of(x))
         return y if Np == N else y[:, :N]
+
+    @staticmethod
+    def forward(ctx, x, weight, offsets, bias):
+        ctx.save_for_backward(x, weight, offsets)
+        ctx.bias_shape = None if bias is None else bias.shape
+        return _GroupedLinearFn.compute(x, weight, offsets, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -211,47 +223,45 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
         raise ValueError(f"weight needs N >= 1 and K >= 1 (got {tuple(weight.shape)})")
     check_groups(x, G, N, K, offsets, bias)
     _same_device(x, weight=weight, offsets=offsets, bias=bias)
-    edges = guard_capture(x, weight, bias)
-    out = _GroupedLinearFn.apply(x, weight, offsets.contiguous(), bias)
-    del edges
-    return out
+    return _apply(_GroupedLinearFn, guard_capture(x, weight, bias), x, weight, offsets.contiguous(), bias)
 
 
 class _MixFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, coeff, experts):
+    def compute(coeff, experts):
         S, E = coeff.shape
-        P = experts[0].numel()
         x = _flat(experts)
-        out = torch.empty(S, *experts.shape[1:], device=experts.device, dtype=experts.dtype)
-        nat.call("fuma_mix_experts", ptr(coeff), coeff.stride(0), coeff.stride(1), ptr(x), S, E, P,
-                 _DTYPES[experts.dtype], ptr(out), stream_of(experts))
-        ctx.save_for_backward(coeff, experts)
+        out = torch.empty((S, *experts.shape[1:]), device=experts.device, dtype=experts.dtype)
+        nat.call("fuma_mix_experts", ptr(coeff), coeff.stride(0), coeff.stride(1), ptr(x), S, E, x.numel() // E,
+                 _DTYPES[experts.dtype], ptr(out), ptr(error_flag(experts.device)), stream_of(experts))
         return out
+
+    @staticmethod
+    def forward(ctx, coeff, experts):
+        ctx.save_for_backward(coeff, experts)
+        return _MixFn.compute(coeff, experts)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         coeff, experts = ctx.saved_tensors
         S, E = coeff.shape
-        P = experts[0].numel()
-        code, s = _DTYPES[experts.dtype], stream_of(experts)
-        g = _flat(g)
-        dc = de = None
-        if ctx.needs_input_grad[0]:
-            dc = torch.zeros(S, E, device=coeff.device) if P == 0 else torch.empty(S, E, device=coeff.device)
-            nbytes = int(nat.load().fuma_mix_experts_work_bytes(S, E, P))
-            if nbytes:
-                work = torch.empty(nbytes, device=coeff.device, dtype=torch.uint8)
-                nat.call("fuma_mix_experts_dcoeff", ptr(g), ptr(_flat(experts)), S, E, P, code, ptr(dc), ptr(work),
-                         nbytes, s)
-        if ctx.needs_input_grad[1]:
-            de = torch.empty(experts.shape, device=experts.device, dtype=experts.dtype)
-            if S == 0:
-                de.zero_()
-            else:
-                nat.call("fuma_mix_experts", ptr(coeff), coeff.stride(1), coeff.stride(0), ptr(g), E, S, P, code,
-                         ptr(de), s)
+        P = experts.numel() // E
+        want_c, want_e = ctx.needs_input_grad
+        dev, code = experts.device, _DTYPES[experts.dtype]
+        if S == 0 or P == 0:
+            return (torch.zeros_like(coeff) if want_c else None), (torch.zeros_like(experts) if want_e else None)
+        dc = de = work = None
+        nbytes = 0
+        if want_c:
+            dc = torch.empty((S, E), device=dev)
+            nbytes = nat.load().fuma_mix_experts_work_bytes(S, E, P, code)
+            work = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        if want_e:
+            de = torch.empty(experts.shape, device=dev, dtype=experts.dtype)
+        g, x = _flat(g), _flat(experts)
+        nat.call("fuma_mix_experts_bwd", ptr(g), ptr(coeff), coeff.stride(0), coeff.stride(1), ptr(x), S, E, P, code,
+                 ptr(dc), ptr(de), ptr(work), nbytes, ptr(error_flag(dev)), stream_of(g))
         return dc, de
 
 
@@ -273,10 +283,7 @@ def mix_experts(coeff: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"coeff must be [systems, experts] for experts [experts, ...] (got {tuple(coeff.shape)} and "
                          f"{tuple(experts.shape)})")
     _same_device(experts, coeff=coeff)
-    edges = guard_capture(coeff, experts)
-    out = _MixFn.apply(coeff, experts)
-    del edges
-    return out
+    return _apply(_MixFn, guard_capture(coeff, experts), coeff, experts)
 
 
 class MoleLinear(nn.Module):

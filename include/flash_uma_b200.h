@@ -367,19 +367,24 @@ int fuma_quantize_rows_fp8(const void* x, int64_t ldx, int64_t T, int32_t K, int
  * transposed codes_t [G, K, ldt], scales_t [G][ceil(K/128)][ceil(N/128)] (the input gradient's operand). */
 int fuma_quantize_weight_fp8(const float* w, int32_t G, int32_t N, int32_t K, void* codes, int64_t ldq, float* scales,
                              void* codes_t, int64_t ldt, float* scales_t, void* stream);
-/* fuma_grouped_linear on such operands (codes [T, ceil16(K)] and [G, N, ceil16(K)]); y of type out_dtype,
- * bias fp32. The input gradient is the same call on the quantised gradient and the transposed weights. */
-int fuma_grouped_linear_fp8(const void* x_codes, const float* x_scales, const void* w_codes, const float* w_scales,
+/* fuma_grouped_linear with such weights: x [T, K] (dtype) is quantised into `work` (fuma_fp8_work_bytes), then
+ * multiplied; y has x's type, bias is fp32. The input gradient is the same call on the output's gradient and the
+ * transposed weights. */
+int64_t fuma_fp8_work_bytes(int64_t T, int32_t K);
+int fuma_grouped_linear_fp8(const void* x, int64_t ldx, const void* w_codes, const float* w_scales,
                             const int64_t* offsets, int32_t G, const float* bias, int32_t bias_rows, int64_t T,
-                            int32_t N, int32_t K, int32_t out_dtype, void* y, int* err_flag, void* stream);
-/* out[s, p] = sum_e coeff[s * stride_s + e * stride_e] experts[e, p], p < P; coeff fp32. With the
- * strides and S, E exchanged, the experts' gradient from the mixed weights' gradient. */
+                            int32_t N, int32_t K, int32_t dtype, void* y, void* work, int64_t work_bytes, int* err_flag,
+                            void* stream);
+/* out[s, p] = sum_e coeff[s * stride_s + e * stride_e] experts[e, p], p < P; coeff fp32, any P. */
 int fuma_mix_experts(const float* coeff, int64_t stride_s, int64_t stride_e, const void* experts, int32_t S, int32_t E,
-                     int64_t P, int32_t dtype, void* out, void* stream);
-/* dcoeff[s, e] = sum_p grad[s, p] experts[e, p], fp32 [S, E], joined in fp64 without atomics. */
-int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P);
-int fuma_mix_experts_dcoeff(const void* grad, const void* experts, int32_t S, int32_t E, int64_t P, int32_t dtype,
-                            float* dcoeff, void* work, int64_t work_bytes, void* stream);
+                     int64_t P, int32_t dtype, void* out, int* err_flag, void* stream);
+/* From grad [S, P]: dcoeff[s, e] = sum_p grad[s, p] experts[e, p], fp32 [S, E], joined in fp64 without atomics, and
+ * dexperts[e, p] = sum_s coeff[s, e] grad[s, p]; either may be NULL. Both together read grad and experts once.
+ * work: fuma_mix_experts_work_bytes when dcoeff is asked for. */
+int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P, int32_t dtype);
+int fuma_mix_experts_bwd(const void* grad, const float* coeff, int64_t stride_s, int64_t stride_e, const void* experts,
+                         int32_t S, int32_t E, int64_t P, int32_t dtype, float* dcoeff, void* dexperts, void* work,
+                         int64_t work_bytes, int* err_flag, void* stream);
 
 #ifdef __cplusplus
 }

@@ -34,7 +34,7 @@ def test_alignment_refused(lib):
     assert lib.fuma_grouped_linear(P + 8, 16, P, P, 3, None, 0, 10, 24, 16, 1, P, None, None) == -2
     assert lib.fuma_grouped_linear_dgrad(P, 24, P + 2, P, 3, 10, 24, 16, 1, P, None, None) == -2
     assert lib.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P + 4, 16, P, None) == -2
-    assert lib.fuma_mix_experts(P, 4, 1, P + 4, 2, 4, 64, 0, P, None) == -2
+    assert lib.fuma_mix_experts(P, 4, 1, P + 4, 2, 4, 64, 0, P, None, None) == -2
 
 
 def test_other_refusals(lib):
@@ -43,13 +43,15 @@ def test_other_refusals(lib):
     assert f.fuma_split_bf16x3(P, 6, 4, 6, P, None) == -1
     assert f.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P, 24, P, None) == -1                        # ldq
     assert f.fuma_quantize_weight_fp8(P, 1, 24, 16, P, 16, P, P, 24, P, None) == -1               # ldt
-    assert f.fuma_grouped_linear_fp8(P, P, P, P, None, 2, None, 0, 10, 24, 16, 1, P, None, None) == -1
-    assert f.fuma_mix_experts(P, 4, 1, P, 2, 0, 64, 0, P, None) == -1
-    assert f.fuma_mix_experts_dcoeff(P, P, 2, 4, 64, 5, P, P, 1 << 20, None) == -1
-    assert f.fuma_mix_experts_dcoeff(P, P, 2, 4, 64, 0, P, P, 4, None) == -1                      # work space
+    assert f.fuma_grouped_linear_fp8(P, 16, P, P, None, 2, None, 0, 10, 24, 16, 1, P, P, 1 << 20, None, None) == -1
+    assert f.fuma_grouped_linear_fp8(P, 16, P, P, P, 2, None, 0, 10, 24, 16, 1, P, P, 100, None, None) == -1   # work space
+    assert f.fuma_mix_experts(P, 4, 1, P, 2, 0, 64, 0, P, None, None) == -1
+    assert f.fuma_mix_experts_bwd(P, P, 4, 1, P, 2, 4, 64, 5, P, P, P, 1 << 20, None, None) == -1
+    assert f.fuma_mix_experts_bwd(P, P, 4, 1, P, 2, 4, 64, 0, P, P, P, 4, None, None) == -1                # work space
+    assert f.fuma_mix_experts_bwd(P, P, 4, 1, P, 2, 4, 64, 0, None, None, P, 1 << 20, None, None) == -1
     # nothing to do: no launch, no device needed
     assert f.fuma_grouped_linear(None, 16, None, None, 3, None, 0, 0, 24, 16, 1, None, None, None) == 0
-    assert f.fuma_mix_experts(None, 4, 1, None, 0, 4, 64, 0, None, None) == 0
+    assert f.fuma_mix_experts(None, 4, 1, None, 0, 4, 64, 0, None, None, None) == 0
 
 
 def test_work_sizes(lib):
@@ -58,7 +60,7 @@ def test_work_sizes(lib):
     assert n(0, 64, 64) == 0 and n(2048, 64, 64) == 0
     assert n(2049, 64, 64) >= 2 * 2 * 64 * 64 * 4
     assert lib.fuma_grouped_bias_grad_work_bytes(1000, 64, 5) >= (2 + 5) * 64 * 4
-    assert lib.fuma_mix_experts_work_bytes(3, 4, 1000) >= 3 * 4 * 4
+    assert lib.fuma_mix_experts_work_bytes(3, 4, 1000, 0) >= 3 * 4 * 4
 
 
 def test_partial_slots_never_meet():
