@@ -216,11 +216,13 @@ def set_probe(p: LaunchProbe | None) -> None:
 
 
 def call(name: str, *args) -> None:
-    lib = load()
+    lib = _lib or load()
     p = _probe
-    ev = p.before(name, args) if p is not None else None
-    rc = getattr(lib, name)(*args)
-    if p is not None:
+    if p is None:
+        rc = getattr(lib, name)(*args)
+    else:
+        ev = p.before(name, args)
+        rc = getattr(lib, name)(*args)
         p.after(name, ev, args)
     if rc != 0:
         msg = lib.fuma_last_error().decode(errors="replace")

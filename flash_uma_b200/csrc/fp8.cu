@@ -6,10 +6,6 @@
 // codes do not depend on how a division rounds; it costs at most one bit of the exponent range
 // of e4m3 and nothing of its precision. A block that holds a value that is not finite gets the scale
 // NaN, which makes every result that depends on it NaN.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
 #include "common.cuh"
 #include "grouped.cuh"
 #include "kernels.h"
@@ -27,33 +23,11 @@ __device__ __forceinline__ float2 block_scale(uint32_t amax_bits) {
   return make_float2(__uint_as_float((uint32_t)(k + 127) << 23), __uint_as_float((uint32_t)(127 - k) << 23));
 }
 
+// two values to e4m3, nearest even, a in the low byte
 __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-}
-
-__device__ __forceinline__ void load8(const void* x, int64_t i, int dtype, float (&v)[8]) {
-  if (dtype == kDtypeF32) {
-    const float4 a = ld4_stream(static_cast<const float*>(x) + i), b = ld4_stream(static_cast<const float*>(x) + i + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
-  const uint4 u = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i));
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float2 f;
-    if (dtype == kDtypeBf16) {
-      __nv_bfloat162 h;
-      memcpy(&h, &w[k], 4);
-      f = __bfloat1622float2(h);
-    } else {
-      __half2 h;
-      memcpy(&h, &w[k], 4);
-      f = __half22float2(h);
-    }
-    v[2 * k] = f.x;
-    v[2 * k + 1] = f.y;
-  }
+  uint16_t q;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(q) : "f"(b), "f"(a));
+  return q;
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -61,36 +35,102 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 }  // namespace
 
 // Rows x [T, K] -> codes [T, ldq] and scales [ceil(K / 128)][T] (block-major: the 128 rows of a GEMM
-// tile read theirs as one run). Half a warp takes one block of one row, 8 values a lane; a
-// thread block takes 16 rows of one k-block at a time, so scales leave as 64-byte runs. Columns
-// [K, ldq) get zero codes. One pass: 2 (4) bytes read, 1 written per value.
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int dtype,
-                                                            int64_t T, int K, uint8_t* __restrict__ codes, int64_t ldq,
+// tile read theirs as one run). 16 lanes (fp32; 16-bit types: 8) take one block of one row with two 16-byte loads each
+// and kQRows such blocks at a time, all loaded before the first reduction; blocks follow one another along the rows, so
+// a thread block reads a run of memory. 16-bit types find the largest magnitude on packed pairs. Columns [K, ldq) get
+// zero codes. One pass: 2 (4) bytes read, 1 written per value. Bound by HBM in fp32, by instructions below
+// it in 16 bits.
+template <int kDtype, int kQRows>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t T, int K,
+                                                            uint8_t* __restrict__ codes, int64_t ldq,
                                                             float* __restrict__ scales) {
-  const int l = threadIdx.x & 15, hrow = threadIdx.x >> 4;
-  const int kblocks = (K + 127) / 128;
-  const int64_t units = (T + 15) / 16 * kblocks;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int64_t row = u / kblocks * 16 + hrow;
-    const int kb = (int)(u % kblocks), k = kb * 128 + l * 8;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (row < T && k < K) load8(x, row * ldx + k, dtype, v);
-    uint32_t m = 0;
+  constexpr bool kF32 = kDtype == kDtypeF32;
+  constexpr int kLanes = kF32 ? 16 : 8, kVals = 128 / kLanes, kUnits = 256 / kLanes;
+  const int l = threadIdx.x % kLanes, h = threadIdx.x / kLanes;
+  const uint32_t kblocks = (uint32_t)(K + 127) / 128;
+  const int64_t units = T * kblocks;
+  for (int64_t u0 = (int64_t)blockIdx.x * (kUnits * kQRows); u0 < units; u0 += (int64_t)gridDim.x * (kUnits * kQRows)) {
+    const int64_t base = u0 / kblocks;
+    const uint32_t rest = (uint32_t)(u0 - base * kblocks) + h;
+    uint4 raw[kQRows][2];
+    uint32_t drow[kQRows];
+    int kb[kQRows];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o));
-    const float2 s = block_scale(m);
-    if (row < T) {
-      if (k < ldq) {
-        uint2 q = make_uint2(0u, 0u);
-        if (s.y != 0.0f) {
-          q.x = e4m3x2(v[0] * s.y, v[1] * s.y) | (e4m3x2(v[2] * s.y, v[3] * s.y) << 16);
-          q.y = e4m3x2(v[4] * s.y, v[5] * s.y) | (e4m3x2(v[6] * s.y, v[7] * s.y) << 16);
-        }
-        *reinterpret_cast<uint2*>(codes + row * ldq + k) = q;
+    for (int i = 0; i < kQRows; ++i) {
+      const uint32_t v = rest + kUnits * i;
+      drow[i] = v / kblocks;
+      kb[i] = (int)(v - drow[i] * kblocks);
+      const int k = kb[i] * 128 + l * kVals;
+      raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (base + drow[i] < T) {   // K is a multiple of 8: a 16-byte load of 16-bit values is all inside or all outside
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) +
+                                                        ((base + drow[i]) * ldx + k) * (kF32 ? 4 : 2));
+        if (k < K) raw[i][0] = __ldcs(p);
+        if (k + kVals / 2 < K) raw[i][1] = __ldcs(p + 1);
       }
-      if (l == 0) scales[(int64_t)kb * T + row] = s.x;
+    }
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w,
+                             raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+      uint32_t m = 0;
+      if constexpr (kF32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, w[j] & 0x7fffffffu);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[j] & 0x7fff7fffu));
+      }
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) {
+        const uint32_t n = __shfl_xor_sync(kFull, m, o);
+        if constexpr (kF32) m = max(m, n);
+        else asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(n));
+      }
+      if constexpr (!kF32) {
+        m = max(m & 0xffffu, m >> 16);
+        if constexpr (kDtype == kDtypeBf16) m <<= 16;
+        else m = __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+      }
+      const float2 s = block_scale(m);
+      const int64_t row = base + drow[i];
+      const int k = kb[i] * 128 + l * kVals;
+      if (row < T) {
+        if (k < ldq) {
+          uint32_t q[kVals / 4];
+#pragma unroll
+          for (int j = 0; j < kVals / 4; ++j) q[j] = 0u;
+          if (s.y != 0.0f) {
+            float f[kVals];
+            if constexpr (kF32) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+            } else if constexpr (kDtype == kDtypeBf16) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                f[2 * j] = __uint_as_float(w[j] << 16);
+                f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                __half2 v2;
+                memcpy(&v2, &w[j], 4);
+                const float2 v = __half22float2(v2);
+                f[2 * j] = v.x;
+                f[2 * j + 1] = v.y;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < kVals / 4; ++j)
+              q[j] = e4m3x2(f[4 * j] * s.y, f[4 * j + 1] * s.y) | (e4m3x2(f[4 * j + 2] * s.y, f[4 * j + 3] * s.y) << 16);
+          }
+          uint8_t* out = codes + row * ldq + k;
+          if constexpr (kF32) *reinterpret_cast<uint2*>(out) = make_uint2(q[0], q[1]);
+          else *reinterpret_cast<uint4*>(out) = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+        if (l == 0) scales[(int64_t)kb[i] * T + row] = s.x;
+      }
     }
   }
 }
@@ -137,11 +177,22 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const float* __res
   }
 }
 
+template <int kDtype, int kQRows>
+static void run_quantize_rows(const void* x, int64_t ldx, int64_t T, int K, void* codes, int64_t ldq, float* scales,
+                              cudaStream_t s) {
+  const int64_t units = T * ((K + 127) / 128);
+  quantize_rows_kernel<kDtype, kQRows><<<grid_resident(quantize_rows_kernel<kDtype, kQRows>, 256, units, (kDtype == kDtypeF32 ? 16 : 32) * kQRows), 256,
+                                         0, s>>>(x, ldx, T, K, static_cast<uint8_t*>(codes), ldq, scales);
+}
+
 void launch_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t T, int K, void* codes, int64_t ldq,
                           float* scales, cudaStream_t s) {
-  const int64_t units = (T + 15) / 16 * ((K + 127) / 128);
-  quantize_rows_kernel<<<grid_resident(quantize_rows_kernel, 256, units, 1), 256, 0, s>>>(
-      x, ldx, dtype, T, K, static_cast<uint8_t*>(codes), ldq, scales);
+  // few rows: one row per thread, so that more blocks share the work
+  const bool few = T * K < (int64_t)4 << 20;
+  auto run = dtype == kDtypeF32    ? (few ? run_quantize_rows<kDtypeF32, 1> : run_quantize_rows<kDtypeF32, 4>)
+             : dtype == kDtypeBf16 ? (few ? run_quantize_rows<kDtypeBf16, 1> : run_quantize_rows<kDtypeBf16, 4>)
+                                   : (few ? run_quantize_rows<kDtypeF16, 1> : run_quantize_rows<kDtypeF16, 4>);
+  run(x, ldx, T, K, codes, ldq, scales, s);
 }
 
 void launch_quantize_weight(const float* w, int G, int N, int K, void* codes, int64_t ldq, float* scales,

@@ -597,67 +597,68 @@ __global__ void __launch_bounds__(kGThreads, 1)
 }
 
 // ---- joining the chunks of the weight gradient --------------------------------------------------
-// dW[g] = sum over the group's chunks, in order, for groups of more than one chunk.
+// dW[g] = sum over the group's chunks, in order, for groups of more than one chunk. Block row y takes the y-th such
+// group (there are at most T / chunk of them), found by a count over all groups: 256 threads with a run each.
 __global__ void __launch_bounds__(256) grouped_join_kernel(const __grid_constant__ GroupedArgs p) {
-  const int64_t n4 = (int64_t)p.M * p.N / 4;
-  const float* work = static_cast<const float*>(p.work);
-  for (int g = blockIdx.y; g < p.G; g += gridDim.y) {
-    const int64_t at = group_at(p.offsets, g, p.T), len = group_len(p.offsets, g, p.T);
-    if (len <= p.chunk) continue;
-    const int chunks = (int)((len + p.chunk - 1) / p.chunk);
-    const int64_t slot = at / p.chunk;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (int64_t)gridDim.x * blockDim.x) {
-      float4 s = ld4_stream(work + (slot * n4 + i) * 4);
-      for (int c = 1; c < chunks; ++c) s += ld4_stream(work + ((p.slots + slot + c) * n4 + i) * 4);
-      const int64_t o = ((int64_t)g * n4 + i) * 4;
-      if (p.out_dtype == kDtypeF32)
-        st4(static_cast<float*>(p.C) + o, s);
-      else
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.C) + o) =
-            make_uint2(pack_half(s.x, s.y, p.out_dtype), pack_half(s.z, s.w, p.out_dtype));
-    }
+  __shared__ int count[8], found;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int per = (p.G + 255) / 256, g0 = threadIdx.x * per, g1 = min(p.G, g0 + per);
+  int n = 0;
+  for (int g = g0; g < g1; ++g) n += group_len(p.offsets, g, p.T) > p.chunk;
+  int incl = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kFull, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) count[w] = incl;
+  if (threadIdx.x == 0) found = -1;
+  __syncthreads();
+  int before = incl - n;
+  for (int i = 0; i < w; ++i) before += count[i];
+  const int y = blockIdx.y;
+  if (before <= y && y < before + n) {
+    for (int g = g0; g < g1; ++g)
+      if (group_len(p.offsets, g, p.T) > p.chunk && before++ == y) found = g;
+  }
+  __syncthreads();
+  const int g = found;
+  if (g < 0) return;
+  const int64_t at = group_at(p.offsets, g, p.T), len = group_len(p.offsets, g, p.T);
+  const int chunks = (int)((len + p.chunk - 1) / p.chunk);
+  const int64_t n4 = (int64_t)p.M * p.N / 4, slot = at / p.chunk;
+  const float* first = static_cast<const float*>(p.work) + slot * n4 * 4;
+  const float* rest = static_cast<const float*>(p.work) + (p.slots + slot) * n4 * 4;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (int64_t)gridDim.x * blockDim.x) {
+    float4 s = ld4_stream(first + i * 4);
+#pragma unroll 4
+    for (int c = 1; c < chunks; ++c) s += ld4_stream(rest + (c * n4 + i) * 4);
+    const int64_t o = ((int64_t)g * n4 + i) * 4;
+    if (p.out_dtype == kDtypeF32)
+      st4(static_cast<float*>(p.C) + o, s);
+    else
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.C) + o) =
+          make_uint2(pack_half(s.x, s.y, p.out_dtype), pack_half(s.z, s.w, p.out_dtype));
   }
 }
 
 // ---- bias gradient ------------------------------------------------------------------------------
-// 8 consecutive values as fp32; i a multiple of 8.
-__device__ __forceinline__ void load8_as_f32(const void* x, int64_t i, int dtype, float (&v)[8]) {
-  if (dtype == kDtypeF32) {
-    const float4 a = ld4_stream(static_cast<const float*>(x) + i), b = ld4_stream(static_cast<const float*>(x) + i + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
-  const uint4 u = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i));
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float2 f;
-    if (dtype == kDtypeBf16) {
-      __nv_bfloat162 h;
-      memcpy(&h, &w[k], 4);
-      f = __bfloat1622float2(h);
-    } else {
-      __half2 h;
-      memcpy(&h, &w[k], 4);
-      f = __half22float2(h);
-    }
-    v[2 * k] = f.x;
-    v[2 * k + 1] = f.y;
-  }
-}
-
 // db[g, n] = sum of dY[t, n] over the rows of group g, in two steps without atomics. The rows are cut at
 // multiples of kSumRows and at the group bounds; the piece of row block b and group g writes its fp32
 // sums to slot b + g. Walking the pieces in row order moves on b or g each time, so the slots are
 // distinct, and there are at most T / kSumRows + G of them. The second step adds a group's
 // pieces in fp64 and rounds once. `shared`: all rows between the first and the last offset count as one group.
-constexpr int kSumRows = 512;
+constexpr int kSumRows = 128;
 
 __device__ __forceinline__ int64_t sum_bound(const int64_t* off, int g, int G, int64_t T, int shared) {
   return group_at(off, shared ? (g ? G : 0) : g, T);
 }
 
-__global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restrict__ x, int64_t ld, int dtype,
+// A block takes the pieces of one row block in 256 columns (8 per lane). Long pieces: the 8 warps share a piece's rows,
+// 8 rows in flight each, and join in shared memory. Row blocks cut into many short pieces (many small groups):
+// a warp per piece, no joining.
+template <int kDtype>
+__global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restrict__ x, int64_t ld,
                                                              const int64_t* __restrict__ off, int G, int shared,
                                                              int64_t T, int N, float* __restrict__ part) {
   __shared__ float sm[8][256 + 8];
@@ -665,62 +666,104 @@ __global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restr
   const int n = blockIdx.y * 256 + lane * 8;
   const int groups = shared ? 1 : G;
   const int64_t b0 = (int64_t)blockIdx.x * kSumRows, b1 = min(T, b0 + kSumRows);
-  // first group that ends behind b0
-  int lo = 0, hi = groups;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (sum_bound(off, mid + 1, G, T, shared) > b0) hi = mid; else lo = mid + 1;
-  }
-  for (int g = lo; g < groups; ++g) {
-    const int64_t ga = sum_bound(off, g, G, T, shared), gb = sum_bound(off, g + 1, G, T, shared);
-    if (ga >= b1) break;
-    const int64_t r0 = max(ga, b0), r1 = min(gb, b1);
+  auto first_behind = [&](int64_t row) {   // first group that ends behind `row`
+    int lo = 0, hi = groups;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sum_bound(off, mid + 1, G, T, shared) > row) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+  };
+  const int g0 = first_behind(b0), g1 = min(groups, first_behind(b1 - 1) + 1);
+  const bool short_pieces = g1 - g0 > 4;
+  const int step = short_pieces ? 1 : 8, w0 = short_pieces ? 0 : w;
+  for (int g = g0 + (short_pieces ? w : 0); g < g1; g += short_pieces ? 8 : 1) {
+    const int64_t r0 = max(sum_bound(off, g, G, T, shared), b0), r1 = min(sum_bound(off, g + 1, G, T, shared), b1);
     if (r0 >= r1) continue;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (n < N) {
-#pragma unroll 4
-      for (int64_t r = r0 + w; r < r1; r += 8) {
-        float v[8];
-        load8_as_f32(x, r * ld + n, dtype, v);
+      for (int64_t r = r0 + w0; r < r1; r += 8 * step) {
+        Raw8<kDtype> raw[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s[k] += v[k];
+        for (int i = 0; i < 8; ++i) {
+          raw[i].zero();
+          if (r + i * step < r1) raw[i].load(x, (r + i * step) * ld + n);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float v[8];
+          raw[i].to_f32(v);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) s[k] += v[k];
+        }
       }
     }
+    float* out = part + ((int64_t)blockIdx.x + g) * N;
+    if (short_pieces) {
+      if (n < N) {
+        st4(out + n, make_float4(s[0], s[1], s[2], s[3]));
+        st4(out + n + 4, make_float4(s[4], s[5], s[6], s[7]));
+      }
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sm[w][lane * 8 + k] = s[k];
-    __syncthreads();
-    const int c = blockIdx.y * 256 + threadIdx.x;
-    if (c < N) {
-      float t = sm[0][threadIdx.x];
+      for (int k = 0; k < 8; ++k) sm[w][lane * 8 + k] = s[k];
+      __syncthreads();
+      const int c = blockIdx.y * 256 + threadIdx.x;
+      if (c < N) {
+        float t = sm[0][threadIdx.x];
 #pragma unroll
-      for (int k = 1; k < 8; ++k) t += sm[k][threadIdx.x];
-      part[((int64_t)blockIdx.x + g) * N + c] = t;
+        for (int k = 1; k < 8; ++k) t += sm[k][threadIdx.x];
+        out[c] = t;
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
-__global__ void __launch_bounds__(256) grouped_colsum_join_kernel(const float* __restrict__ part,
-                                                                  const int64_t* __restrict__ off, int G, int shared,
-                                                                  int64_t T, int N, void* __restrict__ out, int dtype) {
-  __shared__ double sm[8][32];
+// Second step. Groups of many pieces (or few groups): a block of 32 warps per group and 32 columns, the warps sharing
+// the pieces. Many groups of few pieces: a warp per group.
+constexpr int kJoinWarps = 32;
+__global__ void __launch_bounds__(32 * kJoinWarps) grouped_colsum_join_kernel(const float* __restrict__ part,
+                                                                              const int64_t* __restrict__ off, int G,
+                                                                              int shared, int64_t T, int N,
+                                                                              void* __restrict__ out, int dtype, bool by_warp) {
+  __shared__ double sm[kJoinWarps][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int n = blockIdx.x * 32 + lane, groups = shared ? 1 : G;
+  auto store = [&](int g, double t) {
+    const int64_t o = (int64_t)g * N + n;
+    if (dtype == kDtypeF32) static_cast<float*>(out)[o] = (float)t;
+    else if (dtype == kDtypeBf16) static_cast<__nv_bfloat16*>(out)[o] = __double2bfloat16(t);
+    else static_cast<__half*>(out)[o] = __double2half(t);
+  };
+  if (by_warp) {
+    for (int g = blockIdx.y * kJoinWarps + w; g < groups; g += gridDim.y * kJoinWarps) {
+      const int64_t ga = sum_bound(off, g, G, T, shared), gb = sum_bound(off, g + 1, G, T, shared);
+      double s = 0.0;
+      if (n < N) {
+        if (gb > ga)
+#pragma unroll 4
+          for (int64_t b = ga / kSumRows; b <= (gb - 1) / kSumRows; ++b) s += (double)part[(b + g) * N + n];
+        store(g, s);
+      }
+    }
+    return;
+  }
   for (int g = blockIdx.y; g < groups; g += gridDim.y) {
     const int64_t ga = sum_bound(off, g, G, T, shared), gb = sum_bound(off, g + 1, G, T, shared);
     double s = 0.0;
-    if (n < N && gb > ga)
-      for (int64_t b = ga / kSumRows + w; b <= (gb - 1) / kSumRows; b += 8) s += (double)part[(b + g) * N + n];
+    if (n < N && gb > ga) {
+      const int64_t last = (gb - 1) / kSumRows;
+#pragma unroll 4
+      for (int64_t b = ga / kSumRows + w; b <= last; b += kJoinWarps) s += (double)part[(b + g) * N + n];
+    }
     sm[w][lane] = s;
     __syncthreads();
     if (w == 0 && n < N) {
       double t = sm[0][lane];
 #pragma unroll
-      for (int k = 1; k < 8; ++k) t += sm[k][lane];
-      const int64_t o = (int64_t)g * N + n;
-      if (dtype == kDtypeF32) static_cast<float*>(out)[o] = (float)t;
-      else if (dtype == kDtypeBf16) static_cast<__nv_bfloat16*>(out)[o] = __double2bfloat16(t);
-      else static_cast<__half*>(out)[o] = __double2half(t);
+      for (int k = 1; k < kJoinWarps; ++k) t += sm[k][lane];
+      store(g, t);
     }
     __syncthreads();
   }
@@ -896,8 +939,9 @@ int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cuda
   if (st == cudaSuccess && p.T > p.chunk) {
     const int64_t n4 = (int64_t)p.M * p.N / 4;
     int64_t bx = (n4 + 255) / 256;
-    if (bx > 1024) bx = 1024;
-    grouped_join_kernel<<<dim3((unsigned)bx, (unsigned)(p.G < 64 ? p.G : 64)), 256, 0, s>>>(p);
+    if (bx > 512) bx = 512;
+    const int64_t by = p.T / p.chunk < p.G ? p.T / p.chunk : p.G;
+    grouped_join_kernel<<<dim3((unsigned)bx, (unsigned)by), 256, 0, s>>>(p);
     st = cudaGetLastError();
   }
   return (int)st;
@@ -911,13 +955,17 @@ cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const in
                                   int64_t T, int N, float* part, void* out, cudaStream_t s) {
   const int groups = shared ? 1 : G;
   if (T > 0) {
-    grouped_colsum_kernel<<<dim3((unsigned)((T + kSumRows - 1) / kSumRows), (unsigned)((N + 255) / 256)), 256, 0, s>>>(
-        x, ld, dtype, off, G, shared, T, N, part);
+    auto kern = dtype == kDtypeF32 ? grouped_colsum_kernel<kDtypeF32>
+                : dtype == kDtypeBf16 ? grouped_colsum_kernel<kDtypeBf16> : grouped_colsum_kernel<kDtypeF16>;
+    kern<<<dim3((unsigned)((T + kSumRows - 1) / kSumRows), (unsigned)((N + 255) / 256)), 256, 0, s>>>(
+        x, ld, off, G, shared, T, N, part);
     const cudaError_t st = cudaGetLastError();
     if (st != cudaSuccess) return st;
   }
-  grouped_colsum_join_kernel<<<dim3((unsigned)((N + 31) / 32), (unsigned)groups), 256, 0, s>>>(part, off, G, shared, T,
-                                                                                              N, out, dtype);
+  const bool by_warp = groups >= 8 && T / groups < 8 * kSumRows;
+  const int gy = by_warp ? (groups + kJoinWarps - 1) / kJoinWarps : groups;
+  grouped_colsum_join_kernel<<<dim3((unsigned)((N + 31) / 32), (unsigned)gy), 32 * kJoinWarps, 0, s>>>(
+      part, off, G, shared, T, N, out, dtype, by_warp);
   return cudaGetLastError();
 }
 

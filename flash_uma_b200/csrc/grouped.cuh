@@ -1,14 +1,54 @@
 // Arguments shared by the grouped dense maps (grouped.cu), the fp8 quantisation (fp8.cu), the
 // expert mix (mix.cu) and the C ABI.
 #pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
 namespace fuma {
 
 constexpr int kMaxGroups = 4096;   // their work prefix sits in shared memory
 constexpr int kDtypeF32 = 0, kDtypeBf16 = 1, kDtypeF16 = 2;
 constexpr int kErrOffsets = 64;    // group offsets that decrease or leave [0, T]
+
+// 8 consecutive values of a type, 16-byte aligned, loaded first and converted later: kernels that keep several
+// loads in flight take the type as a template argument (a branch on it between the loads makes each wait for the last).
+template <int kDtype>
+struct Raw8 {
+  uint4 w[kDtype == kDtypeF32 ? 2 : 1];
+  __device__ __forceinline__ void zero() {
+    for (auto& u : w) u = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void load(const void* x, int64_t i) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + i * (kDtype == kDtypeF32 ? 4 : 2));
+    w[0] = __ldcs(p);
+    if constexpr (kDtype == kDtypeF32) w[1] = __ldcs(p + 1);
+  }
+  __device__ __forceinline__ void to_f32(float (&v)[8]) const {
+    if constexpr (kDtype == kDtypeF32) {
+      memcpy(v, w, 32);
+    } else {
+      const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float2 f;
+        if constexpr (kDtype == kDtypeBf16) {
+          __nv_bfloat162 h;
+          memcpy(&h, &u[k], 4);
+          f = __bfloat1622float2(h);
+        } else {
+          __half2 h;
+          memcpy(&h, &u[k], 4);
+          f = __half22float2(h);
+        }
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+      }
+    }
+  }
+};
 
 // kind: 0 bf16 / fp16 (dtype), 1 three bf16 planes of fp32, 2 e4m3. Leading dimensions in elements.
 struct GroupedOperands {

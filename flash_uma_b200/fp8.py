@@ -14,7 +14,7 @@ import torch
 
 from . import _native as nat
 from ._native import ptr, stream_of
-from .grouped import _DTYPES, MAX_GROUPS, _apply, _ceil8, _check_dtype, _rows, _same_device, check_groups, guard_capture
+from .grouped import _DTYPES, MAX_GROUPS, _apply, _ceil8, _check_dtype, _opaque, _rows, _same_device, check_groups, guard_capture
 from .linear import error_flag
 
 _BLOCK = 128
@@ -116,7 +116,6 @@ class _Fp8LinearFn(torch.autograd.Function):
         return (dx if weight.Kp == weight.K else dx[:, : weight.K]), None, None, None
 
 
-@torch.compiler.disable
 def fp8_linear(x: torch.Tensor, weight: Fp8Weight, offsets: torch.Tensor | None = None,
                bias: torch.Tensor | None = None) -> torch.Tensor:
     """``y = x_q W_q^T (+ bias)`` with x rounded to e4m3 in row blocks of 128; y has x's type
@@ -127,6 +126,8 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Weight, offsets: torch.Tensor | None 
     float32 [N] or [G, N]. Weights and bias are frozen (a bias that requires a gradient is refused);
     the gradient of x is ``g_q W_q`` with the output's gradient rounded the same way (for forces). A block
     with a value that is not finite makes the results that depend on it NaN."""
+    if torch.compiler.is_compiling():
+        return _opaque(fp8_linear, x, weight, offsets, bias)
     nat.require_cuda(x, offsets, bias)
     if not isinstance(weight, Fp8Weight):
         raise TypeError(f"weight must be an Fp8Weight (got {type(weight).__name__})")
@@ -138,5 +139,5 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Weight, offsets: torch.Tensor | None 
     if offsets is None and weight.G != 1:
         raise ValueError(f"offsets are needed for the weight's {weight.G} matrices")
     check_groups(x, weight.G, weight.N, weight.K, offsets, bias)
-    _same_device(x, weight=weight, offsets=offsets, bias=bias)
+    _same_device(x.device, weight=weight, offsets=offsets, bias=bias)
     return _apply(_Fp8LinearFn, guard_capture(x), x, weight, None if offsets is None else offsets.contiguous(), bias)

@@ -37,10 +37,10 @@ def _check_dtype(name: str, t: torch.Tensor) -> int:
     return code
 
 
-def _same_device(first: torch.Tensor, **others) -> None:
+def _same_device(dev: torch.device, **others) -> None:
     for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {first.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {dev}")
 
 
 # autograd nodes of eager calls, while their graph is alive
@@ -68,12 +68,20 @@ def guard_capture(*inputs) -> bool:
 
 def _apply(fn, capturing: bool, *args):
     """``fn.apply`` where a gradient may be asked for, else its forward alone."""
-    if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
-        return fn.compute(*args)
-    out = fn.apply(*args)
-    if not capturing:
-        _live_nodes.add(out.grad_fn)
-    return out
+    if torch.is_grad_enabled():
+        for t in args:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                out = fn.apply(*args)
+                if not capturing:
+                    _live_nodes.add(out.grad_fn)
+                return out
+    return fn.compute(*args)
+
+
+@torch.compiler.disable
+def _opaque(fn, *args):
+    """A traced call: the kernels sit behind ctypes, so torch.compile runs the call eagerly."""
+    return fn(*args)
 
 
 def _rows(x: torch.Tensor, cols: int) -> torch.Tensor:
@@ -81,16 +89,19 @@ def _rows(x: torch.Tensor, cols: int) -> torch.Tensor:
     elements apart, 16-byte aligned. A copy only where ``x`` is not that already."""
     if x.shape[1] != cols:
         x = torch.nn.functional.pad(x, (0, cols - x.shape[1]))
-    if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < cols or x.data_ptr() % 16 != 0:
+    ld, one = x.stride()
+    if one != 1 or ld % 8 or ld < cols or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
 def _matrices(w: torch.Tensor, N: int, K: int) -> torch.Tensor:
     """``w`` [G, n, k] contiguous, 16-byte aligned, zero-padded to [G, N, K]."""
-    if w.shape[1] != N or w.shape[2] != K:
-        w = torch.nn.functional.pad(w, (0, K - w.shape[2], 0, N - w.shape[1]))
-    w = w.contiguous()
+    _, n, k = w.shape
+    if n != N or k != K:
+        w = torch.nn.functional.pad(w, (0, K - k, 0, N - n))
+    elif not w.is_contiguous():
+        w = w.contiguous()
     return w.clone() if w.data_ptr() % 16 else w
 
 
@@ -184,10 +195,13 @@ class _GroupedLinearFn(torch.autograd.Function):
 
 def check_groups(x: torch.Tensor, G: int, N: int, K: int, offsets: torch.Tensor | None, bias: torch.Tensor | None):
     """The argument checks that the grouped dense maps share."""
-    if x.dim() != 2 or x.shape[1] != K:
-        raise ValueError(f"x must be [rows, {K}] (got {tuple(x.shape)})")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != K:
+        raise ValueError(f"x must be [rows, {K}] (got {tuple(shape)})")
     if not 1 <= G <= MAX_GROUPS:
         raise ValueError(f"the number of groups must be from 1 to {MAX_GROUPS} (got {G})")
+    if N < 1 or K < 1:
+        raise ValueError(f"the matrices need N >= 1 and K >= 1 (got {N} and {K})")
     if offsets is not None:
         if offsets.dtype != torch.int64:
             raise TypeError(f"offsets must be int64 (got {offsets.dtype})")
@@ -197,7 +211,6 @@ def check_groups(x: torch.Tensor, G: int, N: int, K: int, offsets: torch.Tensor 
         raise ValueError(f"bias must be [{N}] or [{G}, {N}] (got {tuple(bias.shape)})")
 
 
-@torch.compiler.disable
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
                    bias: torch.Tensor | None = None) -> torch.Tensor:
     """``y[t] = weight[g] @ x[t] (+ bias)`` for the rows ``offsets[g] <= t < offsets[g + 1]``.
@@ -212,6 +225,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     or 16-byte aligned on a copy. Bad offset values are recorded in the device error flag
     (:func:`flash_uma_b200.linear.check_errors`); an infinite fp32 input may give NaN where fp32
     arithmetic gives an infinity."""
+    if torch.compiler.is_compiling():
+        return _opaque(grouped_linear, x, weight, offsets, bias)
     nat.require_cuda(x, weight, offsets, bias)
     if weight.dim() != 3:
         raise ValueError(f"weight must be [groups, N, K] (got {tuple(weight.shape)})")
@@ -219,11 +234,11 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     _check_dtype("x", x)
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise TypeError("x, weight and bias must have the same dtype")
-    if N < 1 or K < 1:
-        raise ValueError(f"weight needs N >= 1 and K >= 1 (got {tuple(weight.shape)})")
     check_groups(x, G, N, K, offsets, bias)
-    _same_device(x, weight=weight, offsets=offsets, bias=bias)
-    return _apply(_GroupedLinearFn, guard_capture(x, weight, bias), x, weight, offsets.contiguous(), bias)
+    _same_device(x.device, weight=weight, offsets=offsets, bias=bias)
+    if not offsets.is_contiguous():
+        offsets = offsets.contiguous()
+    return _apply(_GroupedLinearFn, guard_capture(x, weight, bias), x, weight, offsets, bias)
 
 
 class _MixFn(torch.autograd.Function):
@@ -266,15 +281,17 @@ class _MixFn(torch.autograd.Function):
 
 
 def _flat(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
-@torch.compiler.disable
 def mix_experts(coeff: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
     """``W[s] = sum_e coeff[s, e] experts[e]``: coeff [S, E] float32 (any strides), experts [E, ...]
     float32, bfloat16 or float16 -> [S, ...] of the experts' type, summed in fp32. Differentiable
     (once) in both; the gradient of coeff is float32, its sum over a matrix joined in fp64."""
+    if torch.compiler.is_compiling():
+        return _opaque(mix_experts, coeff, experts)
     nat.require_cuda(coeff, experts)
     _check_dtype("experts", experts)
     if coeff.dtype != torch.float32:
@@ -282,7 +299,7 @@ def mix_experts(coeff: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
     if experts.dim() < 1 or coeff.dim() != 2 or coeff.shape[1] != experts.shape[0] or experts.shape[0] < 1:
         raise ValueError(f"coeff must be [systems, experts] for experts [experts, ...] (got {tuple(coeff.shape)} and "
                          f"{tuple(experts.shape)})")
-    _same_device(experts, coeff=coeff)
+    _same_device(experts.device, coeff=coeff)
     return _apply(_MixFn, guard_capture(coeff, experts), coeff, experts)
 
 
