@@ -52,11 +52,11 @@ _SIGS = {
     "fuma_coef_to_node_blocked": [_P, _P, _P, _I32, _I64, _I32, _P, _P],
     "fuma_rmsnorm_sh_fwd": [_P, _P, _P, _P, _F32, _I64, _I32, _P, _P, _P],
     "fuma_rmsnorm_sh_bwd": [_P, _P, _P, _P, _P, _I64, _I32, _P, _P],
-    "fuma_grouped_linear": [_P, _I64, _P, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
-    "fuma_grouped_linear_dgrad": [_P, _I64, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
-    "fuma_grouped_linear_wgrad": [_P, _I64, _P, _I64, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I64, _P, _P],
+    "fuma_grouped_linear": [_P, _I64, _P, _P, _P, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
+    "fuma_grouped_linear_dgrad": [_P, _I64, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
+    "fuma_grouped_linear_wgrad": [_P, _I64, _P, _P, _I64, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I64, _P, _P],
     "fuma_grouped_bias_grad": [_P, _I64, _P, _I32, _I32, _I64, _I32, _I32, _P, _P, _I64, _P],
-    "fuma_split_bf16x3": [_P, _I64, _I64, _I32, _P, _P],
+    "fuma_split_blocks": [_P, _I64, _I64, _I32, _P, _I32, _I32, _P, _P, _P],
     "fuma_quantize_rows_fp8": [_P, _I64, _I64, _I32, _I32, _P, _I64, _P, _P],
     "fuma_quantize_weight_fp8": [_P, _I32, _I32, _I32, _P, _I64, _P, _P, _I64, _P, _P],
     "fuma_grouped_linear_fp8": [_P, _I64, _P, _P, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I64, _P, _P],
@@ -69,7 +69,7 @@ _SIGS = {
 _SIZE_SIGS = {
     "fuma_morton_scratch_bytes": [_I64],
     "fuma_neighbor_scratch_bytes": [_I64, _P],
-    "fuma_grouped_wgrad_work_bytes": [_I64, _I32, _I32],
+    "fuma_grouped_wgrad_work_bytes": [_I64, _I32, _I32, _I32],
     "fuma_grouped_bias_grad_work_bytes": [_I64, _I32, _I32],
     "fuma_fp8_work_bytes": [_I64, _I32],
     "fuma_mix_experts_work_bytes": [_I32, _I32, _I64, _I32],

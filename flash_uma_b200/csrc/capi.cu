@@ -699,8 +699,8 @@ int fuma_split_f16(const float* x, int64_t n, float scale, void* hi, void* lo, v
 
 // ---- mixture of linear experts -----------------------------------------------------------------
 
-int64_t fuma_grouped_wgrad_work_bytes(int64_t T, int32_t N, int32_t K) {
-  return T > 0 && N > 0 && K > 0 ? grouped_wgrad_work_bytes(T, N, K) : 0;
+int64_t fuma_grouped_wgrad_work_bytes(int64_t T, int32_t N, int32_t K, int32_t dtype) {
+  return T > 0 && N > 0 && K > 0 ? grouped_wgrad_work_bytes(T, N, K, dtype) : 0;
 }
 
 int64_t fuma_grouped_bias_grad_work_bytes(int64_t T, int32_t N, int32_t groups) {
@@ -736,14 +736,15 @@ int grouped_done(const char* what, int r) {
 
 }  // namespace
 
-int fuma_grouped_linear(const void* x, int64_t ldx, const void* W, const int64_t* offsets, int32_t G,
-                        const void* bias, int32_t bias_rows, int64_t T, int32_t N, int32_t K, int32_t dtype, void* y,
+int fuma_grouped_linear(const void* x, int64_t ldx, const float* x_scales, const void* W, const float* W_scales,
+                        const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows, int64_t T, int32_t N, int32_t K, int32_t dtype, void* y,
                         int* err_flag, void* stream) {
   CHECK(check_grouped("grouped_linear", G, T, N, K, dtype));
   REQUIRE(ldx >= K && ldx % 8 == 0, "grouped_linear: ldx=%lld must be >= K and a multiple of 8", (long long)ldx);
   REQUIRE(!bias || bias_rows == 1 || bias_rows == G, "grouped_linear: bias_rows=%d must be 1 or G", bias_rows);
   if (T == 0) return FUMA_OK;
-  REQUIRE(x && W && y, "grouped_linear: null pointer");
+  REQUIRE(x && W && y && (dtype != kDtypeF32 || (x_scales && W_scales)), "grouped_linear: null pointer");
+  REQUIRE(dtype != kDtypeF32 || ldx == K, "grouped_linear: planes have K columns (ldx=%lld)", (long long)ldx);
   REQUIRE(offsets || G == 1, "grouped_linear: offsets may be NULL for one group only");
   REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(W, "W"); REQUIRE_ALIGNED(y, "y");
   BIND(x);
@@ -752,16 +753,18 @@ int fuma_grouped_linear(const void* x, int64_t ldx, const void* W, const int64_t
   p.offsets = offsets; p.G = G; p.T = T; p.N = N; p.K = K;
   p.C = y; p.ldc = N; p.out_dtype = dtype;
   p.bias = bias; p.bias_rows = bias_rows; p.bias_dtype = dtype;
+  p.scale_a = x_scales; p.scale_b = W_scales; p.blocks_n = (N + 127) / 128; p.scale_slots = split_slots(T, G);
   return grouped_done("grouped_linear", launch_grouped_rows(o, p, false, err_flag, (cudaStream_t)stream));
 }
 
-int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const void* W, const int64_t* offsets, int32_t G,
-                              int64_t T, int32_t N, int32_t K, int32_t dtype, void* dx, int* err_flag, void* stream) {
+int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* W,
+                              const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dx, int* err_flag, void* stream) {
   CHECK(check_grouped("grouped_linear_dgrad", G, T, N, K, dtype));
   REQUIRE(lddy >= N && lddy % 8 == 0, "grouped_linear_dgrad: lddy=%lld must be >= N and a multiple of 8",
           (long long)lddy);
   if (T == 0) return FUMA_OK;
-  REQUIRE(dy && W && dx, "grouped_linear_dgrad: null pointer");
+  REQUIRE(dy && W && dx && (dtype != kDtypeF32 || (dy_scales && W_scales)), "grouped_linear_dgrad: null pointer");
+  REQUIRE(dtype != kDtypeF32 || lddy == N, "grouped_linear_dgrad: planes have N columns (lddy=%lld)", (long long)lddy);
   REQUIRE(offsets || G == 1, "grouped_linear_dgrad: offsets may be NULL for one group only");
   REQUIRE_ALIGNED(dy, "dy"); REQUIRE_ALIGNED(W, "W"); REQUIRE_ALIGNED(dx, "dx");
   BIND(dy);
@@ -769,11 +772,12 @@ int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const void* W, const
   GroupedArgs p{};
   p.offsets = offsets; p.G = G; p.T = T; p.N = K; p.K = N;
   p.C = dx; p.ldc = K; p.out_dtype = dtype;
+  p.scale_a = dy_scales; p.scale_b = W_scales; p.blocks_n = (K + 127) / 128; p.scale_slots = split_slots(T, G);
   return grouped_done("grouped_linear_dgrad", launch_grouped_rows(o, p, true, err_flag, (cudaStream_t)stream));
 }
 
-int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int64_t* offsets,
-                              int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dW, void* work,
+int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* x, int64_t ldx,
+                              const float* x_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dW, void* work,
                               int64_t work_bytes, int* err_flag, void* stream) {
   CHECK(check_grouped("grouped_linear_wgrad", G, T, N, K, dtype));
   REQUIRE(lddy >= N && lddy % 8 == 0 && ldx >= K && ldx % 8 == 0, "grouped_linear_wgrad: bad leading dimensions");
@@ -785,9 +789,10 @@ int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const void* x, int64
         cudaMemsetAsync(dW, 0, (size_t)G * N * K * (dtype == kDtypeF32 ? 4 : 2), (cudaStream_t)stream);
     return st == cudaSuccess ? FUMA_OK : fail((int)st, "grouped_linear_wgrad: %s", cudaGetErrorString(st));
   }
-  REQUIRE(dy && x, "grouped_linear_wgrad: null pointer");
+  REQUIRE(dy && x && (dtype != kDtypeF32 || (dy_scales && x_scales)), "grouped_linear_wgrad: null pointer");
+  REQUIRE(dtype != kDtypeF32 || (lddy == N && ldx == K), "grouped_linear_wgrad: planes have N and K columns");
   REQUIRE(offsets || G == 1, "grouped_linear_wgrad: offsets may be NULL for one group only");
-  const int64_t need = grouped_wgrad_work_bytes(T, N, K);
+  const int64_t need = grouped_wgrad_work_bytes(T, N, K, dtype);
   REQUIRE(work_bytes >= need && (need == 0 || work), "grouped_linear_wgrad: needs %lld bytes of work space, got %lld",
           (long long)need, (long long)work_bytes);
   REQUIRE_ALIGNED(dy, "dy"); REQUIRE_ALIGNED(x, "x");
@@ -796,6 +801,7 @@ int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const void* x, int64
   GroupedArgs p{};
   p.offsets = offsets; p.G = G; p.T = T; p.M = N; p.N = K;
   p.C = dW; p.out_dtype = dtype; p.work = work;
+  p.scale_a = dy_scales; p.scale_b = x_scales; p.blocks_n = (K + 127) / 128; p.scale_slots = split_slots(T, G);
   return grouped_done("grouped_linear_wgrad", launch_grouped_wgrad(o, p, err_flag, (cudaStream_t)stream));
 }
 
@@ -815,15 +821,21 @@ int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets,
   return grouped_done("grouped_bias_grad", (int)st);
 }
 
-int fuma_split_bf16x3(const float* x, int64_t ldx, int64_t rows, int32_t cols, void* out, void* stream) {
-  REQUIRE(rows >= 0 && cols > 0 && cols % 4 == 0, "split_bf16x3: bad shape rows=%lld cols=%d", (long long)rows, cols);
-  REQUIRE(ldx >= cols && ldx % 4 == 0, "split_bf16x3: ldx=%lld must be >= cols and a multiple of 4", (long long)ldx);
+int fuma_split_blocks(const float* x, int64_t ldx, int64_t rows, int32_t cols, const int64_t* offsets, int32_t G,
+                      int32_t mat_rows, void* out, float* scales, void* stream) {
+  REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && cols > 0 && cols % 8 == 0, "split_blocks: bad shape rows=%lld cols=%d",
+          (long long)rows, cols);
+  REQUIRE(ldx >= cols && ldx % 4 == 0, "split_blocks: ldx=%lld must be >= cols and a multiple of 4", (long long)ldx);
+  REQUIRE(mat_rows >= 0 && (mat_rows == 0 || rows % mat_rows == 0), "split_blocks: mat_rows=%d must divide rows", mat_rows);
+  REQUIRE(mat_rows > 0 || (G >= 1 && G <= kMaxGroups && (offsets || G == 1)), "split_blocks: bad groups (G=%d)", G);
   if (rows == 0) return FUMA_OK;
-  REQUIRE(x && out, "split_bf16x3: null pointer");
+  const int64_t slots = mat_rows > 0 ? rows / mat_rows * ((mat_rows + 127) / 128) : split_slots(rows, G);
+  REQUIRE(slots * ((cols + 127) / 128) < (int64_t(1) << 31), "split_blocks: too many blocks");
+  REQUIRE(x && out && scales, "split_blocks: null pointer");
   REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(out, "out");
   BIND(x);
-  launch_split_bf16x3(x, ldx, rows, cols, out, (cudaStream_t)stream);
-  return launched("split_bf16x3");
+  launch_split_blocks(x, ldx, rows, cols, offsets, G, mat_rows, out, scales, (cudaStream_t)stream);
+  return launched("split_blocks");
 }
 
 int fuma_quantize_rows_fp8(const void* x, int64_t ldx, int64_t T, int32_t K, int32_t dtype, void* codes, int64_t ldq,

@@ -14,25 +14,33 @@
 //
 // Element types (kKind):
 //   kHalf    bf16 or fp16 operands, one kind::f16 product per 16 elements of the contraction.
-//   kPlanes  fp32 operands as three bf16 planes x = p0 + p1 + p2 (round to nearest each; 24
-//            bits, the whole fp32 exponent range, so no value needs a scale or is refused).
-//            Six products: p0 q0 in one accumulator; p0 q1, p1 q0, p1 q1, p0 q2, p2 q0 in a
-//            second one, so that the full-size sum takes one truncating addition per 16
-//            elements; what is dropped (p1 q2 and below) is 2^-24 of a product.
+//   kSplit   fp32 operands as two fp16 planes of each 128 x 128 block under the block's own power-of-two
+//            scale 2^k (largest magnitude to [2^14, 2^15)): x = 2^k (hi + lo), hi = fp16(x / 2^k), lo = fp16(x / 2^k
+//            - hi). 22 bits for values down to 2^-18 of the block's largest and 2^-40 of that below, over the
+//            whole fp32 range. Three products, hi hi, hi lo, lo hi, in one accumulator. (Three bf16 planes need no scale,
+//            but six products and half as much again in operand bytes: 178 us against the table's for the same call.)
 //   kFp8     e4m3 operands with fp32 scales: sA[kb][row] for each row and block kb of 128 along the
 //            contraction, sB[g][n / 128][kb] for each 128 x 128 block of W.
 //
 // Accumulation: the tensor core truncates each addition to its fp32 accumulator, which drifts over
-// long sums, and fp8 products of different blocks carry different scales. So TMEM holds the
-// sum of one SEGMENT of the contraction (kHalf: 1024 elements, kPlanes: 128, kFp8: one block of
+// long sums, and the products of different blocks carry different scales. So TMEM holds the
+// sum of one SEGMENT of the contraction (kHalf: 1024 elements, kSplit and kFp8: one block of
 // 128); eight epilogue warps add each segment to fp32 registers, rounded to nearest and with the
-// fp8 scales, while the MMAs of the next segment run in the other TMEM buffer (kPlanes fills
-// TMEM with one buffer of 2 x 256 columns, and the drain of 512 columns per 6,144 cycles of MMA
-// is exposed).
+// block scales, while the MMAs of the next segment run in the other of two TMEM buffers.
+//
+// CTA pairs (kPair, row maps): two CTAs share a 256 x BN tile; each loads its own 128 rows and half of B's columns, and
+// the first issues cta_group::2 MMAs for both. Shared-memory traffic is what bounds the single-CTA tile: per
+// 64 elements of the contraction 48 KB go in by TMA and 48 KB out to the MMAs, 768 cycles at 128 B/cycle against 512 of
+// MMA; a pair moves 32 KB each way.
 //
 // Structure: 384 threads, one CTA per SM. Warp 0 loads operand tiles by TMA into a ring; warp 1
-// allocates TMEM, and its lane 0 issues the MMAs; warps 4-11 are the epilogue. Every wait is bounded.
+// allocates TMEM, and its lane 0 issues the MMAs; warp 2 (weight gradient) clears the rows behind a group's end; warp 3
+// works out the items ahead of time and hands them to the others through a ring (with every warp doing it, 64-bit
+// divisions and dependent loads took 1,000 cycles of each tile's epilogue); warps 4-11 are the epilogue. The MMA
+// thread's own instructions count: 512 cycles of MMA per stage leave no room for descriptors built from scratch
+// (960 cycles per stage measured), so it adds constants to descriptors made once. Every wait is bounded.
 #include <cstdio>
+#include <cstdlib>
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -49,30 +57,29 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kMaxBN = 256;
+constexpr int kCoarse = 256;         // entries of the work prefix in shared memory
 constexpr int kGThreads = 384;      // one control warpgroup (warps 0, 1 work), two epilogue warpgroups
 constexpr int kEpiWarps = 8, kEpiWarp0 = 4;
 // registers per thread: 384 x 168 at launch, moved to the epilogue (128 x (72 + 216 + 216) in all)
 constexpr int kCtrlRegs = 72, kEpiRegs = 216;
-constexpr int kHalf = 0, kPlanes = 1, kFp8 = 2;
+constexpr int kHalf = 0, kSplit = 1, kFp8 = 2;
 constexpr int kModeFwd = 0, kModeDx = 1, kModeDw = 2;
 
-template <int kKind>
+template <int kKind, bool kPair>
 struct GSmem {
-  static constexpr int kP = kKind == kPlanes ? 3 : 1;               // planes per operand
+  static constexpr int kP = kKind == kSplit ? 2 : 1;                // planes per operand
   static constexpr int kElem = kKind == kFp8 ? 1 : 2;               // bytes per element
-  static constexpr int kBK = kKind == kFp8 ? 128 : kKind == kPlanes ? 32 : 64;
-  static constexpr int kRowBytes = kBK * kElem;                     // K-major tile row: 128 B, kPlanes 64 B
+  static constexpr int kBK = kKind == kFp8 ? 128 : kKind == kSplit ? 32 : 64;
+  static constexpr int kRowBytes = kBK * kElem;                     // K-major tile row: 128 B, kSplit 64 B
   static constexpr int kA = kBM * kRowBytes;                        // one plane of the A tile
-  static constexpr int kB = kMaxBN * kRowBytes;
-  static constexpr int kStage = kP * (kA + kB);                     // 48 KB; kPlanes 72 KB
-  static constexpr int kStages = kKind == kPlanes ? 2 : 4;
-  static constexpr int kStaging = kEpiWarps * 2048;
-  static constexpr int kPrefix = (kMaxGroups + 1) * 4 + 60;         // 16-byte multiple
-  static constexpr int kBytes = kStages * kStage + kStaging + 512 /*barriers*/ + kPrefix + 1024 /*alignment*/;
+  static constexpr int kB = (kPair ? kMaxBN / 2 : kMaxBN) * kRowBytes;
+  static constexpr int kStage = kP * (kA + kB);                     // 48 KB; a pair 32 KB in each CTA
+  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kStaging = kEpiWarps * 4096;
+  static constexpr int kPrefix = (kCoarse + 1) * 4 + 12;            // a multiple of 16
+  static constexpr int kBytes = kStages * kStage + kStaging + 640 /*barriers, items*/ + kPrefix + 1024 /*alignment*/;
   static_assert(kBytes <= 227 * 1024, "shared memory plan exceeds 227 KB");
-  static constexpr int kSegBlocks = kKind == kHalf ? 16 : kKind == kPlanes ? 4 : 1;   // k-blocks per segment
-  static constexpr int kAccCols = kP == 3 ? 2 * kMaxBN : kMaxBN;    // main (+ cross)
-  static constexpr int kBufs = 512 / kAccCols;
+  static constexpr int kSegBlocks = kKind == kHalf ? 16 : kKind == kSplit ? 4 : 1;   // k-blocks per segment
 };
 
 // MN-major operand, 128-byte swizzle: a tile is chunks of 64 (16-bit) elements along the tile
@@ -99,22 +106,57 @@ __device__ __forceinline__ uint64_t smem_desc_k64(uint32_t addr) {
   return d;
 }
 
-template <bool kF8>
+// One elected lane of a converged warp issues (the operands are the same in all lanes, so they can sit in uniform
+// registers, which the instruction takes them from).
+#define FUMA_MMA(group, kind)                                                                       \
+  asm volatile(                                                                                     \
+      "{\n\t.reg .pred p, q;\n\t"                                                                   \
+      "elect.sync _|q, 0xffffffff;\n\t"                                                             \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                                   \
+      "@q tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), \
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)                                                          \
+      : "memory")
+
+template <bool kF8, bool kPair>
 __device__ __forceinline__ void mma_issue(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  if constexpr (kF8)
+  if constexpr (kPair) {
+    if constexpr (kF8) FUMA_MMA("2", "f8f6f4");
+    else FUMA_MMA("2", "f16");
+  } else {
+    if constexpr (kF8) FUMA_MMA("1", "f8f6f4");
+    else FUMA_MMA("1", "f16");
+  }
+}
+
+// Arrival of the issued MMAs' completion on `bar`; a pair: on the barrier at that offset in both CTAs. The lane is the one
+// that issued the MMAs (the election of a full warp always gives the same).
+template <bool kPair>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (kPair)
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+        "h"((uint16_t)3)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
+}
+
+__device__ __forceinline__ uint32_t in_cta0(const void* p) {   // the same shared-memory object in the pair's first CTA
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -128,13 +170,24 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
 }
 
-// (x: contiguous, y: rows, z: matrix, w: plane)
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(0), "r"(smem_u32(bar))
-      : "memory");
+// (x: contiguous, y: rows, z: matrix); all planes. Issued by one elected lane of a converged warp. kPair: `bar` is a
+// shared::cluster address, in either CTA of the pair.
+template <bool kPair>
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+        "%4, %5}], [%6];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(0), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(0), "r"(bar)
+        : "memory");
 }
 
 // Group g's start, held inside [0, T] whatever the caller's array says; no array: one group of all rows.
@@ -148,26 +201,16 @@ __device__ __forceinline__ int64_t group_len(const int64_t* off, int g, int64_t 
   return n > 0 ? n : 0;
 }
 
-// Work units of a group: 128-row tiles (row maps), or chunks of `chunk` contraction rows (weight
+// Work units of a group: tiles of kTileM rows (row maps), or chunks of `chunk` contraction rows (weight
 // gradient; a group without rows still has one, which writes zeros).
-template <int kMode>
+template <int kMode, int kTileM>
 __device__ __forceinline__ int group_units(int64_t len, int chunk) {
   if constexpr (kMode == kModeDw) {
     const int64_t n = (len + chunk - 1) / chunk;
     return n > 0 ? (int)n : 1;
   } else {
-    return (int)((len + kBM - 1) / kBM);
+    return (int)((len + kTileM - 1) / kTileM);
   }
-}
-
-// The group that unit u belongs to: the last g with prefix[g] <= u.
-__device__ __forceinline__ int find_group(const int* prefix, int G, int u) {
-  int lo = 0, hi = G;   // prefix[lo] <= u < prefix[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= u) lo = mid; else hi = mid;
-  }
-  return lo;
 }
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b, int dtype) {
@@ -184,29 +227,46 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b, int dtype) {
 
 }  // namespace
 
-// One item's place: group, first row and row count on the M side, first contraction row (weight
-// gradient), columns, k-blocks.
+// One item's place: group, first A row, first column, k-blocks. Rows are this CTA's 128 of the tile.
 struct Item {
-  int g, n0, kblocks;
-  int64_t row0;     // first A row (row maps) or first contraction row (weight gradient)
-  int m0, rows;     // weight gradient: first output row; rows of the tile that exist
-  int tail;         // weight gradient: contraction rows of the last k-block (0: none)
+  int kblocks;      // negative: no more items
+  int g, n0;
+  int nt;           // columns of the tile that exist, rounded up to what the MMA takes
+  int row0;         // first A row (row maps) or first contraction row (weight gradient)
+  int m0, rows;     // weight gradient: first output row; rows of the tile that exist (may be <= 0)
+  int tail;         // weight gradient: contraction rows of the last k-block (0: all)
   int64_t out;      // element offset of (row 0, column 0) of the tile's matrix in the output
-  bool partial;     // weight gradient: goes to the fp32 workspace
+  int slot;         // kSplit: index of the tile's (weight gradient: the first segment's) row block among the scales
+  int partial;      // weight gradient: goes to the fp32 workspace
 };
+constexpr int kRing = 4;
 
-template <int kMode, int kBK>
-__device__ __forceinline__ Item item_at(const GroupedArgs& p, const int* prefix, int item) {
+template <int kMode, int kBK, bool kPair>
+__device__ __forceinline__ Item item_at(const GroupedArgs& p, const int* prefix, int item, int rank) {
+  constexpr int kTileM = kPair ? 2 * kBM : kBM, kStep = kPair ? 32 : 16;
   Item t;
-  t.partial = false;
+  t.partial = 0;
   t.tail = 0;
+  const int tiles = kMode == kModeDw ? p.tiles_m * p.tiles_n : p.tiles_n;
+  const int u = item / tiles, tile = item - u * tiles;
+  // the last group whose units start at or before u: a search over every p.span-th group's start, then a walk
+  int lo = 0, hi = (p.G + p.span - 1) / p.span;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= u) lo = mid; else hi = mid;
+  }
+  int g = lo * p.span, c = u - prefix[lo];
+  int64_t at = group_at(p.offsets, g, p.T), len = group_len(p.offsets, g, p.T);
+  for (int n = group_units<kMode, kTileM>(len, p.chunk); c >= n && g + 1 < p.G;) {
+    c -= n;
+    ++g;
+    at = group_at(p.offsets, g, p.T);
+    len = group_len(p.offsets, g, p.T);
+    n = group_units<kMode, kTileM>(len, p.chunk);
+  }
+  t.g = g;
   if constexpr (kMode == kModeDw) {
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int u = item / tiles, tile = item - u * tiles;
-    t.g = find_group(prefix, p.G, u);
-    const int c = u - prefix[t.g];
-    const int64_t at = group_at(p.offsets, t.g, p.T), len = group_len(p.offsets, t.g, p.T);
-    t.row0 = at + (int64_t)c * p.chunk;
+    t.row0 = (int)(at + (int64_t)c * p.chunk);
     int64_t n = len - (int64_t)c * p.chunk;
     if (n > p.chunk) n = p.chunk;
     t.kblocks = (int)((n + kBK - 1) / kBK);
@@ -216,31 +276,35 @@ __device__ __forceinline__ Item item_at(const GroupedArgs& p, const int* prefix,
     t.rows = p.M - t.m0 < kBM ? p.M - t.m0 : kBM;
     t.partial = len > p.chunk;
     const int64_t slot = at / p.chunk + c;   // chunk 0 in the first half of the slots, see grouped.cuh
-    t.out = (t.partial ? (c == 0 ? slot : p.slots + slot) : (int64_t)t.g) * p.M * p.N + (int64_t)t.m0 * p.N;
+    t.out = (t.partial ? (c == 0 ? slot : p.slots + slot) : (int64_t)g) * p.M * p.N + (int64_t)t.m0 * p.N;
+    t.slot = (int)(at / kBM) + g + c * (p.chunk / kBM);
   } else {
-    const int mt = item / p.tiles_n;
-    t.g = find_group(prefix, p.G, mt);
-    const int64_t at = group_at(p.offsets, t.g, p.T);
-    const int64_t r = (int64_t)(mt - prefix[t.g]) * kBM;
-    const int64_t left = group_len(p.offsets, t.g, p.T) - r;
-    t.row0 = at + r;
+    const int64_t r = (int64_t)c * kTileM + rank * kBM;
+    const int64_t left = len - r;
+    t.row0 = (int)(at + r);
     t.m0 = 0;
-    t.rows = left < kBM ? (int)left : kBM;
-    t.n0 = (item - mt * p.tiles_n) * p.bn;
+    t.rows = left < kBM ? (int)(left < 0 ? 0 : left) : kBM;
+    t.n0 = tile * p.bn;
     t.kblocks = (p.K + kBK - 1) / kBK;
-    t.out = t.row0 * p.ldc;
+    t.out = (at + r) * p.ldc;
+    t.slot = (int)(at / kBM + g + r / kBM);
   }
+  const int cols = p.N - t.n0;
+  t.nt = cols < p.bn ? (cols + kStep - 1) / kStep * kStep : p.bn;
   return t;
 }
 
-template <int kKind, int kMode>
+template <int kKind, int kMode, bool kPair>
 __global__ void __launch_bounds__(kGThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ GroupedArgs p) {
-  using L = GSmem<kKind>;
+  static_assert(!kPair || kMode != kModeDw, "the weight gradient clears rows of a stage, which a pair would share");
+  using L = GSmem<kKind, kPair>;
   constexpr int kP = L::kP, kBK = L::kBK;
+  constexpr bool kScaled = kKind != kHalf;
   constexpr bool kAmn = kMode == kModeDw;                 // A contiguous along the tile
   constexpr bool kBmn = kMode != kModeFwd;
+  constexpr int kTileM = kPair ? 2 * kBM : kBM;
   constexpr uint32_t kChunkMn = kP * kBK * 128;           // bytes between 64-element chunks (planes inside)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -250,37 +314,56 @@ __global__ void __launch_bounds__(kGThreads, 1)
   uint64_t* bar_acc_full = bar_empty + L::kStages;   // [2]
   uint64_t* bar_acc_empty = bar_acc_full + 2;        // [2]
   uint64_t* bar_done = bar_acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_done + 1);
+  uint64_t* bar_clear = bar_done + 1;                // [kStages]
+  uint64_t* bar_item_full = bar_clear + L::kStages;  // [kRing]
+  uint64_t* bar_item_empty = bar_item_full + kRing;  // [kRing]
+  Item* ring = reinterpret_cast<Item*>(bar_item_empty + kRing);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring + kRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* scan = reinterpret_cast<int*>(tmem_slot + 2);   // [kGThreads / 32]
-  int* prefix = reinterpret_cast<int*>(smem_c + L::kStaging + 512);
+  static_assert((3 * L::kStages + 5 + 2 * kRing) * 8 + kRing * sizeof(Item) + (2 + kGThreads / 32) * 4 <= 640, "barrier area");
+  int* prefix = reinterpret_cast<int*>(smem_c + L::kStaging + 640);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kPair ? (int)(blockIdx.x & 1) : 0;       // cluster shape (2, 1, 1)
+  const int first_item = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+  const int item_step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       mbar_init(&bar_full[s], 1);
       mbar_init(&bar_empty[s], 1);
+      mbar_init(&bar_clear[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bar_acc_full[b], 1);
-      mbar_init(&bar_acc_empty[b], kEpiWarps * 32);
+      mbar_init(&bar_acc_empty[b], kEpiWarps * (kPair ? 2 : 1));   // one arrival per epilogue warp
+    }
+    for (int r = 0; r < kRing; ++r) {
+      mbar_init(&bar_item_full[r], 1);
+      // epilogue warps, producer, MMA thread (of a pair's first CTA), clearing warp (weight gradient)
+      mbar_init(&bar_item_empty[r], kEpiWarps + 1 + (rank == 0 ? 1 : 0) + (kMode == kModeDw ? 1 : 0));
     }
     mbar_init(bar_done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(512u)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(512u)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(512u)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
-  // prefix[g] = work units before group g: a contiguous run of groups per thread, then a scan
-  // of the threads' sums
+  // prefix[i] = work units before group i * span: threads 0..255 take `span` groups each, then a scan
   {
-    const int per = (p.G + kGThreads - 1) / kGThreads;
-    const int g0 = threadIdx.x * per, g1 = min(p.G, g0 + per);
+    const int g0 = threadIdx.x * p.span, g1 = threadIdx.x < kCoarse ? min(p.G, g0 + p.span) : 0;
     int sum = 0;
     int bad = 0;
     for (int g = g0; g < g1; ++g) {
@@ -288,7 +371,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
         const int64_t a = p.offsets[g], b = p.offsets[g + 1];
         bad |= a < 0 || b < a || b > p.T;
       }
-      sum += group_units<kMode>(group_len(p.offsets, g, p.T), p.chunk);
+      sum += group_units<kMode, kTileM>(group_len(p.offsets, g, p.T), p.chunk);
     }
     // offsets that decrease or leave [0, T]: recorded, and no item runs (every CTA sees the same array)
     bad = __syncthreads_or(bad);
@@ -304,145 +387,223 @@ __global__ void __launch_bounds__(kGThreads, 1)
     __syncthreads();
     int base = incl - sum;
     for (int w = 0; w < warp; ++w) base += scan[w];
-    for (int g = g0; g < g1; ++g) {
-      prefix[g] = base;
-      if (!bad) base += group_units<kMode>(group_len(p.offsets, g, p.T), p.chunk);
-    }
-    if (g1 == p.G && g0 < g1) prefix[p.G] = base;
+    if (threadIdx.x < kCoarse) prefix[threadIdx.x] = base;
+    if (threadIdx.x == kCoarse) prefix[kCoarse] = base;   // threads from kCoarse on add nothing: the total
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  __syncwarp();
+  if constexpr (kPair) cluster_sync();
+  else __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
-  const int items = prefix[p.G] * (kMode == kModeDw ? p.tiles_m * p.tiles_n : p.tiles_n);
+  const int items = prefix[kCoarse] * (kMode == kModeDw ? p.tiles_m * p.tiles_n : p.tiles_n);
 
   if (warp < kEpiWarp0) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
-  if (warp == 0) {
-    // ---------------- producer
-    if (lane == 0) {
-      const int b_chunks = (p.bn + 63) / 64;
-      const uint32_t bytes = kP * (L::kA + (kBmn ? b_chunks * kBK * 128 : p.bn * L::kRowBytes));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
+    if (warp == 0) {
+      // ---------------- producer (the whole warp runs the loop, one lane issues)
+      const uint32_t smem0 = smem_u32(smem);
+      const uint32_t full0 = __shfl_sync(kFull, kPair ? in_cta0(bar_full) : smem_u32(bar_full), 0);
       int it = 0;
-      for (int item = blockIdx.x; item < items && !*abort_flag; item += gridDim.x) {
-        const Item t = item_at<kMode, kBK>(p, prefix, item);
-        for (int kt = 0; kt < t.kblocks; ++kt, ++it) {
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        ok = __all_sync(kFull, mbar_wait(&bar_item_full[n % kRing], (n / kRing) & 1, abort_flag, p.err, kErrWaitFull));
+        if (!ok) break;
+        const Item& t = ring[n % kRing];
+        const int kblocks = __shfl_sync(kFull, t.kblocks, 0), g = __shfl_sync(kFull, t.g, 0);
+        const int nt = __shfl_sync(kFull, t.nt, 0), n0 = __shfl_sync(kFull, t.n0, 0);
+        const int row0 = __shfl_sync(kFull, t.row0, 0), m0 = kMode == kModeDw ? __shfl_sync(kFull, t.m0, 0) : 0;
+        if (lane == 0) mbar_arrive(&bar_item_empty[n % kRing]);
+        if (kblocks < 0) break;
+        const int cols = kPair ? nt / 2 : nt;             // of B in this CTA
+        const int nb = n0 + rank * cols;
+        const int loads = kBmn ? (cols + 63) / 64 : 1;
+        const uint32_t bytes = kP * (L::kA + loads * (kBmn ? kBK * 128 : p.box_b * L::kRowBytes)) * (kPair ? 2 : 1);
+        for (int kt = 0; kt < kblocks; ++kt, ++it) {
           const int s = it % L::kStages;
-          if (it >= L::kStages &&
-              !mbar_wait(&bar_empty[s], ((it / L::kStages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty))
-            break;
-          uint8_t* a = smem + s * L::kStage;
-          uint8_t* b = a + kP * L::kA;
-          mbar_expect_tx(&bar_full[s], bytes);
+          if (it >= L::kStages) {
+            ok = __all_sync(kFull, mbar_wait(&bar_empty[s], ((it / L::kStages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty));
+            if (!ok) break;
+          }
+          const uint32_t a = smem0 + s * L::kStage, b = a + kP * L::kA, bar = full0 + s * 8;
+          if (rank == 0 && lane == 0) mbar_expect_tx(&bar_full[s], bytes);
+          __syncwarp();
           if constexpr (kAmn) {
+#pragma unroll
             for (int c = 0; c < kBM / 64; ++c)
-              tma_load_4d(a + c * kChunkMn, &tmA, t.m0 + c * 64, (int)t.row0 + kt * kBK, 0, &bar_full[s]);
+              tma_load_4d<kPair>(a + c * kChunkMn, &tmA, m0 + c * 64, row0 + kt * kBK, 0, bar);
           } else {
-            tma_load_4d(a, &tmA, kt * kBK, (int)t.row0, 0, &bar_full[s]);
+            tma_load_4d<kPair>(a, &tmA, kt * kBK, row0, 0, bar);
           }
           if constexpr (kBmn) {
-            const int y = kMode == kModeDw ? (int)t.row0 + kt * kBK : kt * kBK;
-            for (int c = 0; c < b_chunks; ++c)
-              tma_load_4d(b + c * kChunkMn, &tmB, t.n0 + c * 64, y, kMode == kModeDw ? 0 : t.g, &bar_full[s]);
+            const int y = kMode == kModeDw ? row0 + kt * kBK : kt * kBK;
+#pragma unroll
+            for (int c = 0; c < kMaxBN / 64; ++c)
+              if (c < loads) tma_load_4d<kPair>(b + c * kChunkMn, &tmB, nb + c * 64, y, kMode == kModeDw ? 0 : g, bar);
           } else {
-            tma_load_4d(b, &tmB, kt * kBK, t.n0, t.g, &bar_full[s]);
+            tma_load_4d<kPair>(b, &tmB, kt * kBK, nb, g, bar);
           }
         }
       }
-      if (*abort_flag) {
+      if (*abort_flag && rank == 0 && lane == 0) {
         for (int j = it - 1; j >= 0 && j >= it - L::kStages; --j) {
           for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&bar_full[j % L::kStages], (j / L::kStages) & 1); ++i) {
           }
         }
       }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ---------------- MMA issue
-    const uint32_t fmt = p.mma_format;   // operand format bits of the instruction descriptor
-    const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) |
-                           ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-    int it = 0, seg = 0;
-    bool ok = true;
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const Item t = item_at<kMode, kBK>(p, prefix, item);
-      for (int kt = 0; kt < t.kblocks && ok; ++kt, ++it) {
-        const int s = it % L::kStages, buf = seg % L::kBufs;
-        const bool first = kt % L::kSegBlocks == 0;
-        if (first && seg >= L::kBufs)
-          ok = mbar_wait(&bar_acc_empty[buf], ((seg / L::kBufs) - 1) & 1, abort_flag, p.err, kErrWaitAccEmpty);
-        ok = ok && mbar_wait(&bar_full[s], (it / L::kStages) & 1, abort_flag, p.err, kErrWaitFull);
-        ok = __all_sync(kFull, ok);
+      __syncwarp();
+    } else if (warp == 1 && rank == 0) {
+      // ---------------- MMA issue (the whole warp runs the loop, one lane issues)
+      const uint32_t fmt = p.mma_format;   // operand format bits of the instruction descriptor
+      const uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) |
+                              ((uint32_t)(kTileM >> 4) << 24);
+      // descriptors of stage 0, first plane, first step; the rest is constants added to the address field (units of
+      // 16 bytes; shared memory stays below its 14 bits)
+      const uint32_t a0 = smem_u32(smem), b0 = a0 + kP * L::kA;
+      const uint64_t da0 = kAmn ? smem_desc_mn128(a0, kChunkMn) : L::kRowBytes == 64 ? smem_desc_k64(a0) : smem_desc_sw128(a0);
+      const uint64_t db0 = kBmn ? smem_desc_mn128(b0, kChunkMn) : L::kRowBytes == 64 ? smem_desc_k64(b0) : smem_desc_sw128(b0);
+      constexpr uint32_t kStepA = (kAmn ? 2048 : 32) / 16, kStepB = (kBmn ? 2048 : 32) / 16;
+      constexpr uint32_t kPlaneA = (kAmn ? kBK * 128 : L::kA) / 16;
+      const uint32_t plane_b = kBmn ? kBK * 128 / 16 : p.box_b * L::kRowBytes / 16;
+      constexpr int kSteps = kBK * L::kElem / 32;
+      const uint32_t tm = __shfl_sync(kFull, tmem, 0);
+      const uint32_t empty0 = smem_u32(bar_empty), accf0 = smem_u32(bar_acc_full);
+      int s = 0, phase = 0, seg = 0;
+      uint32_t clear_phase = 0;   // one bit per stage
+      bool ok = true;
+      bool ready = false;         // the next stage's barrier was seen complete already
+      for (int n = 0; ok; ++n) {
+        ok = __all_sync(kFull, mbar_wait(&bar_item_full[n % kRing], (n / kRing) & 1, abort_flag, p.err, kErrWaitFull));
         if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint8_t* sa = smem + s * L::kStage;
-        uint8_t* sb = sa + kP * L::kA;
-        int steps = kBK * L::kElem / 32;
-        if constexpr (kMode == kModeDw) {
-          // the last k-block of a group ends inside the tile: the rows behind it belong to the next
-          // group (whatever they hold must not count). Only whole steps of 16 rows run, and
-          // the rest of the last one is cleared in both operands (0 x inf would be NaN).
-          if (kt == t.kblocks - 1 && t.tail) {
-            steps = (t.tail + 15) / 16;
-            const int dead = steps * 16 - t.tail;
-            const int chunks = kBM / 64 * kP, chunks_b = (p.bn + 63) / 64 * kP;
-            for (int i = lane; i < (chunks + chunks_b) * dead * 8; i += 32) {
-              const int c = i / (dead * 8), r = (i / 8) % dead, j = i % 8;
-              uint8_t* base = c < chunks ? sa + c * (kBK * 128) : sb + (c - chunks) * (kBK * 128);
-              *reinterpret_cast<uint4*>(base + (t.tail + r) * 128 + j * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
+        const int kblocks = __shfl_sync(kFull, ring[n % kRing].kblocks, 0), nt = __shfl_sync(kFull, ring[n % kRing].nt, 0);
+        const int tail = kMode == kModeDw ? __shfl_sync(kFull, ring[n % kRing].tail, 0) : 0;
+        if (lane == 0) mbar_arrive(&bar_item_empty[n % kRing]);
+        if (kblocks < 0) break;
+        const uint32_t idesc = idesc0 | ((uint32_t)(nt >> 3) << 17);
+        for (int kt = 0; kt < kblocks; ++kt) {
+          const int buf = seg & 1;
+          const bool first = kt % L::kSegBlocks == 0;
+          if (first && seg >= 2) {
+            ok = __all_sync(kFull, mbar_wait(&bar_acc_empty[buf], ((seg >> 1) - 1) & 1, abort_flag, p.err, kErrWaitAccEmpty));
+            if (!ok) break;
           }
-        }
-        if (lane == 0) {
-          const uint32_t a0 = smem_u32(sa), b0 = smem_u32(sb);
-          const uint32_t acc_main = tmem + (uint32_t)(buf * L::kAccCols), acc_cross = acc_main + kMaxBN;
-          auto desc_a = [&](int plane, int kk) {
-            if constexpr (kAmn) return smem_desc_mn128(a0 + plane * (kBK * 128) + kk * 2048, kChunkMn);
-            else if constexpr (L::kRowBytes == 64) return smem_desc_k64(a0 + plane * L::kA + kk * 32);
-            else return smem_desc_sw128(a0 + kk * 32);
-          };
-          auto desc_b = [&](int plane, int kk) {
-            if constexpr (kBmn) return smem_desc_mn128(b0 + plane * (kBK * 128) + kk * 2048, kChunkMn);
-            else if constexpr (L::kRowBytes == 64) return smem_desc_k64(b0 + plane * (p.bn * L::kRowBytes) + kk * 32);
-            else return smem_desc_sw128(b0 + kk * 32);
-          };
-          for (int kk = 0; kk < steps; ++kk) {
-            const uint32_t acc = (first && kk == 0) ? 0u : 1u;
-            mma_issue<kKind == kFp8>(acc_main, desc_a(0, kk), desc_b(0, kk), idesc, acc);
-            if constexpr (kKind == kPlanes) {
-              mma_issue<false>(acc_cross, desc_a(0, kk), desc_b(1, kk), idesc, acc);
-              mma_issue<false>(acc_cross, desc_a(1, kk), desc_b(0, kk), idesc, 1u);
-              mma_issue<false>(acc_cross, desc_a(1, kk), desc_b(1, kk), idesc, 1u);
-              mma_issue<false>(acc_cross, desc_a(0, kk), desc_b(2, kk), idesc, 1u);
-              mma_issue<false>(acc_cross, desc_a(2, kk), desc_b(0, kk), idesc, 1u);
+          int steps = kSteps;
+          if (kMode == kModeDw && kt == kblocks - 1 && tail) {
+            // the last k-block of a group ends inside the tile: only whole steps of 16 rows run, and warp 2 has
+            // cleared the rest of the last one
+            steps = (tail + 15) / 16;
+            ok = __all_sync(kFull, mbar_wait(&bar_clear[s], (clear_phase >> s) & 1, abort_flag, p.err, kErrWaitSplit));
+            clear_phase ^= 1u << s;
+          } else if (!ready) {
+            ok = __all_sync(kFull, mbar_wait(&bar_full[s], phase, abort_flag, p.err, kErrWaitFull));
+          }
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t da = da0 + (uint32_t)(s * (L::kStage / 16)), db = db0 + (uint32_t)(s * (L::kStage / 16));
+          const uint32_t acc_d = tm + (uint32_t)(buf * kMaxBN);
+          const uint32_t empty = empty0 + s * 8;
+          if (++s == L::kStages) {
+            s = 0;
+            phase ^= 1;
+          }
+          // a look at the next stage's barrier, its latency behind this stage's MMAs
+          const bool peek = mbar_test(&bar_full[s], phase);
+#pragma unroll
+          for (int kk = 0; kk < kSteps; ++kk) {
+            if (kMode == kModeDw && kk >= steps) break;
+            const uint32_t acc = (kk == 0 && first) ? 0u : 1u;
+            const uint64_t dak = da + kk * kStepA, dbk = db + kk * kStepB;
+            if constexpr (kKind == kSplit) {   // the small products first
+              mma_issue<false, kPair>(acc_d, dak, dbk + plane_b, idesc, acc);
+              mma_issue<false, kPair>(acc_d, dak + kPlaneA, dbk, idesc, 1u);
+              mma_issue<false, kPair>(acc_d, dak, dbk, idesc, 1u);
+            } else {
+              mma_issue<kKind == kFp8, kPair>(acc_d, dak, dbk, idesc, acc);
             }
           }
-          mma_commit(&bar_empty[s]);
-          if (kt % L::kSegBlocks == L::kSegBlocks - 1 || kt == t.kblocks - 1) mma_commit(&bar_acc_full[buf]);
+          commit<kPair>(empty);
+          if (kt % L::kSegBlocks == L::kSegBlocks - 1 || kt == kblocks - 1) {
+            commit<kPair>(accf0 + buf * 8);
+            ++seg;
+          }
+          ready = __all_sync(kFull, peek);
         }
-        __syncwarp();
-        if (kt % L::kSegBlocks == L::kSegBlocks - 1 || kt == t.kblocks - 1) ++seg;
       }
-    }
-    if (lane == 0) {
-      mma_commit(bar_done);
+      __syncwarp();
+      if constexpr (kPair)
+        asm volatile(
+            "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar_done))
+            : "memory");
+      else
+        commit<false>(smem_u32(bar_done));
       for (uint32_t i = 0; i < kWaitLimit && !mbar_try(bar_done, 0); ++i) {
       }
+      __syncwarp();
+    } else if (kMode == kModeDw && warp == 2) {
+      // ---------------- clearing: in the last k-block of a group, the rows behind its end belong to the next group and
+      // must not count, whatever they hold; those of the last MMA step are cleared in both operands (0 x inf would be NaN)
+      int it = 0;
+      Item t;
+      for (int n = 0;; ++n) {
+        bool ok = mbar_wait(&bar_item_full[n % kRing], (n / kRing) & 1, abort_flag, p.err, kErrWaitFull);
+        ok = __all_sync(kFull, ok);
+        if (!ok) break;
+        t = ring[n % kRing];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_item_empty[n % kRing]);
+        if (t.kblocks < 0) break;
+        // every stage's barrier in order, also where nothing is to clear: a wait for a phase two ahead of the barrier's
+        // would return at once
+        for (int kt = 0; ok && kt < t.kblocks; ++kt)
+          ok = mbar_wait(&bar_full[(it + kt) % L::kStages], ((it + kt) / L::kStages) & 1, abort_flag, p.err, kErrWaitFull);
+        ok = __all_sync(kFull, ok);
+        if (!ok) break;
+        if (t.tail) {
+          const int s = (it + t.kblocks - 1) % L::kStages;
+          uint8_t* sa = smem + s * L::kStage;
+          uint8_t* sb = sa + kP * L::kA;
+          const int dead = (t.tail + 15) / 16 * 16 - t.tail;
+          const int chunks = kBM / 64 * kP, chunks_b = (t.nt + 63) / 64 * kP;
+          for (int i = lane; i < (chunks + chunks_b) * dead * 8; i += 32) {
+            const int c = i / (dead * 8), r = (i / 8) % dead, j = i % 8;
+            uint8_t* base = c < chunks ? sa + c * (kBK * 128) : sb + (c - chunks) * (kBK * 128);
+            *reinterpret_cast<uint4*>(base + (t.tail + r) * 128 + j * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_clear[s]);
+        }
+        it += t.kblocks;
+      }
+      __syncwarp();
+    } else if (warp == 3) {
+      // ---------------- items
+      if (lane == 0) {
+        int n = 0;
+        for (int item = first_item;; item += item_step, ++n) {
+          if (n >= kRing && !mbar_wait(&bar_item_empty[n % kRing], ((n / kRing) - 1) & 1, abort_flag, p.err, kErrWaitEmpty))
+            break;
+          Item t{};
+          if (item < items) t = item_at<kMode, kBK, kPair>(p, prefix, item, rank);
+          else t.kblocks = -1;
+          ring[n % kRing] = t;
+          mbar_arrive(&bar_item_full[n % kRing]);
+          if (item >= items) break;
+        }
+      }
+      __syncwarp();
     }
-    __syncwarp();
-  }
   } else {
     // ---------------- epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     const int q = warp & 3, half = (warp - kEpiWarp0) >> 2;
-    uint8_t* stage = smem_c + (warp - kEpiWarp0) * 2048;
+    uint8_t* stage = smem_c + (warp - kEpiWarp0) * 4096;
     if constexpr (kMode != kModeDw) {
       // rows before the first and behind the last group: zeros
       const int64_t head = group_at(p.offsets, 0, p.T), tail = group_at(p.offsets, p.G, p.T);
       const int vec = p.N * (p.out_dtype == kDtypeF32 ? 4 : 2) / 16;
-      const int64_t dead = prefix[p.G] || head == tail ? head + (p.T - tail) : 0, n = dead * vec;
+      const int64_t dead = items || head == tail ? head + (p.T - tail) : 0, n = dead * vec;
       for (int64_t i = (int64_t)blockIdx.x * (kEpiWarps * 32) + threadIdx.x - kEpiWarp0 * 32; i < n;
            i += (int64_t)gridDim.x * (kEpiWarps * 32)) {
         const int64_t r = i / vec, row = r < head ? r : tail + (r - head);
@@ -450,64 +611,104 @@ __global__ void __launch_bounds__(kGThreads, 1)
         reinterpret_cast<uint4*>(c)[i - r * vec] = make_uint4(0u, 0u, 0u, 0u);
       }
     }
+    const uint32_t acc_empty[2] = {kPair ? in_cta0(&bar_acc_empty[0]) : smem_u32(&bar_acc_empty[0]),
+                                   kPair ? in_cta0(&bar_acc_empty[1]) : smem_u32(&bar_acc_empty[1])};
     const int hw = p.bn > 128 ? 128 : (p.bn + 63) / 64 * 32;   // columns of this warp: [half * hw, + hw)
     const int col0 = half * hw;
     int seg = 0;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-      const Item t = item_at<kMode, kBK>(p, prefix, item);
+    for (int n = 0;; ++n) {
+      if (!__all_sync(kFull, mbar_wait(&bar_item_full[n % kRing], (n / kRing) & 1, abort_flag, p.err, kErrWaitFull))) break;
+      const Item t = ring[n % kRing];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_item_empty[n % kRing]);
+      if (t.kblocks < 0) break;
       const int segs = (t.kblocks + L::kSegBlocks - 1) / L::kSegBlocks;
       const int n0 = t.n0 + col0;
-      const int ncols = min(min(hw, p.bn - col0), p.N - n0);   // this warp's columns that exist (may be <= 0)
+      const int rows = t.rows - q * 32;                        // of this warp (may be <= 0)
+      const int ncols = rows <= 0 ? 0 : min(min(hw, p.bn - col0), p.N - n0);   // this warp's columns (may be <= 0)
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
       const float* sa = nullptr;
       const float* sb = nullptr;
+      int64_t step_a = 0, step_b = 0;
       float a_next = 1.0f, b_next = 1.0f;
-      if constexpr (kKind == kFp8) {
-        // the scales of one segment ahead, so their latency hides behind the wait for its MMAs
-        const int64_t r = min(t.row0 + q * 32 + lane, p.T - 1);
-        sa = p.scale_a + r;
-        sb = p.scale_b + ((int64_t)t.g * p.blocks_n + min(n0 / 128, p.blocks_n - 1)) * t.kblocks;
-        a_next = sa[0];
-        b_next = sb[0];
+      if constexpr (kScaled) {
+        // the scales are loaded one segment ahead, so that their latency hides behind the wait for its MMAs
+        const int nblk = min(n0 / 128, p.blocks_n - 1);
+        if constexpr (kKind == kFp8) {
+          sa = p.scale_a + min((int64_t)t.row0 + q * 32 + lane, p.T - 1);
+          step_a = p.T;
+        } else if constexpr (kMode == kModeDw) {
+          sa = p.scale_a + (t.m0 / 128) * p.scale_slots + t.slot;
+          step_a = 1;
+        } else {
+          sa = p.scale_a + min((int64_t)t.slot, p.scale_slots - 1);
+          step_a = p.scale_slots;
+        }
+        if constexpr (kMode == kModeDw) {
+          sb = p.scale_b + nblk * p.scale_slots + t.slot;
+          step_b = 1;
+        } else if constexpr (kMode == kModeDx) {   // W's scales are [G][blocks of the contraction][blocks of the columns]
+          sb = p.scale_b + (int64_t)t.g * segs * p.blocks_n + nblk;
+          step_b = p.blocks_n;
+        } else {
+          sb = p.scale_b + ((int64_t)t.g * p.blocks_n + nblk) * segs;
+          step_b = 1;
+        }
+        if (segs) {
+          a_next = *sa;
+          b_next = *sb;
+        }
       }
       bool ok = true;
       for (int sg = 0; sg < segs; ++sg, ++seg) {
-        const int buf = seg % L::kBufs;
+        const int buf = seg & 1;
         const float s_a = a_next, s_b = b_next;   // multiplied after the wait: the loads stay in flight
-        if constexpr (kKind == kFp8) {
-          const int kb = sg + 1 < segs ? sg + 1 : sg;
-          a_next = sa[(int64_t)kb * p.T];
-          b_next = sb[kb];
+        if constexpr (kScaled) {
+          const int nx = sg + 1 < segs ? sg + 1 : sg;
+          a_next = sa[nx * step_a];
+          b_next = sb[nx * step_b];
         }
-        ok = mbar_wait(&bar_acc_full[buf], (seg / L::kBufs) & 1, abort_flag, p.err, kErrWaitAcc);
+        ok = mbar_wait(&bar_acc_full[buf], (seg >> 1) & 1, abort_flag, p.err, kErrWaitAcc);
         ok = __all_sync(kFull, ok && !*abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const float s = s_a * s_b;
-        const uint32_t taddr = tmem + (uint32_t)(buf * L::kAccCols + col0) + ((uint32_t)(q * 32) << 16);
+        // the product of two scales may leave the fp32 range where the result does not: kSplit multiplies by two powers
+        // of two with half the exponent each
+        float s = 1.0f, s2 = 1.0f;
+        if constexpr (kKind == kFp8) s = s_a * s_b;
+        if constexpr (kKind == kSplit) {
+          const int e = (int)(__float_as_uint(s_a) >> 23) + (int)(__float_as_uint(s_b) >> 23) - 254, h = e >> 1;
+          s = __uint_as_float((uint32_t)(h + 127) << 23);
+          s2 = __uint_as_float((uint32_t)(e - h + 127) << 23);
+        }
+        const uint32_t taddr = tmem + (uint32_t)(buf * kMaxBN + col0) + ((uint32_t)(q * 32) << 16);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c * 32 < ncols) {
-            uint32_t r[32];
-            tmem_ld32(taddr + c * 32, r);
+        for (int c = 0; c < 4; c += 2) {
+          if (c * 32 < ncols) {   // two loads in flight; the second may read columns that nobody uses
+            uint32_t r[2][32];
+            tmem_ld32(taddr + c * 32, r[0]);
+            tmem_ld32(taddr + c * 32 + 32, r[1]);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-            for (int u = 0; u < 32; ++u) {
-              if constexpr (kKind == kFp8) acc[c * 32 + u] = fmaf(__uint_as_float(r[u]), s, acc[c * 32 + u]);
-              else acc[c * 32 + u] += __uint_as_float(r[u]);
-            }
-            if constexpr (kKind == kPlanes) {
-              tmem_ld32(taddr + kMaxBN + c * 32, r);
-              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int u = 0; u < 32; ++u) acc[c * 32 + u] += __uint_as_float(r[u]);
-            }
+              for (int u = 0; u < 32; ++u) {
+                float& a = acc[(c + h) * 32 + u];
+                const float v = __uint_as_float(r[h][u]);
+                if constexpr (kKind == kFp8) a = fmaf(v, s, a);
+                else if constexpr (kKind == kSplit) a = fmaf(v * s, s2, a);
+                else a += v;
+              }
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        mbar_arrive(&bar_acc_empty[buf]);
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) arrive_cluster(acc_empty[buf]);
+          else mbar_arrive(&bar_acc_empty[buf]);
+        }
       }
       if (!ok) break;
       if (ncols <= 0) continue;
@@ -537,51 +738,54 @@ __global__ void __launch_bounds__(kGThreads, 1)
           }
         }
       }
-      // rows out: 64 bytes of each of the warp's 32 rows at a time through the staging area (16-byte
-      // chunk j of row r at j ^ ((r >> 1) & 3)), so a store instruction writes 8 rows x 64 bytes
+      // rows out: 128 bytes of each of the warp's 32 rows at a time through the staging area (16-byte
+      // chunk j of row r at j ^ (r & 7)), so a store instruction writes 4 rows x 128 bytes
       const int out_dtype = (kMode == kModeDw && t.partial) ? kDtypeF32 : p.out_dtype;
       uint8_t* out = static_cast<uint8_t*>((kMode == kModeDw && t.partial) ? p.work : p.C);
       const int64_t ld = kMode == kModeDw ? p.N : p.ldc;
-      const int rows = t.rows - q * 32;   // of this warp
-      const int rr = lane >> 2, jj = lane & 3;
+      const int rr = lane >> 3, jj = lane & 7;
       if (out_dtype == kDtypeF32) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          if (c * 16 < ncols) {
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<float4*>(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-                  make_float4(acc[c * 16 + 4 * j], acc[c * 16 + 4 * j + 1], acc[c * 16 + 4 * j + 2], acc[c * 16 + 4 * j + 3]);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = i * 8 + rr;
-              const float4 v = *reinterpret_cast<const float4*>(stage + r * 64 + ((jj ^ ((r >> 1) & 3)) << 4));
-              if (r < rows && c * 16 + jj * 4 < ncols)
-                *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + t.out + (q * 32 + r) * ld + n0 + c * 16 + jj * 4) = v;
-            }
-          }
-        }
-      } else {
+        float* o = reinterpret_cast<float*>(out) + t.out + (int64_t)(q * 32 + rr) * ld + n0 + jj * 4;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           if (c * 32 < ncols) {
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float* a = acc + c * 32 + 8 * j;
-              *reinterpret_cast<uint4*>(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                  make_float4(acc[c * 32 + 4 * j], acc[c * 32 + 4 * j + 1], acc[c * 32 + 4 * j + 2], acc[c * 32 + 4 * j + 3]);
+            __syncwarp();
+            if (c * 32 + jj * 4 < ncols) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + rr;
+                const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + ((jj ^ (r & 7)) << 4));
+                if (r < rows) *reinterpret_cast<float4*>(o + i * 4 * ld + c * 32) = v;
+              }
+            }
+          }
+        }
+      } else {
+        uint16_t* o = reinterpret_cast<uint16_t*>(out) + t.out + (int64_t)(q * 32 + rr) * ld + n0 + jj * 8;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (c * 64 < ncols) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float* a = acc + c * 64 + 8 * j;
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
                   make_uint4(pack_half(a[0], a[1], out_dtype), pack_half(a[2], a[3], out_dtype),
                              pack_half(a[4], a[5], out_dtype), pack_half(a[6], a[7], out_dtype));
             }
             __syncwarp();
+            if (c * 64 + jj * 8 < ncols) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = i * 8 + rr;
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + ((jj ^ ((r >> 1) & 3)) << 4));
-              if (r < rows && c * 32 + jj * 8 < ncols)
-                *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + t.out + (q * 32 + r) * ld + n0 + c * 32 + jj * 8) = v;
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + rr;
+                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((jj ^ (r & 7)) << 4));
+                if (r < rows) *reinterpret_cast<uint4*>(o + i * 4 * ld + c * 64) = v;
+              }
             }
           }
         }
@@ -589,10 +793,15 @@ __global__ void __launch_bounds__(kGThreads, 1)
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  __syncwarp();
+  if constexpr (kPair) cluster_sync();   // neither CTA leaves while the other may still signal or read its shared memory
+  else __syncthreads();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if constexpr (kPair)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
 }
 
@@ -769,36 +978,88 @@ __global__ void __launch_bounds__(32 * kJoinWarps) grouped_colsum_join_kernel(co
   }
 }
 
-// ---- fp32 -> three bf16 planes --------------------------------------------------------------------
-// x = p0 + p1 + p2 with p0 = bf16(x), p1 = bf16(x - p0), p2 = bf16(x - p0 - p1); the differences are
-// exact in fp32. A value that is not finite keeps p0 and zero residuals. 4 values per thread.
-__global__ void __launch_bounds__(256) split_bf16x3_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows,
-                                                           int cols, __nv_bfloat16* __restrict__ out) {
-  const int c4 = cols / 4;
-  const int64_t total = rows * c4, plane = rows * cols;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / c4;
-    const int c = (int)(i - r * c4) * 4;
-    const float4 v = ld4_stream(x + r * ldx + c);
-    const float in[4] = {v.x, v.y, v.z, v.w};
-    __nv_bfloat16 p[3][4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      // beyond the largest bf16 the rounding would give infinity: keep the value below it in p0
-      __nv_bfloat16 h = __float2bfloat16_rn(in[u]);
-      if (__hisinf(h) && fabsf(in[u]) <= 3.402823466e38f) h = __float2bfloat16_rz(in[u]);
-      const float f0 = __bfloat162float(h);
-      const float r1 = fabsf(in[u]) <= 3.402823466e38f ? in[u] - f0 : 0.0f;
-      const __nv_bfloat16 m = __float2bfloat16_rn(r1);
-      p[0][u] = h;
-      p[1][u] = m;
-      p[2][u] = __float2bfloat16_rn(r1 - __bfloat162float(m));
+// ---- fp32 -> two fp16 planes under block scales ------------------------------------------------------
+// One thread block per 128 x 128 block: 16 values of 4 columns per thread, all loaded before the largest magnitude is
+// known, split and written: one pass, 4 bytes in and 4 out per value. Row blocks: of the ragged rows, the
+// 128-row tiles of each group (counted from the group's first row, as the maps cut it; the tile's slot is group
+// start / 128 + group + tile, distinct because one tile or one group further on moves it by at least 1), or, with
+// mat_rows > 0, of matrices of mat_rows rows each. A value that is not finite keeps hi alone and does not set the scale.
+__global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows,
+                                                           int cols, const int64_t* __restrict__ off, int G,
+                                                           int mat_rows, __half* __restrict__ out,
+                                                           float* __restrict__ scales, int64_t slots) {
+  __shared__ uint32_t wmax[8];
+  const int kblocks = (cols + 127) / 128;
+  const int64_t slot = blockIdx.x / kblocks;
+  const int kb = (int)(blockIdx.x - slot * kblocks);
+  int64_t row0, n, scale_at;
+  if (mat_rows > 0) {
+    const int blocks = (mat_rows + 127) / 128;
+    const int64_t m = slot / blocks;
+    const int i = (int)(slot - m * blocks);
+    row0 = m * mat_rows + i * 128;
+    n = mat_rows - i * 128;
+    scale_at = slot * kblocks + kb;
+  } else {
+    int lo = 0, hi = G;   // the last group with start / 128 + group <= slot
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (group_at(off, mid, rows) / 128 + mid <= slot) lo = mid; else hi = mid;
     }
+    const int64_t at = group_at(off, lo, rows), i = slot - (at / 128 + lo);
+    if (i < 0) return;
+    row0 = at + i * 128;
+    n = group_len(off, lo, rows) - i * 128;
+    scale_at = kb * slots + slot;
+  }
+  if (n <= 0) return;
+  if (n > 128) n = 128;
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = kb * 128 + lane * 4;
+  float4 v[16];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
+  for (int i = 0; i < 16; ++i) {
+    const int r = w + 8 * i;
+    v[i] = (r < n && c < cols) ? ld4_stream(x + (row0 + r) * ldx + c) : f4(0.0f);
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float f[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
+      m = max(m, b < 0x7f800000u ? b : 0u);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o));
+  if (lane == 0) wmax[w] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, wmax[i]);
+  int e = (int)(m >> 23) - 127 - 14;
+  if (e < -126) e = -126;
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  if (threadIdx.x == 0) scales[scale_at] = __uint_as_float((uint32_t)(127 + e) << 23);
+  if (c >= cols) return;
+  const int64_t plane = rows * cols;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = w + 8 * i;
+    if (r < n) {
+      const float f[4] = {v[i].x * inv, v[i].y * inv, v[i].z * inv, v[i].w * inv};
+      __half h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        h[j] = __float2half_rn(f[j]);
+        l[j] = __float2half_rn(fabsf(f[j]) <= 3.402823466e38f ? f[j] - __half2float(h[j]) : 0.0f);
+      }
       uint2 u;
-      memcpy(&u, p[k], 8);
-      *reinterpret_cast<uint2*>(out + k * plane + r * cols + c) = u;
+      memcpy(&u, h, 8);
+      *reinterpret_cast<uint2*>(out + (row0 + r) * cols + c) = u;
+      memcpy(&u, l, 8);
+      *reinterpret_cast<uint2*>(out + plane + (row0 + r) * cols + c) = u;
     }
   }
 }
@@ -807,11 +1068,11 @@ __global__ void __launch_bounds__(256) split_bf16x3_kernel(const float* __restri
 
 namespace {
 
-template <int kKind, int kMode>
+template <int kKind, int kMode, bool kPair>
 cudaError_t launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& p, int64_t max_items,
                            cudaStream_t s) {
-  using L = GSmem<kKind>;
-  auto kern = grouped_gemm_kernel<kKind, kMode>;
+  using L = GSmem<kKind, kPair>;
+  auto kern = grouped_gemm_kernel<kKind, kMode, kPair>;
   static thread_local uint64_t configured = 0;  // one bit per device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -820,50 +1081,79 @@ cudaError_t launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const Gro
     if (st != cudaSuccess) return st;
     configured |= uint64_t(1) << (dev & 63);
   }
-  const int64_t sms = sm_count();
-  const int grid = (int)(max_items < 1 ? 1 : max_items < sms ? max_items : sms);
-  kern<<<grid, kGThreads, L::kBytes, s>>>(a, b, p);
-  return cudaGetLastError();
+  if constexpr (kPair) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(sm_count() / 2 * 2));
+    cfg.blockDim = dim3(kGThreads);
+    cfg.dynamicSmemBytes = L::kBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    // as many pairs as run at once: a pair that had to wait for another's end would start its share late
+    static thread_local int resident[64];
+    int& n = resident[dev & 63];
+    if (n == 0 && (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1)) {
+      (void)cudaGetLastError();
+      n = sm_count() / 4;
+    }
+    cfg.gridDim = dim3((unsigned)(2 * (max_items < 1 ? 1 : max_items < n ? max_items : n)));
+    return cudaLaunchKernelEx(&cfg, kern, a, b, p);
+  } else {
+    const int64_t sms = sm_count();
+    const int grid = (int)(max_items < 1 ? 1 : max_items < sms ? max_items : sms);
+    kern<<<grid, kGThreads, L::kBytes, s>>>(a, b, p);
+    return cudaGetLastError();
+  }
 }
 
-// Columns per tile: the whole width in even parts of at most 256 (a multiple of 16, so that
-// N = 640 runs as 3 x 224 and not as 2 x 256 + 128), and narrower tiles, down to 32, while there
+// Columns per tile: the whole width in even parts of at most 256 (so that N = 640 runs as 3 x 224 and not as
+// 2 x 256 + 128), with block scales 256 or 128, and narrower tiles, down to 32, while there
 // would be fewer tiles than SMs: a call of a few rows is bound by how many SMs pull its matrices in.
-// Measured: see the table in the kernel's comment on small calls.
-int pick_bn(int N, int64_t tiles_rows, bool fp8) {
+int pick_bn(int N, int64_t tiles_rows, bool scaled) {
   int bn;
-  if (fp8) {
+  if (scaled) {
     bn = N > 128 ? 256 : 128;   // whole 128-blocks of the scales
   } else {
     const int parts = (N + kMaxBN - 1) / kMaxBN;
-    bn = ((N + parts - 1) / parts + 15) / 16 * 16;
+    bn = ((N + parts - 1) / parts + 31) / 32 * 32;
   }
   while (bn > 32 && tiles_rows * ((N + bn - 1) / bn) < sm_count()) {
-    const int half = fp8 ? bn / 2 : (bn / 2 + 15) / 16 * 16;
-    if (half < 32) break;
+    const int half = scaled ? bn / 2 : (bn / 2 + 31) / 32 * 32;
+    if (half < 32 || half == bn) break;
     bn = half;
   }
   return bn;
 }
 
+// CTA pairs: tiles of 256 rows, when the groups are long enough that the padding of their last tile (128 rows more on
+// average) costs less than what a pair saves, and there are enough tiles for every pair of SMs.
+bool use_pair(int64_t T, int G, int64_t items) { return T >= (int64_t)1024 * G && items >= sm_count() / 2; }
+
 }  // namespace
 
 int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed, int* err, cudaStream_t s) {
-  const bool fp8 = o.kind == kFp8, planes = o.kind == kPlanes;
-  const int esize = fp8 ? 1 : 2, P = planes ? 3 : 1;
-  const int bk = fp8 ? 128 : planes ? 32 : 64;
+  const bool fp8 = o.kind == kFp8, split = o.kind == kSplit;
+  const int esize = fp8 ? 1 : 2, P = split ? 2 : 1;
+  const int bk = fp8 ? 128 : split ? 32 : 64;
   const int64_t groups = p.G < p.T ? p.G : p.T;
   const int64_t tiles_rows = p.T / kBM + groups;   // upper bound: a partial tile per group
-  p.bn = pick_bn(p.N, tiles_rows, fp8);
+  p.bn = pick_bn(p.N, tiles_rows, fp8 || split);
   p.tiles_n = (p.N + p.bn - 1) / p.bn;
   p.tiles_m = 1;
   p.err = err;
   p.chunk = 0;
-  p.mma_format = fp8 ? 0u : (planes || o.dtype == kDtypeBf16) ? 1u : 0u;
+  p.span = (p.G + kCoarse - 1) / kCoarse;
+  p.mma_format = (!fp8 && !split && o.dtype == kDtypeBf16) ? 1u : 0u;
+  const int64_t pair_items = (p.T / (2 * kBM) + groups) * p.tiles_n;
+  const char* pe = getenv("FUMA_PAIR"); const bool pair = (pe ? atoi(pe) != 0 : !fp8) && p.bn > 128 && use_pair(p.T, p.G, pair_items);
+  p.box_b = pair ? p.bn / 2 : p.bn;   // rows of W per load (forward): this CTA's columns, the planes one behind the other
   const CUtensorMapDataType dt = fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                 : (planes || o.dtype == kDtypeBf16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUtensorMapSwizzle ksw = planes ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+                                 : p.mma_format ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapSwizzle ksw = split ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   CUtensorMap ma, mb;
   // A: [T rows, K], planes T * lda apart
   if (!make_map_4d(&ma, dt, o.A, p.K, p.T, 1, P, o.lda * esize, p.T * o.lda * esize, p.T * o.lda * esize, bk, kBM, P,
@@ -873,18 +1163,17 @@ int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed
   // output columns contiguous
   const int64_t brows = transposed ? p.K : p.N, bcols = transposed ? p.N : p.K;
   if (!make_map_4d(&mb, dt, o.B, bcols, brows, p.G, P, o.ldb * esize, brows * o.ldb * esize,
-                   p.G * brows * o.ldb * esize, transposed ? 64 : bk, transposed ? bk : p.bn, P,
+                   p.G * brows * o.ldb * esize, transposed ? 64 : bk, transposed ? bk : p.box_b, P,
                    transposed ? CU_TENSOR_MAP_SWIZZLE_128B : ksw))
     return -1;
   const int64_t items = tiles_rows * p.tiles_n;
   cudaError_t st;
-  if (fp8) st = launch_grouped<kFp8, kModeFwd>(ma, mb, p, items, s);
-  else if (planes)
-    st = transposed ? launch_grouped<kPlanes, kModeDx>(ma, mb, p, items, s)
-                    : launch_grouped<kPlanes, kModeFwd>(ma, mb, p, items, s);
-  else
-    st = transposed ? launch_grouped<kHalf, kModeDx>(ma, mb, p, items, s)
-                    : launch_grouped<kHalf, kModeFwd>(ma, mb, p, items, s);
+#define FUMA_ROWS(kind, mode) (pair ? launch_grouped<kind, mode, true>(ma, mb, p, pair_items, s) \
+                                    : launch_grouped<kind, mode, false>(ma, mb, p, items, s))
+  if (fp8) st = FUMA_ROWS(kFp8, kModeFwd);
+  else if (split) st = transposed ? FUMA_ROWS(kSplit, kModeDx) : FUMA_ROWS(kSplit, kModeFwd);
+  else st = transposed ? FUMA_ROWS(kHalf, kModeDx) : FUMA_ROWS(kHalf, kModeFwd);
+#undef FUMA_ROWS
   return (int)st;
 }
 
@@ -895,38 +1184,40 @@ static int wgrad_chunk(int64_t T, int tiles) {
   int64_t c = T * tiles / ((int64_t)148 * 3);
   if (c < 2048) c = 2048;
   if (c > (1 << 20)) c = 1 << 20;
-  return (int)((c + 63) / 64 * 64);
+  return (int)((c + 127) / 128 * 128);   // whole row blocks of the split's scales
 }
 
-static int wgrad_bn(int N) {
+static int wgrad_bn(int N, bool split) {
+  if (split) return N > 128 ? 256 : 128;   // whole 128-blocks of the scales
   const int parts = (N + kMaxBN - 1) / kMaxBN;
   return ((N + parts - 1) / parts + 15) / 16 * 16;
 }
 
-static int wgrad_tiles(int M, int N) {
-  const int bn = wgrad_bn(N);
+static int wgrad_tiles(int M, int N, bool split) {
+  const int bn = wgrad_bn(N, split);
   return (M + kBM - 1) / kBM * ((N + bn - 1) / bn);
 }
 
-int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N) {
-  const int chunk = wgrad_chunk(T, wgrad_tiles(M, N));
+int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N, int dtype) {
+  const int chunk = wgrad_chunk(T, wgrad_tiles(M, N, dtype == kDtypeF32));
   if (T <= chunk) return 0;
   return 2 * (T / chunk + 1) * (int64_t)M * N * 4;
 }
 
 int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cudaStream_t s) {
-  const bool planes = o.kind == kPlanes;
-  const int P = planes ? 3 : 1, bk = planes ? 32 : 64;
+  const bool split = o.kind == kSplit;
+  const int P = split ? 2 : 1, bk = split ? 32 : 64;
   p.err = err;
-  p.bn = wgrad_bn(p.N);
+  p.bn = wgrad_bn(p.N, split);
   p.tiles_n = (p.N + p.bn - 1) / p.bn;
   p.tiles_m = (p.M + kBM - 1) / kBM;
   p.chunk = wgrad_chunk(p.T, p.tiles_m * p.tiles_n);
   p.slots = p.T / p.chunk + 1;
-  p.mma_format = (planes || o.dtype == kDtypeBf16) ? 1u : 0u;
+  p.span = (p.G + kCoarse - 1) / kCoarse;
+  p.mma_format = (!split && o.dtype == kDtypeBf16) ? 1u : 0u;
   p.ldc = p.N;
-  const CUtensorMapDataType dt = (planes || o.dtype == kDtypeBf16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  p.box_b = 0;
+  const CUtensorMapDataType dt = p.mma_format ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap ma, mb;
   if (!make_map_4d(&ma, dt, o.A, p.M, p.T, 1, P, o.lda * 2, p.T * o.lda * 2, p.T * o.lda * 2, 64, bk, P,
                    CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -934,8 +1225,8 @@ int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cuda
                    CU_TENSOR_MAP_SWIZZLE_128B))
     return -1;
   const int64_t items = (p.T / p.chunk + p.G) * (int64_t)p.tiles_m * p.tiles_n;
-  cudaError_t st = planes ? launch_grouped<kPlanes, kModeDw>(ma, mb, p, items, s)
-                          : launch_grouped<kHalf, kModeDw>(ma, mb, p, items, s);
+  cudaError_t st = split ? launch_grouped<kSplit, kModeDw, false>(ma, mb, p, items, s)
+                         : launch_grouped<kHalf, kModeDw, false>(ma, mb, p, items, s);
   if (st == cudaSuccess && p.T > p.chunk) {
     const int64_t n4 = (int64_t)p.M * p.N / 4;
     int64_t bx = (n4 + 255) / 256;
@@ -969,9 +1260,14 @@ cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const in
   return cudaGetLastError();
 }
 
-void launch_split_bf16x3(const float* x, int64_t ldx, int64_t rows, int cols, void* out, cudaStream_t s) {
-  split_bf16x3_kernel<<<grid_resident(split_bf16x3_kernel, 256, rows * (cols / 4), 256), 256, 0, s>>>(
-      x, ldx, rows, cols, static_cast<__nv_bfloat16*>(out));
+int64_t split_slots(int64_t rows, int G) { return rows / 128 + G; }
+
+void launch_split_blocks(const float* x, int64_t ldx, int64_t rows, int cols, const int64_t* off, int G, int mat_rows,
+                         void* out, float* scales, cudaStream_t s) {
+  const int64_t slots = mat_rows > 0 ? rows / mat_rows * ((mat_rows + 127) / 128) : split_slots(rows, G);
+  const int64_t blocks = slots * ((cols + 127) / 128);
+  split_blocks_kernel<<<(unsigned)blocks, 256, 0, s>>>(x, ldx, rows, cols, off, G, mat_rows, static_cast<__half*>(out),
+                                                       scales, slots);
 }
 
 }  // namespace fuma

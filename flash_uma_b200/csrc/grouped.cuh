@@ -9,7 +9,7 @@
 
 namespace fuma {
 
-constexpr int kMaxGroups = 4096;   // their work prefix sits in shared memory
+constexpr int kMaxGroups = 4096;
 constexpr int kDtypeF32 = 0, kDtypeBf16 = 1, kDtypeF16 = 2;
 constexpr int kErrOffsets = 64;    // group offsets that decrease or leave [0, T]
 
@@ -50,7 +50,7 @@ struct Raw8 {
   }
 };
 
-// kind: 0 bf16 / fp16 (dtype), 1 three bf16 planes of fp32, 2 e4m3. Leading dimensions in elements.
+// kind: 0 bf16 / fp16 (dtype), 1 two fp16 planes of fp32 (split_blocks), 2 e4m3. Leading dimensions in elements.
 struct GroupedOperands {
   const void* A;
   const void* B;
@@ -68,9 +68,12 @@ struct GroupedArgs {
   int out_dtype;
   const void* bias;         // [N] or [G, N] or null
   int bias_rows, bias_dtype;
-  const float* scale_a;     // fp8: [ceil(K / 128)][T]
-  const float* scale_b;     // fp8: [G][blocks_n][ceil(K / 128)]
-  int blocks_n;
+  // fp8: scale_a [ceil(K / 128)][T], scale_b [G][blocks_n][ceil(K / 128)]. Planes: of the row operands
+  // [column blocks][scale_slots], of W [G][ceil(N / 128)][ceil(K / 128)] in the forward's terms.
+  const float* scale_a;
+  const float* scale_b;
+  int blocks_n;             // 128-column blocks of the output
+  int64_t scale_slots;
   // Weight gradient: fp32 partial matrices of groups longer than `chunk` rows. Such a group starts
   // at row a; its chunk 0 takes slot a / chunk, its chunk c >= 1 slot `slots` + a / chunk + c. Two such
   // groups never meet: a group of more than `chunk` rows moves a / chunk on by at least
@@ -81,17 +84,21 @@ struct GroupedArgs {
   int64_t slots;
   int* err;
   // set by the launcher
-  int bn, tiles_m, tiles_n, chunk;
+  int bn, tiles_m, tiles_n, chunk, span, box_b;
   uint32_t mma_format;
 };
 
 int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed, int* err, cudaStream_t s);
 int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cudaStream_t s);
-int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N);
+int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N, int dtype);
 int64_t grouped_colsum_work_bytes(int64_t T, int N, int groups);
 cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const int64_t* off, int G, bool shared,
                                   int64_t T, int N, float* part, void* out, cudaStream_t s);
-void launch_split_bf16x3(const float* x, int64_t ldx, int64_t rows, int cols, void* out, cudaStream_t s);
+// Two fp16 planes [2][rows][cols] and their block scales: of ragged rows (mat_rows 0) [ceil(cols / 128)][split_slots],
+// of matrices of mat_rows rows [matrices][ceil(mat_rows / 128)][ceil(cols / 128)].
+int64_t split_slots(int64_t rows, int G);
+void launch_split_blocks(const float* x, int64_t ldx, int64_t rows, int cols, const int64_t* off, int G, int mat_rows,
+                         void* out, float* scales, cudaStream_t s);
 
 void launch_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t T, int K, void* codes, int64_t ldq,
                           float* scales, cudaStream_t s);

@@ -11,8 +11,8 @@ unlike systems, and for training, every system keeps its own matrix:
 * :class:`MoleLinear`: the two together, a layer.
 
 Counterpart of :class:`~flash_uma_b200.linear.FrozenLinear` (one frozen matrix for all rows) on
-the same tensor cores. Types: fp32 (three bf16 planes per operand, six products: 24 bits and the
-whole fp32 range, no range error), bf16 and fp16 (fp32 sums, one rounding at the end).
+the same tensor cores. Types: fp32 (two fp16 planes per operand under a scale for each 128 x 128 block, three
+products: 22 bits over the whole fp32 range, no range error), bf16 and fp16 (fp32 sums, one rounding at the end).
 :func:`flash_uma_b200.fp8.fp8_linear` is the map on frozen 8-bit weights.
 """
 from __future__ import annotations
@@ -109,25 +109,33 @@ def _ceil8(n: int) -> int:
     return (n + 7) // 8 * 8
 
 
-def _planes(x: torch.Tensor) -> torch.Tensor:
-    """[3, rows, cols] bf16 planes of an fp32 operand [rows, cols] (``fuma_split_bf16x3``)."""
+def _split(x: torch.Tensor, offsets, G: int, mat_rows: int):
+    """The two fp16 planes [2, rows, cols] of an fp32 operand [rows, cols] and their block scales
+    (``fuma_split_blocks``): of ragged rows, or (``mat_rows`` > 0) of matrices of that many rows."""
     rows, cols = x.shape
-    out = torch.empty(3, rows, cols, device=x.device, dtype=torch.bfloat16)
-    nat.call("fuma_split_bf16x3", ptr(x), x.stride(0), rows, cols, ptr(out), stream_of(x))
-    return out
+    out = torch.empty((2, rows, cols), device=x.device, dtype=torch.float16)
+    blocks = rows // mat_rows * ((mat_rows + 127) // 128) if mat_rows else rows // 128 + G
+    scales = torch.empty((cols + 127) // 128 * blocks, device=x.device)
+    nat.call("fuma_split_blocks", ptr(x), x.stride(0), rows, cols, ptr(offsets), G, mat_rows, ptr(out), ptr(scales),
+             stream_of(x))
+    return out, scales
 
 
-def _operand(x: torch.Tensor, cols: int):
-    """(tensor, leading dimension) of a row operand for the C ABI."""
+def _operand(x: torch.Tensor, cols: int, offsets, G: int):
+    """(tensor, leading dimension, scales) of a row operand for the C ABI."""
     x = _rows(x, cols)
     if x.dtype == torch.float32:
-        return _planes(x), cols
-    return x, x.stride(0)
+        planes, scales = _split(x, offsets, G, 0)
+        return planes, cols, scales
+    return x, x.stride(0), None
 
 
-def _weight_operand(w: torch.Tensor) -> torch.Tensor:
-    G, N, K = w.shape
-    return _planes(w.view(G * N, K)) if w.dtype == torch.float32 else w
+def _weight_operand(w: torch.Tensor):
+    """(tensor, scales) of the matrices [G, N, K] for the C ABI."""
+    if w.dtype == torch.float32:
+        G, N, K = w.shape
+        return _split(w.view(G * N, K), None, G, N)
+    return w, None
 
 
 class _GroupedLinearFn(torch.autograd.Function):
@@ -142,9 +150,9 @@ class _GroupedLinearFn(torch.autograd.Function):
             if bias is not None:
                 bias_rows = 1 if bias.dim() == 1 else G
                 bias = torch.nn.functional.pad(bias, (0, Np - N)) if Np != N else bias.contiguous()
-            a, lda = _operand(x, Kp)
-            w = _weight_operand(_matrices(weight, Np, Kp))
-            nat.call("fuma_grouped_linear", ptr(a), lda, ptr(w), ptr(offsets), G, ptr(bias), bias_rows, T, Np, Kp,
+            a, lda, a_s = _operand(x, Kp, offsets, G)
+            w, w_s = _weight_operand(_matrices(weight, Np, Kp))
+            nat.call("fuma_grouped_linear", ptr(a), lda, ptr(a_s), ptr(w), ptr(w_s), ptr(offsets), G, ptr(bias), bias_rows, T, Np, Kp,
                      _DTYPES[x.dtype], ptr(y), ptr(error_flag(x.device)), stream_of(x))
         return y if Np == N else y[:, :N]
 
@@ -166,26 +174,26 @@ class _GroupedLinearFn(torch.autograd.Function):
         dx = dw = db = None
         s, err = stream_of(x), ptr(error_flag(x.device))
         g = _rows(g, Np)
-        a, lda = _operand(g, Np) if T and (want_x or want_w) else (g, Np)
+        a, lda, a_s = _operand(g, Np, offsets, G) if T and (want_x or want_w) else (g, Np, None)
         if want_x:
             dx = torch.empty(T, Kp, device=x.device, dtype=x.dtype)
             if T:
-                w = _weight_operand(_matrices(weight, Np, Kp))
-                nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, ptr(w), ptr(offsets), G, T, Np, Kp, code, ptr(dx),
-                         err, s)
+                w, w_s = _weight_operand(_matrices(weight, Np, Kp))
+                nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, ptr(a_s), ptr(w), ptr(w_s), ptr(offsets), G, T, Np, Kp,
+                         code, ptr(dx), err, s)
             dx = dx if Kp == K else dx[:, :K]
         if want_w:
             dw = torch.empty(G, Np, Kp, device=x.device, dtype=x.dtype)
-            b, ldb = _operand(x, Kp) if T else (x, Kp)
-            nbytes = int(nat.load().fuma_grouped_wgrad_work_bytes(T, Np, Kp))
+            b, ldb, b_s = _operand(x, Kp, offsets, G) if T else (x, Kp, None)
+            nbytes = nat.load().fuma_grouped_wgrad_work_bytes(T, Np, Kp, code)
             work = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
-            nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, ptr(b), ldb, ptr(offsets), G, T, Np, Kp, code, ptr(dw),
-                     ptr(work), nbytes, err, s)
+            nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, ptr(a_s), ptr(b), ldb, ptr(b_s), ptr(offsets), G, T, Np, Kp,
+                     code, ptr(dw), ptr(work), nbytes, err, s)
             dw = dw if (Np, Kp) == (N, K) else dw[:, :N, :K]
         if want_b:
             shared = len(ctx.bias_shape) == 1
             db = torch.empty(*ctx.bias_shape[:-1], Np, device=x.device, dtype=x.dtype)
-            nbytes = int(nat.load().fuma_grouped_bias_grad_work_bytes(T, Np, 1 if shared else G))
+            nbytes = nat.load().fuma_grouped_bias_grad_work_bytes(T, Np, 1 if shared else G)
             work = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
             nat.call("fuma_grouped_bias_grad", ptr(g), g.stride(0) if T else Np, ptr(offsets), G, 1 if shared else 0, T,
                      Np, code, ptr(db), ptr(work), nbytes, s)

@@ -108,7 +108,8 @@ def _close(got, want, S, n, dt, what):
 
 
 SHAPES = [([1], 8, 8, 0, 0), ([1], 512, 512, 0, 0), ([0, 5, 0, 130, 1, 127, 128, 0], 136, 264, 0, 0),
-          ([300, 20], 768, 640, 7, 200), ([17, 0, 40], 13, 7, 2, 1), ([200], 1032, 136, 0, 0)]
+          ([300, 20], 768, 640, 7, 200), ([17, 0, 40], 13, 7, 2, 1), ([200], 1032, 136, 0, 0),
+          ([9001, 0, 257, 8000, 128, 129], 136, 640, 3, 77)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)

@@ -114,6 +114,15 @@ def test_long_groups_cut_over_the_contraction(dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("lens,K,N,head,tail", [([20000], 72, 256, 0, 0), ([9001, 0, 257, 8000, 128, 129], 136, 640, 3, 77),
+                                                ([5000, 5100], 520, 392, 0, 0)])
+def test_long_groups_on_cta_pairs(lens, K, N, head, tail, dt):
+    """Groups long enough for the 256-row tiles of CTA pairs, with last tiles of 1, 128, 129 and 256 rows."""
+    x, w, off, b, gy = _make(lens, K, N, dt, "shared", head, tail)
+    _check(x, w, off, b, gy, dt)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 def test_many_groups(dt):
     g = torch.Generator().manual_seed(5)
     lens = torch.randint(0, 9, (700,), generator=g).tolist()

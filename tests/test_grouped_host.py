@@ -20,27 +20,29 @@ P = 4096   # a 16-byte aligned non-null address that no check reads
     (dict(G=0), b"G=0"), (dict(G=4097), b"G=4097"), (dict(T=-1), b"T=-1"), (dict(T=2 ** 31), b"out of range"),
     (dict(N=12), b"multiples of 8"), (dict(K=0), b"multiples of 8"), (dict(dtype=3), b"dtype=3"),
     (dict(ldx=8), b"ldx=8"), (dict(ldx=20), b"ldx=20"), (dict(bias=P, bias_rows=2), b"bias_rows=2"),
-    (dict(x=None), b"null pointer"), (dict(offsets=None), b"one group only"),
+    (dict(x=None), b"null pointer"), (dict(dtype=0, xs=None), b"null pointer"), (dict(dtype=0, ldx=24), b"planes"), (dict(offsets=None), b"one group only"),
     (dict(T=2 ** 31 - 512, N=2 ** 20, G=1), b"too many output tiles"), (dict(G=4096, N=2 ** 20), b"too large"),
 ])
 def test_grouped_linear_refusals(lib, change, message):
-    a = dict(x=P, ldx=16, W=P, offsets=P, G=3, bias=None, bias_rows=0, T=10, N=24, K=16, dtype=1, y=P)
+    a = dict(x=P, ldx=16, xs=P, W=P, ws=P, offsets=P, G=3, bias=None, bias_rows=0, T=10, N=24, K=16, dtype=1, y=P)
     a.update(change)
     assert lib.fuma_grouped_linear(*a.values(), None, None) == -1
     assert message in lib.fuma_last_error()
 
 
 def test_alignment_refused(lib):
-    assert lib.fuma_grouped_linear(P + 8, 16, P, P, 3, None, 0, 10, 24, 16, 1, P, None, None) == -2
-    assert lib.fuma_grouped_linear_dgrad(P, 24, P + 2, P, 3, 10, 24, 16, 1, P, None, None) == -2
+    assert lib.fuma_grouped_linear(P + 8, 16, None, P, None, P, 3, None, 0, 10, 24, 16, 1, P, None, None) == -2
+    assert lib.fuma_grouped_linear_dgrad(P, 24, None, P + 2, None, P, 3, 10, 24, 16, 1, P, None, None) == -2
     assert lib.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P + 4, 16, P, None) == -2
     assert lib.fuma_mix_experts(P, 4, 1, P + 4, 2, 4, 64, 0, P, None, None) == -2
 
 
 def test_other_refusals(lib):
     f = lib
-    assert f.fuma_grouped_linear_dgrad(P, 16, P, P, 3, 10, 24, 16, 1, P, None, None) == -1        # lddy < N
-    assert f.fuma_split_bf16x3(P, 6, 4, 6, P, None) == -1
+    assert f.fuma_grouped_linear_dgrad(P, 16, None, P, None, P, 3, 10, 24, 16, 1, P, None, None) == -1   # lddy < N
+    assert f.fuma_split_blocks(P, 12, 4, 12, P, 1, 0, P, P, None) == -1                           # cols
+    assert f.fuma_split_blocks(P, 16, 10, 16, None, 0, 4, P, P, None) == -1                       # mat_rows
+    assert f.fuma_split_blocks(P, 16, 10, 16, None, 2, 0, P, P, None) == -1                       # no offsets
     assert f.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P, 24, P, None) == -1                        # ldq
     assert f.fuma_quantize_weight_fp8(P, 1, 24, 16, P, 16, P, P, 24, P, None) == -1               # ldt
     assert f.fuma_grouped_linear_fp8(P, 16, P, P, None, 2, None, 0, 10, 24, 16, 1, P, P, 1 << 20, None, None) == -1
@@ -50,15 +52,15 @@ def test_other_refusals(lib):
     assert f.fuma_mix_experts_bwd(P, P, 4, 1, P, 2, 4, 64, 0, P, P, P, 4, None, None) == -1                # work space
     assert f.fuma_mix_experts_bwd(P, P, 4, 1, P, 2, 4, 64, 0, None, None, P, 1 << 20, None, None) == -1
     # nothing to do: no launch, no device needed
-    assert f.fuma_grouped_linear(None, 16, None, None, 3, None, 0, 0, 24, 16, 1, None, None, None) == 0
+    assert f.fuma_grouped_linear(None, 16, None, None, None, None, 3, None, 0, 0, 24, 16, 1, None, None, None) == 0
     assert f.fuma_mix_experts(None, 4, 1, None, 0, 4, 64, 0, None, None, None) == 0
 
 
 def test_work_sizes(lib):
     """The weight gradient's work space holds two slots per chunk bound of the rows; none for short batches."""
     n = lib.fuma_grouped_wgrad_work_bytes
-    assert n(0, 64, 64) == 0 and n(2048, 64, 64) == 0
-    assert n(2049, 64, 64) >= 2 * 2 * 64 * 64 * 4
+    assert n(0, 64, 64, 1) == 0 and n(2048, 64, 64, 1) == 0
+    assert n(2049, 64, 64, 1) >= 2 * 2 * 64 * 64 * 4
     assert lib.fuma_grouped_bias_grad_work_bytes(1000, 64, 5) >= (2 + 5) * 64 * 4
     assert lib.fuma_mix_experts_work_bytes(3, 4, 1000, 0) >= 3 * 4 * 4
 
@@ -80,6 +82,23 @@ def test_partial_slots_never_meet():
                     assert c == 0 or s >= slots
                     used.add(s)
             a += n
+
+
+def test_row_block_slots_never_meet():
+    """The slot rule of the fp32 split's block scales (group start / 128 + group + tile), restated: distinct, in range,
+    and found again by the kernel's search."""
+    g = torch.Generator().manual_seed(1)
+    for _ in range(300):
+        lens = (torch.rand(15, generator=g) ** 2 * 500).long().tolist()
+        starts = [sum(lens[:i]) for i in range(len(lens))]
+        slots, used = sum(lens) // 128 + len(lens), set()
+        for k, (a, n) in enumerate(zip(starts, lens)):
+            for i in range(-(-n // 128)):
+                s = a // 128 + k + i
+                assert s not in used and s < slots
+                used.add(s)
+                found = max(j for j in range(len(lens)) if starts[j] // 128 + j <= s)
+                assert found == k and s - (starts[found] // 128 + found) == i
 
 
 def test_cpu_tensors_refused():
