@@ -360,6 +360,26 @@ bool make_map_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, 
   return true;
 }
 
+bool make_map_5d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, int64_t cols, int64_t rows,
+                 int64_t mats, int64_t planes, int64_t row_bytes, int64_t mat_bytes, int64_t plane_bytes, int box_rows,
+                 int box_chunks, int box_planes) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[5] = {64, (cuuint64_t)rows, (cuuint64_t)(cols / 64), (cuuint64_t)mats, (cuuint64_t)planes};
+  cuuint64_t strides[4] = {(cuuint64_t)row_bytes, 128, (cuuint64_t)mat_bytes, (cuuint64_t)plane_bytes};
+  cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_chunks, 1, (cuuint32_t)box_planes};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(map, dtype, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    snprintf(g_map_err, sizeof(g_map_err),
+             "cuTensorMapEncodeTiled failed (CUresult %d) for base=%p cols=%lld rows=%lld matrices=%lld ld=%lldB", (int)r,
+             base, (long long)cols, (long long)rows, (long long)mats, (long long)row_bytes);
+    return false;
+  }
+  return true;
+}
+
 namespace {
 
 // fp32 operand: box 32 x box_rows (128-byte rows), 128-byte swizzle.

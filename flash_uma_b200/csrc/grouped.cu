@@ -190,6 +190,25 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// The same with the tile in one go: (64 columns, rows, chunks of 64 columns, matrix, plane), for widths that are whole chunks.
+template <bool kPair>
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int y, int chunk, int z, uint32_t bar) {
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+        "%4, %5, %6}], [%7];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(chunk), "r"(z), "r"(0), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+        "[%7];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(chunk), "r"(z), "r"(0), "r"(bar)
+        : "memory");
+}
+
 // Group g's start, held inside [0, T] whatever the caller's array says; no array: one group of all rows.
 __device__ __forceinline__ int64_t group_at(const int64_t* off, int g, int64_t T) {
   if (!off) return g ? T : 0;
@@ -201,16 +220,13 @@ __device__ __forceinline__ int64_t group_len(const int64_t* off, int g, int64_t 
   return n > 0 ? n : 0;
 }
 
-// Work units of a group: tiles of kTileM rows (row maps), or chunks of `chunk` contraction rows (weight
-// gradient; a group without rows still has one, which writes zeros).
+// Work units of a group: its tiles of kTileM rows (row maps), or the parts that its contraction is cut into (weight
+// gradient: even parts of at most `cap` blocks of 128 rows; a group without rows has one, which writes zeros).
 template <int kMode, int kTileM>
-__device__ __forceinline__ int group_units(int64_t len, int chunk) {
-  if constexpr (kMode == kModeDw) {
-    const int64_t n = (len + chunk - 1) / chunk;
-    return n > 0 ? (int)n : 1;
-  } else {
-    return (int)((len + kTileM - 1) / kTileM);
-  }
+__device__ __forceinline__ int group_units(int64_t len, int cap) {
+  const int n = (int)((len + kTileM - 1) / kTileM);
+  if constexpr (kMode == kModeDw) return n ? (n + cap - 1) / cap : 1;
+  else return n;
 }
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b, int dtype) {
@@ -233,64 +249,87 @@ struct Item {
   int g, n0;
   int nt;           // columns of the tile that exist, rounded up to what the MMA takes
   int row0;         // first A row (row maps) or first contraction row (weight gradient)
-  int m0, rows;     // weight gradient: first output row; rows of the tile that exist (may be <= 0)
+  int m0, rows;     // weight gradient: first output row; rows of the tile that exist (may be 0)
   int tail;         // weight gradient: contraction rows of the last k-block (0: all)
-  int64_t out;      // element offset of (row 0, column 0) of the tile's matrix in the output
   int slot;         // kSplit: index of the tile's (weight gradient: the first segment's) row block among the scales
-  int partial;      // weight gradient: goes to the fp32 workspace
+  int partial;      // weight gradient: 1 + the workspace matrix that takes the sum, or 0
+  int pad[2];
 };
 constexpr int kRing = 4;
 
-template <int kMode, int kBK, bool kPair>
-__device__ __forceinline__ Item item_at(const GroupedArgs& p, const int* prefix, int item, int rank) {
-  constexpr int kTileM = kPair ? 2 * kBM : kBM, kStep = kPair ? 32 : 16;
-  Item t;
-  t.partial = 0;
-  t.tail = 0;
-  const int tiles = kMode == kModeDw ? p.tiles_m * p.tiles_n : p.tiles_n;
-  const int u = item / tiles, tile = item - u * tiles;
-  // the last group whose units start at or before u: a search over every p.span-th group's start, then a walk
+// The group that unit u falls into, and its units before u: a search over every p.span-th group's start, then a walk.
+template <int kMode, int kTileM>
+__device__ __forceinline__ int find_group(const GroupedArgs& p, const int* prefix, int u, int& c, int64_t& at, int64_t& len) {
   int lo = 0, hi = (p.G + p.span - 1) / p.span;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (prefix[mid] <= u) lo = mid; else hi = mid;
   }
-  int g = lo * p.span, c = u - prefix[lo];
-  int64_t at = group_at(p.offsets, g, p.T), len = group_len(p.offsets, g, p.T);
-  for (int n = group_units<kMode, kTileM>(len, p.chunk); c >= n && g + 1 < p.G;) {
+  int g = lo * p.span;
+  c = u - prefix[lo];
+  at = group_at(p.offsets, g, p.T);
+  len = group_len(p.offsets, g, p.T);
+  for (int n = group_units<kMode, kTileM>(len, p.cap); c >= n && g + 1 < p.G;) {
     c -= n;
     ++g;
     at = group_at(p.offsets, g, p.T);
     len = group_len(p.offsets, g, p.T);
-    n = group_units<kMode, kTileM>(len, p.chunk);
+    n = group_units<kMode, kTileM>(len, p.cap);
   }
-  t.g = g;
-  if constexpr (kMode == kModeDw) {
-    t.row0 = (int)(at + (int64_t)c * p.chunk);
-    int64_t n = len - (int64_t)c * p.chunk;
-    if (n > p.chunk) n = p.chunk;
-    t.kblocks = (int)((n + kBK - 1) / kBK);
-    t.tail = (int)(n % kBK);
-    t.m0 = (tile / p.tiles_n) * kBM;
-    t.n0 = (tile % p.tiles_n) * p.bn;
-    t.rows = p.M - t.m0 < kBM ? p.M - t.m0 : kBM;
-    t.partial = len > p.chunk;
-    const int64_t slot = at / p.chunk + c;   // chunk 0 in the first half of the slots, see grouped.cuh
-    t.out = (t.partial ? (c == 0 ? slot : p.slots + slot) : (int64_t)g) * p.M * p.N + (int64_t)t.m0 * p.N;
-    t.slot = (int)(at / kBM) + g + c * (p.chunk / kBM);
-  } else {
-    const int64_t r = (int64_t)c * kTileM + rank * kBM;
-    const int64_t left = len - r;
-    t.row0 = (int)(at + r);
-    t.m0 = 0;
-    t.rows = left < kBM ? (int)(left < 0 ? 0 : left) : kBM;
-    t.n0 = tile * p.bn;
-    t.kblocks = (p.K + kBK - 1) / kBK;
-    t.out = (at + r) * p.ldc;
-    t.slot = (int)(at / kBM + g + r / kBM);
-  }
-  const int cols = p.N - t.n0;
-  t.nt = cols < p.bn ? (cols + kStep - 1) / kStep * kStep : p.bn;
+  return g;
+}
+
+template <bool kPair>
+__device__ __forceinline__ int tile_columns(const GroupedArgs& p, int n0) {
+  constexpr int kStep = kPair ? 32 : 16;
+  const int cols = p.N - n0;
+  return cols < p.bn ? (cols + kStep - 1) / kStep * kStep : p.bn;
+}
+
+// Row maps: item -> tile.
+template <int kBK, bool kPair>
+__device__ __forceinline__ Item row_item(const GroupedArgs& p, const int* prefix, int item, int rank) {
+  constexpr int kTileM = kPair ? 2 * kBM : kBM;
+  Item t{};
+  const int u = item / p.tiles_n;
+  int c;
+  int64_t at, len;
+  t.g = find_group<kModeFwd, kTileM>(p, prefix, u, c, at, len);
+  const int64_t r = (int64_t)c * kTileM + rank * kBM, left = len - r;
+  t.row0 = (int)(at + r);
+  t.rows = left < kBM ? (int)(left < 0 ? 0 : left) : kBM;
+  t.n0 = (item - u * p.tiles_n) * p.bn;
+  t.kblocks = (p.K + kBK - 1) / kBK;
+  t.slot = (int)(at / kBM + t.g + r / kBM);
+  t.nt = tile_columns<kPair>(p, t.n0);
+  return t;
+}
+
+// Weight gradient: item -> a part of a group's contraction and an output tile, the tiles of a part one after the other, so
+// that the CTAs work on the same rows at the same time and all but the first find them in L2. (One line of all tiles cut into
+// equal stretches balances better and loses more to rows read again from HBM: 172 us against 141 at 120,000 rows.) Parts of
+// cut groups go to the workspace, slot 2 * (first block) / cap + part: see grouped.cuh.
+template <int kBK>
+__device__ __forceinline__ Item wgrad_item(const GroupedArgs& p, const int* prefix, int item) {
+  Item t{};
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int u = item / tiles, tile = item - u * tiles;
+  int c;
+  int64_t at, len;
+  t.g = find_group<kModeDw, kBM>(p, prefix, u, c, at, len);
+  const int blocks = (int)((len + kBM - 1) / kBM), parts = blocks > p.cap ? (blocks + p.cap - 1) / p.cap : 1;
+  const int each = (blocks + parts - 1) / parts;
+  const int64_t r0 = (int64_t)c * each * kBM, r1 = r0 + (int64_t)each * kBM;
+  const int n = r0 < len ? (int)((r1 < len ? r1 : len) - r0) : 0;
+  t.row0 = (int)(at + r0);
+  t.kblocks = (n + kBK - 1) / kBK;
+  t.tail = n % kBK;
+  t.m0 = (tile / p.tiles_n) * kBM;
+  t.n0 = (tile % p.tiles_n) * p.bn;
+  t.rows = p.M - t.m0 < kBM ? p.M - t.m0 : kBM;
+  t.slot = (int)(at / kBM) + t.g + c * each;
+  t.nt = tile_columns<false>(p, t.n0);
+  if (parts > 1) t.partial = 1 + (int)(2 * (at / kBM) / p.cap) + c;
   return t;
 }
 
@@ -371,7 +410,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
         const int64_t a = p.offsets[g], b = p.offsets[g + 1];
         bad |= a < 0 || b < a || b > p.T;
       }
-      sum += group_units<kMode, kTileM>(group_len(p.offsets, g, p.T), p.chunk);
+      sum += group_units<kMode, kTileM>(group_len(p.offsets, g, p.T), p.cap);
     }
     // offsets that decrease or leave [0, T]: recorded, and no item runs (every CTA sees the same array)
     bad = __syncthreads_or(bad);
@@ -396,7 +435,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
   else __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
-  const int items = prefix[kCoarse] * (kMode == kModeDw ? p.tiles_m * p.tiles_n : p.tiles_n);
+  const int units = prefix[kCoarse];
 
   if (warp < kEpiWarp0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
@@ -417,7 +456,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
         if (kblocks < 0) break;
         const int cols = kPair ? nt / 2 : nt;             // of B in this CTA
         const int nb = n0 + rank * cols;
-        const int loads = kBmn ? (cols + 63) / 64 : 1;
+        const int loads = !kBmn ? 1 : p.wide_b ? p.box_b / 64 : (cols + 63) / 64;   // chunks of B that arrive
         const uint32_t bytes = kP * (L::kA + loads * (kBmn ? kBK * 128 : p.box_b * L::kRowBytes)) * (kPair ? 2 : 1);
         for (int kt = 0; kt < kblocks; ++kt, ++it) {
           const int s = it % L::kStages;
@@ -428,18 +467,27 @@ __global__ void __launch_bounds__(kGThreads, 1)
           const uint32_t a = smem0 + s * L::kStage, b = a + kP * L::kA, bar = full0 + s * 8;
           if (rank == 0 && lane == 0) mbar_expect_tx(&bar_full[s], bytes);
           __syncwarp();
+          // (one load where the width allows: each takes the producer about 100 cycles, and a stage's MMAs 512)
           if constexpr (kAmn) {
+            if (p.wide_a) {
+              tma_load_5d<kPair>(a, &tmA, row0 + kt * kBK, m0 / 64, 0, bar);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kBM / 64; ++c)
-              tma_load_4d<kPair>(a + c * kChunkMn, &tmA, m0 + c * 64, row0 + kt * kBK, 0, bar);
+              for (int c = 0; c < kBM / 64; ++c)
+                tma_load_4d<kPair>(a + c * kChunkMn, &tmA, m0 + c * 64, row0 + kt * kBK, 0, bar);
+            }
           } else {
             tma_load_4d<kPair>(a, &tmA, kt * kBK, row0, 0, bar);
           }
           if constexpr (kBmn) {
-            const int y = kMode == kModeDw ? row0 + kt * kBK : kt * kBK;
+            const int y = kMode == kModeDw ? row0 + kt * kBK : kt * kBK, z = kMode == kModeDw ? 0 : g;
+            if (p.wide_b) {
+              tma_load_5d<kPair>(b, &tmB, y, nb / 64, z, bar);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kMaxBN / 64; ++c)
-              if (c < loads) tma_load_4d<kPair>(b + c * kChunkMn, &tmB, nb + c * 64, y, kMode == kModeDw ? 0 : g, bar);
+              for (int c = 0; c < kMaxBN / 64; ++c)
+                if (c < loads) tma_load_4d<kPair>(b + c * kChunkMn, &tmB, nb + c * 64, y, z, bar);
+            }
           } else {
             tma_load_4d<kPair>(b, &tmB, kt * kBK, nb, g, bar);
           }
@@ -460,11 +508,13 @@ __global__ void __launch_bounds__(kGThreads, 1)
       // descriptors of stage 0, first plane, first step; the rest is constants added to the address field (units of
       // 16 bytes; shared memory stays below its 14 bits)
       const uint32_t a0 = smem_u32(smem), b0 = a0 + kP * L::kA;
-      const uint64_t da0 = kAmn ? smem_desc_mn128(a0, kChunkMn) : L::kRowBytes == 64 ? smem_desc_k64(a0) : smem_desc_sw128(a0);
-      const uint64_t db0 = kBmn ? smem_desc_mn128(b0, kChunkMn) : L::kRowBytes == 64 ? smem_desc_k64(b0) : smem_desc_sw128(b0);
+      // MN-major tiles: loaded chunk by chunk, a chunk's planes follow one another; in one go, a plane's chunks do
+      const uint32_t chunk_a = p.wide_a ? kBK * 128 : kChunkMn, chunk_b = p.wide_b ? kBK * 128 : kChunkMn;
+      const uint64_t da0 = kAmn ? smem_desc_mn128(a0, chunk_a) : L::kRowBytes == 64 ? smem_desc_k64(a0) : smem_desc_sw128(a0);
+      const uint64_t db0 = kBmn ? smem_desc_mn128(b0, chunk_b) : L::kRowBytes == 64 ? smem_desc_k64(b0) : smem_desc_sw128(b0);
       constexpr uint32_t kStepA = (kAmn ? 2048 : 32) / 16, kStepB = (kBmn ? 2048 : 32) / 16;
-      constexpr uint32_t kPlaneA = (kAmn ? kBK * 128 : L::kA) / 16;
-      const uint32_t plane_b = kBmn ? kBK * 128 / 16 : p.box_b * L::kRowBytes / 16;
+      const uint32_t plane_a = (!kAmn ? L::kA : p.wide_a ? kBM / 64 * kBK * 128 : kBK * 128) / 16;
+      const uint32_t plane_b = (!kBmn ? p.box_b * L::kRowBytes : p.wide_b ? p.box_b / 64 * (kBK * 128) : kBK * 128) / 16;
       constexpr int kSteps = kBK * L::kElem / 32;
       const uint32_t tm = __shfl_sync(kFull, tmem, 0);
       const uint32_t empty0 = smem_u32(bar_empty), accf0 = smem_u32(bar_acc_full);
@@ -515,7 +565,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
             const uint64_t dak = da + kk * kStepA, dbk = db + kk * kStepB;
             if constexpr (kKind == kSplit) {   // the small products first
               mma_issue<false, kPair>(acc_d, dak, dbk + plane_b, idesc, acc);
-              mma_issue<false, kPair>(acc_d, dak + kPlaneA, dbk, idesc, 1u);
+              mma_issue<false, kPair>(acc_d, dak + plane_a, dbk, idesc, 1u);
               mma_issue<false, kPair>(acc_d, dak, dbk, idesc, 1u);
             } else {
               mma_issue<kKind == kFp8, kPair>(acc_d, dak, dbk, idesc, acc);
@@ -564,7 +614,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
           uint8_t* sa = smem + s * L::kStage;
           uint8_t* sb = sa + kP * L::kA;
           const int dead = (t.tail + 15) / 16 * 16 - t.tail;
-          const int chunks = kBM / 64 * kP, chunks_b = (t.nt + 63) / 64 * kP;
+          const int chunks = kBM / 64 * kP, chunks_b = (p.wide_b ? p.box_b / 64 : (t.nt + 63) / 64) * kP;
           for (int i = lane; i < (chunks + chunks_b) * dead * 8; i += 32) {
             const int c = i / (dead * 8), r = (i / 8) % dead, j = i % 8;
             uint8_t* base = c < chunks ? sa + c * (kBK * 128) : sb + (c - chunks) * (kBK * 128);
@@ -580,17 +630,22 @@ __global__ void __launch_bounds__(kGThreads, 1)
     } else if (warp == 3) {
       // ---------------- items
       if (lane == 0) {
-        int n = 0;
-        for (int item = first_item;; item += item_step, ++n) {
+        auto publish = [&](int n, const Item& t) {
           if (n >= kRing && !mbar_wait(&bar_item_empty[n % kRing], ((n / kRing) - 1) & 1, abort_flag, p.err, kErrWaitEmpty))
-            break;
-          Item t{};
-          if (item < items) t = item_at<kMode, kBK, kPair>(p, prefix, item, rank);
-          else t.kblocks = -1;
+            return false;
           ring[n % kRing] = t;
           mbar_arrive(&bar_item_full[n % kRing]);
-          if (item >= items) break;
-        }
+          return t.kblocks >= 0;
+        };
+        const int items = units * (kMode == kModeDw ? p.tiles_m * p.tiles_n : p.tiles_n);
+        auto make = [&](int item) {
+          if constexpr (kMode == kModeDw) return wgrad_item<kBK>(p, prefix, item);
+          else return row_item<kBK, kPair>(p, prefix, item, rank);
+        };
+        Item last{};
+        last.kblocks = -1;
+        int item = first_item;
+        for (int n = 0; publish(n, item < items ? make(item) : last); ++n) item += item_step;
       }
       __syncwarp();
     }
@@ -603,7 +658,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
       // rows before the first and behind the last group: zeros
       const int64_t head = group_at(p.offsets, 0, p.T), tail = group_at(p.offsets, p.G, p.T);
       const int vec = p.N * (p.out_dtype == kDtypeF32 ? 4 : 2) / 16;
-      const int64_t dead = items || head == tail ? head + (p.T - tail) : 0, n = dead * vec;
+      const int64_t dead = units || head == tail ? head + (p.T - tail) : 0, n = dead * vec;
       for (int64_t i = (int64_t)blockIdx.x * (kEpiWarps * 32) + threadIdx.x - kEpiWarp0 * 32; i < n;
            i += (int64_t)gridDim.x * (kEpiWarps * 32)) {
         const int64_t r = i / vec, row = r < head ? r : tail + (r - head);
@@ -739,13 +794,17 @@ __global__ void __launch_bounds__(kGThreads, 1)
         }
       }
       // rows out: 128 bytes of each of the warp's 32 rows at a time through the staging area (16-byte
-      // chunk j of row r at j ^ (r & 7)), so a store instruction writes 4 rows x 128 bytes
-      const int out_dtype = (kMode == kModeDw && t.partial) ? kDtypeF32 : p.out_dtype;
-      uint8_t* out = static_cast<uint8_t*>((kMode == kModeDw && t.partial) ? p.work : p.C);
+      // chunk j of row r at j ^ (r & 7)), so a store instruction writes 4 rows x 128 bytes. (TMA stores from the staging
+      // area queue behind the producer's loads: the fp8 map took 128 us with them and 107 without.)
+      const bool partial = kMode == kModeDw && t.partial;
+      const int out_dtype = partial ? kDtypeF32 : p.out_dtype;
       const int64_t ld = kMode == kModeDw ? p.N : p.ldc;
+      const int64_t y0 = (kMode == kModeDw ? (int64_t)(partial ? t.partial - 1 : t.g) * p.M + t.m0 : t.row0) + q * 32;
+      const int x0 = n0;
+      uint8_t* out = static_cast<uint8_t*>(partial ? p.work : p.C);
       const int rr = lane >> 3, jj = lane & 7;
       if (out_dtype == kDtypeF32) {
-        float* o = reinterpret_cast<float*>(out) + t.out + (int64_t)(q * 32 + rr) * ld + n0 + jj * 4;
+        float* o = reinterpret_cast<float*>(out) + (y0 + rr) * ld + x0 + jj * 4;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           if (c * 32 < ncols) {
@@ -766,7 +825,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
           }
         }
       } else {
-        uint16_t* o = reinterpret_cast<uint16_t*>(out) + t.out + (int64_t)(q * 32 + rr) * ld + n0 + jj * 8;
+        uint16_t* o = reinterpret_cast<uint16_t*>(out) + (y0 + rr) * ld + x0 + jj * 8;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (c * 64 < ncols) {
@@ -806,14 +865,15 @@ __global__ void __launch_bounds__(kGThreads, 1)
 }
 
 // ---- joining the chunks of the weight gradient --------------------------------------------------
-// dW[g] = sum over the group's chunks, in order, for groups of more than one chunk. Block row y takes the y-th such
-// group (there are at most T / chunk of them), found by a count over all groups: 256 threads with a run each.
+// dW[g] = sum over the group's parts, in order, for groups that were cut. Block row y takes the y-th such
+// group (there are fewer than T / 128 / cap of them), found by a count over all groups: 256 threads with a run each.
 __global__ void __launch_bounds__(256) grouped_join_kernel(const __grid_constant__ GroupedArgs p) {
   __shared__ int count[8], found;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int per = (p.G + 255) / 256, g0 = threadIdx.x * per, g1 = min(p.G, g0 + per);
+  const int64_t most = (int64_t)p.cap * kBM;
   int n = 0;
-  for (int g = g0; g < g1; ++g) n += group_len(p.offsets, g, p.T) > p.chunk;
+  for (int g = g0; g < g1; ++g) n += group_len(p.offsets, g, p.T) > most;
   int incl = n;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -828,20 +888,19 @@ __global__ void __launch_bounds__(256) grouped_join_kernel(const __grid_constant
   const int y = blockIdx.y;
   if (before <= y && y < before + n) {
     for (int g = g0; g < g1; ++g)
-      if (group_len(p.offsets, g, p.T) > p.chunk && before++ == y) found = g;
+      if (group_len(p.offsets, g, p.T) > most && before++ == y) found = g;
   }
   __syncthreads();
   const int g = found;
   if (g < 0) return;
   const int64_t at = group_at(p.offsets, g, p.T), len = group_len(p.offsets, g, p.T);
-  const int chunks = (int)((len + p.chunk - 1) / p.chunk);
-  const int64_t n4 = (int64_t)p.M * p.N / 4, slot = at / p.chunk;
-  const float* first = static_cast<const float*>(p.work) + slot * n4 * 4;
-  const float* rest = static_cast<const float*>(p.work) + (p.slots + slot) * n4 * 4;
+  const int parts = group_units<kModeDw, kBM>(len, p.cap);
+  const int64_t n4 = (int64_t)p.M * p.N / 4;
+  const float* work = static_cast<const float*>(p.work) + 2 * (at / kBM) / p.cap * n4 * 4;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (int64_t)gridDim.x * blockDim.x) {
-    float4 s = ld4_stream(first + i * 4);
+    float4 s = ld4_stream(work + i * 4);
 #pragma unroll 4
-    for (int c = 1; c < chunks; ++c) s += ld4_stream(rest + (c * n4 + i) * 4);
+    for (int c = 1; c < parts; ++c) s += ld4_stream(work + (c * n4 + i) * 4);
     const int64_t o = ((int64_t)g * n4 + i) * 4;
     if (p.out_dtype == kDtypeF32)
       st4(static_cast<float*>(p.C) + o, s);
@@ -1069,8 +1128,7 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restri
 namespace {
 
 template <int kKind, int kMode, bool kPair>
-cudaError_t launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& p, int64_t max_items,
-                           cudaStream_t s) {
+cudaError_t launch_grouped(const CUtensorMap (&m)[2], const GroupedArgs& p, int64_t max_items, cudaStream_t s) {
   using L = GSmem<kKind, kPair>;
   auto kern = grouped_gemm_kernel<kKind, kMode, kPair>;
   static thread_local uint64_t configured = 0;  // one bit per device
@@ -1101,25 +1159,25 @@ cudaError_t launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const Gro
       n = sm_count() / 4;
     }
     cfg.gridDim = dim3((unsigned)(2 * (max_items < 1 ? 1 : max_items < n ? max_items : n)));
-    return cudaLaunchKernelEx(&cfg, kern, a, b, p);
+    return cudaLaunchKernelEx(&cfg, kern, m[0], m[1], p);
   } else {
     const int64_t sms = sm_count();
     const int grid = (int)(max_items < 1 ? 1 : max_items < sms ? max_items : sms);
-    kern<<<grid, kGThreads, L::kBytes, s>>>(a, b, p);
+    kern<<<grid, kGThreads, L::kBytes, s>>>(m[0], m[1], p);
     return cudaGetLastError();
   }
 }
 
-// Columns per tile: the whole width in even parts of at most 256 (so that N = 640 runs as 3 x 224 and not as
-// 2 x 256 + 128), with block scales 256 or 128, and narrower tiles, down to 32, while there
+// Columns per tile: the whole width in even parts of at most 256, multiples of `step` (with block scales 256 or 128), and
+// narrower tiles, down to 32, while there
 // would be fewer tiles than SMs: a call of a few rows is bound by how many SMs pull its matrices in.
-int pick_bn(int N, int64_t tiles_rows, bool scaled) {
+int pick_bn(int N, int64_t tiles_rows, bool scaled, int step) {
   int bn;
   if (scaled) {
     bn = N > 128 ? 256 : 128;   // whole 128-blocks of the scales
   } else {
     const int parts = (N + kMaxBN - 1) / kMaxBN;
-    bn = ((N + parts - 1) / parts + 31) / 32 * 32;
+    bn = ((N + parts - 1) / parts + step - 1) / step * step;
   }
   while (bn > 32 && tiles_rows * ((N + bn - 1) / bn) < sm_count()) {
     const int half = scaled ? bn / 2 : (bn / 2 + 31) / 32 * 32;
@@ -1141,35 +1199,38 @@ int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed
   const int bk = fp8 ? 128 : split ? 32 : 64;
   const int64_t groups = p.G < p.T ? p.G : p.T;
   const int64_t tiles_rows = p.T / kBM + groups;   // upper bound: a partial tile per group
-  p.bn = pick_bn(p.N, tiles_rows, fp8 || split);
+  p.bn = pick_bn(p.N, tiles_rows, fp8 || split, transposed ? 64 : 32);   // transposed: whole chunks of 64
   p.tiles_n = (p.N + p.bn - 1) / p.bn;
   p.tiles_m = 1;
   p.err = err;
-  p.chunk = 0;
   p.span = (p.G + kCoarse - 1) / kCoarse;
   p.mma_format = (!fp8 && !split && o.dtype == kDtypeBf16) ? 1u : 0u;
   const int64_t pair_items = (p.T / (2 * kBM) + groups) * p.tiles_n;
   const char* pe = getenv("FUMA_PAIR"); const bool pair = (pe ? atoi(pe) != 0 : !fp8) && p.bn > 128 && use_pair(p.T, p.G, pair_items);
-  p.box_b = pair ? p.bn / 2 : p.bn;   // rows of W per load (forward): this CTA's columns, the planes one behind the other
+  p.box_b = pair ? p.bn / 2 : p.bn;   // columns of the tile in this CTA: rows of W per load (forward)
+  p.wide_b = transposed && p.N % (pair ? 128 : 64) == 0 && p.box_b % 64 == 0;
+  p.wide_a = 0;
   const CUtensorMapDataType dt = fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                  : p.mma_format ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUtensorMapSwizzle ksw = split ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-  CUtensorMap ma, mb;
+  CUtensorMap m[2];
   // A: [T rows, K], planes T * lda apart
-  if (!make_map_4d(&ma, dt, o.A, p.K, p.T, 1, P, o.lda * esize, p.T * o.lda * esize, p.T * o.lda * esize, bk, kBM, P,
+  if (!make_map_4d(&m[0], dt, o.A, p.K, p.T, 1, P, o.lda * esize, p.T * o.lda * esize, p.T * o.lda * esize, bk, kBM, P,
                    ksw))
     return -1;
   // W: forward [G, N, K] with K contiguous along the contraction; input gradient [G, K, N] with the
   // output columns contiguous
   const int64_t brows = transposed ? p.K : p.N, bcols = transposed ? p.N : p.K;
-  if (!make_map_4d(&mb, dt, o.B, bcols, brows, p.G, P, o.ldb * esize, brows * o.ldb * esize,
-                   p.G * brows * o.ldb * esize, transposed ? 64 : bk, transposed ? bk : p.box_b, P,
-                   transposed ? CU_TENSOR_MAP_SWIZZLE_128B : ksw))
+  if (p.wide_b ? !make_map_5d(&m[1], dt, o.B, bcols, brows, p.G, P, o.ldb * 2, brows * o.ldb * 2, p.G * brows * o.ldb * 2,
+                              bk, p.box_b / 64, P)
+               : !make_map_4d(&m[1], dt, o.B, bcols, brows, p.G, P, o.ldb * esize, brows * o.ldb * esize,
+                              p.G * brows * o.ldb * esize, transposed ? 64 : bk, transposed ? bk : p.box_b, P,
+                              transposed ? CU_TENSOR_MAP_SWIZZLE_128B : ksw))
     return -1;
   const int64_t items = tiles_rows * p.tiles_n;
   cudaError_t st;
-#define FUMA_ROWS(kind, mode) (pair ? launch_grouped<kind, mode, true>(ma, mb, p, pair_items, s) \
-                                    : launch_grouped<kind, mode, false>(ma, mb, p, items, s))
+#define FUMA_ROWS(kind, mode) (pair ? launch_grouped<kind, mode, true>(m, p, pair_items, s) \
+                                    : launch_grouped<kind, mode, false>(m, p, items, s))
   if (fp8) st = FUMA_ROWS(kFp8, kModeFwd);
   else if (split) st = transposed ? FUMA_ROWS(kSplit, kModeDx) : FUMA_ROWS(kSplit, kModeFwd);
   else st = transposed ? FUMA_ROWS(kHalf, kModeDx) : FUMA_ROWS(kHalf, kModeFwd);
@@ -1177,31 +1238,27 @@ int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed
   return (int)st;
 }
 
-// Rows of the contraction per work item of the weight gradient: long groups are cut so that about
-// three rounds of tiles fill the SMs, but not below 2048 rows, where writing and joining the fp32
-// partial matrices costs as much as the products.
-static int wgrad_chunk(int64_t T, int tiles) {
-  int64_t c = T * tiles / ((int64_t)148 * 3);
-  if (c < 2048) c = 2048;
-  if (c > (1 << 20)) c = 1 << 20;
-  return (int)((c + 127) / 128 * 128);   // whole row blocks of the split's scales
-}
-
 static int wgrad_bn(int N, bool split) {
   if (split) return N > 128 ? 256 : 128;   // whole 128-blocks of the scales
   const int parts = (N + kMaxBN - 1) / kMaxBN;
-  return ((N + parts - 1) / parts + 15) / 16 * 16;
+  return ((N + parts - 1) / parts + 63) / 64 * 64;
 }
 
-static int wgrad_tiles(int M, int N, bool split) {
+// Blocks of 128 rows per part of the weight gradient: long groups are cut so that the parts fill the SMs about twice
+// over, but not below 16, where writing and joining the fp32 matrices costs as much as the products. At 120,000 rows in 16
+// groups, 640 x 768: twice 134 + 17 us (products + joining), three times 140 + 22, four times 130 + 26.
+static int wgrad_cap(int64_t T, int M, int N, bool split) {
   const int bn = wgrad_bn(N, split);
-  return (M + kBM - 1) / kBM * ((N + bn - 1) / bn);
+  const int64_t tiles = (int64_t)((M + kBM - 1) / kBM) * ((N + bn - 1) / bn);
+  int64_t cap = T / kBM * tiles / ((int64_t)sm_count() * 2);
+  if (cap < 16) cap = 16;
+  return cap > (1 << 13) ? 1 << 13 : (int)cap;
 }
 
 int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N, int dtype) {
-  const int chunk = wgrad_chunk(T, wgrad_tiles(M, N, dtype == kDtypeF32));
-  if (T <= chunk) return 0;
-  return 2 * (T / chunk + 1) * (int64_t)M * N * 4;
+  const int cap = wgrad_cap(T, M, N, dtype == kDtypeF32);
+  if (T <= (int64_t)cap * kBM) return 0;
+  return (2 * (T / kBM) / cap + 2) * (int64_t)M * N * 4;
 }
 
 int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cudaStream_t s) {
@@ -1211,28 +1268,31 @@ int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cuda
   p.bn = wgrad_bn(p.N, split);
   p.tiles_n = (p.N + p.bn - 1) / p.bn;
   p.tiles_m = (p.M + kBM - 1) / kBM;
-  p.chunk = wgrad_chunk(p.T, p.tiles_m * p.tiles_n);
-  p.slots = p.T / p.chunk + 1;
   p.span = (p.G + kCoarse - 1) / kCoarse;
   p.mma_format = (!split && o.dtype == kDtypeBf16) ? 1u : 0u;
   p.ldc = p.N;
-  p.box_b = 0;
+  p.box_b = p.bn;
+  p.wide_a = p.M % 64 == 0;
+  p.wide_b = p.N % 64 == 0;
+  p.cap = wgrad_cap(p.T, p.M, p.N, split);
   const CUtensorMapDataType dt = p.mma_format ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap ma, mb;
-  if (!make_map_4d(&ma, dt, o.A, p.M, p.T, 1, P, o.lda * 2, p.T * o.lda * 2, p.T * o.lda * 2, 64, bk, P,
-                   CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_map_4d(&mb, dt, o.B, p.N, p.T, 1, P, o.ldb * 2, p.T * o.ldb * 2, p.T * o.ldb * 2, 64, bk, P,
-                   CU_TENSOR_MAP_SWIZZLE_128B))
+  CUtensorMap m[2];
+  auto operand = [&](CUtensorMap* map, const void* base, int cols, int64_t ld, bool wide, int chunks) {
+    return wide ? make_map_5d(map, dt, base, cols, p.T, 1, P, ld * 2, p.T * ld * 2, p.T * ld * 2, bk, chunks, P)
+                : make_map_4d(map, dt, base, cols, p.T, 1, P, ld * 2, p.T * ld * 2, p.T * ld * 2, 64, bk, P,
+                              CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  if (!operand(&m[0], o.A, p.M, o.lda, p.wide_a, kBM / 64) || !operand(&m[1], o.B, p.N, o.ldb, p.wide_b, p.bn / 64))
     return -1;
-  const int64_t items = (p.T / p.chunk + p.G) * (int64_t)p.tiles_m * p.tiles_n;
-  cudaError_t st = split ? launch_grouped<kSplit, kModeDw, false>(ma, mb, p, items, s)
-                         : launch_grouped<kHalf, kModeDw, false>(ma, mb, p, items, s);
-  if (st == cudaSuccess && p.T > p.chunk) {
+  const int64_t items = (p.T / kBM / p.cap + p.G) * (int64_t)p.tiles_m * p.tiles_n;
+  cudaError_t st = split ? launch_grouped<kSplit, kModeDw, false>(m, p, items, s)
+                         : launch_grouped<kHalf, kModeDw, false>(m, p, items, s);
+  if (st == cudaSuccess && p.T > (int64_t)p.cap * kBM) {
     const int64_t n4 = (int64_t)p.M * p.N / 4;
     int64_t bx = (n4 + 255) / 256;
     if (bx > 512) bx = 512;
-    const int64_t by = p.T / p.chunk < p.G ? p.T / p.chunk : p.G;
-    grouped_join_kernel<<<dim3((unsigned)bx, (unsigned)by), 256, 0, s>>>(p);
+    const int64_t long_groups = p.T / ((int64_t)p.cap * kBM);
+    grouped_join_kernel<<<dim3((unsigned)bx, (unsigned)(long_groups < p.G ? long_groups : p.G)), 256, 0, s>>>(p);
     st = cudaGetLastError();
   }
   return (int)st;

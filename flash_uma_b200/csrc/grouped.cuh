@@ -74,17 +74,14 @@ struct GroupedArgs {
   const float* scale_b;
   int blocks_n;             // 128-column blocks of the output
   int64_t scale_slots;
-  // Weight gradient: fp32 partial matrices of groups longer than `chunk` rows. Such a group starts
-  // at row a; its chunk 0 takes slot a / chunk, its chunk c >= 1 slot `slots` + a / chunk + c. Two such
-  // groups never meet: a group of more than `chunk` rows moves a / chunk on by at least
-  // floor(len / chunk) >= 1 for the next one, whose later chunks then start at least
-  // floor(len / chunk) + 1 > ceil(len / chunk) - 1 slots further on. Both ranges end at or before
-  // T / chunk + 1 = `slots`.
+  // Weight gradient: fp32 matrices of the parts of groups longer than cap blocks of 128 rows. Such a group that starts in
+  // block A (of absolute rows) and has b > cap blocks takes slots floor(2 A / cap) + part, part < q = ceil(b / cap). The next
+  // such group starts in block A + b - 1 or later, so its first slot is at least floor(2 (b - 1) / cap) >= 2 (q - 1) >= q
+  // further on. All slots are below 2 (T / 128) / cap + 2.
   void* work;
-  int64_t slots;
   int* err;
   // set by the launcher
-  int bn, tiles_m, tiles_n, chunk, span, box_b;
+  int bn, tiles_m, tiles_n, cap, span, box_b, wide_a, wide_b;
   uint32_t mma_format;
 };
 

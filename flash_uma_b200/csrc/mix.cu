@@ -204,12 +204,12 @@ __global__ void __launch_bounds__(256) mix_dcoeff_join_kernel(const float* __res
 // a cross accumulator. dc leaves TMEM for fp32 registers after every tile, each addition there rounded to
 // nearest, and each CTA's sums go to a slot of their own.
 //
-// 640 threads, one CTA per SM: warp 0 issues the MMAs; warps 4-11 load R and X through registers (any
-// alignment; two warpgroups take turns, so one's loads are in flight while the other converts), warps 12-19
-// are the epilogue.
+// 640 threads, one CTA per SM: warp 0 issues the MMAs; warp 4 loads 16-bit R and X by TMA, or warps 4-11 load them through
+// registers (fp32, and rows of any alignment; two warpgroups take turns, so one's loads are in flight while the
+// other converts); warps 12-19 are the epilogue.
 constexpr int kMixTcThreads = 640;
 constexpr int kMixTcMax = 128;   // rows of A, of R and of X
-constexpr int kMixCtrlRegs = 48, kMixLoadRegs = 88, kMixEpiRegs = 128;   // 640 x 96 at launch = 128 x (48 + 2 x 88 + 2 x 128)
+constexpr int kMixCtrlRegs = 48, kMixLoadRegs = 104, kMixEpiRegs = 112;   // 640 x 96 at launch = 128 x (48 + 2 x 104 + 2 x 112)
 
 struct MixTcArgs {
   const float* c;
@@ -221,6 +221,7 @@ struct MixTcArgs {
   int M, K;
   int64_t P;
   int stages;
+  int tma;               // 16-bit rows loaded by TMA
   int* err;
 };
 
@@ -234,12 +235,21 @@ __device__ __forceinline__ uint64_t mix_desc_mn(uint32_t addr, uint32_t chunk) {
   return d;
 }
 
+// One elected lane of a converged warp issues.
 __device__ __forceinline__ void mix_mma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void mix_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
       : "memory");
 }
 
@@ -285,7 +295,9 @@ struct MixTc {
 };
 
 template <typename T, bool kDc>
-__global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_constant__ MixTcArgs p) {
+__global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_constant__ CUtensorMap tmR,
+                                                                       const __grid_constant__ CUtensorMap tmX,
+                                                                       const __grid_constant__ MixTcArgs p) {
   using L = MixTc<T>;
   constexpr bool kF32 = L::kF32;
   using H = std::conditional_t<kF32, __nv_bfloat16, T>;   // operand type
@@ -315,7 +327,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 8; ++s) {
-      mbar_init(&bar_full[s], 128);
+      mbar_init(&bar_full[s], p.tma ? 1 : 128);
       mbar_init(&bar_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -383,34 +395,38 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       const uint32_t fmt = kFp16 ? 0u : 1u;
       const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(kBN >> 3) << 17) | (8u << 24);
       const uint32_t idesc_dc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(rm >> 3) << 17) | (8u << 24);
-      int it = 0;
+      // the whole warp runs the loop and one lane issues; descriptors are made once (first stage, first plane, first step)
+      // and moved by their address fields, in units of 16 bytes: up to 72 MMAs of 32 cycles make a tile
+      const uint32_t a0 = smem_u32(smem_a), r0 = smem_u32(smem);
+      const uint64_t da0 = smem_desc_sw128(a0), db0 = mix_desc_mn(r0, kPR * rk * 128);
+      const uint64_t ra0 = smem_desc_sw128(r0), xb0 = smem_desc_sw128(r0 + tile_r);
+      const uint32_t plane_a = kc * rm * 8, plane_r = rk * 8, plane_x = rm * 8;
+      const uint32_t tm = __shfl_sync(kFull, tmem, 0);
+      const int ksteps = rk / 16;
+      int it = 0, s = 0, phase = 0;
       bool ok = true;
       for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++it) {
-        const int s = it % p.stages, buf = it & 1;
+        const int buf = it & 1;
         ok = it < 2 || mbar_wait(&bar_acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, p.err, kErrWaitAccEmpty);
-        ok = ok && mbar_wait(&bar_full[s], (it / p.stages) & 1, abort_flag, p.err, kErrWaitFull);
+        ok = ok && mbar_wait(&bar_full[s], phase, abort_flag, p.err, kErrWaitFull);
         ok = __all_sync(kFull, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t a0 = smem_u32(smem_a), r0 = smem_u32(smem + s * stage_bytes), x0 = r0 + tile_r;
-        const uint32_t d1 = tmem + buf * L::kD1;
-        if (lane == 0) {
-          for (int kk = 0; kk < rk / 16; ++kk) {
-            const uint32_t acc = kk ? 1u : 0u;
-            auto da = [&](int q) { return smem_desc_sw128(a0 + (q * kc + kk / 4) * rm * 128 + (kk & 3) * 32); };
-            auto db = [&](int q) { return mix_desc_mn(r0 + q * rk * 128 + kk * 2048, kPR * rk * 128); };
-            mix_mma(d1, da(0), db(0), idesc, acc);
-            if constexpr (kF32) {
-              const uint32_t cross = d1 + kBN;
-              mix_mma(cross, da(0), db(1), idesc, acc);
-              mix_mma(cross, da(1), db(0), idesc, 1u);
-              mix_mma(cross, da(1), db(1), idesc, 1u);
-              mix_mma(cross, da(0), db(2), idesc, 1u);
-              mix_mma(cross, da(2), db(0), idesc, 1u);
-            } else {
-              mix_mma(d1, da(1), db(0), idesc, 1u);
-              mix_mma(d1, da(2), db(0), idesc, 1u);
-            }
+        const uint32_t at = (uint32_t)(s * (stage_bytes / 16)), d1 = tm + buf * L::kD1;
+        for (int kk = 0; kk < ksteps; ++kk) {
+          const uint32_t acc = kk ? 1u : 0u;
+          const uint64_t da = da0 + (uint32_t)((kk >> 2) * rm * 8 + (kk & 3) * 2), db = db0 + at + kk * 128;
+          mix_mma(d1, da, db, idesc, acc);
+          if constexpr (kF32) {
+            const uint32_t cross = d1 + kBN;
+            mix_mma(cross, da, db + plane_r, idesc, acc);
+            mix_mma(cross, da + plane_a, db, idesc, 1u);
+            mix_mma(cross, da + plane_a, db + plane_r, idesc, 1u);
+            mix_mma(cross, da, db + 2 * plane_r, idesc, 1u);
+            mix_mma(cross, da + 2 * plane_a, db, idesc, 1u);
+          } else {
+            mix_mma(d1, da + plane_a, db, idesc, 1u);
+            mix_mma(d1, da + 2 * plane_a, db, idesc, 1u);
           }
         }
         if constexpr (kDc) {
@@ -418,50 +434,76 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
           ok = __all_sync(kFull, ok);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (lane == 0) {
-            for (int kk = 0; kk < kBN / 16; ++kk) {
-              const uint32_t acc = kk ? 1u : 0u;
-              auto da = [&](int q) {
-                return smem_desc_sw128(r0 + (kk / 4) * kPR * rk * 128 + q * rk * 128 + (kk & 3) * 32);
-              };
-              auto db = [&](int q) {
-                return smem_desc_sw128(x0 + (kk / 4) * kPR * rm * 128 + q * rm * 128 + (kk & 3) * 32);
-              };
-              mix_mma(dc_tmem, da(0), db(0), idesc_dc, acc);
-              if constexpr (kF32) {
-                const uint32_t cross = dc_tmem + 128;
-                mix_mma(cross, da(0), db(1), idesc_dc, acc);
-                mix_mma(cross, da(1), db(0), idesc_dc, 1u);
-                mix_mma(cross, da(1), db(1), idesc_dc, 1u);
-                mix_mma(cross, da(0), db(2), idesc_dc, 1u);
-                mix_mma(cross, da(2), db(0), idesc_dc, 1u);
-              }
+          const uint32_t dc = tm + 2 * L::kD1;
+#pragma unroll
+          for (int kk = 0; kk < kBN / 16; ++kk) {
+            const uint32_t acc = kk ? 1u : 0u;
+            const uint64_t da = ra0 + at + (uint32_t)((kk >> 2) * kPR * rk * 8 + (kk & 3) * 2);
+            const uint64_t db = xb0 + at + (uint32_t)((kk >> 2) * kPR * rm * 8 + (kk & 3) * 2);
+            mix_mma(dc, da, db, idesc_dc, acc);
+            if constexpr (kF32) {
+              const uint32_t cross = dc + 128;
+              mix_mma(cross, da, db + plane_x, idesc_dc, acc);
+              mix_mma(cross, da + plane_r, db, idesc_dc, 1u);
+              mix_mma(cross, da + plane_r, db + plane_x, idesc_dc, 1u);
+              mix_mma(cross, da, db + 2 * plane_x, idesc_dc, 1u);
+              mix_mma(cross, da + 2 * plane_r, db, idesc_dc, 1u);
             }
           }
         }
-        if (lane == 0) {
-          mma_commit(&bar_empty[s]);
-          mma_commit(&bar_acc_full[buf]);
+        mix_commit(&bar_empty[s]);
+        mix_commit(&bar_acc_full[buf]);
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1;
         }
-        __syncwarp();
       }
-      if (lane == 0) {
-        mma_commit(bar_done);
-        for (uint32_t i = 0; i < kWaitLimit && !mbar_try(bar_done, 0); ++i) {
-        }
+      __syncwarp();
+      mix_commit(bar_done);
+      for (uint32_t i = 0; i < kWaitLimit && !mbar_try(bar_done, 0); ++i) {
       }
       __syncwarp();
     }
   } else if (warp < 12) {
     // ---------------- loads: this warpgroup's tiles are every second one of the CTA's
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMixLoadRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMixLoadRegs));
     const int wg = (warp - 4) >> 2, t = threadIdx.x - 128 - wg * 128;
+    if (!kF32 && p.tma) {
+      // 16-bit matrices whose rows TMA can address: one warp, [64 columns x all rows] per load
+      if (warp == 4) {
+        int it = 0;
+        bool ok = true;
+        for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++it) {
+          const int s = it % p.stages;
+          ok = it < p.stages || mbar_wait(&bar_empty[s], ((it / p.stages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
+          ok = __all_sync(kFull, ok);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_expect_tx(&bar_full[s], stage_bytes);
+            uint8_t* st = smem + s * stage_bytes;
+#pragma unroll
+            for (int c = 0; c < L::kChunks; ++c) {
+              tma_load_2d(st + c * rk * 128, &tmR, (int)(tile * kBN) + c * 64, 0, &bar_full[s]);
+              if (kDc) tma_load_2d(st + tile_r + c * rm * 128, &tmX, (int)(tile * kBN) + c * 64, 0, &bar_full[s]);
+            }
+          }
+          __syncwarp();
+        }
+        if (*abort_flag && lane == 0) {
+          for (int j = it - 1; j >= 0 && j >= it - p.stages; --j) {
+            for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&bar_full[j % p.stages], (j / p.stages) & 1); ++i) {
+            }
+          }
+        }
+        __syncwarp();
+      }
+    } else {
     const T* R = static_cast<const T*>(p.R);
     const T* X = static_cast<const T*>(p.X);
     const bool vec = p.P % L::kUnit == 0;
     const int units = (rk + (kDc ? rm : 0)) / 8;     // 16-byte units of this thread: 16 per row, 8 rows per round
     const int u = t & 15, row0 = t >> 4;
-    constexpr int kBatch = 4;
+    constexpr int kBatch = 8;
     int it = wg;
     bool ok = true;
     for (int64_t tile = blockIdx.x + (int64_t)wg * gridDim.x; tile < tiles && ok; tile += 2 * (int64_t)gridDim.x, it += 2) {
@@ -528,6 +570,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&bar_full[s]);
+    }
     }
   } else {
     // ---------------- epilogue: TMEM lane quadrant q, half of the columns
@@ -721,8 +764,17 @@ cudaError_t run_tc(MixTcArgs p, cudaStream_t s) {
   p.stages = tc_stages<T>(p.K, p.M, kDc);
   const int m = p.M < kMixTcMax ? p.M : kMixTcMax;
   const int smem = MixTc<T>::kFixed + MixTc<T>::coeff_bytes(p.K, m) + p.stages * MixTc<T>::stage_bytes(p.K, m, kDc);
+  CUtensorMap mr{}, mx{};
+  p.tma = 0;
+  if constexpr (sizeof(T) == 2) {
+    const CUtensorMapDataType dt =
+        std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    p.tma = p.P % 8 == 0 && p.P < ((int64_t)1 << 31) - 256 &&
+            make_map_t(&mr, dt, p.R, p.K, p.P, p.P * 2, 64, ceil16(p.K), CU_TENSOR_MAP_SWIZZLE_128B) &&
+            (!kDc || make_map_t(&mx, dt, p.X, p.M, p.P, p.P * 2, 64, ceil16(m), CU_TENSOR_MAP_SWIZZLE_128B));
+  }
   kern<<<dim3((unsigned)tc_grid(p.P, MixTc<T>::kBN), (unsigned)((p.M + kMixTcMax - 1) / kMixTcMax)), kMixTcThreads, smem,
-         s>>>(p);
+         s>>>(mr, mx, p);
   return cudaGetLastError();
 }
 

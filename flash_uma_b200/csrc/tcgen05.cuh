@@ -107,5 +107,10 @@ bool make_map_t(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, i
 bool make_map_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, int64_t cols, int64_t rows,
                  int64_t mats, int64_t planes, int64_t row_bytes, int64_t mat_bytes, int64_t plane_bytes, int box_cols,
                  int box_rows, int box_planes, CUtensorMapSwizzle swz);
+// The same array of 16-bit values seen as (64 columns, rows, chunks of 64 columns, matrices, planes), cols a multiple of 64:
+// boxes of box_chunks chunks land chunk by chunk, each [box_rows][64] with a 128-byte swizzle.
+bool make_map_5d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, int64_t cols, int64_t rows,
+                 int64_t mats, int64_t planes, int64_t row_bytes, int64_t mat_bytes, int64_t plane_bytes, int box_rows,
+                 int box_chunks, int box_planes);
 
 }  // namespace fuma

@@ -57,29 +57,31 @@ def test_other_refusals(lib):
 
 
 def test_work_sizes(lib):
-    """The weight gradient's work space holds two slots per chunk bound of the rows; none for short batches."""
+    """The weight gradient's work space holds the parts of cut groups; none for short batches."""
     n = lib.fuma_grouped_wgrad_work_bytes
     assert n(0, 64, 64, 1) == 0 and n(2048, 64, 64, 1) == 0
-    assert n(2049, 64, 64, 1) >= 2 * 2 * 64 * 64 * 4
+    assert n(2049, 64, 64, 1) >= 2 * 64 * 64 * 4
     assert lib.fuma_grouped_bias_grad_work_bytes(1000, 64, 5) >= (2 + 5) * 64 * 4
     assert lib.fuma_mix_experts_work_bytes(3, 4, 1000, 0) >= 3 * 4 * 4
 
 
-def test_partial_slots_never_meet():
-    """The slot rule of the weight gradient's partial matrices, restated: over random group lengths no two
-    chunks share a slot and all stay inside the work space."""
+def test_part_slots_never_meet():
+    """The slot rule of the weight gradient's partial matrices, restated: over random group lengths no two parts share a
+    slot, all stay inside the work space, and the parts cover each group's blocks of 128 rows once."""
     g = torch.Generator().manual_seed(0)
-    chunk = 64
-    for _ in range(300):
-        lens = (torch.rand(12, generator=g) ** 3 * 400).long().tolist()
+    for trial in range(400):
+        cap = int(torch.randint(2, 30, (1,), generator=g))
+        lens = (torch.rand(12, generator=g) ** 3 * 128 * cap * 5).long().tolist()
         T, a, used = sum(lens), 0, set()
-        slots = T // chunk + 1
         for n in lens:
-            if n > chunk:
-                for c in range(-(-n // chunk)):
-                    s = a // chunk if c == 0 else slots + a // chunk + c
-                    assert s not in used and 0 <= s < 2 * slots
-                    assert c == 0 or s >= slots
+            blocks = -(-n // 128)
+            if blocks > cap:
+                parts = -(-blocks // cap)
+                each = -(-blocks // parts)
+                assert each <= cap
+                for c in range(parts):
+                    s = 2 * (a // 128) // cap + c
+                    assert s not in used and 0 <= s < 2 * (T // 128) // cap + 2
                     used.add(s)
             a += n
 
