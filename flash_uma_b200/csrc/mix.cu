@@ -200,13 +200,21 @@ __global__ void __launch_bounds__(256) mix_dcoeff_join_kernel(const float* __res
 //
 // 16-bit matrices: the coefficients are three planes of the matrices' type that add up to their 24 bits (fp16: each row
 // of A scaled by a power of two into fp16's range first, undone in the epilogue), so every product is
-// exact. fp32 matrices: three bf16 planes on both sides and the six products of grouped.cu, in a main and
-// a cross accumulator. dc leaves TMEM for fp32 registers after every tile, each addition there rounded to
-// nearest, and each CTA's sums go to a slot of their own.
+// exact. fp32: two fp16 planes on both sides, hi = fp16(x / s), lo = fp16(x / s - hi), and the products lo hi, hi lo,
+// hi hi: s is a power of two per row of A and per tile of R and of X (largest magnitude to [2^14, 2^15); 22 bits for values
+// down to 2^-18 of the tile's largest, 2^-40 of that below). Three bf16 planes need no scale, but six products, and the
+// MMAs (N = 64 takes 60 cycles) were then what the backward pass waited for: 312 us at 128 x 64 x 524,288.
+// dc leaves TMEM for fp32 registers after every tile (fp32, with the tiles' scales) or every 256 columns, each addition
+// there rounded to nearest, and each CTA's sums go to a slot of their own.
 //
-// 640 threads, one CTA per SM: warp 0 issues the MMAs; warp 4 loads 16-bit R and X by TMA, or warps 4-11 load them through
-// registers (fp32, and rows of any alignment; two warpgroups take turns, so one's loads are in flight while the
-// other converts); warps 12-19 are the epilogue.
+// A tile is a short piece of up to 256 rows that lie megabytes apart. Loads and stores of the threads' own ran at 1.7 TB/s on
+// it (8 warps, 256 bytes per row; a read of the same bytes), TMA at 6.5, so rows that TMA can address (16-byte multiples)
+// come and go by TMA.
+//
+// 640 threads, one CTA per SM: warp 0 issues the MMAs; warp 1 loads R and X by TMA: 16-bit values to where the MMAs read
+// them, fp32 to a raw buffer, from which warps 4-11 take a whole tile into registers (its largest magnitude has to be
+// known before it is split) and write the planes. Rows of any other length go through the registers of warps 4-11 (16 bits:
+// two warpgroups take turns). Warps 12-19 are the epilogue.
 constexpr int kMixTcThreads = 640;
 constexpr int kMixTcMax = 128;   // rows of A, of R and of X
 constexpr int kMixCtrlRegs = 48, kMixLoadRegs = 104, kMixEpiRegs = 112;   // 640 x 96 at launch = 128 x (48 + 2 x 104 + 2 x 112)
@@ -220,8 +228,8 @@ struct MixTcArgs {
   float* part;           // backward only: [gridDim.x][K][M]
   int M, K;
   int64_t P;
-  int stages;
-  int tma;               // 16-bit rows loaded by TMA
+  int stages;            // of operand tiles
+  int tma;               // rows that TMA can address (fp32: two raw buffers)
   int* err;
 };
 
@@ -265,17 +273,34 @@ __device__ __forceinline__ void mix_tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// x as three numbers of type H that add up to it: H(x), H(x - p0), H(x - p0 - p1). Not finite: p0 alone.
-template <typename H>
-__device__ __forceinline__ void three_planes(float x, H (&p)[3]) {
-  H h = from_f32<H>(x);
+__device__ __forceinline__ void mix_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// x as kN numbers of type H that add up to it: H(x), H(x - p0), ... Not finite: p0 alone.
+template <typename H, int kN>
+__device__ __forceinline__ void split_planes(float x, H (&p)[kN]) {
+  p[0] = from_f32<H>(x);
   if constexpr (__is_same(H, __nv_bfloat16))
-    if (__hisinf(h) && fabsf(x) <= 3.402823466e38f) h = __float2bfloat16_rz(x);
-  const float r1 = fabsf(x) <= 3.402823466e38f ? x - to_f32(h) : 0.0f;
-  const H m = from_f32<H>(r1);
-  p[0] = h;
-  p[1] = m;
-  p[2] = from_f32<H>(r1 - to_f32(m));
+    if (__hisinf(p[0]) && fabsf(x) <= 3.402823466e38f) p[0] = __float2bfloat16_rz(x);
+  float r = fabsf(x) <= 3.402823466e38f ? x - to_f32(p[0]) : 0.0f;
+#pragma unroll
+  for (int i = 1; i < kN; ++i) {
+    p[i] = from_f32<H>(r);
+    r -= to_f32(p[i]);
+  }
+}
+
+// The power of two that brings the largest magnitude (its bits) to [2^14, 2^15), and its inverse.
+__device__ __forceinline__ float2 fp16_scale(uint32_t amax_bits) {
+  int e = (int)(amax_bits >> 23) - 127 - 14;
+  if (e < -126) e = -126;
+  return make_float2(__uint_as_float((uint32_t)(127 + e) << 23), __uint_as_float((uint32_t)(127 - e) << 23));
 }
 
 __host__ __device__ inline int ceil16(int n) { return (n + 15) / 16 * 16; }
@@ -284,12 +309,13 @@ template <typename T>
 struct MixTc {
   static constexpr bool kF32 = sizeof(T) == 4;
   static constexpr int kBN = kF32 ? 64 : 128;          // columns per tile
-  static constexpr int kPlanesR = kF32 ? 3 : 1;
+  static constexpr int kPlanesR = kF32 ? 2 : 1;
+  static constexpr int kPlanesA = kF32 ? 2 : 3;
   static constexpr int kChunks = kBN / 64;
   static constexpr int kUnit = kF32 ? 4 : 8;           // values per 16 bytes of global memory
-  static constexpr int kD1 = kF32 ? 2 * kBN : kBN;     // TMEM columns of one out buffer (main + cross)
+  static constexpr int kDcTiles = kF32 ? 1 : 256 / kBN;   // tiles per drain of dc
   static int stage_bytes(int K, int M, bool dc) { return kPlanesR * kChunks * 128 * (ceil16(K) + (dc ? ceil16(M) : 0)); }
-  static int coeff_bytes(int K, int M) { return 3 * ((K + 63) / 64) * ceil16(M) * 128; }
+  static int coeff_bytes(int K, int M) { return kPlanesA * ((K + 63) / 64) * ceil16(M) * 128; }
   static constexpr int kStaging = 8 * 4096;
   static constexpr int kFixed = kStaging + 1024 /*barriers, row scales*/ + 1024 /*alignment*/;
 };
@@ -297,12 +323,13 @@ struct MixTc {
 template <typename T, bool kDc>
 __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_constant__ CUtensorMap tmR,
                                                                        const __grid_constant__ CUtensorMap tmX,
+                                                                       const __grid_constant__ CUtensorMap tmO,
                                                                        const __grid_constant__ MixTcArgs p) {
   using L = MixTc<T>;
   constexpr bool kF32 = L::kF32;
-  using H = std::conditional_t<kF32, __nv_bfloat16, T>;   // operand type
-  constexpr bool kFp16 = __is_same(T, __half);
-  constexpr int kBN = L::kBN, kPR = L::kPlanesR;
+  using H = std::conditional_t<kF32, __half, T>;          // operand type
+  constexpr bool kFp16 = __is_same(H, __half);
+  constexpr int kBN = L::kBN, kPR = L::kPlanesR, kPA = L::kPlanesA;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int m_first = blockIdx.y * kMixTcMax;             // forward: slices of 128 rows of A
@@ -312,30 +339,43 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
   const int stage_bytes = tile_r + tile_x;
   // [stages][A planes][staging][barriers]: the MMA reads 128 rows of a tile that holds fewer; what lies
   // behind is read too (rows of the result that nobody reads), and stays inside this block
+  const int raw_bytes = (rk + (kDc ? rm : 0)) * kBN * 4;   // fp32: one raw buffer
   uint8_t* smem_a = smem + p.stages * stage_bytes;
-  uint8_t* smem_c = smem_a + 3 * kc * rm * 128;
+  uint8_t* smem_c = smem_a + kPA * kc * rm * 128;
+  uint8_t* smem_raw_tile = smem_c + L::kStaging + 1024;    // behind the barriers
   uint64_t* bar_full = reinterpret_cast<uint64_t*>(smem_c + L::kStaging);
   uint64_t* bar_empty = bar_full + 8;
   uint64_t* bar_acc_full = bar_empty + 8;
   uint64_t* bar_acc_empty = bar_acc_full + 2;
   uint64_t* bar_dc_empty = bar_acc_empty + 2;
-  uint64_t* bar_done = bar_dc_empty + 1;
+  uint64_t* bar_dc_full = bar_dc_empty + 2;
+  uint64_t* bar_raw_full = bar_dc_full + 2;
+  uint64_t* bar_raw_empty = bar_raw_full + 2;
+  uint64_t* bar_done = bar_raw_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* row_scale = reinterpret_cast<float*>(tmem_slot + 2);   // [128]
+  float2* tile_scale = reinterpret_cast<float2*>(row_scale + 128);   // fp32: [8] of R and X, by tile
+  uint32_t* tile_max = reinterpret_cast<uint32_t*>(tile_scale + 8);  // fp32: [8][2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 8; ++s) {
-      mbar_init(&bar_full[s], p.tma ? 1 : 128);
+      mbar_init(&bar_full[s], kF32 ? 256 : p.tma ? 1 : 128);
       mbar_init(&bar_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bar_acc_full[b], 1);
       mbar_init(&bar_acc_empty[b], 256);
     }
-    mbar_init(bar_dc_empty, 256);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bar_dc_empty[b], 256);
+      mbar_init(&bar_dc_full[b], 1);
+      mbar_init(&bar_raw_full[b], 1);
+      mbar_init(&bar_raw_empty[b], 256);
+    }
     mbar_init(bar_done, 1);
+    for (int i = 0; i < 16; ++i) tile_max[i] = 0;
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -363,19 +403,18 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
-      int e = (int)(mx >> 23) - 127 - 14;
-      if (e < -126) e = -126;
-      inv = __uint_as_float((uint32_t)(127 - e) << 23);
-      if (lane == 0) row_scale[m] = __uint_as_float((uint32_t)(127 + e) << 23);
+      const float2 sc = fp16_scale(mx);
+      inv = sc.y;
+      if (lane == 0) row_scale[m] = sc.x;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int k = lane + 32 * j;
       if (k < kc * 64) {
-        H pl[3];
-        three_planes<H>(v[j] * inv, pl);
+        H pl[kPA];
+        split_planes<H, kPA>(v[j] * inv, pl);
 #pragma unroll
-        for (int q = 0; q < 3; ++q)
+        for (int q = 0; q < kPA; ++q)
           *reinterpret_cast<H*>(smem_a + (q * kc + k / 64) * rm * 128 + m * 128 + ((((k & 63) >> 3) ^ (m & 7)) << 4) +
                                 (k & 7) * 2) = pl[q];
       }
@@ -387,16 +426,16 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   const int64_t tiles = (p.P + kBN - 1) / kBN;
-  const uint32_t dc_tmem = tmem + 2 * L::kD1;   // dc: main at +0, cross at +128
+  const uint32_t dc_tmem = tmem + 2 * kBN;
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMixCtrlRegs));
     if (warp == 0) {
-      const uint32_t fmt = kFp16 ? 0u : 1u;
+      const uint32_t fmt = kFp16 ? 0u : 1u;   // fp16 or bf16
       const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(kBN >> 3) << 17) | (8u << 24);
       const uint32_t idesc_dc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(rm >> 3) << 17) | (8u << 24);
       // the whole warp runs the loop and one lane issues; descriptors are made once (first stage, first plane, first step)
-      // and moved by their address fields, in units of 16 bytes: up to 72 MMAs of 32 cycles make a tile
+      // and moved by their address fields, in units of 16 bytes: up to 40 short MMAs make a tile
       const uint32_t a0 = smem_u32(smem_a), r0 = smem_u32(smem);
       const uint64_t da0 = smem_desc_sw128(a0), db0 = mix_desc_mn(r0, kPR * rk * 128);
       const uint64_t ra0 = smem_desc_sw128(r0), xb0 = smem_desc_sw128(r0 + tile_r);
@@ -412,47 +451,46 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
         ok = __all_sync(kFull, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t at = (uint32_t)(s * (stage_bytes / 16)), d1 = tm + buf * L::kD1;
+        const uint32_t at = (uint32_t)(s * (stage_bytes / 16)), d1 = tm + buf * kBN;
         for (int kk = 0; kk < ksteps; ++kk) {
           const uint32_t acc = kk ? 1u : 0u;
           const uint64_t da = da0 + (uint32_t)((kk >> 2) * rm * 8 + (kk & 3) * 2), db = db0 + at + kk * 128;
-          mix_mma(d1, da, db, idesc, acc);
-          if constexpr (kF32) {
-            const uint32_t cross = d1 + kBN;
-            mix_mma(cross, da, db + plane_r, idesc, acc);
-            mix_mma(cross, da + plane_a, db, idesc, 1u);
-            mix_mma(cross, da + plane_a, db + plane_r, idesc, 1u);
-            mix_mma(cross, da, db + 2 * plane_r, idesc, 1u);
-            mix_mma(cross, da + 2 * plane_a, db, idesc, 1u);
+          if constexpr (kF32) {   // the small products first
+            mix_mma(d1, da + plane_a, db, idesc, acc);
+            mix_mma(d1, da, db + plane_r, idesc, 1u);
+            mix_mma(d1, da, db, idesc, 1u);
           } else {
+            mix_mma(d1, da, db, idesc, acc);
             mix_mma(d1, da + plane_a, db, idesc, 1u);
             mix_mma(d1, da + 2 * plane_a, db, idesc, 1u);
           }
         }
         if constexpr (kDc) {
-          ok = it < 1 || mbar_wait(bar_dc_empty, (it - 1) & 1, abort_flag, p.err, kErrWaitAccEmpty);
-          ok = __all_sync(kFull, ok);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t dc = tm + 2 * L::kD1;
+          const int dci = it % L::kDcTiles, dcn = it / L::kDcTiles;
+          if (dci == 0) {
+            ok = dcn < 2 || mbar_wait(&bar_dc_empty[dcn & 1], ((dcn >> 1) - 1) & 1, abort_flag, p.err, kErrWaitAccEmpty);
+            ok = __all_sync(kFull, ok);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+          const uint32_t dc = tm + 2 * kBN + (dcn & 1) * 128;
 #pragma unroll
           for (int kk = 0; kk < kBN / 16; ++kk) {
-            const uint32_t acc = kk ? 1u : 0u;
+            const uint32_t acc = kk || dci ? 1u : 0u;
             const uint64_t da = ra0 + at + (uint32_t)((kk >> 2) * kPR * rk * 8 + (kk & 3) * 2);
             const uint64_t db = xb0 + at + (uint32_t)((kk >> 2) * kPR * rm * 8 + (kk & 3) * 2);
-            mix_mma(dc, da, db, idesc_dc, acc);
             if constexpr (kF32) {
-              const uint32_t cross = dc + 128;
-              mix_mma(cross, da, db + plane_x, idesc_dc, acc);
-              mix_mma(cross, da + plane_r, db, idesc_dc, 1u);
-              mix_mma(cross, da + plane_r, db + plane_x, idesc_dc, 1u);
-              mix_mma(cross, da, db + 2 * plane_x, idesc_dc, 1u);
-              mix_mma(cross, da + 2 * plane_r, db, idesc_dc, 1u);
+              mix_mma(dc, da + plane_r, db, idesc_dc, acc);
+              mix_mma(dc, da, db + plane_x, idesc_dc, 1u);
+              mix_mma(dc, da, db, idesc_dc, 1u);
+            } else {
+              mix_mma(dc, da, db, idesc_dc, acc);
             }
           }
         }
         mix_commit(&bar_empty[s]);
         mix_commit(&bar_acc_full[buf]);
+        if (kDc && (it % L::kDcTiles == L::kDcTiles - 1 || tile + gridDim.x >= tiles)) mix_commit(&bar_dc_full[it / L::kDcTiles & 1]);
         if (++s == p.stages) {
           s = 0;
           phase ^= 1;
@@ -464,66 +502,153 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       }
       __syncwarp();
     }
-  } else if (warp < 12) {
-    // ---------------- loads: this warpgroup's tiles are every second one of the CTA's
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMixLoadRegs));
-    const int wg = (warp - 4) >> 2, t = threadIdx.x - 128 - wg * 128;
-    if (!kF32 && p.tma) {
-      // 16-bit matrices whose rows TMA can address: one warp, [64 columns x all rows] per load
-      if (warp == 4) {
-        int it = 0;
-        bool ok = true;
-        for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++it) {
-          const int s = it % p.stages;
-          ok = it < p.stages || mbar_wait(&bar_empty[s], ((it / p.stages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
-          ok = __all_sync(kFull, ok);
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_expect_tx(&bar_full[s], stage_bytes);
-            uint8_t* st = smem + s * stage_bytes;
+    if (warp == 1 && p.tma) {
+      // ---------------- TMA loads: [64 columns x all rows] each
+      uint64_t* full = kF32 ? bar_raw_full : bar_full;
+      uint64_t* empty = kF32 ? bar_raw_empty : bar_empty;
+      const int depth = kF32 ? 2 : p.stages, bytes = kF32 ? raw_bytes : stage_bytes;
+      uint8_t* base = kF32 ? smem_raw_tile : smem;
+      const int row_bytes = kF32 ? 256 : 128;
+      int it = 0;
+      bool ok = true;
+      for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++it) {
+        const int s = it % depth;
+        ok = it < depth || mbar_wait(&empty[s], ((it / depth) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
+        ok = __all_sync(kFull, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(&full[s], bytes);
+          uint8_t* st = base + s * bytes;
 #pragma unroll
-            for (int c = 0; c < L::kChunks; ++c) {
-              tma_load_2d(st + c * rk * 128, &tmR, (int)(tile * kBN) + c * 64, 0, &bar_full[s]);
-              if (kDc) tma_load_2d(st + tile_r + c * rm * 128, &tmX, (int)(tile * kBN) + c * 64, 0, &bar_full[s]);
-            }
-          }
-          __syncwarp();
-        }
-        if (*abort_flag && lane == 0) {
-          for (int j = it - 1; j >= 0 && j >= it - p.stages; --j) {
-            for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&bar_full[j % p.stages], (j / p.stages) & 1); ++i) {
-            }
+          for (int c = 0; c < L::kChunks; ++c) {
+            tma_load_2d(st + c * rk * row_bytes, &tmR, (int)(tile * kBN) + c * 64, 0, &full[s]);
+            if (kDc)
+              tma_load_2d(st + L::kChunks * rk * row_bytes + c * rm * row_bytes, &tmX, (int)(tile * kBN) + c * 64, 0, &full[s]);
           }
         }
         __syncwarp();
       }
-    } else {
+      if (*abort_flag && lane == 0) {
+        for (int j = it - 1; j >= 0 && j >= it - depth; --j) {
+          for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&full[j % depth], (j / depth) & 1); ++i) {
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp < 12) {
+    // ---------------- loads: this warpgroup's tiles are every second one of the CTA's
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMixLoadRegs));
+    const int wg = (warp - 4) >> 2, t = threadIdx.x - 128 - wg * 128;
     const T* R = static_cast<const T*>(p.R);
     const T* X = static_cast<const T*>(p.X);
-    const bool vec = p.P % L::kUnit == 0;
-    const int units = (rk + (kDc ? rm : 0)) / 8;     // 16-byte units of this thread: 16 per row, 8 rows per round
-    const int u = t & 15, row0 = t >> 4;
+    const int u = t & 15;                            // 16 units of 16 bytes per row of a tile
+    if constexpr (kF32) {
+      // both warpgroups, 16 rows of the tile a round
+      const int t2 = t + wg * 128, row0 = t2 >> 4;
+      const int rounds_r = rk / 16, rounds = rounds_r + (kDc ? rm / 16 : 0);
+      const int64_t step = 16 * p.P;
+      int it = 0;
+      for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
+        const int s = it % p.stages;
+        const int64_t col = tile * kBN + u * 4;
+        const float* src_r = R + row0 * p.P + col;
+        const float* src_x = X + row0 * p.P + col - rounds_r * step;
+        uint4 v[kDc ? 16 : 8];
+        uint32_t mr = 0, mx = 0;
+        if (p.tma) {
+          mbar_wait(&bar_raw_full[it & 1], (it >> 1) & 1, abort_flag, p.err, kErrWaitFull);   // (a failed one: see below)
+          const uint8_t* raw = smem_raw_tile + (it & 1) * raw_bytes + row0 * 256 + u * 16;
+#pragma unroll
+          for (int j = 0; j < (kDc ? 16 : 8); ++j)   // X's rows follow R's
+            v[j] = j < rounds ? *reinterpret_cast<const uint4*>(raw + j * 4096) : make_uint4(0u, 0u, 0u, 0u);
+          mbar_arrive(&bar_raw_empty[it & 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < (kDc ? 16 : 8); ++j) {
+            const bool is_x = kDc && j >= rounds_r;
+            const int row = row0 + (is_x ? j - rounds_r : j) * 16;
+            const float* src = (is_x ? src_x : src_r) + j * step;
+            v[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (j < rounds && row < (is_x ? M : K)) {
+              float h[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) h[i] = col + i < p.P ? src[i] : 0.0f;
+              memcpy(&v[j], h, 16);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < (kDc ? 16 : 8); ++j) {
+          uint32_t m = 0;
+          const uint32_t x[4] = {v[j].x & 0x7fffffffu, v[j].y & 0x7fffffffu, v[j].z & 0x7fffffffu, v[j].w & 0x7fffffffu};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m = max(m, x[i] < 0x7f800000u ? x[i] : 0u);
+          if (kDc && j >= rounds_r) mx = max(mx, m);
+          else mr = max(mr, m);
+        }
+        mr = __reduce_max_sync(kFull, mr);
+        if (kDc) mx = __reduce_max_sync(kFull, mx);
+        uint32_t* tm = tile_max + (it & 7) * 2;
+        if (lane == 0) {
+          atomicMax(tm, mr);
+          if (kDc) atomicMax(tm + 1, mx);
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float2 sr = fp16_scale(tm[0]), sx = fp16_scale(kDc ? tm[1] : 0u);
+        if (t2 == 0) {
+          tile_scale[it & 7] = make_float2(sr.x, sx.x);
+          // four tiles on: nobody is there before three more barriers, and everybody has left it
+          tile_max[((it + 4) & 7) * 2] = tile_max[((it + 4) & 7) * 2 + 1] = 0u;
+        }
+        // (no end of the loop after a failed wait: the other threads count on this one at the barrier above)
+        const bool ok = it < p.stages || mbar_wait(&bar_empty[s], ((it / p.stages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
+        uint8_t* dst = smem + s * stage_bytes + row0 * 128 + ((((u >> 1) ^ row0) & 7) << 4) + (u & 1) * 8;
+        if (ok) {
+#pragma unroll
+          for (int j = 0; j < (kDc ? 16 : 8); ++j) {
+            if (j >= rounds) break;
+            const bool is_x = kDc && j >= rounds_r;
+            const float inv = is_x ? sx.y : sr.y;
+            uint8_t* at = dst + (is_x ? tile_r + (j - rounds_r) * 2048 : j * 2048);
+            const float f[4] = {__uint_as_float(v[j].x) * inv, __uint_as_float(v[j].y) * inv, __uint_as_float(v[j].z) * inv,
+                                __uint_as_float(v[j].w) * inv};
+            const __half2 h01 = __floats2half2_rn(f[0], f[1]), h23 = __floats2half2_rn(f[2], f[3]);
+            const float2 g01 = __half22float2(h01), g23 = __half22float2(h23);
+            // a value that is not finite: lo = 0 (x - hi would be NaN either way; the result is not finite)
+            const __half2 l01 = __floats2half2_rn(fabsf(f[0]) <= 65504.0f ? f[0] - g01.x : 0.0f,
+                                                  fabsf(f[1]) <= 65504.0f ? f[1] - g01.y : 0.0f);
+            const __half2 l23 = __floats2half2_rn(fabsf(f[2]) <= 65504.0f ? f[2] - g23.x : 0.0f,
+                                                  fabsf(f[3]) <= 65504.0f ? f[3] - g23.y : 0.0f);
+            *reinterpret_cast<uint2*>(at) = make_uint2(h2_bits(h01), h2_bits(h23));
+            *reinterpret_cast<uint2*>(at + (is_x ? rm : rk) * 128) = make_uint2(h2_bits(l01), h2_bits(l23));
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&bar_full[s]);
+      }
+    } else if (!p.tma) {
+    const int rounds_r = rk / 8, rounds = rounds_r + (kDc ? rm / 8 : 0);   // 8 rows a round, 16 units of 16 bytes per row
+    const int row0 = t >> 4;
+    const int64_t step = 8 * p.P;
     constexpr int kBatch = 8;
     int it = wg;
     bool ok = true;
     for (int64_t tile = blockIdx.x + (int64_t)wg * gridDim.x; tile < tiles && ok; tile += 2 * (int64_t)gridDim.x, it += 2) {
       const int s = it % p.stages;
       const int64_t col = tile * kBN + u * L::kUnit;
-      uint8_t* st = smem + s * stage_bytes;
+      const T* src_r = R + row0 * p.P + col;
+      const T* src_x = X + row0 * p.P + col - rounds_r * step;
       uint4 v[2][kBatch];
       auto fetch = [&](int j0, uint4 (&d)[kBatch]) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-          const int row = row0 + (j0 + b) * 8;
+          const int j = j0 + b;
+          const bool is_x = kDc && j >= rounds_r;
+          const int row = row0 + (is_x ? j - rounds_r : j) * 8;
+          const T* src = (is_x ? src_x : src_r) + j * step;
           d[b] = make_uint4(0u, 0u, 0u, 0u);
-          if (j0 + b >= units) continue;
-          const bool is_x = kDc && row >= rk;
-          const int r = is_x ? row - rk : row;
-          if (r >= (is_x ? M : K)) continue;
-          const T* src = (is_x ? X : R) + (int64_t)r * p.P + col;
-          if (vec) {
-            if (col < p.P) d[b] = __ldcs(reinterpret_cast<const uint4*>(src));
-          } else {
+          if (j < rounds && row < (is_x ? M : K)) {
             T h[L::kUnit];
 #pragma unroll
             for (int i = 0; i < L::kUnit; ++i) h[i] = col + i < p.P ? src[i] : from_f32<T>(0.0f);
@@ -534,36 +659,23 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       fetch(0, v[0]);
       if (it >= p.stages) ok = mbar_wait(&bar_empty[s], ((it / p.stages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
       if (!ok) break;
+      // this thread's 16 bytes in row row0 of a tile; rows 8 further on are 1024 bytes on and
+      // have the same swizzle
+      uint8_t* dst = smem + s * stage_bytes + row0 * 128 + (((u ^ row0) & 7) << 4);
 #pragma unroll 1
-      for (int j0 = 0; j0 < units; j0 += 2 * kBatch) {
+      for (int j0 = 0; j0 < rounds; j0 += 2 * kBatch) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int j = j0 + half * kBatch;
-          if (j < units) {
-            if (j + kBatch < units) fetch(j + kBatch, v[half ^ 1]);
+          if (j < rounds) {
+            if (j + kBatch < rounds) fetch(j + kBatch, v[half ^ 1]);
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-              const int row = row0 + (j + b) * 8;
-              if (j + b >= units) continue;
-              const bool is_x = kDc && row >= rk;
-              const int r = is_x ? row - rk : row, rows = is_x ? rm : rk;
-              uint8_t* base = st + (is_x ? tile_r : 0) + r * 128;
-              if constexpr (kF32) {
-                const float f[4] = {__uint_as_float(v[half][b].x), __uint_as_float(v[half][b].y),
-                                    __uint_as_float(v[half][b].z), __uint_as_float(v[half][b].w)};
-                H pl[4][3];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) three_planes<H>(f[i], pl[i]);
-#pragma unroll
-                for (int q = 0; q < 3; ++q) {
-                  const H h[4] = {pl[0][q], pl[1][q], pl[2][q], pl[3][q]};
-                  uint2 w;
-                  memcpy(&w, h, 8);
-                  *reinterpret_cast<uint2*>(base + q * rows * 128 + (((u >> 1) ^ (r & 7)) << 4) + (u & 1) * 8) = w;
-                }
-              } else {
-                *reinterpret_cast<uint4*>(base + (u >> 3) * rows * 128 + (((u & 7) ^ (r & 7)) << 4)) = v[half][b];
-              }
+              if (j + b >= rounds) break;
+              const bool is_x = kDc && j + b >= rounds_r;
+              const int plane = (is_x ? rm : rk) * 128;
+              uint8_t* at = dst + (is_x ? tile_r + (j + b - rounds_r) * 1024 : (j + b) * 1024);
+              *reinterpret_cast<uint4*>(at + (u >> 3) * plane) = v[half][b];
             }
           }
         }
@@ -578,7 +690,6 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
     const int q = warp & 3, half = (warp - 12) >> 2;
     uint8_t* stage = smem_c + (warp - 12) * 4096;
     T* out = static_cast<T*>(p.out);
-    const bool vec = p.P % L::kUnit == 0;
     constexpr int kHalfCols = kBN / 2;                   // 32 fp32 or 64 16-bit values: 128 bytes per row
     const int dc_half = (rm + 63) / 64 * 32;             // dc columns of this warp: [half * dc_half, + dc_half), at most 64
     float acc[kDc ? 64 : 1];
@@ -593,45 +704,54 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t lanes = (uint32_t)(q * 32) << 16;
-      if constexpr (kDc) {
+      const float2 ts = kF32 ? tile_scale[it & 7] : make_float2(1.0f, 1.0f);   // the ring is longer than anyone is ahead
+      auto drain_dc = [&]() {   // TMEM's sum of the last tiles to registers, rounded to nearest
+        const int dcn = it / L::kDcTiles;
+        bool full = mbar_wait(&bar_dc_full[dcn & 1], (dcn >> 1) & 1, abort_flag, p.err, kErrWaitAcc);
+        full = __all_sync(kFull, full && !*abort_flag);
+        if (!full) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // (powers of two; their product may leave the fp32 range where the result does not)
+        const int e = (int)(__float_as_uint(ts.x) >> 23) + (int)(__float_as_uint(ts.y) >> 23) - 254, eh = e >> 1;
+        const float s1 = __uint_as_float((uint32_t)(eh + 127) << 23), s2 = __uint_as_float((uint32_t)(e - eh + 127) << 23);
         if (q * 32 < K) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (c * 32 < dc_half && half * dc_half + c * 32 < M) {
-              uint32_t r[32];
-              mix_tmem_ld32(dc_tmem + half * dc_half + c * 32 + lanes, r);
+          for (int c = 0; c < 4; ++c) {
+            if (c * 16 < dc_half && half * dc_half + c * 16 < M) {
+              uint32_t r[16];
+              mix_tmem_ld16(dc_tmem + (dcn & 1) * 128 + half * dc_half + c * 16 + lanes, r);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) acc[c * 32 + i] += __uint_as_float(r[i]);
-              if constexpr (kF32) {
-                mix_tmem_ld32(dc_tmem + 128 + half * dc_half + c * 32 + lanes, r);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) acc[c * 32 + i] += __uint_as_float(r[i]);
+              for (int i = 0; i < 16; ++i) {
+                if constexpr (kF32) acc[c * 16 + i] = fmaf(__uint_as_float(r[i]) * s1, s2, acc[c * 16 + i]);
+                else acc[c * 16 + i] += __uint_as_float(r[i]);
               }
             }
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        mbar_arrive(bar_dc_empty);
-      }
+        mbar_arrive(&bar_dc_empty[dcn & 1]);
+        return true;
+      };
       if (q * 32 < M) {
-        const uint32_t d1 = tmem + buf * L::kD1 + half * kHalfCols + lanes;
+        const uint32_t d1 = tmem + buf * kBN + half * kHalfCols + lanes;
         const int rows = min(32, M - q * 32);
+        if (p.tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < kHalfCols / 32; ++c) {
-          uint32_t r[32];
-          mix_tmem_ld32(d1 + c * 32, r);
           if constexpr (kF32) {
-            uint32_t x[32];
-            mix_tmem_ld32(d1 + kBN + c * 32, x);
+            uint32_t r[32];
+            mix_tmem_ld32(d1, r);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                  make_float4(__uint_as_float(r[4 * j]) + __uint_as_float(x[4 * j]),
-                              __uint_as_float(r[4 * j + 1]) + __uint_as_float(x[4 * j + 1]),
-                              __uint_as_float(r[4 * j + 2]) + __uint_as_float(x[4 * j + 2]),
-                              __uint_as_float(r[4 * j + 3]) + __uint_as_float(x[4 * j + 3]));
+            for (int j = 0; j < 8; ++j) {
+              float o[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(r[4 * j + i]) * scale * ts.x;
+              *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(o[0], o[1], o[2], o[3]);
+            }
           } else {
+            uint32_t r[32];
+            mix_tmem_ld32(d1 + c * 32, r);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               T h[8];
@@ -648,16 +768,15 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
         __syncwarp();
         const int64_t c0 = tile * kBN + half * kHalfCols;
         T* o = out + (int64_t)(m_first + q * 32) * p.P + c0;
-        if (vec) {
-          const int rr = lane >> 3, j = lane & 7;
-          if (c0 + j * L::kUnit < p.P) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = i * 4 + rr;
-              if (r < rows)
-                __stcs(reinterpret_cast<uint4*>(o + r * p.P + j * L::kUnit),
-                       *reinterpret_cast<const uint4*>(stage + r * 128 + ((j ^ (r & 7)) << 4)));
-            }
+        if (p.tma) {   // rows behind the last and columns behind P are clipped
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                             reinterpret_cast<uint64_t>(&tmO)),
+                         "r"((int)c0), "r"(m_first + q * 32), "r"(smem_u32(stage))
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else {
           for (int r = 0; r < rows; ++r)
@@ -671,7 +790,12 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         mbar_arrive(&bar_acc_empty[buf]);
       }
+      if constexpr (kDc) {
+        if ((it % L::kDcTiles == L::kDcTiles - 1 || tile + gridDim.x >= tiles) && !drain_dc()) break;
+      }
     }
+    if (p.tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the staging area outlives its reads
+    __syncwarp();
     if constexpr (kDc) {
       const int s = q * 32 + lane;   // dc row; its columns are the experts (rows of X)
       if (s < K) {
@@ -735,10 +859,13 @@ cudaError_t run_dcoeff(const void* dW, const void* X, int S, int E, int64_t P, f
 
 constexpr int kSmemLimit = 227 * 1024;
 
+// Operand stages that fit beside the coefficients, the staging area and, in fp32, two raw tiles.
 template <typename T>
-int tc_stages(int K, int M, bool dc) {
-  const int room = kSmemLimit - MixTc<T>::kFixed - MixTc<T>::coeff_bytes(K, M < kMixTcMax ? M : kMixTcMax);
-  const int n = room / MixTc<T>::stage_bytes(K, M < kMixTcMax ? M : kMixTcMax, dc);
+int tc_stages(int K, int M, bool dc, bool raw) {
+  const int m = M < kMixTcMax ? M : kMixTcMax;
+  const int tile = MixTc<T>::stage_bytes(K, m, dc);
+  const int raw_bytes = raw && sizeof(T) == 4 ? 2 * (tile / MixTc<T>::kPlanesR / 2 * 4) : 0;
+  const int n = (kSmemLimit - MixTc<T>::kFixed - MixTc<T>::coeff_bytes(K, m) - raw_bytes) / tile;
   return n < 4 ? n : 4;
 }
 
@@ -761,26 +888,30 @@ cudaError_t run_tc(MixTcArgs p, cudaStream_t s) {
     if (st != cudaSuccess) return st;
     configured |= uint64_t(1) << (dev & 63);
   }
-  p.stages = tc_stages<T>(p.K, p.M, kDc);
   const int m = p.M < kMixTcMax ? p.M : kMixTcMax;
-  const int smem = MixTc<T>::kFixed + MixTc<T>::coeff_bytes(p.K, m) + p.stages * MixTc<T>::stage_bytes(p.K, m, kDc);
-  CUtensorMap mr{}, mx{};
-  p.tma = 0;
-  if constexpr (sizeof(T) == 2) {
-    const CUtensorMapDataType dt =
-        std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    p.tma = p.P % 8 == 0 && p.P < ((int64_t)1 << 31) - 256 &&
-            make_map_t(&mr, dt, p.R, p.K, p.P, p.P * 2, 64, ceil16(p.K), CU_TENSOR_MAP_SWIZZLE_128B) &&
-            (!kDc || make_map_t(&mx, dt, p.X, p.M, p.P, p.P * 2, 64, ceil16(m), CU_TENSOR_MAP_SWIZZLE_128B));
-  }
+  constexpr bool kF32 = sizeof(T) == 4;
+  CUtensorMap mr{}, mx{}, mo{};
+  const CUtensorMapDataType dt = kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                             : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapSwizzle sw = kF32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+  const int64_t pitch = p.P * (int64_t)sizeof(T);
+  p.tma = pitch % 16 == 0 && p.P < ((int64_t)1 << 31) - 256 && tc_stages<T>(p.K, p.M, kDc, true) >= 1 &&
+          make_map_t(&mr, dt, p.R, p.K, p.P, pitch, 64, ceil16(p.K), sw) &&
+          (!kDc || make_map_t(&mx, dt, p.X, p.M, p.P, pitch, 64, ceil16(m), sw)) &&
+          make_map_t(&mo, dt, p.out, p.M, p.P, pitch, 128 / sizeof(T), 32, CU_TENSOR_MAP_SWIZZLE_128B);
+  p.stages = tc_stages<T>(p.K, p.M, kDc, p.tma);
+  const int tile = MixTc<T>::stage_bytes(p.K, m, kDc);
+  const int smem = MixTc<T>::kFixed + MixTc<T>::coeff_bytes(p.K, m) + p.stages * tile +
+                   (kF32 && p.tma ? 2 * (tile / MixTc<T>::kPlanesR / 2 * 4) : 0);
   kern<<<dim3((unsigned)tc_grid(p.P, MixTc<T>::kBN), (unsigned)((p.M + kMixTcMax - 1) / kMixTcMax)), kMixTcThreads, smem,
-         s>>>(mr, mx, p);
+         s>>>(mr, mx, mo, p);
   return cudaGetLastError();
 }
 
 template <typename T>
 bool tc_fits(int K, int M, bool dc) {
-  return K <= kMixTcMax && (!dc || M <= kMixTcMax) && tc_stages<T>(K, M, dc) >= 1;
+  return K <= kMixTcMax && (!dc || M <= kMixTcMax) && tc_stages<T>(K, M, dc, false) >= 1;
 }
 
 template <typename T>
