@@ -1206,7 +1206,7 @@ int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed
   p.span = (p.G + kCoarse - 1) / kCoarse;
   p.mma_format = (!fp8 && !split && o.dtype == kDtypeBf16) ? 1u : 0u;
   const int64_t pair_items = (p.T / (2 * kBM) + groups) * p.tiles_n;
-  const char* pe = getenv("FUMA_PAIR"); const bool pair = (pe ? atoi(pe) != 0 : !fp8) && p.bn > 128 && use_pair(p.T, p.G, pair_items);
+  const bool pair = !fp8 && p.bn > 128 && use_pair(p.T, p.G, pair_items);
   p.box_b = pair ? p.bn / 2 : p.bn;   // columns of the tile in this CTA: rows of W per load (forward)
   p.wide_b = transposed && p.N % (pair ? 128 : 64) == 0 && p.box_b % 64 == 0;
   p.wide_a = 0;

@@ -212,12 +212,12 @@ __global__ void __launch_bounds__(256) mix_dcoeff_join_kernel(const float* __res
 // come and go by TMA.
 //
 // 640 threads, one CTA per SM: warp 0 issues the MMAs; warp 1 loads R and X by TMA: 16-bit values to where the MMAs read
-// them, fp32 to a raw buffer, from which warps 4-11 take a whole tile into registers (its largest magnitude has to be
-// known before it is split) and write the planes. Rows of any other length go through the registers of warps 4-11 (16 bits:
+// them, fp32 to a raw buffer, from which warps 4-11 write the planes (in a second pass: the tile's largest magnitude has to be
+// known first). Rows of any other length go through the registers of warps 4-11 (16 bits:
 // two warpgroups take turns). Warps 12-19 are the epilogue.
 constexpr int kMixTcThreads = 640;
 constexpr int kMixTcMax = 128;   // rows of A, of R and of X
-constexpr int kMixCtrlRegs = 48, kMixLoadRegs = 104, kMixEpiRegs = 112;   // 640 x 96 at launch = 128 x (48 + 2 x 104 + 2 x 112)
+constexpr int kMixCtrlRegs = 48, kMixLoadRegs = 88, kMixEpiRegs = 128;   // 640 x 96 at launch = 128 x (48 + 2 x 88 + 2 x 128)
 
 struct MixTcArgs {
   const float* c;
@@ -229,7 +229,7 @@ struct MixTcArgs {
   int M, K;
   int64_t P;
   int stages;            // of operand tiles
-  int tma;               // rows that TMA can address (fp32: two raw buffers)
+  int tma;               // rows that TMA can address: 1, in fp32 the number of raw buffers (1 to 4); else 0
   int* err;
 };
 
@@ -317,7 +317,7 @@ struct MixTc {
   static int stage_bytes(int K, int M, bool dc) { return kPlanesR * kChunks * 128 * (ceil16(K) + (dc ? ceil16(M) : 0)); }
   static int coeff_bytes(int K, int M) { return kPlanesA * ((K + 63) / 64) * ceil16(M) * 128; }
   static constexpr int kStaging = 8 * 4096;
-  static constexpr int kFixed = kStaging + 1024 /*barriers, row scales*/ + 1024 /*alignment*/;
+  static constexpr int kFixed = kStaging + 1024 /*barriers, scales*/ + 1024 /*alignment*/;
 };
 
 template <typename T, bool kDc>
@@ -350,18 +350,18 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
   uint64_t* bar_dc_empty = bar_acc_empty + 2;
   uint64_t* bar_dc_full = bar_dc_empty + 2;
   uint64_t* bar_raw_full = bar_dc_full + 2;
-  uint64_t* bar_raw_empty = bar_raw_full + 2;
-  uint64_t* bar_done = bar_raw_empty + 2;
+  uint64_t* bar_raw_empty = bar_raw_full + 4;
+  uint64_t* bar_done = bar_raw_empty + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* row_scale = reinterpret_cast<float*>(tmem_slot + 2);   // [128]
   float2* tile_scale = reinterpret_cast<float2*>(row_scale + 128);   // fp32: [8] of R and X, by tile
-  uint32_t* tile_max = reinterpret_cast<uint32_t*>(tile_scale + 8);  // fp32: [8][2]
+  uint32_t* tile_max = reinterpret_cast<uint32_t*>(tile_scale + 8);  // fp32: [8][4]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 8; ++s) {
-      mbar_init(&bar_full[s], kF32 ? 256 : p.tma ? 1 : 128);
+      mbar_init(&bar_full[s], !kF32 && p.tma ? 1 : 128);
       mbar_init(&bar_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -371,11 +371,14 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bar_dc_empty[b], 256);
       mbar_init(&bar_dc_full[b], 1);
+
+    }
+    for (int b = 0; b < 4; ++b) {
       mbar_init(&bar_raw_full[b], 1);
-      mbar_init(&bar_raw_empty[b], 256);
+      mbar_init(&bar_raw_empty[b], 128);
     }
     mbar_init(bar_done, 1);
-    for (int i = 0; i < 16; ++i) tile_max[i] = 0;
+    for (int i = 0; i < 32; ++i) tile_max[i] = 0;
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       // ---------------- TMA loads: [64 columns x all rows] each
       uint64_t* full = kF32 ? bar_raw_full : bar_full;
       uint64_t* empty = kF32 ? bar_raw_empty : bar_empty;
-      const int depth = kF32 ? 2 : p.stages, bytes = kF32 ? raw_bytes : stage_bytes;
+      const int depth = kF32 ? p.tma : p.stages, bytes = kF32 ? raw_bytes : stage_bytes;
       uint8_t* base = kF32 ? smem_raw_tile : smem;
       const int row_bytes = kF32 ? 256 : 128;
       int it = 0;
@@ -538,100 +541,100 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
     }
   } else if (warp < 12) {
     // ---------------- loads: this warpgroup's tiles are every second one of the CTA's
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMixLoadRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMixLoadRegs));
     const int wg = (warp - 4) >> 2, t = threadIdx.x - 128 - wg * 128;
     const T* R = static_cast<const T*>(p.R);
     const T* X = static_cast<const T*>(p.X);
     const int u = t & 15;                            // 16 units of 16 bytes per row of a tile
     if constexpr (kF32) {
-      // both warpgroups, 16 rows of the tile a round
-      const int t2 = t + wg * 128, row0 = t2 >> 4;
-      const int rounds_r = rk / 16, rounds = rounds_r + (kDc ? rm / 16 : 0);
-      const int64_t step = 16 * p.P;
-      int it = 0;
-      for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
-        const int s = it % p.stages;
+      // the warpgroups take turns; a warpgroup goes twice over its tile, 8 rows a round: its largest magnitude, then the planes
+      const int row0 = t >> 4;
+      const int rounds_r = rk / 8, rounds = rounds_r + (kDc ? rm / 8 : 0);
+      int it = wg;
+      for (int64_t tile = blockIdx.x + (int64_t)wg * gridDim.x; tile < tiles; tile += 2 * (int64_t)gridDim.x, it += 2) {
+        const int s = it % p.stages, rb = p.tma ? it % p.tma : 0;
         const int64_t col = tile * kBN + u * 4;
-        const float* src_r = R + row0 * p.P + col;
-        const float* src_x = X + row0 * p.P + col - rounds_r * step;
-        uint4 v[kDc ? 16 : 8];
-        uint32_t mr = 0, mx = 0;
-        if (p.tma) {
-          mbar_wait(&bar_raw_full[it & 1], (it >> 1) & 1, abort_flag, p.err, kErrWaitFull);   // (a failed one: see below)
-          const uint8_t* raw = smem_raw_tile + (it & 1) * raw_bytes + row0 * 256 + u * 16;
+        const uint8_t* raw = smem_raw_tile + rb * raw_bytes + row0 * 256 + u * 16;
+        auto value = [&](int j) {   // this thread's 4 columns in row row0 + 8 j of the tile; X's rows follow R's
+          if (p.tma) return *reinterpret_cast<const uint4*>(raw + j * 2048);
+          const bool is_x = kDc && j >= rounds_r;
+          const int row = row0 + (is_x ? j - rounds_r : j) * 8;
+          const float* src = (is_x ? X : R) + (int64_t)row * p.P + col;
+          float h[4];
 #pragma unroll
-          for (int j = 0; j < (kDc ? 16 : 8); ++j)   // X's rows follow R's
-            v[j] = j < rounds ? *reinterpret_cast<const uint4*>(raw + j * 4096) : make_uint4(0u, 0u, 0u, 0u);
-          mbar_arrive(&bar_raw_empty[it & 1]);
-        } else {
+          for (int i = 0; i < 4; ++i) h[i] = row < (is_x ? M : K) && col + i < p.P ? src[i] : 0.0f;
+          uint4 w;
+          memcpy(&w, h, 16);
+          return w;
+        };
+        // (no end of the loop after a failed wait: the other threads count on this one at the barriers below)
+        if (p.tma) mbar_wait(&bar_raw_full[rb], (it / p.tma) & 1, abort_flag, p.err, kErrWaitFull);
+        // the tile's largest magnitudes, as bits: of R's rows and of X's. `all`: with values that are not finite, which is
+        // what tells that there are any; a second round then leaves them out
+        uint32_t* tm = tile_max + (it & 7) * 4;
+        auto largest = [&](bool all, uint32_t* out) {
+          uint32_t m2[2] = {0, 0};
 #pragma unroll
-          for (int j = 0; j < (kDc ? 16 : 8); ++j) {
-            const bool is_x = kDc && j >= rounds_r;
-            const int row = row0 + (is_x ? j - rounds_r : j) * 16;
-            const float* src = (is_x ? src_x : src_r) + j * step;
-            v[j] = make_uint4(0u, 0u, 0u, 0u);
-            if (j < rounds && row < (is_x ? M : K)) {
-              float h[4];
+          for (int h = 0; h < (kDc ? 2 : 1); ++h) {
+            uint32_t m = 0;
+#pragma unroll 4
+            for (int j = h ? rounds_r : 0; j < (h ? rounds : rounds_r); ++j) {
+              const uint4 w = value(j);
+              uint32_t x[4] = {w.x & 0x7fffffffu, w.y & 0x7fffffffu, w.z & 0x7fffffffu, w.w & 0x7fffffffu};
+              if (!all)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) h[i] = col + i < p.P ? src[i] : 0.0f;
-              memcpy(&v[j], h, 16);
+                for (int i = 0; i < 4; ++i) x[i] = x[i] < 0x7f800000u ? x[i] : 0u;
+              m = __vimax3_u32(m, x[0], __vimax3_u32(x[1], x[2], x[3]));
             }
+            m2[h] = __reduce_max_sync(kFull, m);
+            if (lane == 0) atomicMax(out + h, m2[h]);
           }
-        }
-#pragma unroll
-        for (int j = 0; j < (kDc ? 16 : 8); ++j) {
-          uint32_t m = 0;
-          const uint32_t x[4] = {v[j].x & 0x7fffffffu, v[j].y & 0x7fffffffu, v[j].z & 0x7fffffffu, v[j].w & 0x7fffffffu};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m = max(m, x[i] < 0x7f800000u ? x[i] : 0u);
-          if (kDc && j >= rounds_r) mx = max(mx, m);
-          else mr = max(mr, m);
-        }
-        mr = __reduce_max_sync(kFull, mr);
-        if (kDc) mx = __reduce_max_sync(kFull, mx);
-        uint32_t* tm = tile_max + (it & 7) * 2;
-        if (lane == 0) {
-          atomicMax(tm, mr);
-          if (kDc) atomicMax(tm + 1, mx);
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float2 sr = fp16_scale(tm[0]), sx = fp16_scale(kDc ? tm[1] : 0u);
-        if (t2 == 0) {
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+          return make_uint2(out[0], kDc ? out[1] : 0u);
+        };
+        uint2 big = largest(true, tm);
+        const bool odd = big.x >= 0x7f800000u || big.y >= 0x7f800000u;   // the same in all 128 threads
+        if (odd) big = largest(false, tm + 2);
+        const float2 sr = fp16_scale(big.x), sx = fp16_scale(big.y);
+        if (t == 0) {
           tile_scale[it & 7] = make_float2(sr.x, sx.x);
-          // four tiles on: nobody is there before three more barriers, and everybody has left it
-          tile_max[((it + 4) & 7) * 2] = tile_max[((it + 4) & 7) * 2 + 1] = 0u;
+          // four tiles on: this warpgroup's too, nobody is there before another barrier, and everybody has left it
+          *reinterpret_cast<uint4*>(tile_max + ((it + 4) & 7) * 4) = make_uint4(0u, 0u, 0u, 0u);
         }
-        // (no end of the loop after a failed wait: the other threads count on this one at the barrier above)
         const bool ok = it < p.stages || mbar_wait(&bar_empty[s], ((it / p.stages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
         uint8_t* dst = smem + s * stage_bytes + row0 * 128 + ((((u >> 1) ^ row0) & 7) << 4) + (u & 1) * 8;
         if (ok) {
 #pragma unroll
-          for (int j = 0; j < (kDc ? 16 : 8); ++j) {
-            if (j >= rounds) break;
-            const bool is_x = kDc && j >= rounds_r;
-            const float inv = is_x ? sx.y : sr.y;
-            uint8_t* at = dst + (is_x ? tile_r + (j - rounds_r) * 2048 : j * 2048);
-            const float f[4] = {__uint_as_float(v[j].x) * inv, __uint_as_float(v[j].y) * inv, __uint_as_float(v[j].z) * inv,
-                                __uint_as_float(v[j].w) * inv};
-            const __half2 h01 = __floats2half2_rn(f[0], f[1]), h23 = __floats2half2_rn(f[2], f[3]);
-            const float2 g01 = __half22float2(h01), g23 = __half22float2(h23);
-            // a value that is not finite: lo = 0 (x - hi would be NaN either way; the result is not finite)
-            const __half2 l01 = __floats2half2_rn(fabsf(f[0]) <= 65504.0f ? f[0] - g01.x : 0.0f,
-                                                  fabsf(f[1]) <= 65504.0f ? f[1] - g01.y : 0.0f);
-            const __half2 l23 = __floats2half2_rn(fabsf(f[2]) <= 65504.0f ? f[2] - g23.x : 0.0f,
-                                                  fabsf(f[3]) <= 65504.0f ? f[3] - g23.y : 0.0f);
-            *reinterpret_cast<uint2*>(at) = make_uint2(h2_bits(h01), h2_bits(h23));
-            *reinterpret_cast<uint2*>(at + (is_x ? rm : rk) * 128) = make_uint2(h2_bits(l01), h2_bits(l23));
+          for (int h = 0; h < (kDc ? 2 : 1); ++h) {
+            const float inv = h ? sx.y : sr.y;
+            const int plane = (h ? rm : rk) * 128;
+            uint8_t* at = dst + (h ? tile_r - rounds_r * 1024 : 0);
+#pragma unroll 4
+            for (int j = h ? rounds_r : 0; j < (h ? rounds : rounds_r); ++j) {
+              const uint4 w = value(j);
+              const float f[4] = {__uint_as_float(w.x) * inv, __uint_as_float(w.y) * inv, __uint_as_float(w.z) * inv,
+                                  __uint_as_float(w.w) * inv};
+              const __half2 h01 = __floats2half2_rn(f[0], f[1]), h23 = __floats2half2_rn(f[2], f[3]);
+              const float2 g01 = __half22float2(h01), g23 = __half22float2(h23);
+              float d[4] = {f[0] - g01.x, f[1] - g01.y, f[2] - g23.x, f[3] - g23.y};
+              if (odd)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = fabsf(f[i]) <= 65504.0f ? d[i] : 0.0f;   // not finite: hi alone
+              const __half2 l01 = __floats2half2_rn(d[0], d[1]), l23 = __floats2half2_rn(d[2], d[3]);
+              *reinterpret_cast<uint2*>(at + j * 1024) = make_uint2(h2_bits(h01), h2_bits(h23));
+              *reinterpret_cast<uint2*>(at + j * 1024 + plane) = make_uint2(h2_bits(l01), h2_bits(l23));
+            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(&bar_full[s]);
+        if (p.tma) mbar_arrive(&bar_raw_empty[rb]);
       }
     } else if (!p.tma) {
     const int rounds_r = rk / 8, rounds = rounds_r + (kDc ? rm / 8 : 0);   // 8 rows a round, 16 units of 16 bytes per row
     const int row0 = t >> 4;
     const int64_t step = 8 * p.P;
-    constexpr int kBatch = 8;
+    constexpr int kBatch = 4;
     int it = wg;
     bool ok = true;
     for (int64_t tile = blockIdx.x + (int64_t)wg * gridDim.x; tile < tiles && ok; tile += 2 * (int64_t)gridDim.x, it += 2) {
@@ -859,12 +862,12 @@ cudaError_t run_dcoeff(const void* dW, const void* X, int S, int E, int64_t P, f
 
 constexpr int kSmemLimit = 227 * 1024;
 
-// Operand stages that fit beside the coefficients, the staging area and, in fp32, two raw tiles.
+// Operand stages that fit beside the coefficients, the staging area and, in fp32, `raw` raw tiles.
 template <typename T>
-int tc_stages(int K, int M, bool dc, bool raw) {
+int tc_stages(int K, int M, bool dc, int raw) {
   const int m = M < kMixTcMax ? M : kMixTcMax;
   const int tile = MixTc<T>::stage_bytes(K, m, dc);
-  const int raw_bytes = raw && sizeof(T) == 4 ? 2 * (tile / MixTc<T>::kPlanesR / 2 * 4) : 0;
+  const int raw_bytes = sizeof(T) == 4 ? raw * (tile / MixTc<T>::kPlanesR / 2 * 4) : 0;
   const int n = (kSmemLimit - MixTc<T>::kFixed - MixTc<T>::coeff_bytes(K, m) - raw_bytes) / tile;
   return n < 4 ? n : 4;
 }
@@ -896,14 +899,17 @@ cudaError_t run_tc(MixTcArgs p, cudaStream_t s) {
                                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapSwizzle sw = kF32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
   const int64_t pitch = p.P * (int64_t)sizeof(T);
-  p.tma = pitch % 16 == 0 && p.P < ((int64_t)1 << 31) - 256 && tc_stages<T>(p.K, p.M, kDc, true) >= 1 &&
+  // fp32: two raw buffers (one per splitting warpgroup) come first, then two operand stages, then more raw buffers
+  const int raw = !kF32 ? 1 : tc_stages<T>(p.K, p.M, kDc, 4) >= 2 ? 4 : tc_stages<T>(p.K, p.M, kDc, 2) >= 1 ? 2 : 1;
+  const bool tma = pitch % 16 == 0 && p.P < ((int64_t)1 << 31) - 256 && tc_stages<T>(p.K, p.M, kDc, raw) >= 1 &&
           make_map_t(&mr, dt, p.R, p.K, p.P, pitch, 64, ceil16(p.K), sw) &&
           (!kDc || make_map_t(&mx, dt, p.X, p.M, p.P, pitch, 64, ceil16(m), sw)) &&
           make_map_t(&mo, dt, p.out, p.M, p.P, pitch, 128 / sizeof(T), 32, CU_TENSOR_MAP_SWIZZLE_128B);
+  p.tma = tma ? raw : 0;
   p.stages = tc_stages<T>(p.K, p.M, kDc, p.tma);
   const int tile = MixTc<T>::stage_bytes(p.K, m, kDc);
   const int smem = MixTc<T>::kFixed + MixTc<T>::coeff_bytes(p.K, m) + p.stages * tile +
-                   (kF32 && p.tma ? 2 * (tile / MixTc<T>::kPlanesR / 2 * 4) : 0);
+                   (kF32 ? p.tma * (tile / MixTc<T>::kPlanesR / 2 * 4) : 0);
   kern<<<dim3((unsigned)tc_grid(p.P, MixTc<T>::kBN), (unsigned)((p.M + kMixTcMax - 1) / kMixTcMax)), kMixTcThreads, smem,
          s>>>(mr, mx, mo, p);
   return cudaGetLastError();
@@ -911,7 +917,7 @@ cudaError_t run_tc(MixTcArgs p, cudaStream_t s) {
 
 template <typename T>
 bool tc_fits(int K, int M, bool dc) {
-  return K <= kMixTcMax && (!dc || M <= kMixTcMax) && tc_stages<T>(K, M, dc, false) >= 1;
+  return K <= kMixTcMax && (!dc || M <= kMixTcMax) && tc_stages<T>(K, M, dc, 0) >= 1;
 }
 
 template <typename T>
