@@ -713,10 +713,12 @@ int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P, int32_t dty
 
 namespace {
 
+int64_t ceil8(int64_t n) { return (n + 7) / 8 * 8; }
+
 int check_grouped(const char* what, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype) {
   REQUIRE(G >= 1 && G <= kMaxGroups, "%s: G=%d must be from 1 to %d", what, G, kMaxGroups);
   REQUIRE(T >= 0 && T < (int64_t(1) << 31) - 256, "%s: T=%lld out of range", what, (long long)T);
-  REQUIRE(N > 0 && N % 8 == 0 && K > 0 && K % 8 == 0, "%s: N=%d and K=%d must be positive multiples of 8", what, N, K);
+  REQUIRE(N > 0 && K > 0, "%s: N=%d and K=%d must be positive", what, N, K);
   REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "%s: dtype=%d must be 0 (fp32), 1 (bf16) or 2 (fp16)", what, dtype);
   REQUIRE((int64_t)G * (N > K ? N : K) < (int64_t(1) << 31), "%s: G * max(N, K) too large", what);
   REQUIRE((T / 128 + G) * (int64_t)((N > K ? N : K) / 32 + 1) < (int64_t(1) << 31), "%s: too many output tiles", what);
@@ -736,42 +738,44 @@ int grouped_done(const char* what, int r) {
 
 }  // namespace
 
-int fuma_grouped_linear(const void* x, int64_t ldx, const float* x_scales, const void* W, const float* W_scales,
-                        const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows, int64_t T, int32_t N, int32_t K, int32_t dtype, void* y,
+int fuma_grouped_linear(const void* x, int64_t ldx, const float* x_scales, const void* W, int64_t ldw,
+                        const float* W_scales, const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows, int64_t T, int32_t N, int32_t K, int32_t dtype, void* y,
                         int* err_flag, void* stream) {
   CHECK(check_grouped("grouped_linear", G, T, N, K, dtype));
-  REQUIRE(ldx >= K && ldx % 8 == 0, "grouped_linear: ldx=%lld must be >= K and a multiple of 8", (long long)ldx);
+  REQUIRE(ldx >= K && ldx % 8 == 0 && ldw >= K && ldw % 8 == 0,
+          "grouped_linear: ldx=%lld and ldw=%lld must be >= K and multiples of 8", (long long)ldx, (long long)ldw);
   REQUIRE(!bias || bias_rows == 1 || bias_rows == G, "grouped_linear: bias_rows=%d must be 1 or G", bias_rows);
   if (T == 0) return FUMA_OK;
   REQUIRE(x && W && y && (dtype != kDtypeF32 || (x_scales && W_scales)), "grouped_linear: null pointer");
-  REQUIRE(dtype != kDtypeF32 || ldx == K, "grouped_linear: planes have K columns (ldx=%lld)", (long long)ldx);
+  REQUIRE(dtype != kDtypeF32 || (ldx == ceil8(K) && ldw == ceil8(K)), "grouped_linear: planes have K columns rounded up to 8");
   REQUIRE(offsets || G == 1, "grouped_linear: offsets may be NULL for one group only");
   REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(W, "W"); REQUIRE_ALIGNED(y, "y");
   BIND(x);
-  GroupedOperands o{x, W, ldx, K, dtype == kDtypeF32 ? 1 : 0, dtype};
+  GroupedOperands o{x, W, ldx, ldw, dtype == kDtypeF32 ? 1 : 0, dtype};
   GroupedArgs p{};
   p.offsets = offsets; p.G = G; p.T = T; p.N = N; p.K = K;
-  p.C = y; p.ldc = N; p.out_dtype = dtype;
+  p.C = y; p.out_dtype = dtype;
   p.bias = bias; p.bias_rows = bias_rows; p.bias_dtype = dtype;
   p.scale_a = x_scales; p.scale_b = W_scales; p.blocks_n = (N + 127) / 128; p.scale_slots = split_slots(T, G);
   return grouped_done("grouped_linear", launch_grouped_rows(o, p, false, err_flag, (cudaStream_t)stream));
 }
 
 int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* W,
-                              const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dx, int* err_flag, void* stream) {
+                              int64_t ldw, const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dx, int* err_flag, void* stream) {
   CHECK(check_grouped("grouped_linear_dgrad", G, T, N, K, dtype));
-  REQUIRE(lddy >= N && lddy % 8 == 0, "grouped_linear_dgrad: lddy=%lld must be >= N and a multiple of 8",
-          (long long)lddy);
+  REQUIRE(lddy >= N && lddy % 8 == 0 && ldw >= K && ldw % 8 == 0,
+          "grouped_linear_dgrad: lddy=%lld (>= N) and ldw=%lld (>= K) must be multiples of 8", (long long)lddy, (long long)ldw);
   if (T == 0) return FUMA_OK;
   REQUIRE(dy && W && dx && (dtype != kDtypeF32 || (dy_scales && W_scales)), "grouped_linear_dgrad: null pointer");
-  REQUIRE(dtype != kDtypeF32 || lddy == N, "grouped_linear_dgrad: planes have N columns (lddy=%lld)", (long long)lddy);
+  REQUIRE(dtype != kDtypeF32 || (lddy == ceil8(N) && ldw == ceil8(K)),
+          "grouped_linear_dgrad: planes have N and K columns rounded up to 8");
   REQUIRE(offsets || G == 1, "grouped_linear_dgrad: offsets may be NULL for one group only");
   REQUIRE_ALIGNED(dy, "dy"); REQUIRE_ALIGNED(W, "W"); REQUIRE_ALIGNED(dx, "dx");
   BIND(dy);
-  GroupedOperands o{dy, W, lddy, K, dtype == kDtypeF32 ? 1 : 0, dtype};
+  GroupedOperands o{dy, W, lddy, ldw, dtype == kDtypeF32 ? 1 : 0, dtype};
   GroupedArgs p{};
   p.offsets = offsets; p.G = G; p.T = T; p.N = K; p.K = N;
-  p.C = dx; p.ldc = K; p.out_dtype = dtype;
+  p.C = dx; p.out_dtype = dtype;
   p.scale_a = dy_scales; p.scale_b = W_scales; p.blocks_n = (K + 127) / 128; p.scale_slots = split_slots(T, G);
   return grouped_done("grouped_linear_dgrad", launch_grouped_rows(o, p, true, err_flag, (cudaStream_t)stream));
 }
@@ -790,7 +794,8 @@ int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const float* dy_scal
     return st == cudaSuccess ? FUMA_OK : fail((int)st, "grouped_linear_wgrad: %s", cudaGetErrorString(st));
   }
   REQUIRE(dy && x && (dtype != kDtypeF32 || (dy_scales && x_scales)), "grouped_linear_wgrad: null pointer");
-  REQUIRE(dtype != kDtypeF32 || (lddy == N && ldx == K), "grouped_linear_wgrad: planes have N and K columns");
+  REQUIRE(dtype != kDtypeF32 || (lddy == ceil8(N) && ldx == ceil8(K)),
+          "grouped_linear_wgrad: planes have N and K columns rounded up to 8");
   REQUIRE(offsets || G == 1, "grouped_linear_wgrad: offsets may be NULL for one group only");
   const int64_t need = grouped_wgrad_work_bytes(T, N, K, dtype);
   REQUIRE(work_bytes >= need && (need == 0 || work), "grouped_linear_wgrad: needs %lld bytes of work space, got %lld",
@@ -808,13 +813,12 @@ int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const float* dy_scal
 int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets, int32_t G, int32_t shared, int64_t T,
                            int32_t N, int32_t dtype, void* db, void* work, int64_t work_bytes, void* stream) {
   CHECK(check_grouped("grouped_bias_grad", G, T, N, N, dtype));
-  REQUIRE(lddy >= N && lddy % 8 == 0, "grouped_bias_grad: lddy=%lld must be >= N and a multiple of 8", (long long)lddy);
+  REQUIRE(lddy >= N, "grouped_bias_grad: lddy=%lld must be >= N", (long long)lddy);
   REQUIRE(db && (T == 0 || dy), "grouped_bias_grad: null pointer");
   REQUIRE(offsets || G == 1, "grouped_bias_grad: offsets may be NULL for one group only");
   const int64_t need = T > 0 ? grouped_colsum_work_bytes(T, N, shared ? 1 : G) : 0;
   REQUIRE(work_bytes >= need && (need == 0 || work), "grouped_bias_grad: needs %lld bytes of work space, got %lld",
           (long long)need, (long long)work_bytes);
-  if (T > 0) REQUIRE_ALIGNED(dy, "dy");
   BIND(db);
   const cudaError_t st = launch_grouped_colsum(dy, lddy, dtype, offsets, G, shared != 0, T, N,
                                                static_cast<float*>(work), db, (cudaStream_t)stream);
@@ -823,31 +827,45 @@ int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets,
 
 int fuma_split_blocks(const float* x, int64_t ldx, int64_t rows, int32_t cols, const int64_t* offsets, int32_t G,
                       int32_t mat_rows, void* out, float* scales, void* stream) {
-  REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && cols > 0 && cols % 8 == 0, "split_blocks: bad shape rows=%lld cols=%d",
-          (long long)rows, cols);
-  REQUIRE(ldx >= cols && ldx % 4 == 0, "split_blocks: ldx=%lld must be >= cols and a multiple of 4", (long long)ldx);
+  REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && cols > 0, "split_blocks: bad shape rows=%lld cols=%d", (long long)rows,
+          cols);
+  REQUIRE(ldx >= cols, "split_blocks: ldx=%lld must be >= cols", (long long)ldx);
   REQUIRE(mat_rows >= 0 && (mat_rows == 0 || rows % mat_rows == 0), "split_blocks: mat_rows=%d must divide rows", mat_rows);
   REQUIRE(mat_rows > 0 || (G >= 1 && G <= kMaxGroups && (offsets || G == 1)), "split_blocks: bad groups (G=%d)", G);
   if (rows == 0) return FUMA_OK;
   const int64_t slots = mat_rows > 0 ? rows / mat_rows * ((mat_rows + 127) / 128) : split_slots(rows, G);
   REQUIRE(slots * ((cols + 127) / 128) < (int64_t(1) << 31), "split_blocks: too many blocks");
   REQUIRE(x && out && scales, "split_blocks: null pointer");
-  REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(out, "out");
+  REQUIRE_ALIGNED(out, "out");
   BIND(x);
   launch_split_blocks(x, ldx, rows, cols, offsets, G, mat_rows, out, scales, (cudaStream_t)stream);
   return launched("split_blocks");
 }
 
+int fuma_pad_rows(const void* x, int64_t ldx, int64_t rows, int32_t cols, void* out, int64_t ldo, const int64_t* offsets,
+                  int32_t G, int32_t mat_rows, int64_t T, void* stream) {
+  REQUIRE(rows >= 0 && cols > 0 && ldx >= cols, "pad_rows: bad shape rows=%lld cols=%d ldx=%lld", (long long)rows, cols,
+          (long long)ldx);
+  REQUIRE(ldo >= cols && ldo % 8 == 0, "pad_rows: ldo=%lld must be >= cols and a multiple of 8", (long long)ldo);
+  REQUIRE(!offsets || (G >= 1 && mat_rows > 0 && rows == (int64_t)G * mat_rows), "pad_rows: rows must be G * mat_rows");
+  if (rows == 0) return FUMA_OK;
+  REQUIRE(x && out, "pad_rows: null pointer");
+  REQUIRE_ALIGNED(out, "out");
+  BIND(x);
+  launch_pad_rows(x, ldx, rows, cols, out, ldo, offsets, mat_rows, T, (cudaStream_t)stream);
+  return launched("pad_rows");
+}
+
 int fuma_quantize_rows_fp8(const void* x, int64_t ldx, int64_t T, int32_t K, int32_t dtype, void* codes, int64_t ldq,
                            float* scales, void* stream) {
-  REQUIRE(T >= 0 && T < (int64_t(1) << 31) && K > 0 && K % 8 == 0, "quantize_rows_fp8: bad shape T=%lld K=%d",
+  REQUIRE(T >= 0 && T < (int64_t(1) << 31) && K > 0, "quantize_rows_fp8: bad shape T=%lld K=%d",
           (long long)T, K);
   REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "quantize_rows_fp8: dtype=%d must be 0, 1 or 2", dtype);
-  REQUIRE(ldx >= K && ldx % 8 == 0, "quantize_rows_fp8: ldx=%lld must be >= K and a multiple of 8", (long long)ldx);
+  REQUIRE(ldx >= K, "quantize_rows_fp8: ldx=%lld must be >= K", (long long)ldx);
   REQUIRE(ldq == (K + 15) / 16 * 16, "quantize_rows_fp8: ldq=%lld must be K rounded up to 16", (long long)ldq);
   if (T == 0) return FUMA_OK;
   REQUIRE(x && codes && scales, "quantize_rows_fp8: null pointer");
-  REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(codes, "codes");
+  REQUIRE_ALIGNED(codes, "codes");
   BIND(x);
   launch_quantize_rows(x, ldx, dtype, T, K, codes, ldq, scales, (cudaStream_t)stream);
   return launched("quantize_rows_fp8");
@@ -876,14 +894,14 @@ int fuma_grouped_linear_fp8(const void* x, int64_t ldx, const void* w_codes, con
                             int32_t N, int32_t K, int32_t dtype, void* y, void* work, int64_t work_bytes, int* err_flag,
                             void* stream) {
   CHECK(check_grouped("grouped_linear_fp8", G, T, N, K, dtype));
-  REQUIRE(ldx >= K && ldx % 8 == 0, "grouped_linear_fp8: ldx=%lld must be >= K and a multiple of 8", (long long)ldx);
+  REQUIRE(ldx >= K, "grouped_linear_fp8: ldx=%lld must be >= K", (long long)ldx);
   REQUIRE(!bias || bias_rows == 1 || bias_rows == G, "grouped_linear_fp8: bias_rows=%d must be 1 or G", bias_rows);
   if (T == 0) return FUMA_OK;
   REQUIRE(x && w_codes && w_scales && y && work, "grouped_linear_fp8: null pointer");
   REQUIRE(offsets || G == 1, "grouped_linear_fp8: offsets may be NULL for one group only");
   REQUIRE(work_bytes >= fuma_fp8_work_bytes(T, K), "grouped_linear_fp8: needs %lld bytes of work space, got %lld",
           (long long)fuma_fp8_work_bytes(T, K), (long long)work_bytes);
-  REQUIRE_ALIGNED(x, "x"); REQUIRE_ALIGNED(w_codes, "w_codes"); REQUIRE_ALIGNED(y, "y"); REQUIRE_ALIGNED(work, "work");
+  REQUIRE_ALIGNED(w_codes, "w_codes"); REQUIRE_ALIGNED(y, "y"); REQUIRE_ALIGNED(work, "work");
   BIND(x);
   const int64_t ld = (K + 15) / 16 * 16;
   uint8_t* codes = static_cast<uint8_t*>(work);
@@ -893,7 +911,7 @@ int fuma_grouped_linear_fp8(const void* x, int64_t ldx, const void* w_codes, con
   GroupedOperands o{codes, w_codes, ld, ld, 2, 0};
   GroupedArgs p{};
   p.offsets = offsets; p.G = G; p.T = T; p.N = N; p.K = K;
-  p.C = y; p.ldc = N; p.out_dtype = dtype;
+  p.C = y; p.out_dtype = dtype;
   p.bias = bias; p.bias_rows = bias_rows; p.bias_dtype = kDtypeF32;
   p.scale_a = scales; p.scale_b = w_scales; p.blocks_n = (N + 127) / 128;
   return grouped_done("grouped_linear_fp8", launch_grouped_rows(o, p, false, err_flag, (cudaStream_t)stream));

@@ -40,7 +40,8 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 // a thread block reads a run of memory. 16-bit types find the largest magnitude on packed pairs. Columns [K, ldq) get
 // zero codes. One pass: 2 (4) bytes read, 1 written per value. Bound by HBM in fp32, by instructions below
 // it in 16 bits.
-template <int kDtype, int kQRows>
+// kVec: rows 16-byte aligned.
+template <int kDtype, int kQRows, bool kVec>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t T, int K,
                                                             uint8_t* __restrict__ codes, int64_t ldq,
                                                             float* __restrict__ scales) {
@@ -62,7 +63,24 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
       kb[i] = (int)(v - drow[i] * kblocks);
       const int k = kb[i] * 128 + l * kVals;
       raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
-      if (base + drow[i] < T) {   // K is a multiple of 8: a 16-byte load of 16-bit values is all inside or all outside
+      if (!kVec) {
+        if (base + drow[i] < T && k < K) {
+          constexpr int kSize = kF32 ? 4 : 2;
+          uint8_t b[32];
+          const uint8_t* src = static_cast<const uint8_t*>(x) + ((base + drow[i]) * ldx + k) * kSize;
+#pragma unroll
+          for (int j = 0; j < kVals; ++j) {
+            if constexpr (kF32) {
+              const uint32_t e = k + j < K ? *reinterpret_cast<const uint32_t*>(src + 4 * j) : 0u;
+              memcpy(b + 4 * j, &e, 4);
+            } else {
+              const uint16_t e = k + j < K ? *reinterpret_cast<const uint16_t*>(src + 2 * j) : (uint16_t)0;
+              memcpy(b + 2 * j, &e, 2);
+            }
+          }
+          memcpy(raw[i], b, 32);
+        }
+      } else if (base + drow[i] < T) {   // K is a multiple of 8: a 16-byte load is all inside or all outside
         const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) +
                                                         ((base + drow[i]) * ldx + k) * (kF32 ? 4 : 2));
         if (k < K) raw[i][0] = __ldcs(p);
@@ -177,21 +195,29 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const float* __res
   }
 }
 
-template <int kDtype, int kQRows>
+template <int kDtype, int kQRows, bool kVec>
 static void run_quantize_rows(const void* x, int64_t ldx, int64_t T, int K, void* codes, int64_t ldq, float* scales,
                               cudaStream_t s) {
   const int64_t units = T * ((K + 127) / 128);
-  quantize_rows_kernel<kDtype, kQRows><<<grid_resident(quantize_rows_kernel<kDtype, kQRows>, 256, units, (kDtype == kDtypeF32 ? 16 : 32) * kQRows), 256,
-                                         0, s>>>(x, ldx, T, K, static_cast<uint8_t*>(codes), ldq, scales);
+  auto kern = quantize_rows_kernel<kDtype, kQRows, kVec>;
+  kern<<<grid_resident(kern, 256, units, (kDtype == kDtypeF32 ? 16 : 32) * kQRows), 256, 0, s>>>(
+      x, ldx, T, K, static_cast<uint8_t*>(codes), ldq, scales);
+}
+
+template <int kDtype>
+static void any_quantize_rows(const void* x, int64_t ldx, int64_t T, int K, void* codes, int64_t ldq, float* scales,
+                              cudaStream_t s) {
+  // few rows: one block per lane group, so that more thread blocks share the work
+  const bool few = T * K < (int64_t)4 << 20, vec = ldx % 8 == 0 && K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  auto run = vec ? (few ? run_quantize_rows<kDtype, 1, true> : run_quantize_rows<kDtype, 4, true>)
+                 : run_quantize_rows<kDtype, 1, false>;
+  run(x, ldx, T, K, codes, ldq, scales, s);
 }
 
 void launch_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t T, int K, void* codes, int64_t ldq,
                           float* scales, cudaStream_t s) {
-  // few rows: one row per thread, so that more blocks share the work
-  const bool few = T * K < (int64_t)4 << 20;
-  auto run = dtype == kDtypeF32    ? (few ? run_quantize_rows<kDtypeF32, 1> : run_quantize_rows<kDtypeF32, 4>)
-             : dtype == kDtypeBf16 ? (few ? run_quantize_rows<kDtypeBf16, 1> : run_quantize_rows<kDtypeBf16, 4>)
-                                   : (few ? run_quantize_rows<kDtypeF16, 1> : run_quantize_rows<kDtypeF16, 4>);
+  auto run = dtype == kDtypeF32 ? any_quantize_rows<kDtypeF32>
+             : dtype == kDtypeBf16 ? any_quantize_rows<kDtypeBf16> : any_quantize_rows<kDtypeF16>;
   run(x, ldx, T, K, codes, ldq, scales, s);
 }
 

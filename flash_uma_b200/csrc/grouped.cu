@@ -40,7 +40,6 @@
 // thread's own instructions count: 512 cycles of MMA per stage leave no room for descriptors built from scratch
 // (960 cycles per stage measured), so it adds constants to descriptors made once. Every wait is bounded.
 #include <cstdio>
-#include <cstdlib>
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -337,7 +336,8 @@ template <int kKind, int kMode, bool kPair>
 __global__ void __launch_bounds__(kGThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ GroupedArgs p) {
-  static_assert(!kPair || kMode != kModeDw, "the weight gradient clears rows of a stage, which a pair would share");
+  static_assert(!kPair || (kMode != kModeDw && kKind == kHalf),
+                "the weight gradient clears rows of a stage, which a pair would share; pairs are for 16-bit operands");
   using L = GSmem<kKind, kPair>;
   constexpr int kP = L::kP, kBK = L::kBK;
   constexpr bool kScaled = kKind != kHalf;
@@ -657,13 +657,16 @@ __global__ void __launch_bounds__(kGThreads, 1)
     if constexpr (kMode != kModeDw) {
       // rows before the first and behind the last group: zeros
       const int64_t head = group_at(p.offsets, 0, p.T), tail = group_at(p.offsets, p.G, p.T);
-      const int vec = p.N * (p.out_dtype == kDtypeF32 ? 4 : 2) / 16;
-      const int64_t dead = units || head == tail ? head + (p.T - tail) : 0, n = dead * vec;
+      const int esize = p.out_dtype == kDtypeF32 ? 4 : 2, row_bytes = p.N * esize;
+      const int unit = p.N % 8 ? esize : 16, units_row = row_bytes / unit;
+      const int64_t dead = units || head == tail ? head + (p.T - tail) : 0, n = dead * units_row;
       for (int64_t i = (int64_t)blockIdx.x * (kEpiWarps * 32) + threadIdx.x - kEpiWarp0 * 32; i < n;
            i += (int64_t)gridDim.x * (kEpiWarps * 32)) {
-        const int64_t r = i / vec, row = r < head ? r : tail + (r - head);
-        uint8_t* c = static_cast<uint8_t*>(p.C) + row * p.ldc * (p.out_dtype == kDtypeF32 ? 4 : 2);
-        reinterpret_cast<uint4*>(c)[i - r * vec] = make_uint4(0u, 0u, 0u, 0u);
+        const int64_t r = i / units_row, row = r < head ? r : tail + (r - head);
+        uint8_t* c = static_cast<uint8_t*>(p.C) + row * row_bytes + (i - r * units_row) * unit;
+        if (unit == 16) *reinterpret_cast<uint4*>(c) = make_uint4(0u, 0u, 0u, 0u);
+        else if (unit == 4) *reinterpret_cast<uint32_t*>(c) = 0u;
+        else *reinterpret_cast<uint16_t*>(c) = 0u;
       }
     }
     const uint32_t acc_empty[2] = {kPair ? in_cta0(&bar_acc_empty[0]) : smem_u32(&bar_acc_empty[0]),
@@ -798,7 +801,8 @@ __global__ void __launch_bounds__(kGThreads, 1)
       // area queue behind the producer's loads: the fp8 map took 128 us with them and 107 without.)
       const bool partial = kMode == kModeDw && t.partial;
       const int out_dtype = partial ? kDtypeF32 : p.out_dtype;
-      const int64_t ld = kMode == kModeDw ? p.N : p.ldc;
+      const int64_t ld = partial ? p.ldw : p.N;
+      const bool rows16 = kPair || partial || p.N % 8 == 0;   // output rows in 16-byte steps (pairs: always)
       const int64_t y0 = (kMode == kModeDw ? (int64_t)(partial ? t.partial - 1 : t.g) * p.M + t.m0 : t.row0) + q * 32;
       const int x0 = n0;
       uint8_t* out = static_cast<uint8_t*>(partial ? p.work : p.C);
@@ -814,7 +818,12 @@ __global__ void __launch_bounds__(kGThreads, 1)
               *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
                   make_float4(acc[c * 32 + 4 * j], acc[c * 32 + 4 * j + 1], acc[c * 32 + 4 * j + 2], acc[c * 32 + 4 * j + 3]);
             __syncwarp();
-            if (c * 32 + jj * 4 < ncols) {
+            if (!rows16) {
+              if (c * 32 + lane < ncols)
+                for (int r = 0; r < min(rows, 32); ++r)
+                  reinterpret_cast<float*>(out)[(y0 + r) * ld + x0 + c * 32 + lane] =
+                      *reinterpret_cast<const float*>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+            } else if (c * 32 + jj * 4 < ncols) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const int r = i * 4 + rr;
@@ -838,7 +847,16 @@ __global__ void __launch_bounds__(kGThreads, 1)
                              pack_half(a[4], a[5], out_dtype), pack_half(a[6], a[7], out_dtype));
             }
             __syncwarp();
-            if (c * 64 + jj * 8 < ncols) {
+            if (!rows16) {
+              for (int r = 0; r < min(rows, 32); ++r)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const int k = h * 32 + lane;
+                  if (c * 64 + k < ncols)
+                    reinterpret_cast<uint16_t*>(out)[(y0 + r) * ld + x0 + c * 64 + k] =
+                        *reinterpret_cast<const uint16_t*>(stage + r * 128 + (((k >> 3) ^ (r & 7)) << 4) + (k & 7) * 2);
+                }
+            } else if (c * 64 + jj * 8 < ncols) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const int r = i * 4 + rr;
@@ -895,18 +913,32 @@ __global__ void __launch_bounds__(256) grouped_join_kernel(const __grid_constant
   if (g < 0) return;
   const int64_t at = group_at(p.offsets, g, p.T), len = group_len(p.offsets, g, p.T);
   const int parts = group_units<kModeDw, kBM>(len, p.cap);
-  const int64_t n4 = (int64_t)p.M * p.N / 4;
+  const int w4 = p.ldw / 4;                  // the parts' rows are padded to 8 columns
+  const int64_t n4 = (int64_t)p.M * w4;
   const float* work = static_cast<const float*>(p.work) + 2 * (at / kBM) / p.cap * n4 * 4;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (int64_t)gridDim.x * blockDim.x) {
     float4 s = ld4_stream(work + i * 4);
 #pragma unroll 4
     for (int c = 1; c < parts; ++c) s += ld4_stream(work + (c * n4 + i) * 4);
-    const int64_t o = ((int64_t)g * n4 + i) * 4;
-    if (p.out_dtype == kDtypeF32)
-      st4(static_cast<float*>(p.C) + o, s);
-    else
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.C) + o) =
-          make_uint2(pack_half(s.x, s.y, p.out_dtype), pack_half(s.z, s.w, p.out_dtype));
+    if (p.ldw == p.N) {
+      const int64_t o = ((int64_t)g * n4 + i) * 4;
+      if (p.out_dtype == kDtypeF32)
+        st4(static_cast<float*>(p.C) + o, s);
+      else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.C) + o) =
+            make_uint2(pack_half(s.x, s.y, p.out_dtype), pack_half(s.z, s.w, p.out_dtype));
+    } else {
+      const int64_t m = i / w4;
+      const int n = (int)(i - m * w4) * 4;
+      const int64_t o = ((int64_t)g * p.M + m) * p.N + n;
+      const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (n + k >= p.N) break;
+        if (p.out_dtype == kDtypeF32) static_cast<float*>(p.C)[o + k] = v[k];
+        else static_cast<uint16_t*>(p.C)[o + k] = (uint16_t)(pack_half(v[k], 0.0f, p.out_dtype) & 0xffffu);
+      }
+    }
   }
 }
 
@@ -925,7 +957,8 @@ __device__ __forceinline__ int64_t sum_bound(const int64_t* off, int g, int G, i
 // A block takes the pieces of one row block in 256 columns (8 per lane). Long pieces: the 8 warps share a piece's rows,
 // 8 rows in flight each, and join in shared memory. Row blocks cut into many short pieces (many small groups):
 // a warp per piece, no joining.
-template <int kDtype>
+// kVec: rows 16-byte aligned.
+template <int kDtype, bool kVec>
 __global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restrict__ x, int64_t ld,
                                                              const int64_t* __restrict__ off, int G, int shared,
                                                              int64_t T, int N, float* __restrict__ part) {
@@ -955,7 +988,10 @@ __global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restr
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           raw[i].zero();
-          if (r + i * step < r1) raw[i].load(x, (r + i * step) * ld + n);
+          if (r + i * step < r1) {
+            if constexpr (kVec) raw[i].load(x, (r + i * step) * ld + n);
+            else raw[i].load_some(x, (r + i * step) * ld + n, min(8, N - n));
+          }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -968,9 +1004,15 @@ __global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restr
     }
     float* out = part + ((int64_t)blockIdx.x + g) * N;
     if (short_pieces) {
-      if (n < N) {
-        st4(out + n, make_float4(s[0], s[1], s[2], s[3]));
-        st4(out + n + 4, make_float4(s[4], s[5], s[6], s[7]));
+      if constexpr (kVec) {
+        if (n < N) {
+          st4(out + n, make_float4(s[0], s[1], s[2], s[3]));
+          st4(out + n + 4, make_float4(s[4], s[5], s[6], s[7]));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (n + k < N) out[n + k] = s[k];
       }
     } else {
 #pragma unroll
@@ -1043,6 +1085,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) grouped_colsum_join_kernel(co
 // 128-row tiles of each group (counted from the group's first row, as the maps cut it; the tile's slot is group
 // start / 128 + group + tile, distinct because one tile or one group further on moves it by at least 1), or, with
 // mat_rows > 0, of matrices of mat_rows rows each. A value that is not finite keeps hi alone and does not set the scale.
+// kVec: rows 16-byte aligned. Planes [rows][ldp], ldp = cols rounded up to 8.
+template <bool kVec>
 __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows,
                                                            int cols, const int64_t* __restrict__ off, int G,
                                                            int mat_rows, __half* __restrict__ out,
@@ -1079,7 +1123,18 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restri
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int r = w + 8 * i;
-    v[i] = (r < n && c < cols) ? ld4_stream(x + (row0 + r) * ldx + c) : f4(0.0f);
+    v[i] = f4(0.0f);
+    if (r < n) {
+      const float* src = x + (row0 + r) * ldx + c;
+      if constexpr (kVec) {
+        if (c < cols) v[i] = ld4_stream(src);
+      } else {
+        if (c < cols) v[i].x = __ldcs(src);
+        if (c + 1 < cols) v[i].y = __ldcs(src + 1);
+        if (c + 2 < cols) v[i].z = __ldcs(src + 2);
+        if (c + 3 < cols) v[i].w = __ldcs(src + 3);
+      }
+    }
   }
   uint32_t m = 0;
 #pragma unroll
@@ -1101,8 +1156,9 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restri
   if (e < -126) e = -126;
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
   if (threadIdx.x == 0) scales[scale_at] = __uint_as_float((uint32_t)(127 + e) << 23);
-  if (c >= cols) return;
-  const int64_t plane = rows * cols;
+  const int ldp = (cols + 7) / 8 * 8;
+  if (c >= ldp) return;
+  const int64_t plane = rows * ldp;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int r = w + 8 * i;
@@ -1116,9 +1172,9 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restri
       }
       uint2 u;
       memcpy(&u, h, 8);
-      *reinterpret_cast<uint2*>(out + (row0 + r) * cols + c) = u;
+      *reinterpret_cast<uint2*>(out + (row0 + r) * ldp + c) = u;
       memcpy(&u, l, 8);
-      *reinterpret_cast<uint2*>(out + plane + (row0 + r) * cols + c) = u;
+      *reinterpret_cast<uint2*>(out + plane + (row0 + r) * ldp + c) = u;
     }
   }
 }
@@ -1187,9 +1243,14 @@ int pick_bn(int N, int64_t tiles_rows, bool scaled, int step) {
   return bn;
 }
 
-// CTA pairs: tiles of 256 rows, when the groups are long enough that the padding of their last tile (128 rows more on
-// average) costs less than what a pair saves, and there are enough tiles for every pair of SMs.
-bool use_pair(int64_t T, int G, int64_t items) { return T >= (int64_t)1024 * G && items >= sm_count() / 2; }
+// CTA pairs (16-bit operands only): tiles of 256 rows, when the groups are long enough that the padding of their last tile
+// (128 rows more on average) costs less than what a pair saves, and there are 8 tiles or more for every pair of SMs: with
+// fewer, the last round's idle SMs cost what the pairs save. bf16, forward and input gradient: 120,000 rows in 16 groups,
+// 640 -> 768 columns, 108 and 99 us, single CTAs 115 and 123; 32,768 rows in 32 groups, 512 -> 512 (4 tiles a pair), 26.7
+// and 26.4 us, single 25.6 and 25.5. At 30,011 rows in 8 groups in fp32 pairs are slower (55.2 and 53.6 us, single 51.6
+// and 50.9), and so they are in fp8 (184 us, 110): both have scales to fetch and sums to drain between the products,
+// which a pair does in step.
+bool use_pair(int64_t T, int G, int64_t items) { return T >= (int64_t)1024 * G && items >= (int64_t)4 * sm_count(); }
 
 }  // namespace
 
@@ -1206,7 +1267,7 @@ int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed
   p.span = (p.G + kCoarse - 1) / kCoarse;
   p.mma_format = (!fp8 && !split && o.dtype == kDtypeBf16) ? 1u : 0u;
   const int64_t pair_items = (p.T / (2 * kBM) + groups) * p.tiles_n;
-  const bool pair = !fp8 && p.bn > 128 && use_pair(p.T, p.G, pair_items);
+  const bool pair = o.kind == kHalf && p.N % 8 == 0 && p.bn > 128 && use_pair(p.T, p.G, pair_items);
   p.box_b = pair ? p.bn / 2 : p.bn;   // columns of the tile in this CTA: rows of W per load (forward)
   p.wide_b = transposed && p.N % (pair ? 128 : 64) == 0 && p.box_b % 64 == 0;
   p.wide_a = 0;
@@ -1229,12 +1290,16 @@ int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed
     return -1;
   const int64_t items = tiles_rows * p.tiles_n;
   cudaError_t st;
-#define FUMA_ROWS(kind, mode) (pair ? launch_grouped<kind, mode, true>(m, p, pair_items, s) \
-                                    : launch_grouped<kind, mode, false>(m, p, items, s))
-  if (fp8) st = FUMA_ROWS(kFp8, kModeFwd);
-  else if (split) st = transposed ? FUMA_ROWS(kSplit, kModeDx) : FUMA_ROWS(kSplit, kModeFwd);
-  else st = transposed ? FUMA_ROWS(kHalf, kModeDx) : FUMA_ROWS(kHalf, kModeFwd);
-#undef FUMA_ROWS
+  if (pair)
+    st = transposed ? launch_grouped<kHalf, kModeDx, true>(m, p, pair_items, s)
+                    : launch_grouped<kHalf, kModeFwd, true>(m, p, pair_items, s);
+  else if (fp8) st = launch_grouped<kFp8, kModeFwd, false>(m, p, items, s);
+  else if (split)
+    st = transposed ? launch_grouped<kSplit, kModeDx, false>(m, p, items, s)
+                    : launch_grouped<kSplit, kModeFwd, false>(m, p, items, s);
+  else
+    st = transposed ? launch_grouped<kHalf, kModeDx, false>(m, p, items, s)
+                    : launch_grouped<kHalf, kModeFwd, false>(m, p, items, s);
   return (int)st;
 }
 
@@ -1258,7 +1323,7 @@ static int wgrad_cap(int64_t T, int M, int N, bool split) {
 int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N, int dtype) {
   const int cap = wgrad_cap(T, M, N, dtype == kDtypeF32);
   if (T <= (int64_t)cap * kBM) return 0;
-  return (2 * (T / kBM) / cap + 2) * (int64_t)M * N * 4;
+  return (2 * (T / kBM) / cap + 2) * (int64_t)M * ((N + 7) / 8 * 8) * 4;
 }
 
 int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cudaStream_t s) {
@@ -1270,7 +1335,7 @@ int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cuda
   p.tiles_m = (p.M + kBM - 1) / kBM;
   p.span = (p.G + kCoarse - 1) / kCoarse;
   p.mma_format = (!split && o.dtype == kDtypeBf16) ? 1u : 0u;
-  p.ldc = p.N;
+  p.ldw = (p.N + 7) / 8 * 8;
   p.box_b = p.bn;
   p.wide_a = p.M % 64 == 0;
   p.wide_b = p.N % 64 == 0;
@@ -1288,7 +1353,7 @@ int launch_grouped_wgrad(const GroupedOperands& o, GroupedArgs p, int* err, cuda
   cudaError_t st = split ? launch_grouped<kSplit, kModeDw, false>(m, p, items, s)
                          : launch_grouped<kHalf, kModeDw, false>(m, p, items, s);
   if (st == cudaSuccess && p.T > (int64_t)p.cap * kBM) {
-    const int64_t n4 = (int64_t)p.M * p.N / 4;
+    const int64_t n4 = (int64_t)p.M * p.ldw / 4;
     int64_t bx = (n4 + 255) / 256;
     if (bx > 512) bx = 512;
     const int64_t long_groups = p.T / ((int64_t)p.cap * kBM);
@@ -1306,8 +1371,10 @@ cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const in
                                   int64_t T, int N, float* part, void* out, cudaStream_t s) {
   const int groups = shared ? 1 : G;
   if (T > 0) {
-    auto kern = dtype == kDtypeF32 ? grouped_colsum_kernel<kDtypeF32>
-                : dtype == kDtypeBf16 ? grouped_colsum_kernel<kDtypeBf16> : grouped_colsum_kernel<kDtypeF16>;
+    const bool vec = ld % 8 == 0 && N % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    auto kern = dtype == kDtypeF32    ? (vec ? grouped_colsum_kernel<kDtypeF32, true> : grouped_colsum_kernel<kDtypeF32, false>)
+                : dtype == kDtypeBf16 ? (vec ? grouped_colsum_kernel<kDtypeBf16, true> : grouped_colsum_kernel<kDtypeBf16, false>)
+                                      : (vec ? grouped_colsum_kernel<kDtypeF16, true> : grouped_colsum_kernel<kDtypeF16, false>);
     kern<<<dim3((unsigned)((T + kSumRows - 1) / kSumRows), (unsigned)((N + 255) / 256)), 256, 0, s>>>(
         x, ld, off, G, shared, T, N, part);
     const cudaError_t st = cudaGetLastError();
@@ -1326,8 +1393,35 @@ void launch_split_blocks(const float* x, int64_t ldx, int64_t rows, int cols, co
                          void* out, float* scales, cudaStream_t s) {
   const int64_t slots = mat_rows > 0 ? rows / mat_rows * ((mat_rows + 127) / 128) : split_slots(rows, G);
   const int64_t blocks = slots * ((cols + 127) / 128);
-  split_blocks_kernel<<<(unsigned)blocks, 256, 0, s>>>(x, ldx, rows, cols, off, G, mat_rows, static_cast<__half*>(out),
-                                                       scales, slots);
+  const bool vec = ldx % 4 == 0 && cols % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  auto kern = vec ? split_blocks_kernel<true> : split_blocks_kernel<false>;
+  kern<<<(unsigned)blocks, 256, 0, s>>>(x, ldx, rows, cols, off, G, mat_rows, static_cast<__half*>(out), scales, slots);
+}
+
+// 16-bit rows to a 16-byte pitch (for TMA), 8 values per thread; columns behind the last are left as they are (the tensor
+// maps end before them). With offsets: rows of matrices (mat_rows each) whose group has no rows are left out.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t rows, int cols,
+                                                       uint16_t* __restrict__ out, int64_t ldo,
+                                                       const int64_t* __restrict__ off, int mat_rows, int64_t T) {
+  const int c8 = (cols + 7) / 8;
+  const int64_t total = rows * c8;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / c8;
+    const int c = (int)(i - r * c8) * 8;
+    if (off && group_len(off, (int)(r / mat_rows), T) == 0) continue;
+    uint16_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? x[r * ldx + c + k] : 0;
+    uint4 u;
+    memcpy(&u, v, 16);
+    *reinterpret_cast<uint4*>(out + r * ldo + c) = u;
+  }
+}
+
+void launch_pad_rows(const void* x, int64_t ldx, int64_t rows, int cols, void* out, int64_t ldo, const int64_t* off,
+                     int mat_rows, int64_t T, cudaStream_t s) {
+  pad_rows_kernel<<<grid_resident(pad_rows_kernel, 256, rows * ((cols + 7) / 8), 256), 256, 0, s>>>(
+      static_cast<const uint16_t*>(x), ldx, rows, cols, static_cast<uint16_t*>(out), ldo, off, mat_rows, T);
 }
 
 }  // namespace fuma

@@ -26,6 +26,21 @@ struct Raw8 {
     w[0] = __ldcs(p);
     if constexpr (kDtype == kDtypeF32) w[1] = __ldcs(p + 1);
   }
+  __device__ __forceinline__ void load_some(const void* x, int64_t i, int n) {   // any alignment, n <= 8 values
+    constexpr int kSize = kDtype == kDtypeF32 ? 4 : 2;
+    uint8_t b[8 * kSize];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (kSize == 4) {
+        const uint32_t v = k < n ? static_cast<const uint32_t*>(x)[i + k] : 0u;
+        memcpy(b + 4 * k, &v, 4);
+      } else {
+        const uint16_t v = k < n ? static_cast<const uint16_t*>(x)[i + k] : (uint16_t)0;
+        memcpy(b + 2 * k, &v, 2);
+      }
+    }
+    memcpy(w, b, sizeof(b));
+  }
   __device__ __forceinline__ void to_f32(float (&v)[8]) const {
     if constexpr (kDtype == kDtypeF32) {
       memcpy(v, w, 32);
@@ -63,8 +78,7 @@ struct GroupedArgs {
   int G;
   int64_t T;                // rows of the ragged operand(s)
   int M, N, K;              // row maps: N output columns, contraction K. Weight gradient: dW is [G, M, N].
-  void* C;
-  int64_t ldc;
+  void* C;                  // contiguous
   int out_dtype;
   const void* bias;         // [N] or [G, N] or null
   int bias_rows, bias_dtype;
@@ -81,7 +95,7 @@ struct GroupedArgs {
   void* work;
   int* err;
   // set by the launcher
-  int bn, tiles_m, tiles_n, cap, span, box_b, wide_a, wide_b;
+  int bn, tiles_m, tiles_n, cap, ldw, span, box_b, wide_a, wide_b;
   uint32_t mma_format;
 };
 
@@ -91,11 +105,15 @@ int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N, int dtype);
 int64_t grouped_colsum_work_bytes(int64_t T, int N, int groups);
 cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const int64_t* off, int G, bool shared,
                                   int64_t T, int N, float* part, void* out, cudaStream_t s);
-// Two fp16 planes [2][rows][cols] and their block scales: of ragged rows (mat_rows 0) [ceil(cols / 128)][split_slots],
+// Two fp16 planes [2][rows][cols rounded up to 8] and their block scales: of ragged rows (mat_rows 0) [ceil(cols / 128)][split_slots],
 // of matrices of mat_rows rows [matrices][ceil(mat_rows / 128)][ceil(cols / 128)].
 int64_t split_slots(int64_t rows, int G);
 void launch_split_blocks(const float* x, int64_t ldx, int64_t rows, int cols, const int64_t* off, int G, int mat_rows,
                          void* out, float* scales, cudaStream_t s);
+
+// 16-bit rows copied to a pitch of ldo (a multiple of 8) elements; see the kernel.
+void launch_pad_rows(const void* x, int64_t ldx, int64_t rows, int cols, void* out, int64_t ldo, const int64_t* off,
+                     int mat_rows, int64_t T, cudaStream_t s);
 
 void launch_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t T, int K, void* codes, int64_t ldq,
                           float* scales, cudaStream_t s);

@@ -14,7 +14,8 @@ import torch
 
 from . import _native as nat
 from ._native import ptr, stream_of
-from .grouped import _DTYPES, MAX_GROUPS, _apply, _ceil8, _check_dtype, _opaque, _rows, _same_device, check_groups, guard_capture
+from .grouped import (_DTYPES, MAX_GROUPS, _apply, _check_dtype, _opaque, _same_device, _unit_stride, check_groups,
+                      guard_capture)
 from .linear import error_flag
 
 _BLOCK = 128
@@ -44,16 +45,15 @@ class Fp8Weight:
             raise ValueError(f"the number of groups must be from 1 to {MAX_GROUPS} (got {self.G})")
         if self.N < 1 or self.K < 1:
             raise ValueError(f"weight needs N >= 1 and K >= 1 (got {tuple(weight.shape)})")
-        self.Np, self.Kp = _ceil8(self.N), _ceil8(self.K)
-        w = torch.nn.functional.pad(w.float(), (0, self.Kp - self.K, 0, self.Np - self.N)).contiguous()
-        dev, G, Np, Kp = w.device, self.G, self.Np, self.Kp
+        w = w.float().contiguous()
+        dev, G, N, K = w.device, self.G, self.N, self.K
         self.device = dev
-        self.codes = torch.empty(G, Np, _ceil16(Kp), device=dev, dtype=torch.uint8)
-        self.scales = torch.empty(G, _blocks(Np), _blocks(Kp), device=dev)
-        self.codes_t = torch.empty(G, Kp, _ceil16(Np), device=dev, dtype=torch.uint8)
-        self.scales_t = torch.empty(G, _blocks(Kp), _blocks(Np), device=dev)
-        nat.call("fuma_quantize_weight_fp8", ptr(w), G, Np, Kp, ptr(self.codes), _ceil16(Kp), ptr(self.scales),
-                 ptr(self.codes_t), _ceil16(Np), ptr(self.scales_t), stream_of(w))
+        self.codes = torch.empty((G, N, _ceil16(K)), device=dev, dtype=torch.uint8)
+        self.scales = torch.empty((G, _blocks(N), _blocks(K)), device=dev)
+        self.codes_t = torch.empty((G, K, _ceil16(N)), device=dev, dtype=torch.uint8)
+        self.scales_t = torch.empty((G, _blocks(K), _blocks(N)), device=dev)
+        nat.call("fuma_quantize_weight_fp8", ptr(w), G, N, K, ptr(self.codes), _ceil16(K), ptr(self.scales),
+                 ptr(self.codes_t), _ceil16(N), ptr(self.scales_t), stream_of(w))
 
     def dequantize(self) -> torch.Tensor:
         """The values that the codes stand for, fp32 [G, N, K]."""
@@ -69,12 +69,12 @@ def quantize_rows(x: torch.Tensor):
     code = _check_dtype("x", x)
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be [rows, K] with K >= 1 (got {tuple(x.shape)})")
-    T, Kp = x.shape[0], _ceil8(x.shape[1])
-    x = _rows(x, Kp)
-    codes = torch.empty(T, _ceil16(Kp), device=x.device, dtype=torch.uint8)
-    scales = torch.empty(_blocks(Kp), T, device=x.device)
+    T, K = x.shape
+    x = _unit_stride(x)
+    codes = torch.empty((T, _ceil16(K)), device=x.device, dtype=torch.uint8)
+    scales = torch.empty((_blocks(K), T), device=x.device)
     if T:
-        nat.call("fuma_quantize_rows_fp8", ptr(x), x.stride(0), T, Kp, code, ptr(codes), _ceil16(Kp), ptr(scales),
+        nat.call("fuma_quantize_rows_fp8", ptr(x), x.stride(0), T, K, code, ptr(codes), _ceil16(K), ptr(scales),
                  stream_of(x))
     return codes, scales
 
@@ -83,7 +83,7 @@ def _product(x, w_codes, w_scales, offsets, bias, N, K):
     T, G = x.shape[0], w_codes.shape[0]
     y = torch.empty((T, N), device=x.device, dtype=x.dtype)
     if T:
-        x = _rows(x, K)
+        x = _unit_stride(x)
         nbytes = nat.load().fuma_fp8_work_bytes(T, K)   # the quantised rows and their scales
         work = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
         nat.call("fuma_grouped_linear_fp8", ptr(x), x.stride(0), ptr(w_codes), ptr(w_scales), ptr(offsets), G, ptr(bias),
@@ -96,10 +96,8 @@ class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def compute(x, weight, offsets, bias):
         if bias is not None:
-            pad = weight.Np - weight.N
-            bias = torch.nn.functional.pad(bias, (0, pad)) if pad else bias.contiguous()
-        y = _product(x, weight.codes, weight.scales, offsets, bias, weight.Np, weight.Kp)
-        return y if weight.Np == weight.N else y[:, : weight.N]
+            bias = bias.contiguous()
+        return _product(x, weight.codes, weight.scales, offsets, bias, weight.N, weight.K)
 
     @staticmethod
     def forward(ctx, x, weight, offsets, bias):
@@ -112,8 +110,7 @@ class _Fp8LinearFn(torch.autograd.Function):
     def backward(ctx, g):
         weight = ctx.weight
         offsets = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        dx = _product(g, weight.codes_t, weight.scales_t, offsets, None, weight.Kp, weight.Np)
-        return (dx if weight.Kp == weight.K else dx[:, : weight.K]), None, None, None
+        return _product(g, weight.codes_t, weight.scales_t, offsets, None, weight.K, weight.N), None, None, None
 
 
 def fp8_linear(x: torch.Tensor, weight: Fp8Weight, offsets: torch.Tensor | None = None,

@@ -84,25 +84,10 @@ def _opaque(fn, *args):
     return fn(*args)
 
 
-def _rows(x: torch.Tensor, cols: int) -> torch.Tensor:
-    """``x`` [T, >= width] as an operand: ``cols`` (a multiple of 8) columns, rows a multiple of 8
-    elements apart, 16-byte aligned. A copy only where ``x`` is not that already."""
-    if x.shape[1] != cols:
-        x = torch.nn.functional.pad(x, (0, cols - x.shape[1]))
+def _unit_stride(x: torch.Tensor) -> torch.Tensor:
+    """``x`` [rows, cols] with contiguous rows (any pitch); a copy only where it is not that already."""
     ld, one = x.stride()
-    if one != 1 or ld % 8 or ld < cols or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
-def _matrices(w: torch.Tensor, N: int, K: int) -> torch.Tensor:
-    """``w`` [G, n, k] contiguous, 16-byte aligned, zero-padded to [G, N, K]."""
-    _, n, k = w.shape
-    if n != N or k != K:
-        w = torch.nn.functional.pad(w, (0, K - k, 0, N - n))
-    elif not w.is_contiguous():
-        w = w.contiguous()
-    return w.clone() if w.data_ptr() % 16 else w
+    return x if (one == 1 or x.shape[1] == 1) and ld >= x.shape[1] else x.clone(memory_format=torch.contiguous_format)
 
 
 def _ceil8(n: int) -> int:
@@ -110,10 +95,10 @@ def _ceil8(n: int) -> int:
 
 
 def _split(x: torch.Tensor, offsets, G: int, mat_rows: int):
-    """The two fp16 planes [2, rows, cols] of an fp32 operand [rows, cols] and their block scales
+    """The two fp16 planes [2, rows, cols rounded up to 8] of an fp32 operand [rows, cols] and their block scales
     (``fuma_split_blocks``): of ragged rows, or (``mat_rows`` > 0) of matrices of that many rows."""
     rows, cols = x.shape
-    out = torch.empty((2, rows, cols), device=x.device, dtype=torch.float16)
+    out = torch.empty((2, rows, _ceil8(cols)), device=x.device, dtype=torch.float16)
     blocks = rows // mat_rows * ((mat_rows + 127) // 128) if mat_rows else rows // 128 + G
     scales = torch.empty((cols + 127) // 128 * blocks, device=x.device)
     nat.call("fuma_split_blocks", ptr(x), x.stride(0), rows, cols, ptr(offsets), G, mat_rows, ptr(out), ptr(scales),
@@ -121,21 +106,36 @@ def _split(x: torch.Tensor, offsets, G: int, mat_rows: int):
     return out, scales
 
 
-def _operand(x: torch.Tensor, cols: int, offsets, G: int):
-    """(tensor, leading dimension, scales) of a row operand for the C ABI."""
-    x = _rows(x, cols)
+def _operand(x: torch.Tensor, offsets, G: int):
+    """(tensor, leading dimension, scales) of a row operand for the C ABI: 16-bit rows a multiple of 16 bytes apart and
+    aligned to that (a copy where they are not), fp32 as planes."""
+    x = _unit_stride(x)
+    rows, cols = x.shape
     if x.dtype == torch.float32:
         planes, scales = _split(x, offsets, G, 0)
-        return planes, cols, scales
-    return x, x.stride(0), None
+        return planes, _ceil8(cols), scales
+    ld = x.stride(0)
+    if ld % 8 or x.data_ptr() % 16:
+        out = torch.empty((rows, _ceil8(cols)), device=x.device, dtype=x.dtype)
+        nat.call("fuma_pad_rows", ptr(x), ld, rows, cols, ptr(out), _ceil8(cols), None, 0, 0, 0, stream_of(x))
+        return out, _ceil8(cols), None
+    return x, ld, None
 
 
-def _weight_operand(w: torch.Tensor):
-    """(tensor, scales) of the matrices [G, N, K] for the C ABI."""
+def _weight_operand(w: torch.Tensor, offsets, T: int):
+    """(tensor, leading dimension, scales) of the matrices [G, N, K] for the C ABI, likewise; a copy leaves out the
+    matrices of groups without rows."""
+    if not w.is_contiguous():
+        w = w.contiguous()
+    G, N, K = w.shape
     if w.dtype == torch.float32:
-        G, N, K = w.shape
-        return _split(w.view(G * N, K), None, G, N)
-    return w, None
+        planes, scales = _split(w.view(G * N, K), None, G, N)
+        return planes, _ceil8(K), scales
+    if K % 8 or w.data_ptr() % 16:
+        out = torch.empty((G, N, _ceil8(K)), device=w.device, dtype=w.dtype)
+        nat.call("fuma_pad_rows", ptr(w), K, G * N, K, ptr(out), _ceil8(K), ptr(offsets), G, N, T, stream_of(w))
+        return out, _ceil8(K), None
+    return w, K, None
 
 
 class _GroupedLinearFn(torch.autograd.Function):
@@ -143,18 +143,17 @@ class _GroupedLinearFn(torch.autograd.Function):
     def compute(x, weight, offsets, bias):
         T = x.shape[0]
         G, N, K = weight.shape
-        Np, Kp = _ceil8(N), _ceil8(K)
-        y = torch.empty((T, Np), device=x.device, dtype=x.dtype)
+        y = torch.empty((T, N), device=x.device, dtype=x.dtype)
         if T:
             bias_rows = 0
             if bias is not None:
                 bias_rows = 1 if bias.dim() == 1 else G
-                bias = torch.nn.functional.pad(bias, (0, Np - N)) if Np != N else bias.contiguous()
-            a, lda, a_s = _operand(x, Kp, offsets, G)
-            w, w_s = _weight_operand(_matrices(weight, Np, Kp))
-            nat.call("fuma_grouped_linear", ptr(a), lda, ptr(a_s), ptr(w), ptr(w_s), ptr(offsets), G, ptr(bias), bias_rows, T, Np, Kp,
-                     _DTYPES[x.dtype], ptr(y), ptr(error_flag(x.device)), stream_of(x))
-        return y if Np == N else y[:, :N]
+                bias = bias.contiguous()
+            a, lda, a_s = _operand(x, offsets, G)
+            w, ldw, w_s = _weight_operand(weight, offsets, T)
+            nat.call("fuma_grouped_linear", ptr(a), lda, ptr(a_s), ptr(w), ldw, ptr(w_s), ptr(offsets), G, ptr(bias),
+                     bias_rows, T, N, K, _DTYPES[x.dtype], ptr(y), ptr(error_flag(x.device)), stream_of(x))
+        return y
 
     @staticmethod
     def forward(ctx, x, weight, offsets, bias):
@@ -168,36 +167,33 @@ class _GroupedLinearFn(torch.autograd.Function):
         x, weight, offsets = ctx.saved_tensors
         T = x.shape[0]
         G, N, K = weight.shape
-        Np, Kp = _ceil8(N), _ceil8(K)
-        code = _DTYPES[x.dtype]
+        dev, dt = x.device, x.dtype
+        code = _DTYPES[dt]
         want_x, want_w, _, want_b = ctx.needs_input_grad
         dx = dw = db = None
-        s, err = stream_of(x), ptr(error_flag(x.device))
-        g = _rows(g, Np)
-        a, lda, a_s = _operand(g, Np, offsets, G) if T and (want_x or want_w) else (g, Np, None)
+        s, err = stream_of(x), ptr(error_flag(dev))
+        g = _unit_stride(g)
+        a, lda, a_s = _operand(g, offsets, G) if T and (want_x or want_w) else (g, _ceil8(N), None)
         if want_x:
-            dx = torch.empty(T, Kp, device=x.device, dtype=x.dtype)
+            dx = torch.empty((T, K), device=dev, dtype=dt)
             if T:
-                w, w_s = _weight_operand(_matrices(weight, Np, Kp))
-                nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, ptr(a_s), ptr(w), ptr(w_s), ptr(offsets), G, T, Np, Kp,
-                         code, ptr(dx), err, s)
-            dx = dx if Kp == K else dx[:, :K]
+                w, ldw, w_s = _weight_operand(weight, offsets, T)
+                nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, ptr(a_s), ptr(w), ldw, ptr(w_s), ptr(offsets), G, T, N,
+                         K, code, ptr(dx), err, s)
         if want_w:
-            dw = torch.empty(G, Np, Kp, device=x.device, dtype=x.dtype)
-            b, ldb, b_s = _operand(x, Kp, offsets, G) if T else (x, Kp, None)
-            nbytes = nat.load().fuma_grouped_wgrad_work_bytes(T, Np, Kp, code)
-            work = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
-            nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, ptr(a_s), ptr(b), ldb, ptr(b_s), ptr(offsets), G, T, Np, Kp,
+            dw = torch.empty((G, N, K), device=dev, dtype=dt)
+            b, ldb, b_s = _operand(x, offsets, G) if T else (x, _ceil8(K), None)
+            nbytes = nat.load().fuma_grouped_wgrad_work_bytes(T, N, K, code)
+            work = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+            nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, ptr(a_s), ptr(b), ldb, ptr(b_s), ptr(offsets), G, T, N, K,
                      code, ptr(dw), ptr(work), nbytes, err, s)
-            dw = dw if (Np, Kp) == (N, K) else dw[:, :N, :K]
         if want_b:
             shared = len(ctx.bias_shape) == 1
-            db = torch.empty(*ctx.bias_shape[:-1], Np, device=x.device, dtype=x.dtype)
-            nbytes = nat.load().fuma_grouped_bias_grad_work_bytes(T, Np, 1 if shared else G)
-            work = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
-            nat.call("fuma_grouped_bias_grad", ptr(g), g.stride(0) if T else Np, ptr(offsets), G, 1 if shared else 0, T,
-                     Np, code, ptr(db), ptr(work), nbytes, s)
-            db = db if Np == N else db[..., :N]
+            db = torch.empty(ctx.bias_shape, device=dev, dtype=dt)
+            nbytes = nat.load().fuma_grouped_bias_grad_work_bytes(T, N, 1 if shared else G)
+            work = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+            nat.call("fuma_grouped_bias_grad", ptr(g), g.stride(0) if T else N, ptr(offsets), G, 1 if shared else 0, T, N,
+                     code, ptr(db), ptr(work), nbytes, s)
         return dx, dw, None, db
 
 
@@ -229,8 +225,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     float16. Returns [T, N]; rows outside [offsets[0], offsets[G]) come back as zeros and get zero
     gradients. Differentiable in x, weight and bias (once); repeated calls give the same bits.
 
-    K and N that are not multiples of 8 run on zero-padded copies, rows that are not contiguous
-    or 16-byte aligned on a copy. Bad offset values are recorded in the device error flag
+    16-bit operands whose rows are not contiguous, aligned to 16 bytes and a multiple of 16 bytes apart (an
+    odd K, say) run on a copy. Bad offset values are recorded in the device error flag
     (:func:`flash_uma_b200.linear.check_errors`); an infinite fp32 input may give NaN where fp32
     arithmetic gives an infinity."""
     if torch.compiler.is_compiling():

@@ -332,20 +332,20 @@ int fuma_morton_reorder_noalloc(const float* pos, const int64_t* Z, const int64_
  * launch needs no host copy of it; empty groups are allowed, rows outside [offsets[0],
  * offsets[G]) are written as zeros, and offsets may be NULL for one group of all rows. Offsets that
  * decrease or leave [0, T] put 64 into err_flag (the results are then undefined, all accesses stay in
- * bounds). 1 <= G <= 4096; N and K multiples of 8; leading dimensions (elements) multiples of 8;
- * arrays 16-byte aligned. Work space: see the *_work_bytes functions (0: may be NULL).
+ * bounds). 1 <= G <= 4096; any N and K; leading dimensions (elements) of the operands multiples
+ * of 8 (fuma_pad_rows makes such a copy), arrays 16-byte aligned; outputs contiguous. Work space: see the *_work_bytes functions (0: may be NULL).
  *
  * fp32 operands come as two fp16 planes and their block scales (fuma_split_blocks: x and dy as ragged rows under
- * the same offsets, W with mat_rows = N; the leading dimension is then the column count). Results and
+ * the same offsets, W with mat_rows = N; the leading dimension is then the column count rounded up to 8). Results and
  * biases are fp32. For the 16-bit types the scales are NULL.
  *
  * y[t, n] = sum_k x[t, k] W[g, n, k] + bias (bias_rows 1: bias[n], G: bias[g, n]; may be NULL) */
-int fuma_grouped_linear(const void* x, int64_t ldx, const float* x_scales, const void* W, const float* W_scales,
-                        const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows, int64_t T, int32_t N,
+int fuma_grouped_linear(const void* x, int64_t ldx, const float* x_scales, const void* W, int64_t ldw,
+                        const float* W_scales, const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows, int64_t T, int32_t N,
                         int32_t K, int32_t dtype, void* y, int* err_flag, void* stream);
 /* dx[t, k] = sum_n dy[t, n] W[g, n, k] */
 int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* W,
-                              const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K,
+                              int64_t ldw, const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K,
                               int32_t dtype, void* dx, int* err_flag, void* stream);
 /* dW[g, n, k] = sum over the rows of g of dy[t, n] x[t, k]; zeros for a group without rows. No
  * atomics: the same call gives the same bits. */
@@ -357,13 +357,17 @@ int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const float* dy_scal
 int64_t fuma_grouped_bias_grad_work_bytes(int64_t T, int32_t N, int32_t groups);
 int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets, int32_t G, int32_t shared, int64_t T,
                            int32_t N, int32_t dtype, void* db, void* work, int64_t work_bytes, void* stream);
-/* fp32 [rows, cols] (rows ldx floats apart, cols a multiple of 8) -> two fp16 planes out [2][rows][cols] and block scales:
+/* fp32 [rows, cols] (rows ldx floats apart) -> two fp16 planes out [2][rows][cols rounded up to 8] and block scales:
  * x = scale (hi + lo), scale the power of two (at least 2^-126) that brings a 128 x 128 block's largest finite magnitude
  * to [2^14, 2^15). mat_rows = 0: ragged rows, blocks counted from each group's first row, scales
  * [ceil(cols / 128)][rows / 128 + G]; rows outside the groups are not written. mat_rows > 0: matrices of mat_rows rows,
  * scales [rows / mat_rows][ceil(mat_rows / 128)][ceil(cols / 128)]. */
 int fuma_split_blocks(const float* x, int64_t ldx, int64_t rows, int32_t cols, const int64_t* offsets, int32_t G,
                       int32_t mat_rows, void* out, float* scales, void* stream);
+/* 16-bit rows copied to a pitch of ldo elements (a multiple of 8; columns behind the last hold nothing). offsets (may be
+ * NULL): x is G matrices of mat_rows rows, and those of groups without rows (of T) are left out. */
+int fuma_pad_rows(const void* x, int64_t ldx, int64_t rows, int32_t cols, void* out, int64_t ldo, const int64_t* offsets,
+                  int32_t G, int32_t mat_rows, int64_t T, void* stream);
 /* Block-scaled e4m3 operands: a block of 128 values is stored as codes times the smallest power of two
  * (at least 2^-126) that brings its largest magnitude to 448 or below, rounded to nearest even; a block
  * with a value that is not finite gets the scale NaN.

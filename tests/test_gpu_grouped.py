@@ -85,7 +85,11 @@ SHAPES = [
     ([0, 5, 0, 130, 1, 0, 127, 128, 0], 72, 136, 0, 0),
     ([300, 20], 256, 264, 7, 200),
     ([33, 200, 64], 520, 392, 0, 3),
-    ([17, 0, 40], 13, 7, 2, 1),          # odd widths: padded copies
+    ([17, 0, 40], 13, 7, 2, 1),          # odd widths
+    ([9, 1], 1, 1, 1, 0),
+    ([50, 130, 0, 2], 65, 129, 0, 3),
+    ([40, 0, 300], 535, 583, 1, 0),
+    ([31], 260, 131, 0, 0),
     ([129], 1032, 520, 0, 0),
 ]
 
@@ -106,16 +110,18 @@ def test_forward_and_gradients(shape, bias, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-def test_long_groups_cut_over_the_contraction(dt):
+@pytest.mark.parametrize("K,N", [(72, 40), (71, 33), (70, 44)])
+def test_long_groups_cut_over_the_contraction(dt, K, N):
     """Groups longer than one chunk of the weight gradient, next to short and empty ones, with chunk
     ends inside tiles."""
-    x, w, off, b, gy = _make([2047, 5001, 0, 2049, 6200, 3], 72, 40, dt, "group", 1, 5)
+    x, w, off, b, gy = _make([2047, 5001, 0, 2049, 6200, 3], K, N, dt, "group", 1, 5)
     _check(x, w, off, b, gy, dt)
 
 
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("lens,K,N,head,tail", [([20000], 72, 256, 0, 0), ([9001, 0, 257, 8000, 128, 129], 136, 640, 3, 77),
-                                                ([5000, 5100], 520, 392, 0, 0)])
+                                                ([5000, 5100], 520, 392, 0, 0), ([60000, 60001], 264, 264, 0, 0),
+                                                ([30001, 0, 20000, 257, 25128, 129], 520, 640, 3, 77)])
 def test_long_groups_on_cta_pairs(lens, K, N, head, tail, dt):
     """Groups long enough for the 256-row tiles of CTA pairs, with last tiles of 1, 128, 129 and 256 rows."""
     x, w, off, b, gy = _make(lens, K, N, dt, "shared", head, tail)

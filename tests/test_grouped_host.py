@@ -18,29 +18,31 @@ P = 4096   # a 16-byte aligned non-null address that no check reads
 
 @pytest.mark.parametrize("change,message", [
     (dict(G=0), b"G=0"), (dict(G=4097), b"G=4097"), (dict(T=-1), b"T=-1"), (dict(T=2 ** 31), b"out of range"),
-    (dict(N=12), b"multiples of 8"), (dict(K=0), b"multiples of 8"), (dict(dtype=3), b"dtype=3"),
+    (dict(N=0), b"positive"), (dict(K=0), b"positive"), (dict(ldw=8), b"ldw=8"), (dict(ldw=20), b"ldw=20"), (dict(dtype=3), b"dtype=3"),
     (dict(ldx=8), b"ldx=8"), (dict(ldx=20), b"ldx=20"), (dict(bias=P, bias_rows=2), b"bias_rows=2"),
     (dict(x=None), b"null pointer"), (dict(dtype=0, xs=None), b"null pointer"), (dict(dtype=0, ldx=24), b"planes"), (dict(offsets=None), b"one group only"),
     (dict(T=2 ** 31 - 512, N=2 ** 20, G=1), b"too many output tiles"), (dict(G=4096, N=2 ** 20), b"too large"),
 ])
 def test_grouped_linear_refusals(lib, change, message):
-    a = dict(x=P, ldx=16, xs=P, W=P, ws=P, offsets=P, G=3, bias=None, bias_rows=0, T=10, N=24, K=16, dtype=1, y=P)
+    a = dict(x=P, ldx=16, xs=P, W=P, ldw=16, ws=P, offsets=P, G=3, bias=None, bias_rows=0, T=10, N=24, K=16, dtype=1, y=P)
     a.update(change)
     assert lib.fuma_grouped_linear(*a.values(), None, None) == -1
     assert message in lib.fuma_last_error()
 
 
 def test_alignment_refused(lib):
-    assert lib.fuma_grouped_linear(P + 8, 16, None, P, None, P, 3, None, 0, 10, 24, 16, 1, P, None, None) == -2
-    assert lib.fuma_grouped_linear_dgrad(P, 24, None, P + 2, None, P, 3, 10, 24, 16, 1, P, None, None) == -2
+    assert lib.fuma_grouped_linear(P + 8, 16, None, P, 16, None, P, 3, None, 0, 10, 24, 16, 1, P, None, None) == -2
+    assert lib.fuma_grouped_linear_dgrad(P, 24, None, P + 2, 16, None, P, 3, 10, 24, 16, 1, P, None, None) == -2
     assert lib.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P + 4, 16, P, None) == -2
     assert lib.fuma_mix_experts(P, 4, 1, P + 4, 2, 4, 64, 0, P, None, None) == -2
 
 
 def test_other_refusals(lib):
     f = lib
-    assert f.fuma_grouped_linear_dgrad(P, 16, None, P, None, P, 3, 10, 24, 16, 1, P, None, None) == -1   # lddy < N
-    assert f.fuma_split_blocks(P, 12, 4, 12, P, 1, 0, P, P, None) == -1                           # cols
+    assert f.fuma_grouped_linear_dgrad(P, 16, None, P, 16, None, P, 3, 10, 24, 16, 1, P, None, None) == -1   # lddy < N
+    assert f.fuma_split_blocks(P, 8, 4, 12, P, 1, 0, P, P, None) == -1                            # ldx
+    assert f.fuma_pad_rows(P, 12, 4, 12, P, 12, None, 0, 0, 0, None) == -1                        # ldo
+    assert f.fuma_pad_rows(P, 12, 5, 12, P, 16, P, 2, 2, 9, None) == -1                           # rows != G * mat_rows
     assert f.fuma_split_blocks(P, 16, 10, 16, None, 0, 4, P, P, None) == -1                       # mat_rows
     assert f.fuma_split_blocks(P, 16, 10, 16, None, 2, 0, P, P, None) == -1                       # no offsets
     assert f.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P, 24, P, None) == -1                        # ldq
@@ -52,7 +54,7 @@ def test_other_refusals(lib):
     assert f.fuma_mix_experts_bwd(P, P, 4, 1, P, 2, 4, 64, 0, P, P, P, 4, None, None) == -1                # work space
     assert f.fuma_mix_experts_bwd(P, P, 4, 1, P, 2, 4, 64, 0, None, None, P, 1 << 20, None, None) == -1
     # nothing to do: no launch, no device needed
-    assert f.fuma_grouped_linear(None, 16, None, None, None, None, 3, None, 0, 0, 24, 16, 1, None, None, None) == 0
+    assert f.fuma_grouped_linear(None, 16, None, None, 16, None, None, 3, None, 0, 0, 24, 16, 1, None, None, None) == 0
     assert f.fuma_mix_experts(None, 4, 1, None, 0, 4, 64, 0, None, None, None) == 0
 
 
