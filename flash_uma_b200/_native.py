@@ -56,7 +56,7 @@ _SIGS = {
     "fuma_grouped_linear_dgrad": [_P, _I64, _P, _P, _I64, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P],
     "fuma_grouped_linear_wgrad": [_P, _I64, _P, _P, _I64, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I64, _P, _P],
     "fuma_grouped_bias_grad": [_P, _I64, _P, _I32, _I32, _I64, _I32, _I32, _P, _P, _I64, _P],
-    "fuma_split_blocks": [_P, _I64, _I64, _I32, _P, _I32, _I32, _P, _P, _P],
+    "fuma_split_blocks": [_P, _I64, _I64, _I32, _P, _I32, _I32, _I64, _P, _P, _P],
     "fuma_pad_rows": [_P, _I64, _I64, _I32, _P, _I64, _P, _I32, _I32, _I64, _P],
     "fuma_quantize_rows_fp8": [_P, _I64, _I64, _I32, _I32, _P, _I64, _P, _P],
     "fuma_quantize_weight_fp8": [_P, _I32, _I32, _I32, _P, _I64, _P, _P, _I64, _P, _P],

@@ -826,19 +826,20 @@ int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets,
 }
 
 int fuma_split_blocks(const float* x, int64_t ldx, int64_t rows, int32_t cols, const int64_t* offsets, int32_t G,
-                      int32_t mat_rows, void* out, float* scales, void* stream) {
+                      int32_t mat_rows, int64_t T, void* out, float* scales, void* stream) {
   REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && cols > 0, "split_blocks: bad shape rows=%lld cols=%d", (long long)rows,
           cols);
   REQUIRE(ldx >= cols, "split_blocks: ldx=%lld must be >= cols", (long long)ldx);
   REQUIRE(mat_rows >= 0 && (mat_rows == 0 || rows % mat_rows == 0), "split_blocks: mat_rows=%d must divide rows", mat_rows);
-  REQUIRE(mat_rows > 0 || (G >= 1 && G <= kMaxGroups && (offsets || G == 1)), "split_blocks: bad groups (G=%d)", G);
+  REQUIRE(mat_rows > 0 ? !offsets || rows == (int64_t)G * mat_rows : G >= 1 && G <= kMaxGroups && (offsets || G == 1),
+          "split_blocks: bad groups (G=%d)", G);
   if (rows == 0) return FUMA_OK;
   const int64_t slots = mat_rows > 0 ? rows / mat_rows * ((mat_rows + 127) / 128) : split_slots(rows, G);
   REQUIRE(slots * ((cols + 127) / 128) < (int64_t(1) << 31), "split_blocks: too many blocks");
   REQUIRE(x && out && scales, "split_blocks: null pointer");
   REQUIRE_ALIGNED(out, "out");
   BIND(x);
-  launch_split_blocks(x, ldx, rows, cols, offsets, G, mat_rows, out, scales, (cudaStream_t)stream);
+  launch_split_blocks(x, ldx, rows, cols, offsets, G, mat_rows, T, out, scales, (cudaStream_t)stream);
   return launched("split_blocks");
 }
 
@@ -847,7 +848,8 @@ int fuma_pad_rows(const void* x, int64_t ldx, int64_t rows, int32_t cols, void* 
   REQUIRE(rows >= 0 && cols > 0 && ldx >= cols, "pad_rows: bad shape rows=%lld cols=%d ldx=%lld", (long long)rows, cols,
           (long long)ldx);
   REQUIRE(ldo >= cols && ldo % 8 == 0, "pad_rows: ldo=%lld must be >= cols and a multiple of 8", (long long)ldo);
-  REQUIRE(!offsets || (G >= 1 && mat_rows > 0 && rows == (int64_t)G * mat_rows), "pad_rows: rows must be G * mat_rows");
+  REQUIRE(!offsets || (G >= 1 && G <= kMaxGroups && mat_rows > 0 && rows == (int64_t)G * mat_rows),
+          "pad_rows: rows must be G * mat_rows");
   if (rows == 0) return FUMA_OK;
   REQUIRE(x && out, "pad_rows: null pointer");
   REQUIRE_ALIGNED(out, "out");

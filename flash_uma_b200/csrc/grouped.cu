@@ -680,6 +680,23 @@ __global__ void __launch_bounds__(kGThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_item_empty[n % kRing]);
       if (t.kblocks < 0) break;
+      if (kMode == kModeDw && t.kblocks == 0) {   // a group without rows: this item's share of its matrix, as one run
+        const int esize = p.out_dtype == kDtypeF32 ? 4 : 2, unit = 16 / esize;
+        const int64_t n = (int64_t)p.M * p.N, share = (n + p.tiles_m * p.tiles_n - 1) / (p.tiles_m * p.tiles_n);
+        const int64_t i0 = min((t.m0 / kBM * p.tiles_n + t.n0 / p.bn) * share, n), i1 = min(i0 + share, n);
+        const int64_t a = t.g * n + i0, b = t.g * n + i1;
+        const int64_t lo = min((a + unit - 1) / unit * unit, b), hi = max(b / unit * unit, lo);   // 16-byte steps in [lo, hi)
+        const int tid = threadIdx.x - kEpiWarp0 * 32;
+        uint8_t* c = static_cast<uint8_t*>(p.C);
+        for (int64_t i = lo + (int64_t)tid * unit; i < hi; i += (int64_t)kEpiWarps * 32 * unit)
+          *reinterpret_cast<uint4*>(c + i * esize) = make_uint4(0u, 0u, 0u, 0u);
+        const int64_t e = tid < unit ? a + tid : hi + (tid - unit);   // the ends, at most unit - 1 elements each
+        if (tid < 2 * unit && e < (tid < unit ? lo : b)) {
+          if (esize == 4) reinterpret_cast<float*>(c)[e] = 0.0f;
+          else reinterpret_cast<uint16_t*>(c)[e] = 0;
+        }
+        continue;
+      }
       const int segs = (t.kblocks + L::kSegBlocks - 1) / L::kSegBlocks;
       const int n0 = t.n0 + col0;
       const int rows = t.rows - q * 32;                        // of this warp (may be <= 0)
@@ -820,6 +837,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
             __syncwarp();
             if (!rows16) {
               if (c * 32 + lane < ncols)
+#pragma unroll 4
                 for (int r = 0; r < min(rows, 32); ++r)
                   reinterpret_cast<float*>(out)[(y0 + r) * ld + x0 + c * 32 + lane] =
                       *reinterpret_cast<const float*>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
@@ -848,14 +866,16 @@ __global__ void __launch_bounds__(kGThreads, 1)
             }
             __syncwarp();
             if (!rows16) {
-              for (int r = 0; r < min(rows, 32); ++r)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const int k = h * 32 + lane;
-                  if (c * 64 + k < ncols)
-                    reinterpret_cast<uint16_t*>(out)[(y0 + r) * ld + x0 + c * 64 + k] =
+              for (int h = 0; h < 2; ++h) {
+                const int k = h * 32 + lane;
+                uint16_t* col = reinterpret_cast<uint16_t*>(out) + y0 * ld + x0 + c * 64 + k;
+                if (c * 64 + k < ncols)
+#pragma unroll 4
+                  for (int r = 0; r < min(rows, 32); ++r)
+                    col[r * ld] =
                         *reinterpret_cast<const uint16_t*>(stage + r * 128 + (((k >> 3) ^ (r & 7)) << 4) + (k & 7) * 2);
-                }
+              }
             } else if (c * 64 + jj * 8 < ncols) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
@@ -1080,16 +1100,17 @@ __global__ void __launch_bounds__(32 * kJoinWarps) grouped_colsum_join_kernel(co
 }
 
 // ---- fp32 -> two fp16 planes under block scales ------------------------------------------------------
-// One thread block per 128 x 128 block: 16 values of 4 columns per thread, all loaded before the largest magnitude is
-// known, split and written: one pass, 4 bytes in and 4 out per value. Row blocks: of the ragged rows, the
+// One thread block per 128 x 128 block: 8 columns of 8 rows per thread, all loaded before the largest magnitude is
+// known, split and written: one pass, 4 bytes in and 4 out per value. 16-byte stores: 66 us where 4 columns of 16 rows
+// took 79 (and 66 with registers for a third resident block, which spills). Row blocks: of the ragged rows, the
 // 128-row tiles of each group (counted from the group's first row, as the maps cut it; the tile's slot is group
 // start / 128 + group + tile, distinct because one tile or one group further on moves it by at least 1), or, with
-// mat_rows > 0, of matrices of mat_rows rows each. A value that is not finite keeps hi alone and does not set the scale.
+// mat_rows > 0, of matrices of mat_rows rows each, but (given offsets) those of groups without rows. A value that is not finite keeps hi alone and does not set the scale.
 // kVec: rows 16-byte aligned. Planes [rows][ldp], ldp = cols rounded up to 8.
 template <bool kVec>
 __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows,
                                                            int cols, const int64_t* __restrict__ off, int G,
-                                                           int mat_rows, __half* __restrict__ out,
+                                                           int mat_rows, int64_t T, __half* __restrict__ out,
                                                            float* __restrict__ scales, int64_t slots) {
   __shared__ uint32_t wmax[8];
   const int kblocks = (cols + 127) / 128;
@@ -1099,6 +1120,7 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restri
   if (mat_rows > 0) {
     const int blocks = (mat_rows + 127) / 128;
     const int64_t m = slot / blocks;
+    if (off && group_len(off, (int)m, T) == 0) return;
     const int i = (int)(slot - m * blocks);
     row0 = m * mat_rows + i * 128;
     n = mat_rows - i * 128;
@@ -1118,34 +1140,36 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restri
   if (n <= 0) return;
   if (n > 128) n = 128;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = kb * 128 + lane * 4;
-  float4 v[16];
+  const int c = kb * 128 + (lane & 15) * 8, r0 = w * 2 + (lane >> 4);
+  float v[8][8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = w + 8 * i;
-    v[i] = f4(0.0f);
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
     if (r < n) {
       const float* src = x + (row0 + r) * ldx + c;
       if constexpr (kVec) {
-        if (c < cols) v[i] = ld4_stream(src);
+        if (c < cols) {
+          const float4 a = ld4_stream(src), b = ld4_stream(src + 4);
+          v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
+          v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
+        }
       } else {
-        if (c < cols) v[i].x = __ldcs(src);
-        if (c + 1 < cols) v[i].y = __ldcs(src + 1);
-        if (c + 2 < cols) v[i].z = __ldcs(src + 2);
-        if (c + 3 < cols) v[i].w = __ldcs(src + 3);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (c + k < cols) v[i][k] = __ldcs(src + k);
       }
     }
   }
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float f[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+  for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = __float_as_uint(v[i][j]) & 0x7fffffffu;
       m = max(m, b < 0x7f800000u ? b : 0u);
     }
-  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o));
   if (lane == 0) wmax[w] = m;
@@ -1160,21 +1184,21 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restri
   if (c >= ldp) return;
   const int64_t plane = rows * ldp;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = w + 8 * i;
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i;
     if (r < n) {
-      const float f[4] = {v[i].x * inv, v[i].y * inv, v[i].z * inv, v[i].w * inv};
-      __half h[4], l[4];
+      __half h[8], l[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        h[j] = __float2half_rn(f[j]);
-        l[j] = __float2half_rn(fabsf(f[j]) <= 3.402823466e38f ? f[j] - __half2float(h[j]) : 0.0f);
+      for (int j = 0; j < 8; ++j) {
+        const float f = v[i][j] * inv;
+        h[j] = __float2half_rn(f);
+        l[j] = __float2half_rn(fabsf(f) <= 3.402823466e38f ? f - __half2float(h[j]) : 0.0f);
       }
-      uint2 u;
-      memcpy(&u, h, 8);
-      *reinterpret_cast<uint2*>(out + (row0 + r) * ldp + c) = u;
-      memcpy(&u, l, 8);
-      *reinterpret_cast<uint2*>(out + plane + (row0 + r) * ldp + c) = u;
+      uint4 u;
+      memcpy(&u, h, 16);
+      *reinterpret_cast<uint4*>(out + (row0 + r) * ldp + c) = u;
+      memcpy(&u, l, 16);
+      *reinterpret_cast<uint4*>(out + plane + (row0 + r) * ldp + c) = u;
     }
   }
 }
@@ -1390,38 +1414,53 @@ cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const in
 int64_t split_slots(int64_t rows, int G) { return rows / 128 + G; }
 
 void launch_split_blocks(const float* x, int64_t ldx, int64_t rows, int cols, const int64_t* off, int G, int mat_rows,
-                         void* out, float* scales, cudaStream_t s) {
+                         int64_t T, void* out, float* scales, cudaStream_t s) {
   const int64_t slots = mat_rows > 0 ? rows / mat_rows * ((mat_rows + 127) / 128) : split_slots(rows, G);
   const int64_t blocks = slots * ((cols + 127) / 128);
-  const bool vec = ldx % 4 == 0 && cols % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  const bool vec = ldx % 4 == 0 && cols % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   auto kern = vec ? split_blocks_kernel<true> : split_blocks_kernel<false>;
-  kern<<<(unsigned)blocks, 256, 0, s>>>(x, ldx, rows, cols, off, G, mat_rows, static_cast<__half*>(out), scales, slots);
+  kern<<<(unsigned)blocks, 256, 0, s>>>(x, ldx, rows, cols, off, G, mat_rows, T, static_cast<__half*>(out), scales, slots);
 }
 
-// 16-bit rows to a 16-byte pitch (for TMA), 8 values per thread; columns behind the last are left as they are (the tensor
-// maps end before them). With offsets: rows of matrices (mat_rows each) whose group has no rows are left out.
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t rows, int cols,
+// 16-bit rows to a 16-byte pitch (for TMA): 8 values per lane in aligned 4-byte loads (a load covers a byte that is needed, so
+// it stays in the allocation), as many lanes on a row as it has chunks. Columns behind the last hold nothing (the tensor maps
+// end before them). Block column y is a matrix of mat_rows rows, left out if its group has no rows; without offsets, the
+// one run of rows. Bound by HBM: 120,001
+// rows of 641 and 767 values, 980 MB read and written, in 174 us.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t mat_rows, int cols,
                                                        uint16_t* __restrict__ out, int64_t ldo,
-                                                       const int64_t* __restrict__ off, int mat_rows, int64_t T) {
-  const int c8 = (cols + 7) / 8;
-  const int64_t total = rows * c8;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / c8;
-    const int c = (int)(i - r * c8) * 8;
-    if (off && group_len(off, (int)(r / mat_rows), T) == 0) continue;
-    uint16_t v[8];
+                                                       const int64_t* __restrict__ off, int64_t T, int lanes) {
+  if (off && group_len(off, blockIdx.y, T) == 0) return;
+  const int c8 = (cols + 7) / 8, per = 256 / lanes, l = threadIdx.x & (lanes - 1);
+  const int64_t row0 = (int64_t)blockIdx.y * mat_rows;
+  for (int64_t m = (int64_t)blockIdx.x * per + threadIdx.x / lanes; m < mat_rows; m += (int64_t)gridDim.x * per) {
+    const uint16_t* src = x + (row0 + m) * ldx;
+    uint4* dst = reinterpret_cast<uint4*>(out + (row0 + m) * ldo);
+    const bool odd = reinterpret_cast<uintptr_t>(src) & 2;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(src - odd);
+#pragma unroll 4
+    for (int j = l; j < c8; j += lanes) {
+      uint32_t w[5];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? x[r * ldx + c + k] : 0;
-    uint4 u;
-    memcpy(&u, v, 16);
-    *reinterpret_cast<uint4*>(out + r * ldo + c) = u;
+      for (int k = 0; k < 5; ++k) w[k] = j * 8 + 2 * k < cols + odd ? __ldcs(words + j * 4 + k) : 0u;
+      uint4 u;
+      u.x = odd ? __funnelshift_r(w[0], w[1], 16) : w[0];
+      u.y = odd ? __funnelshift_r(w[1], w[2], 16) : w[1];
+      u.z = odd ? __funnelshift_r(w[2], w[3], 16) : w[2];
+      u.w = odd ? __funnelshift_r(w[3], w[4], 16) : w[3];
+      dst[j] = u;
+    }
   }
 }
 
 void launch_pad_rows(const void* x, int64_t ldx, int64_t rows, int cols, void* out, int64_t ldo, const int64_t* off,
                      int mat_rows, int64_t T, cudaStream_t s) {
-  pad_rows_kernel<<<grid_resident(pad_rows_kernel, 256, rows * ((cols + 7) / 8), 256), 256, 0, s>>>(
-      static_cast<const uint16_t*>(x), ldx, rows, cols, static_cast<uint16_t*>(out), ldo, off, mat_rows, T);
+  int lanes = 1;
+  while (lanes < 32 && lanes < (cols + 7) / 8) lanes *= 2;
+  const int64_t m = off ? mat_rows : rows, mats = off ? rows / mat_rows : 1;
+  const int64_t want = (m + 256 / lanes - 1) / (256 / lanes), most = (int64_t)8 * sm_count();
+  pad_rows_kernel<<<dim3((unsigned)(want < most ? want : most), (unsigned)mats), 256, 0, s>>>(
+      static_cast<const uint16_t*>(x), ldx, m, cols, static_cast<uint16_t*>(out), ldo, off, T, lanes);
 }
 
 }  // namespace fuma

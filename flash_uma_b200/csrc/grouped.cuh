@@ -109,7 +109,7 @@ cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const in
 // of matrices of mat_rows rows [matrices][ceil(mat_rows / 128)][ceil(cols / 128)].
 int64_t split_slots(int64_t rows, int G);
 void launch_split_blocks(const float* x, int64_t ldx, int64_t rows, int cols, const int64_t* off, int G, int mat_rows,
-                         void* out, float* scales, cudaStream_t s);
+                         int64_t T, void* out, float* scales, cudaStream_t s);
 
 // 16-bit rows copied to a pitch of ldo (a multiple of 8) elements; see the kernel.
 void launch_pad_rows(const void* x, int64_t ldx, int64_t rows, int cols, void* out, int64_t ldo, const int64_t* off,

@@ -14,7 +14,7 @@ import torch
 
 from . import _native as nat
 from ._native import ptr, stream_of
-from .grouped import (_DTYPES, MAX_GROUPS, _apply, _check_dtype, _opaque, _same_device, _unit_stride, check_groups,
+from .grouped import (_DTYPES, MAX_GROUPS, _apply, _check_dtype, _once, _opaque, _same_device, _unit_stride, check_groups,
                       guard_capture)
 from .linear import error_flag
 
@@ -106,7 +106,7 @@ class _Fp8LinearFn(torch.autograd.Function):
         return _Fp8LinearFn.compute(x, weight, offsets, bias)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         weight = ctx.weight
         offsets = ctx.saved_tensors[0] if ctx.saved_tensors else None

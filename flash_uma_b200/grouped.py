@@ -17,6 +17,7 @@ products: 22 bits over the whole fp32 range, no range error), bf16 and fp16 (fp3
 """
 from __future__ import annotations
 
+import threading
 import weakref
 
 import torch
@@ -45,6 +46,7 @@ def _same_device(dev: torch.device, **others) -> None:
 
 # autograd nodes of eager calls, while their graph is alive
 _live_nodes: "weakref.WeakSet" = weakref.WeakSet()
+_live_lock = threading.Lock()
 
 
 def guard_capture(*inputs) -> bool:
@@ -56,7 +58,9 @@ def guard_capture(*inputs) -> bool:
         return False
     if torch.is_grad_enabled():
         leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
-        for node in list(_live_nodes):
+        with _live_lock:
+            nodes = list(_live_nodes)
+        for node in nodes:
             for edge, _ in node.next_functions:
                 held = getattr(edge, "variable", None)
                 if held is not None and any(held is t for t in leaves):
@@ -73,9 +77,19 @@ def _apply(fn, capturing: bool, *args):
             if isinstance(t, torch.Tensor) and t.requires_grad:
                 out = fn.apply(*args)
                 if not capturing:
-                    _live_nodes.add(out.grad_fn)
+                    with _live_lock:
+                        _live_nodes.add(out.grad_fn)
                 return out
     return fn.compute(*args)
+
+
+def _once(backward):
+    """``once_differentiable`` only where a second derivative may be asked for: its bookkeeping costs 5 us a call."""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 @torch.compiler.disable
@@ -94,15 +108,16 @@ def _ceil8(n: int) -> int:
     return (n + 7) // 8 * 8
 
 
-def _split(x: torch.Tensor, offsets, G: int, mat_rows: int):
+def _split(x: torch.Tensor, offsets, G: int, mat_rows: int, T: int):
     """The two fp16 planes [2, rows, cols rounded up to 8] of an fp32 operand [rows, cols] and their block scales
-    (``fuma_split_blocks``): of ragged rows, or (``mat_rows`` > 0) of matrices of that many rows."""
+    (``fuma_split_blocks``): of ragged rows, or (``mat_rows`` > 0) of matrices of that many rows, those of groups
+    with rows (of T)."""
     rows, cols = x.shape
     out = torch.empty((2, rows, _ceil8(cols)), device=x.device, dtype=torch.float16)
     blocks = rows // mat_rows * ((mat_rows + 127) // 128) if mat_rows else rows // 128 + G
     scales = torch.empty((cols + 127) // 128 * blocks, device=x.device)
-    nat.call("fuma_split_blocks", ptr(x), x.stride(0), rows, cols, ptr(offsets), G, mat_rows, ptr(out), ptr(scales),
-             stream_of(x))
+    nat.call("fuma_split_blocks", ptr(x), x.stride(0), rows, cols, ptr(offsets), G, mat_rows, T, ptr(out),
+             ptr(scales), stream_of(x))
     return out, scales
 
 
@@ -112,7 +127,7 @@ def _operand(x: torch.Tensor, offsets, G: int):
     x = _unit_stride(x)
     rows, cols = x.shape
     if x.dtype == torch.float32:
-        planes, scales = _split(x, offsets, G, 0)
+        planes, scales = _split(x, offsets, G, 0, rows)
         return planes, _ceil8(cols), scales
     ld = x.stride(0)
     if ld % 8 or x.data_ptr() % 16:
@@ -129,7 +144,7 @@ def _weight_operand(w: torch.Tensor, offsets, T: int):
         w = w.contiguous()
     G, N, K = w.shape
     if w.dtype == torch.float32:
-        planes, scales = _split(w.view(G * N, K), None, G, N)
+        planes, scales = _split(w.view(G * N, K), offsets, G, N, T)
         return planes, _ceil8(K), scales
     if K % 8 or w.data_ptr() % 16:
         out = torch.empty((G, N, _ceil8(K)), device=w.device, dtype=w.dtype)
@@ -140,56 +155,64 @@ def _weight_operand(w: torch.Tensor, offsets, T: int):
 
 class _GroupedLinearFn(torch.autograd.Function):
     @staticmethod
-    def compute(x, weight, offsets, bias):
+    def compute(x, weight, offsets, bias, keep_x=False, keep_w=False):
+        """y; with ``keep_x`` or ``keep_w``, y and those of the two operands as the kernels read them: the same bytes that
+        the backward pass needs again (fp32: planes instead of the values), laid out once."""
         T = x.shape[0]
         G, N, K = weight.shape
         y = torch.empty((T, N), device=x.device, dtype=x.dtype)
+        a, w = (x, _ceil8(K), None), (weight, _ceil8(K), None)
         if T:
             bias_rows = 0
             if bias is not None:
                 bias_rows = 1 if bias.dim() == 1 else G
                 bias = bias.contiguous()
-            a, lda, a_s = _operand(x, offsets, G)
-            w, ldw, w_s = _weight_operand(weight, offsets, T)
-            nat.call("fuma_grouped_linear", ptr(a), lda, ptr(a_s), ptr(w), ldw, ptr(w_s), ptr(offsets), G, ptr(bias),
-                     bias_rows, T, N, K, _DTYPES[x.dtype], ptr(y), ptr(error_flag(x.device)), stream_of(x))
+            a, w = _operand(x, offsets, G), _weight_operand(weight, offsets, T)
+            nat.call("fuma_grouped_linear", ptr(a[0]), a[1], ptr(a[2]), ptr(w[0]), w[1], ptr(w[2]), ptr(offsets), G,
+                     ptr(bias), bias_rows, T, N, K, _DTYPES[x.dtype], ptr(y), ptr(error_flag(x.device)), stream_of(x))
+        if keep_x or keep_w:
+            return y, a if keep_x else (None, 0, None), w if keep_w else (None, 0, None)
         return y
 
     @staticmethod
     def forward(ctx, x, weight, offsets, bias):
-        ctx.save_for_backward(x, weight, offsets)
-        ctx.bias_shape = None if bias is None else bias.shape
-        return _GroupedLinearFn.compute(x, weight, offsets, bias)
+        want_x, want_w, _, _ = ctx.needs_input_grad
+        a = w = (None, 0, None)
+        out = _GroupedLinearFn.compute(x, weight, offsets, bias, want_w, want_x)
+        if want_w or want_x:
+            out, a, w = out
+        ctx.save_for_backward(a[0], a[2], w[0], w[2], offsets)
+        ctx.lds = a[1], w[1]
+        ctx.shapes = x.shape[0], weight.shape, None if bias is None else bias.shape
+        return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
-        x, weight, offsets = ctx.saved_tensors
-        T = x.shape[0]
-        G, N, K = weight.shape
-        dev, dt = x.device, x.dtype
+        b, b_s, w, w_s, offsets = ctx.saved_tensors
+        ldb, ldw = ctx.lds
+        T, (G, N, K), bias_shape = ctx.shapes
+        dev, dt = g.device, g.dtype
         code = _DTYPES[dt]
         want_x, want_w, _, want_b = ctx.needs_input_grad
         dx = dw = db = None
-        s, err = stream_of(x), ptr(error_flag(dev))
+        s, err = stream_of(g), ptr(error_flag(dev))
         g = _unit_stride(g)
         a, lda, a_s = _operand(g, offsets, G) if T and (want_x or want_w) else (g, _ceil8(N), None)
         if want_x:
             dx = torch.empty((T, K), device=dev, dtype=dt)
             if T:
-                w, ldw, w_s = _weight_operand(weight, offsets, T)
                 nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, ptr(a_s), ptr(w), ldw, ptr(w_s), ptr(offsets), G, T, N,
                          K, code, ptr(dx), err, s)
         if want_w:
             dw = torch.empty((G, N, K), device=dev, dtype=dt)
-            b, ldb, b_s = _operand(x, offsets, G) if T else (x, _ceil8(K), None)
             nbytes = nat.load().fuma_grouped_wgrad_work_bytes(T, N, K, code)
             work = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
             nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, ptr(a_s), ptr(b), ldb, ptr(b_s), ptr(offsets), G, T, N, K,
                      code, ptr(dw), ptr(work), nbytes, err, s)
         if want_b:
-            shared = len(ctx.bias_shape) == 1
-            db = torch.empty(ctx.bias_shape, device=dev, dtype=dt)
+            shared = len(bias_shape) == 1
+            db = torch.empty(bias_shape, device=dev, dtype=dt)
             nbytes = nat.load().fuma_grouped_bias_grad_work_bytes(T, N, 1 if shared else G)
             work = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
             nat.call("fuma_grouped_bias_grad", ptr(g), g.stride(0) if T else N, ptr(offsets), G, 1 if shared else 0, T, N,
@@ -261,7 +284,7 @@ class _MixFn(torch.autograd.Function):
         return _MixFn.compute(coeff, experts)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         coeff, experts = ctx.saved_tensors
         S, E = coeff.shape
@@ -277,7 +300,7 @@ class _MixFn(torch.autograd.Function):
             nbytes = nat.load().fuma_mix_experts_work_bytes(S, E, P, code)
             work = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         if want_e:
-            de = torch.empty(experts.shape, device=dev, dtype=experts.dtype)
+            de = torch.empty_like(experts, memory_format=torch.contiguous_format)
         g, x = _flat(g), _flat(experts)
         nat.call("fuma_mix_experts_bwd", ptr(g), ptr(coeff), coeff.stride(0), coeff.stride(1), ptr(x), S, E, P, code,
                  ptr(dc), ptr(de), ptr(work), nbytes, ptr(error_flag(dev)), stream_of(g))

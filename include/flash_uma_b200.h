@@ -361,9 +361,10 @@ int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets,
  * x = scale (hi + lo), scale the power of two (at least 2^-126) that brings a 128 x 128 block's largest finite magnitude
  * to [2^14, 2^15). mat_rows = 0: ragged rows, blocks counted from each group's first row, scales
  * [ceil(cols / 128)][rows / 128 + G]; rows outside the groups are not written. mat_rows > 0: matrices of mat_rows rows,
- * scales [rows / mat_rows][ceil(mat_rows / 128)][ceil(cols / 128)]. */
+ * scales [rows / mat_rows][ceil(mat_rows / 128)][ceil(cols / 128)]; with offsets, the matrices of groups without rows
+ * (of T) are not written. */
 int fuma_split_blocks(const float* x, int64_t ldx, int64_t rows, int32_t cols, const int64_t* offsets, int32_t G,
-                      int32_t mat_rows, void* out, float* scales, void* stream);
+                      int32_t mat_rows, int64_t T, void* out, float* scales, void* stream);
 /* 16-bit rows copied to a pitch of ldo elements (a multiple of 8; columns behind the last hold nothing). offsets (may be
  * NULL): x is G matrices of mat_rows rows, and those of groups without rows (of T) are left out. */
 int fuma_pad_rows(const void* x, int64_t ldx, int64_t rows, int32_t cols, void* out, int64_t ldo, const int64_t* offsets,

@@ -40,11 +40,11 @@ def test_alignment_refused(lib):
 def test_other_refusals(lib):
     f = lib
     assert f.fuma_grouped_linear_dgrad(P, 16, None, P, 16, None, P, 3, 10, 24, 16, 1, P, None, None) == -1   # lddy < N
-    assert f.fuma_split_blocks(P, 8, 4, 12, P, 1, 0, P, P, None) == -1                            # ldx
+    assert f.fuma_split_blocks(P, 8, 4, 12, P, 1, 0, 0, P, P, None) == -1                            # ldx
     assert f.fuma_pad_rows(P, 12, 4, 12, P, 12, None, 0, 0, 0, None) == -1                        # ldo
     assert f.fuma_pad_rows(P, 12, 5, 12, P, 16, P, 2, 2, 9, None) == -1                           # rows != G * mat_rows
-    assert f.fuma_split_blocks(P, 16, 10, 16, None, 0, 4, P, P, None) == -1                       # mat_rows
-    assert f.fuma_split_blocks(P, 16, 10, 16, None, 2, 0, P, P, None) == -1                       # no offsets
+    assert f.fuma_split_blocks(P, 16, 10, 16, None, 0, 4, 0, P, P, None) == -1                       # mat_rows
+    assert f.fuma_split_blocks(P, 16, 10, 16, None, 2, 0, 0, P, P, None) == -1                       # no offsets
     assert f.fuma_quantize_rows_fp8(P, 16, 4, 16, 1, P, 24, P, None) == -1                        # ldq
     assert f.fuma_quantize_weight_fp8(P, 1, 24, 16, P, 16, P, P, 24, P, None) == -1               # ldt
     assert f.fuma_grouped_linear_fp8(P, 16, P, P, None, 2, None, 0, 10, 24, 16, 1, P, P, 1 << 20, None, None) == -1
