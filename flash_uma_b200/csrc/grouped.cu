@@ -18,7 +18,8 @@
 //            scale 2^k (largest magnitude to [2^14, 2^15)): x = 2^k (hi + lo), hi = fp16(x / 2^k), lo = fp16(x / 2^k
 //            - hi). 22 bits for values down to 2^-18 of the block's largest and 2^-40 of that below, over the
 //            whole fp32 range. Three products, hi hi, hi lo, lo hi, in one accumulator. (Three bf16 planes need no scale,
-//            but six products and half as much again in operand bytes: 178 us against the table's for the same call.)
+//            but six products and half as much again in operand bytes: 260 us where this takes 162, at 30,000 rows
+//            in 32 groups, 1024 -> 512.)
 //   kFp8     e4m3 operands with fp32 scales: sA[kb][row] for each row and block kb of 128 along the
 //            contraction, sB[g][n / 128][kb] for each 128 x 128 block of W.
 //
@@ -975,8 +976,9 @@ __device__ __forceinline__ int64_t sum_bound(const int64_t* off, int g, int G, i
 }
 
 // A block takes the pieces of one row block in 256 columns (8 per lane). Long pieces: the 8 warps share a piece's rows,
-// 8 rows in flight each, and join in shared memory. Row blocks cut into many short pieces (many small groups):
-// a warp per piece, no joining.
+// 8 rows in flight each, and join in shared memory. Row blocks cut into more than 4 pieces (many small groups):
+// a warp per piece, no joining. 20,000 rows of 512 bf16 in 2,000 groups: 10.8 us, sharing every piece 28.2; 50,021 rows of
+// 392 in 301 groups: 17.2, a warp per piece 80.2.
 // kVec: rows 16-byte aligned.
 template <int kDtype, bool kVec>
 __global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restrict__ x, int64_t ld,
@@ -1249,8 +1251,11 @@ cudaError_t launch_grouped(const CUtensorMap (&m)[2], const GroupedArgs& p, int6
 }
 
 // Columns per tile: the whole width in even parts of at most 256, multiples of `step` (with block scales 256 or 128), and
-// narrower tiles, down to 32, while there
-// would be fewer tiles than SMs: a call of a few rows is bound by how many SMs pull its matrices in.
+// narrower tiles, down to 32, while there are no more of them than SMs: a call of a few rows is bound by how many SMs pull
+// its matrices in, but a second round of tiles costs more than narrow tiles save. `tiles_rows` is what groups of any
+// length have on average, half a tile more than their rows each. bf16: 24 rows,
+// 768 -> 640, 8.1 us, at full width 9.3; 1,000 rows in 4 groups 9.1, at full width 10.3, 32 wide (two rounds) 11.7;
+// 4,000 rows in 8 groups, 512 -> 512, 8.8, at full width 9.8.
 int pick_bn(int N, int64_t tiles_rows, bool scaled, int step) {
   int bn;
   if (scaled) {
@@ -1259,9 +1264,9 @@ int pick_bn(int N, int64_t tiles_rows, bool scaled, int step) {
     const int parts = (N + kMaxBN - 1) / kMaxBN;
     bn = ((N + parts - 1) / parts + step - 1) / step * step;
   }
-  while (bn > 32 && tiles_rows * ((N + bn - 1) / bn) < sm_count()) {
+  for (;;) {
     const int half = scaled ? bn / 2 : (bn / 2 + 31) / 32 * 32;
-    if (half < 32 || half == bn) break;
+    if (half < 32 || half == bn || tiles_rows * ((N + half - 1) / half) > sm_count()) break;
     bn = half;
   }
   return bn;
@@ -1284,7 +1289,7 @@ int launch_grouped_rows(const GroupedOperands& o, GroupedArgs p, bool transposed
   const int bk = fp8 ? 128 : split ? 32 : 64;
   const int64_t groups = p.G < p.T ? p.G : p.T;
   const int64_t tiles_rows = p.T / kBM + groups;   // upper bound: a partial tile per group
-  p.bn = pick_bn(p.N, tiles_rows, fp8 || split, transposed ? 64 : 32);   // transposed: whole chunks of 64
+  p.bn = pick_bn(p.N, p.T / kBM + (groups + 1) / 2, fp8 || split, transposed ? 64 : 32);   // transposed: whole chunks of 64
   p.tiles_n = (p.N + p.bn - 1) / p.bn;
   p.tiles_m = 1;
   p.err = err;
@@ -1404,6 +1409,8 @@ cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const in
     const cudaError_t st = cudaGetLastError();
     if (st != cudaSuccess) return st;
   }
+  // few pieces per group: a warp joins a group's (2,000 groups of 10 rows: 8.5 us, a block per group 180; 16 groups of 7,500
+  // rows the other way round: 5.4 us, a warp per group 8.1)
   const bool by_warp = groups >= 8 && T / groups < 8 * kSumRows;
   const int gy = by_warp ? (groups + kJoinWarps - 1) / kJoinWarps : groups;
   grouped_colsum_join_kernel<<<dim3((unsigned)((N + 31) / 32), (unsigned)gy), 32 * kJoinWarps, 0, s>>>(

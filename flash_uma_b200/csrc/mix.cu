@@ -877,8 +877,17 @@ int tc_grid(int64_t P, int bn) {
   return (int)(tiles < sm_count() ? tiles : sm_count());
 }
 
-// Few coefficients: the vector kernels, whose blocks start at once, and several to an SM.
-bool use_tc(int S, int E) { return (int64_t)S * E >= 64; }
+// Forward: few coefficients go to the vector kernel, whose blocks start at once, and several to an SM; its time grows
+// with S E, that of the tensor-core kernel hardly. Rows that TMA cannot read (not a multiple of 16 bytes apart) cost the latter more. us, vector and
+// tensor cores, for matrices of 491,520 values (odd: 102,307): bf16 S E = 128 19.8, 17.6 (of 16,384 values 4.3, 5.1), 512
+// 36.7, 19.2; odd 1024 15.0, 21.7, 2048 25.1, 23.0; fp32 512 38.2, 53.6, 1024 54.8, 54.6, 2048 90.6, 56.7; odd 2048
+// 23.5, 34.9. Both gradients at once always go to the tensor cores, which read the matrices once: bf16 S E = 8 28 + 4,
+// vector 10 + 127 + 4; fp32 84 + 4, vector 10 + 125 + 4.
+template <typename T>
+bool use_tc(int S, int E, int64_t P) {
+  const bool aligned = P * sizeof(T) % 16 == 0;
+  return (int64_t)S * E >= (sizeof(T) == 2 ? (aligned ? 256 : 2048) : (aligned ? 1024 : 4096));
+}
 
 template <typename T, bool kDc>
 cudaError_t run_tc(MixTcArgs p, cudaStream_t s) {
@@ -923,7 +932,7 @@ bool tc_fits(int K, int M, bool dc) {
 template <typename T>
 cudaError_t any_mix(const float* c, int64_t cs, int64_t ce, const void* X, int S, int E, int64_t P, void* out, int* err,
                     cudaStream_t s) {
-  if (use_tc(S, E) && tc_fits<T>(E, S, false)) {
+  if (use_tc<T>(S, E, P) && tc_fits<T>(E, S, false)) {
     MixTcArgs p{};
     p.c = c; p.cm = cs; p.ck = ce; p.R = X; p.out = out; p.M = S; p.K = E; p.P = P; p.err = err;
     return run_tc<T, false>(p, s);
@@ -933,7 +942,7 @@ cudaError_t any_mix(const float* c, int64_t cs, int64_t ce, const void* X, int S
 
 template <typename T>
 int64_t bwd_splits(int S, int E, int64_t P) {
-  if (use_tc(S, E) && tc_fits<T>(S, E, true)) return tc_grid(P, MixTc<T>::kBN);
+  if (tc_fits<T>(S, E, true)) return tc_grid(P, MixTc<T>::kBN);
   const int64_t share = dcoeff_share(S, E, P);
   return (P + share - 1) / share;
 }
@@ -941,7 +950,7 @@ int64_t bwd_splits(int S, int E, int64_t P) {
 template <typename T>
 cudaError_t any_bwd(const float* c, int64_t cs, int64_t ce, const void* dW, const void* X, int S, int E, int64_t P,
                     float* dc, void* dX, float* part, int* err, cudaStream_t s) {
-  if (dc && dX && use_tc(S, E) && tc_fits<T>(S, E, true)) {
+  if (dc && dX && tc_fits<T>(S, E, true)) {
     MixTcArgs p{};
     p.c = c; p.cm = ce; p.ck = cs; p.R = dW; p.X = X; p.out = dX; p.part = part; p.M = E; p.K = S; p.P = P; p.err = err;
     const cudaError_t st = run_tc<T, true>(p, s);
