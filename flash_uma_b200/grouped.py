@@ -11,8 +11,8 @@ unlike systems, and for training, every system keeps its own matrix:
 * :class:`MoleLinear`: the two together, a layer.
 
 Counterpart of :class:`~flash_uma_b200.linear.FrozenLinear` (one frozen matrix for all rows) on
-the same tensor cores. Types: fp32 (two fp16 planes per operand under a scale for each 128 x 128 block, three
-products: 22 bits over the whole fp32 range, no range error), bf16 and fp16 (fp32 sums, one rounding at the end).
+the same tensor cores. Types: fp32 (two fp16 planes per operand under a scale for each block, three products:
+22 bits, or 2^-39 of the block's largest magnitude where that is more; the whole fp32 range, no range error), bf16 and fp16 (fp32 sums, one rounding at the end).
 :func:`flash_uma_b200.fp8.fp8_linear` is the map on frozen 8-bit weights.
 """
 from __future__ import annotations
@@ -25,7 +25,7 @@ import torch.nn as nn
 
 from . import _native as nat
 from ._native import ptr, stream_of
-from .linear import error_flag
+from .linear import _err_flags, error_flag
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_GROUPS = 4096
@@ -56,6 +56,8 @@ def guard_capture(*inputs) -> bool:
     invalidates the capture or ends the process. Seen are the eager calls of this module and of fp8."""
     if not torch.cuda.is_current_stream_capturing():
         return False
+    if inputs[0].device.index not in _err_flags:   # it would be made in the graph's memory, and cleared by every replay
+        raise RuntimeError("the first call on a device cannot be captured into a CUDA graph: run one before the capture")
     if torch.is_grad_enabled():
         leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
         with _live_lock:
@@ -250,8 +252,12 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
 
     16-bit operands whose rows are not contiguous, aligned to 16 bytes and a multiple of 16 bytes apart (an
     odd K, say) run on a copy. Bad offset values are recorded in the device error flag
-    (:func:`flash_uma_b200.linear.check_errors`); an infinite fp32 input may give NaN where fp32
-    arithmetic gives an infinity."""
+    (:func:`flash_uma_b200.linear.check_errors`).
+
+    fp32: each operand is taken to 2^-22 of itself or, in a 128 x 128 block (128 rows of one group, from its first row,
+    and 128 columns) of widely different magnitudes, to 2^-39 of the block's largest; an infinite input may give NaN
+    where fp32 arithmetic gives an infinity. A training call keeps the operands as the kernels read them for the backward
+    pass: fp32 planes take the place of x and weight, at the same size."""
     if torch.compiler.is_compiling():
         return _opaque(grouped_linear, x, weight, offsets, bias)
     nat.require_cuda(x, weight, offsets, bias)
@@ -316,7 +322,9 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
 def mix_experts(coeff: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
     """``W[s] = sum_e coeff[s, e] experts[e]``: coeff [S, E] float32 (any strides), experts [E, ...]
     float32, bfloat16 or float16 -> [S, ...] of the experts' type, summed in fp32. Differentiable
-    (once) in both; the gradient of coeff is float32, its sum over a matrix joined in fp64."""
+    (once) in both; the gradient of coeff is float32, its sum over a matrix joined in fp64. Large fp32 mixes run
+    on the tensor cores with the precision of :func:`grouped_linear`'s fp32 maps, a block being the same 64 values
+    of all matrices; a value that is not finite makes the results that depend on it not finite."""
     if torch.compiler.is_compiling():
         return _opaque(mix_experts, coeff, experts)
     nat.require_cuda(coeff, experts)

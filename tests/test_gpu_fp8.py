@@ -58,7 +58,7 @@ def _values(T, K, dt, seed=0):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("T,K", [(1, 8), (1, 128), (17, 136), (130, 520), (33, 13), (1000, 1024)])
+@pytest.mark.parametrize("T,K", [(1, 8), (1, 128), (17, 136), (130, 520), (33, 13), (7, 1), (300, 535), (1000, 1024)])
 def test_quantize_rows(T, K, dt):
     from flash_uma_b200.fp8 import quantize_rows
     x = _values(T, K, dt)
@@ -108,7 +108,8 @@ def _close(got, want, S, n, dt, what):
 
 
 SHAPES = [([1], 8, 8, 0, 0), ([1], 512, 512, 0, 0), ([0, 5, 0, 130, 1, 127, 128, 0], 136, 264, 0, 0),
-          ([300, 20], 768, 640, 7, 200), ([17, 0, 40], 13, 7, 2, 1), ([200], 1032, 136, 0, 0),
+          ([300, 20], 768, 640, 7, 200), ([17, 0, 40], 13, 7, 2, 1), ([200], 1032, 136, 0, 0), ([9, 1], 1, 1, 1, 0),
+          ([40, 0, 300], 535, 583, 1, 0), ([31], 260, 131, 0, 0),
           ([9001, 0, 257, 8000, 128, 129], 136, 640, 3, 77)]
 
 
@@ -207,3 +208,50 @@ def test_refusals():
         Fp8Weight(w[0, 0])
     with pytest.raises(TypeError):
         quantize_rows(x.double())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_strides_alignment_streams_and_replay(dt):
+    """Rows that are strided, transposed or off 16 bytes, another stream and a captured call on new data give the bits of the
+    contiguous eager call."""
+    from flash_uma_b200.fp8 import Fp8Weight, fp8_linear
+    g = torch.Generator(device=DEV).manual_seed(5)
+    T, G, N, K = 140, 3, 72, 200
+    w8 = Fp8Weight(torch.randn(G, N, K, device=DEV, generator=g))
+    off = torch.tensor([1, 60, 60, 139], device=DEV)
+    b = torch.randn(G, N, device=DEV, generator=g)
+    x = torch.randn(T, K, device=DEV, generator=g).to(dt)
+    gy = torch.randn(T, N, device=DEV, generator=g).to(dt)
+
+    def run(x, gy):
+        x = x.detach().requires_grad_(True)
+        y = fp8_linear(x, w8, off, b)
+        return y.detach(), torch.autograd.grad(y, x, gy)[0]
+    want = run(x, gy)
+    wide = torch.zeros(T, K + 3, device=DEV, dtype=dt)[:, 1:K + 1].copy_(x)
+    gt = gy.t().contiguous().t()
+    for xi, gi in ((wide, gt), (x.t().contiguous().t(), gy.flip(0).flip(0)[:, :N])):
+        assert all(torch.equal(p, q) for p, q in zip(run(xi, gi), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run(x, gy)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(other, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(x, gy)
+    x.mul_(3.0)
+    graph.replay()
+    assert all(torch.equal(p, q) for p, q in zip(out, run(x, gy)))
+
+
+def test_rows_past_32_bit_offsets():
+    from flash_uma_b200.fp8 import Fp8Weight, fp8_linear
+    T, K, N, n = 2 ** 21 + 5, 1032, 8, 300
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.zeros(T, K, device=DEV, dtype=torch.bfloat16)
+    x[-n:] = torch.randn(n, K, device=DEV, generator=g).bfloat16()
+    w8 = Fp8Weight(torch.randn(N, K, device=DEV, generator=g))
+    y = fp8_linear(x, w8)
+    assert torch.equal(y[-n:], fp8_linear(x[-n:].contiguous(), w8)) and not y[:-n].any()

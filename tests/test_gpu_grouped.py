@@ -386,3 +386,227 @@ def test_mole_layer(dt):
     slope = sum((gr.double() * u).sum() for gr, u in zip(grads, d))
     size = sum((gr.double() * u).norm() for gr, u in zip(grads, d))
     assert abs(slope - (up - dn) / (2 * h)) <= (8 * _half(dt) + 1e-6) * size * 4
+
+
+# ---- what a user may do with them ------------------------------------------------------------------
+
+def test_fp32_blocks_of_mixed_magnitudes():
+    """Rows, columns and matrices whose magnitudes differ by up to 2^40 within a block. A block is scaled so that its largest
+    magnitude M is below 2^15, where the second plane's smallest step is 2^-24 and its rounding 2^-25: 2^-39 M, or 2^-22 of
+    the value itself. So besides the bound of :func:`_close` (with 12 2^-24 of S for the planes in it) each product
+    may be off by 2^-39 (M_x |w| + |x| M_w); M over the whole operand is at least a block's."""
+    lens, K, N = [300, 20, 129], 200, 136
+    x, w, off, b, gy = _make(lens, K, N, torch.float32, None, 0, 0, 7)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    mag = lambda n: 2.0 ** torch.randint(-20, 21, (n, 1), device=DEV, generator=g)   # noqa: E731
+    x, gy = x * mag(x.shape[0]), gy * mag(x.shape[0])
+    w = w * mag(N)
+    from flash_uma_b200.grouped import grouped_linear
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = grouped_linear(xl, wl, off)
+    dx, dw = torch.autograd.grad(y, [xl, wl], gy)
+    Y, Sy, DX, Sx, DW, Sw, _, _ = _oracle(x, w, off, b, gy)
+    X, W, GY = x.double().abs(), w.double().abs(), gy.double().abs()
+    Mx, Mw, Mg = X.max(), W.max(), GY.max()
+    o = off.tolist()
+    for i in range(len(lens)):
+        r = slice(o[i], o[i + 1])
+        for got, want, S, n, extra in (
+                (y.detach()[r], Y[r], Sy[r], K, Mx * W[i].sum(1)[None] + Mw * X[r].sum(1)[:, None]),
+                (dx[r], DX[r], Sx[r], N, Mg * W[i].sum(0)[None] + Mw * GY[r].sum(1)[:, None]),
+                (dw[i], DW[i], Sw[i], lens[i], Mg * X[r].sum(0)[None] + Mx * GY[r].sum(0)[:, None])):
+            tol = (n / 16 + 12) * 2.0 ** -23 * S + 2.0 ** -39 * extra
+            assert (got.double() - want).abs().le(tol).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("S,E,P", [(3, 5, 304), (40, 33, 304), (40, 33, 305), (70, 70, 640)])
+def test_mix_not_finite_values_stay_in_their_column(S, E, P, dt):
+    """NaN or an infinity in expert e0 at p0 reaches W[:, p0] and dc[:, e0]; in the gradient of W[s0] at p1, dX[:, p1]
+    and dc[s0, :]; everything else keeps its value to the rounding of the results."""
+    from flash_uma_b200.grouped import mix_experts
+    g = torch.Generator(device=DEV).manual_seed(2)
+    c = torch.rand(S, E, device=DEV, generator=g) + 0.5
+    x = torch.randn(E, P, device=DEV, generator=g).to(dt)
+    gw = torch.randn(S, P, device=DEV, generator=g).to(dt)
+    e0, p0, s0, p1 = E // 2, 65, S // 2, P - 1
+
+    def run(x, gw):
+        cl, xl = c.clone().requires_grad_(True), x.clone().requires_grad_(True)
+        w = mix_experts(cl, xl)
+        return (w.detach(), *torch.autograd.grad(w, [cl, xl], gw))
+    w0, dc0, dx0 = run(x, gw)
+    for bad in (float("nan"), float("inf")):
+        x1, gw1 = x.clone(), gw.clone()
+        x1[e0, p0], gw1[s0, p1] = bad, bad
+        w, dc, dx = run(x1, gw1)
+        assert not w[:, p0].isfinite().any() and not dx[:, p1].isfinite().any()
+        assert not dc[:, e0].isfinite().any() and not dc[s0].isfinite().any()
+        for got, want, dim, i in ((w, w0, 1, p0), (dx, dx0, 1, p1)):
+            keep = torch.arange(P, device=DEV) != i
+            # a tile's scale may change with its largest finite value: the planes' bound on either side
+            tol = 4 * _half(dt) * want.abs() + 2.0 ** -16
+            assert (got - want).abs().le(tol).index_select(dim, keep.nonzero()[:, 0]).all()
+        keep_s, keep_e = torch.arange(S, device=DEV) != s0, torch.arange(E, device=DEV) != e0
+        assert torch.allclose(dc[keep_s][:, keep_e], dc0[keep_s][:, keep_e], rtol=1e-4, atol=1e-3)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_mix_operands_of_any_layout_and_single_gradients(dt):
+    """Expanded and strided coefficients, experts and gradients that are not contiguous or aligned, and each gradient
+    alone, against the contiguous call with both."""
+    from flash_uma_b200.grouped import mix_experts
+    g = torch.Generator(device=DEV).manual_seed(4)
+    S, E, N, K = 12, 34, 24, 40
+    c = torch.randn(S, E, device=DEV, generator=g)
+    x = torch.randn(E, N, K, device=DEV, generator=g).to(dt)
+    gw = torch.randn(S, N, K, device=DEV, generator=g).to(dt)
+
+    def run(c, x, gw, grads=(True, True)):
+        c, x = c.detach().requires_grad_(grads[0]), x.detach().requires_grad_(grads[1])
+        w = mix_experts(c, x)
+        got = torch.autograd.grad(w, [t for t in (c, x) if t.requires_grad], gw)
+        return (w.detach(), *got)
+    w, dc, dx = run(c, x, gw)
+    xt = x.permute(1, 2, 0).contiguous().permute(2, 0, 1)
+    off = torch.empty(x.numel() + 1, device=DEV, dtype=dt)[1:].view(x.shape).copy_(x)
+    gt = gw.transpose(1, 2).contiguous().transpose(1, 2)
+    ct = torch.empty(E, 2 * S, device=DEV).t()[::2].copy_(c)
+    for xi in (xt, off):
+        for p, q in zip(run(ct, xi, gt), (w, dc, dx)):
+            assert torch.equal(p, q)
+    # one gradient alone may take another kernel: fp32 sums in another order
+    s_c = gw.double().abs().flatten(1) @ x.double().abs().flatten(1).T
+    s_x = torch.einsum("se,snk->enk", c.double().abs(), gw.double().abs())
+    assert (run(c, x, gw, (True, False))[1] - dc).double().abs().le((2 * N * K + 40) * 2.0 ** -24 * s_c).all()
+    assert (run(c, x, gw, (False, True))[1].double() - dx.double()).abs().le(
+        2 * _half(dt) * dx.double().abs() + (S + 60) * 2.0 ** -24 * s_x).all()
+    one = torch.randn(1, E, device=DEV, generator=g).expand(S, E).requires_grad_(True)
+    y = mix_experts(one, x)
+    assert torch.equal(y[0], y[-1])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_two_captured_layers_replayed_in_turn(dt):
+    """A layer's training step, small and with groups long enough for CTA pairs and for cut weight gradients, captured twice in
+    one memory pool and replayed alternately on new data, gives the eager call's bits."""
+    from flash_uma_b200.grouped import MoleLinear
+    g = torch.Generator(device=DEV).manual_seed(6)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)   # noqa: E731
+    steps = []
+    for lens, E, N, K in (([5, 0, 130], 3, 72, 40), ([9000, 31000], 40, 520, 136)):
+        off = torch.tensor([0] + lens, device=DEV).cumsum(0)
+        layer = MoleLinear((r(E, N, K) * K ** -0.5).to(dt), r(N).to(dt))
+        x, gy = r(sum(lens), K).to(dt).requires_grad_(True), r(sum(lens), N).to(dt)
+        coeff = torch.rand(len(lens), E, device=DEV, generator=g).requires_grad_(True)
+
+        def step(layer=layer, x=x, coeff=coeff, off=off, gy=gy):
+            y = layer(x, coeff, off)
+            return (y.detach(), *torch.autograd.grad(y, [x, coeff, layer.experts, layer.bias], gy))
+        steps.append((step, x, coeff))
+    for step, _, _ in steps:
+        step()
+    pool = torch.cuda.graph_pool_handle()
+    graphs, outs = [], []
+    for step, _, _ in steps:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(step())
+        graphs.append(graph)
+    for i in (0, 1, 0, 1):
+        step, x, coeff = steps[i]
+        with torch.no_grad():
+            x.mul_(-0.5)
+            coeff.add_(0.25)
+        graphs[i].replay()
+        got = [t.clone() for t in outs[i]]
+        assert all(torch.equal(p, q) for p, q in zip(got, step()))
+
+
+def test_layer_under_torch_compile():
+    """The layer's calls are opaque to a trace and run eagerly, with gradients."""
+    from flash_uma_b200.grouped import MoleLinear
+    g = torch.Generator(device=DEV).manual_seed(9)
+    off = torch.tensor([0, 40, 57], device=DEV)
+    layer = MoleLinear(torch.randn(4, 24, 16, device=DEV, generator=g), torch.randn(24, device=DEV, generator=g))
+    x = torch.randn(57, 16, device=DEV, generator=g).requires_grad_(True)
+    c = torch.rand(2, 4, device=DEV, generator=g).requires_grad_(True)
+    f = lambda x, c: layer(x * 2, torch.softmax(c, 1), off) + 1   # noqa: E731
+    want = f(x, c)
+    got = torch.compile(f, backend="eager")(x, c)
+    assert torch.equal(got, want)
+    for p, q in zip(torch.autograd.grad(got.sum(), [x, c]), torch.autograd.grad(want.sum(), [x, c])):
+        assert torch.equal(p, q)
+
+
+def test_first_call_in_a_capture_is_refused():
+    """The device's error flag would be made in the graph's memory."""
+    from flash_uma_b200 import linear
+    from flash_uma_b200.grouped import mix_experts
+    c, x = torch.rand(2, 4, device=DEV), torch.rand(4, 8, device=DEV)
+    mix_experts(c, x)
+    held = dict(linear._err_flags)
+    linear._err_flags.clear()
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            with pytest.raises(RuntimeError, match="first call"):
+                mix_experts(c, x)
+            torch.zeros(1, device=DEV)
+    finally:
+        linear._err_flags.update(held)
+
+
+def test_gradient_of_an_expanded_bias_and_of_a_row_taken_twice():
+    """Autograd joins what the operator gives for inputs that were broadcast or used twice."""
+    from flash_uma_b200.grouped import grouped_linear
+    x, w, off, b, gy = _make([33, 0, 90], 48, 40, torch.float32, "shared", 1, 2)
+    X, W, B = (t.clone().requires_grad_(True) for t in (x[:1], w[:1], b))
+    y = grouped_linear(X.expand(x.shape[0], -1), W.expand(3, -1, -1), off, B.expand(3, -1))
+    got = torch.autograd.grad(y, [X, W, B], gy)
+    live = gy.double()[1:124]
+    assert torch.allclose(got[0].double(), (live @ w[0].double()).sum(0, keepdim=True), rtol=1e-5, atol=1e-4)
+    assert torch.allclose(got[1][0].double(), live.sum(0)[:, None] * x[0].double()[None], rtol=1e-5, atol=1e-4)
+    assert torch.allclose(got[2].double(), live.sum(0), rtol=1e-5, atol=1e-4)
+
+
+def test_rows_past_32_bit_offsets():
+    """2^21 + 5 rows of 1032 values: the last group starts behind element 2^31 of x and of dx."""
+    from flash_uma_b200 import linear
+    from flash_uma_b200.grouped import grouped_linear
+    T, K, N, n = 2 ** 21 + 5, 1032, 16, 300
+    dt = torch.bfloat16
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.zeros(T, K, device=DEV, dtype=dt)
+    x[-n:] = torch.randn(n, K, device=DEV, generator=g).to(dt)
+    gy = torch.zeros(T, N, device=DEV, dtype=dt)
+    gy[-n:] = torch.randn(n, N, device=DEV, generator=g).to(dt)
+    w = torch.randn(2, N, K, device=DEV, generator=g).to(dt)
+    off = torch.tensor([0, T - n + 100, T - 1], device=DEV)
+    xl, wl = x.requires_grad_(True), w.clone().requires_grad_(True)
+    y = grouped_linear(xl, wl, off)
+    dx, dw = torch.autograd.grad(y, [xl, wl], gy)
+    linear.check_errors()
+    small = _oracle(x.detach()[-n:], w, torch.tensor([0, 100, n - 1], device=DEV), None, gy[-n:])
+    _close(y.detach()[-n:], small[0], small[1], K, dt, "y")
+    _close(dx[-n:], small[2], small[3], N, dt, "dx")
+    _close(dw, small[4], small[5], T, dt, "dw")
+    assert not y.detach()[:-n].any() and not dx[:-n].any()
+
+
+def test_mix_past_32_bit_offsets():
+    """Matrices of 2^31 + 8 values, more than a tensor map addresses."""
+    from flash_uma_b200.grouped import mix_experts
+    P, dt = 2 ** 31 + 8, torch.bfloat16
+    c = torch.tensor([[0.75, -1.5]], device=DEV).requires_grad_(True)
+    x = torch.zeros(2, P, device=DEV, dtype=dt)
+    x[0, -3:], x[1, -5:] = 2.0, 0.5
+    x[0, :7] = 1.0
+    x.requires_grad_(True)
+    w = mix_experts(c, x)
+    gw = torch.zeros(1, P, device=DEV, dtype=dt)
+    gw[0, -4:], gw[0, 0] = 1.0, 8.0
+    dc, dx = torch.autograd.grad(w, [c, x], gw)
+    assert w.detach()[0, -6:].tolist() == [0.0, -0.75, -0.75, 0.75, 0.75, 0.75] and w.detach()[0, :8].tolist() == [0.75] * 7 + [0]
+    assert dc.tolist() == [[14.0, 2.0]]
+    assert dx[0, -5:].tolist() == [0.0] + [0.75] * 4 and dx[1, -5:].tolist() == [0.0] + [-1.5] * 4
+    assert dx[:, 0].tolist() == [6.0, -12.0] and int((dx != 0).sum()) == 10
