@@ -739,8 +739,8 @@ int grouped_done(const char* what, int r) {
 }  // namespace
 
 int fuma_grouped_linear(const void* x, int64_t ldx, const float* x_scales, const void* W, int64_t ldw,
-                        const float* W_scales, const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows, int64_t T, int32_t N, int32_t K, int32_t dtype, void* y,
-                        int* err_flag, void* stream) {
+                        const float* W_scales, const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows,
+                        int64_t T, int32_t N, int32_t K, int32_t dtype, void* y, int* err_flag, void* stream) {
   CHECK(check_grouped("grouped_linear", G, T, N, K, dtype));
   REQUIRE(ldx >= K && ldx % 8 == 0 && ldw >= K && ldw % 8 == 0,
           "grouped_linear: ldx=%lld and ldw=%lld must be >= K and multiples of 8", (long long)ldx, (long long)ldw);
@@ -760,8 +760,9 @@ int fuma_grouped_linear(const void* x, int64_t ldx, const float* x_scales, const
   return grouped_done("grouped_linear", launch_grouped_rows(o, p, false, err_flag, (cudaStream_t)stream));
 }
 
-int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* W,
-                              int64_t ldw, const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dx, int* err_flag, void* stream) {
+int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* W, int64_t ldw,
+                              const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K,
+                              int32_t dtype, void* dx, int* err_flag, void* stream) {
   CHECK(check_grouped("grouped_linear_dgrad", G, T, N, K, dtype));
   REQUIRE(lddy >= N && lddy % 8 == 0 && ldw >= K && ldw % 8 == 0,
           "grouped_linear_dgrad: lddy=%lld (>= N) and ldw=%lld (>= K) must be multiples of 8", (long long)lddy, (long long)ldw);
@@ -781,10 +782,12 @@ int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const float* dy_scal
 }
 
 int fuma_grouped_linear_wgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* x, int64_t ldx,
-                              const float* x_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype, void* dW, void* work,
-                              int64_t work_bytes, int* err_flag, void* stream) {
+                              const float* x_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K,
+                              int32_t dtype, void* dW, void* work, int64_t work_bytes, int* err_flag, void* stream) {
   CHECK(check_grouped("grouped_linear_wgrad", G, T, N, K, dtype));
   REQUIRE(lddy >= N && lddy % 8 == 0 && ldx >= K && ldx % 8 == 0, "grouped_linear_wgrad: bad leading dimensions");
+  REQUIRE((T / 128 + G) * (int64_t)((N + 127) / 128) * ((K + 127) / 128) < (int64_t(1) << 31),
+          "grouped_linear_wgrad: too many output tiles");
   REQUIRE(dW, "grouped_linear_wgrad: null pointer");
   REQUIRE_ALIGNED(dW, "dW");
   BIND(dW);

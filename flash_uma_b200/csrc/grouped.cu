@@ -1107,7 +1107,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) grouped_colsum_join_kernel(co
 // took 79 (and 66 with registers for a third resident block, which spills). Row blocks: of the ragged rows, the
 // 128-row tiles of each group (counted from the group's first row, as the maps cut it; the tile's slot is group
 // start / 128 + group + tile, distinct because one tile or one group further on moves it by at least 1), or, with
-// mat_rows > 0, of matrices of mat_rows rows each, but (given offsets) those of groups without rows. A value that is not finite keeps hi alone and does not set the scale.
+// mat_rows > 0, of matrices of mat_rows rows each, but (given offsets) those of groups without rows. A value that is not
+// finite keeps hi alone and does not set the scale.
 // kVec: rows 16-byte aligned. Planes [rows][ldp], ldp = cols rounded up to 8.
 template <bool kVec>
 __global__ void __launch_bounds__(256) split_blocks_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows,

@@ -105,7 +105,8 @@ int64_t grouped_wgrad_work_bytes(int64_t T, int M, int N, int dtype);
 int64_t grouped_colsum_work_bytes(int64_t T, int N, int groups);
 cudaError_t launch_grouped_colsum(const void* x, int64_t ld, int dtype, const int64_t* off, int G, bool shared,
                                   int64_t T, int N, float* part, void* out, cudaStream_t s);
-// Two fp16 planes [2][rows][cols rounded up to 8] and their block scales: of ragged rows (mat_rows 0) [ceil(cols / 128)][split_slots],
+// Two fp16 planes [2][rows][cols rounded up to 8] and their block scales: of ragged rows (mat_rows 0)
+// [ceil(cols / 128)][split_slots],
 // of matrices of mat_rows rows [matrices][ceil(mat_rows / 128)][ceil(cols / 128)].
 int64_t split_slots(int64_t rows, int G);
 void launch_split_blocks(const float* x, int64_t ldx, int64_t rows, int cols, const int64_t* off, int G, int mat_rows,

@@ -878,10 +878,11 @@ int tc_grid(int64_t P, int bn) {
 }
 
 // Forward: few coefficients go to the vector kernel, whose blocks start at once, and several to an SM; its time grows
-// with S E, that of the tensor-core kernel hardly. Rows that TMA cannot read (not a multiple of 16 bytes apart) cost the latter more. us, vector and
-// tensor cores, for matrices of 491,520 values (odd: 102,307): bf16 S E = 128 19.8, 17.6 (of 16,384 values 4.3, 5.1), 512
-// 36.7, 19.2; odd 1024 15.0, 21.7, 2048 25.1, 23.0; fp32 512 38.2, 53.6, 1024 54.8, 54.6, 2048 90.6, 56.7; odd 2048
-// 23.5, 34.9. Both gradients at once always go to the tensor cores, which read the matrices once: bf16 S E = 8 28 + 4,
+// with S E, that of the tensor-core kernel hardly. Rows that TMA cannot read (not a multiple of 16 bytes apart) cost the
+// latter more. us, vector and tensor cores, for matrices of 491,520 values (odd: 102,307):
+//   bf16  S E = 128  19.8, 17.6 (of 16,384 values 4.3, 5.1); 512  36.7, 19.2;  odd 1024  15.0, 21.7; 2048  25.1, 23.0
+//   fp32  S E = 512  38.2, 53.6; 1024  54.8, 54.6; 2048  90.6, 56.7;           odd 2048  23.5, 34.9
+// Both gradients at once always go to the tensor cores, which read the matrices once: bf16 S E = 8 28 + 4,
 // vector 10 + 127 + 4; fp32 84 + 4, vector 10 + 125 + 4.
 template <typename T>
 bool use_tc(int S, int E, int64_t P) {

@@ -333,7 +333,8 @@ int fuma_morton_reorder_noalloc(const float* pos, const int64_t* Z, const int64_
  * offsets[G]) are written as zeros, and offsets may be NULL for one group of all rows. Offsets that
  * decrease or leave [0, T] put 64 into err_flag (the results are then undefined, all accesses stay in
  * bounds). 1 <= G <= 4096; any N and K; leading dimensions (elements) of the operands multiples
- * of 8 (fuma_pad_rows makes such a copy), arrays 16-byte aligned; outputs contiguous. Work space: see the *_work_bytes functions (0: may be NULL).
+ * of 8 (fuma_pad_rows makes such a copy), arrays 16-byte aligned; outputs contiguous. Work space: see the *_work_bytes
+ * functions (0: may be NULL); calls that overlap need one each.
  *
  * fp32 operands come as two fp16 planes and their block scales (fuma_split_blocks: x and dy as ragged rows under
  * the same offsets, W with mat_rows = N; the leading dimension is then the column count rounded up to 8). Results and
@@ -341,11 +342,11 @@ int fuma_morton_reorder_noalloc(const float* pos, const int64_t* Z, const int64_
  *
  * y[t, n] = sum_k x[t, k] W[g, n, k] + bias (bias_rows 1: bias[n], G: bias[g, n]; may be NULL) */
 int fuma_grouped_linear(const void* x, int64_t ldx, const float* x_scales, const void* W, int64_t ldw,
-                        const float* W_scales, const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows, int64_t T, int32_t N,
-                        int32_t K, int32_t dtype, void* y, int* err_flag, void* stream);
+                        const float* W_scales, const int64_t* offsets, int32_t G, const void* bias, int32_t bias_rows,
+                        int64_t T, int32_t N, int32_t K, int32_t dtype, void* y, int* err_flag, void* stream);
 /* dx[t, k] = sum_n dy[t, n] W[g, n, k] */
-int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* W,
-                              int64_t ldw, const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K,
+int fuma_grouped_linear_dgrad(const void* dy, int64_t lddy, const float* dy_scales, const void* W, int64_t ldw,
+                              const float* W_scales, const int64_t* offsets, int32_t G, int64_t T, int32_t N, int32_t K,
                               int32_t dtype, void* dx, int* err_flag, void* stream);
 /* dW[g, n, k] = sum over the rows of g of dy[t, n] x[t, k]; zeros for a group without rows. No
  * atomics: the same call gives the same bits. */
