@@ -981,7 +981,7 @@ __device__ __forceinline__ int64_t sum_bound(const int64_t* off, int g, int G, i
 // 392 in 301 groups: 17.2, a warp per piece 80.2.
 // kVec: rows 16-byte aligned.
 template <int kDtype, bool kVec>
-__global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restrict__ x, int64_t ld,
+__global__ void __launch_bounds__(256, kVec ? 4 : 2) grouped_colsum_kernel(const void* __restrict__ x, int64_t ld,
                                                              const int64_t* __restrict__ off, int G, int shared,
                                                              int64_t T, int N, float* __restrict__ part) {
   __shared__ float sm[8][256 + 8];
@@ -989,15 +989,21 @@ __global__ void __launch_bounds__(256) grouped_colsum_kernel(const void* __restr
   const int n = blockIdx.y * 256 + lane * 8;
   const int groups = shared ? 1 : G;
   const int64_t b0 = (int64_t)blockIdx.x * kSumRows, b1 = min(T, b0 + kSumRows);
-  auto first_behind = [&](int64_t row) {   // first group that ends behind `row`
-    int lo = 0, hi = groups;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (sum_bound(off, mid + 1, G, T, shared) > row) hi = mid; else lo = mid + 1;
-    }
-    return lo;
-  };
-  const int g0 = first_behind(b0), g1 = min(groups, first_behind(b1 - 1) + 1);
+  // the groups of the block's rows: from the first that ends behind b0 to the first that ends behind b1 - 1, by counting
+  // those that end before (independent loads; a binary search's dependent ones took longer than the sums of 128 rows)
+  __shared__ int count[8];
+  int n_end = 0;   // ends <= b0, and in the upper half ends < b1
+  for (int g = threadIdx.x; g < groups; g += 256) {
+    const int64_t end = sum_bound(off, g + 1, G, T, shared);
+    n_end += (end <= b0) + ((end < b1) << 16);
+  }
+  n_end = __reduce_add_sync(kFull, n_end);
+  if (lane == 0) count[w] = n_end;
+  __syncthreads();
+  n_end = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) n_end += count[i];
+  const int g0 = n_end & 0xffff, g1 = min(groups, (n_end >> 16) + 1);
   const bool short_pieces = g1 - g0 > 4;
   const int step = short_pieces ? 1 : 8, w0 = short_pieces ? 0 : w;
   for (int g = g0 + (short_pieces ? w : 0); g < g1; g += short_pieces ? 8 : 1) {
@@ -1086,7 +1092,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) grouped_colsum_join_kernel(co
     double s = 0.0;
     if (n < N && gb > ga) {
       const int64_t last = (gb - 1) / kSumRows;
-#pragma unroll 4
+#pragma unroll 8
       for (int64_t b = ga / kSumRows + w; b <= last; b += kJoinWarps) s += (double)part[(b + g) * N + n];
     }
     sm[w][lane] = s;
