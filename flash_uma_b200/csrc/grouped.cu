@@ -977,8 +977,9 @@ __device__ __forceinline__ int64_t sum_bound(const int64_t* off, int g, int G, i
 
 // A block takes the pieces of one row block in 256 columns (8 per lane). Long pieces: the 8 warps share a piece's rows,
 // 8 rows in flight each, and join in shared memory. Row blocks cut into more than 4 pieces (many small groups):
-// a warp per piece, no joining. 20,000 rows of 512 bf16 in 2,000 groups: 10.8 us, sharing every piece 28.2; 50,021 rows of
-// 392 in 301 groups: 17.2, a warp per piece 80.2.
+// a warp per piece, no joining. 20,000 rows of 512 bf16 in 2,000 groups: 9.2 us, sharing every piece 28; 50,021 rows of
+// 392 in 301 groups: 15.7, a warp per piece 80. Bound by latency (120,000 rows of 640: 154 MB in 34 us); all of a block's
+// rows in registers ahead of the offsets took 64.
 // kVec: rows 16-byte aligned.
 template <int kDtype, bool kVec>
 __global__ void __launch_bounds__(256, kVec ? 4 : 2) grouped_colsum_kernel(const void* __restrict__ x, int64_t ld,
