@@ -49,6 +49,21 @@ _live_nodes: "weakref.WeakSet" = weakref.WeakSet()
 _live_lock = threading.Lock()
 
 
+def _leaves_below(nodes) -> list:
+    """The leaf tensors that the autograd graphs of ``nodes`` end in."""
+    found, seen, stack = [], set(), list(nodes)
+    while stack:
+        node = stack.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        leaf = getattr(node, "variable", None)
+        if leaf is not None:
+            found.append(leaf)
+        stack.extend(n for n, _ in node.next_functions)
+    return found
+
+
 def guard_capture(*inputs) -> bool:
     """True if the current stream is capturing. Refuses to put a call on leaf tensors into a CUDA graph capture
     while an eager graph of the same leaves is alive: autograd keeps one gradient node per leaf, bound to the
@@ -60,15 +75,13 @@ def guard_capture(*inputs) -> bool:
         raise RuntimeError("the first call on a device cannot be captured into a CUDA graph: run one before the capture")
     if torch.is_grad_enabled():
         leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
+        leaves += _leaves_below(t.grad_fn for t in inputs if t is not None and t.grad_fn is not None)
         with _live_lock:
             nodes = list(_live_nodes)
-        for node in nodes:
-            for edge, _ in node.next_functions:
-                held = getattr(edge, "variable", None)
-                if held is not None and any(held is t for t in leaves):
-                    raise RuntimeError("a CUDA graph capture of this call needs the results of earlier eager calls on "
-                                       "the same leaf tensors to be released or detached first (their autograd graph "
-                                       "is alive)")
+        held = {id(t) for t in _leaves_below(nodes)} if leaves else ()
+        if any(id(t) in held for t in leaves):
+            raise RuntimeError("a CUDA graph capture of this call needs the results of earlier eager calls on the same "
+                               "leaf tensors to be released or detached first (their autograd graph is alive)")
     return True
 
 

@@ -129,9 +129,10 @@ def test_long_groups_on_cta_pairs(lens, K, N, head, tail, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-def test_many_groups(dt):
+@pytest.mark.parametrize("G", [700, 4096])
+def test_many_groups(dt, G):
     g = torch.Generator().manual_seed(5)
-    lens = torch.randint(0, 9, (700,), generator=g).tolist()
+    lens = torch.randint(0, 9, (G,), generator=g).tolist()
     x, w, off, b, gy = _make(lens, 40, 24, dt, "group")
     _check(x, w, off, b, gy, dt)
 
@@ -610,3 +611,61 @@ def test_mix_past_32_bit_offsets():
     assert dc.tolist() == [[14.0, 2.0]]
     assert dx[0, -5:].tolist() == [0.0] + [0.75] * 4 and dx[1, -5:].tolist() == [0.0] + [-1.5] * 4
     assert dx[:, 0].tolist() == [6.0, -12.0] and int((dx != 0).sum()) == 10
+
+
+def test_capture_while_an_eager_graph_of_the_layer_lives_is_refused():
+    """Also where the shared leaf is behind another operator (the router's logits, behind a softmax)."""
+    from flash_uma_b200.grouped import MoleLinear
+    g = torch.Generator(device=DEV).manual_seed(9)
+    off = torch.tensor([0, 40, 57], device=DEV)
+    layer = MoleLinear(torch.randn(4, 24, 16, device=DEV, generator=g)).requires_grad_(False)
+    x = torch.randn(57, 16, device=DEV, generator=g)
+    logits = torch.randn(2, 4, device=DEV, generator=g).requires_grad_(True)
+
+    def step():
+        y = layer(x, torch.softmax(logits, 1), off)
+        return torch.autograd.grad(y.sum(), logits)[0]
+    want = step()
+    held = layer(x, torch.softmax(logits, 1), off)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="eager"):
+            step()
+        torch.zeros(1, device=DEV)
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    assert torch.equal(got, want)
+
+
+def test_two_threads_on_two_streams():
+    from flash_uma_b200.grouped import MoleLinear
+    import threading
+    g = torch.Generator(device=DEV).manual_seed(9)
+    off = torch.tensor([0, 400, 457], device=DEV)
+    layer = MoleLinear(torch.randn(4, 72, 56, device=DEV, generator=g), torch.randn(72, device=DEV, generator=g))
+    x = torch.randn(457, 56, device=DEV, generator=g)
+    c = torch.rand(2, 4, device=DEV, generator=g)
+
+    def step():
+        xl = x.clone().requires_grad_(True)
+        y = layer(xl, c, off)
+        return (y.detach(), *torch.autograd.grad(y.sum(), [xl, layer.experts, layer.bias]))   # an expanded gradient
+    want, bad = step(), []
+    torch.cuda.synchronize()
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = step()
+                s.synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, want)):
+                    bad.append(1)
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
