@@ -48,10 +48,10 @@ class Fp8Weight:
         w = w.float().contiguous()
         dev, G, N, K = w.device, self.G, self.N, self.K
         self.device = dev
-        self.codes = torch.empty((G, N, _ceil16(K)), device=dev, dtype=torch.uint8)
-        self.scales = torch.empty((G, _blocks(N), _blocks(K)), device=dev)
-        self.codes_t = torch.empty((G, K, _ceil16(N)), device=dev, dtype=torch.uint8)
-        self.scales_t = torch.empty((G, _blocks(K), _blocks(N)), device=dev)
+        self.codes = w.new_empty((G, N, _ceil16(K)), dtype=torch.uint8)
+        self.scales = w.new_empty((G, _blocks(N), _blocks(K)))
+        self.codes_t = w.new_empty((G, K, _ceil16(N)), dtype=torch.uint8)
+        self.scales_t = w.new_empty((G, _blocks(K), _blocks(N)))
         nat.call("fuma_quantize_weight_fp8", ptr(w), G, N, K, ptr(self.codes), _ceil16(K), ptr(self.scales),
                  ptr(self.codes_t), _ceil16(N), ptr(self.scales_t), stream_of(w))
 
@@ -71,8 +71,8 @@ def quantize_rows(x: torch.Tensor):
         raise ValueError(f"x must be [rows, K] with K >= 1 (got {tuple(x.shape)})")
     T, K = x.shape
     x = _unit_stride(x)
-    codes = torch.empty((T, _ceil16(K)), device=x.device, dtype=torch.uint8)
-    scales = torch.empty((_blocks(K), T), device=x.device)
+    codes = x.new_empty((T, _ceil16(K)), dtype=torch.uint8)
+    scales = x.new_empty((_blocks(K), T), dtype=torch.float32)
     if T:
         nat.call("fuma_quantize_rows_fp8", ptr(x), x.stride(0), T, K, code, ptr(codes), _ceil16(K), ptr(scales),
                  stream_of(x))
@@ -81,11 +81,11 @@ def quantize_rows(x: torch.Tensor):
 
 def _product(x, w_codes, w_scales, offsets, bias, N, K):
     T, G = x.shape[0], w_codes.shape[0]
-    y = torch.empty((T, N), device=x.device, dtype=x.dtype)
+    y = x.new_empty((T, N))
     if T:
         x = _unit_stride(x)
         nbytes = nat.load().fuma_fp8_work_bytes(T, K)   # the quantised rows and their scales
-        work = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+        work = x.new_empty(nbytes, dtype=torch.uint8)
         nat.call("fuma_grouped_linear_fp8", ptr(x), x.stride(0), ptr(w_codes), ptr(w_scales), ptr(offsets), G, ptr(bias),
                  0 if bias is None else (1 if bias.dim() == 1 else G), T, N, K, _DTYPES[x.dtype], ptr(y), ptr(work),
                  nbytes, ptr(error_flag(x.device)), stream_of(x))

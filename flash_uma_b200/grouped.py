@@ -128,9 +128,9 @@ def _split(x: torch.Tensor, offsets, G: int, mat_rows: int, T: int):
     (``fuma_split_blocks``): of ragged rows, or (``mat_rows`` > 0) of matrices of that many rows, those of groups
     with rows (of T)."""
     rows, cols = x.shape
-    out = torch.empty((2, rows, _ceil8(cols)), device=x.device, dtype=torch.float16)
+    out = x.new_empty((2, rows, _ceil8(cols)), dtype=torch.float16)
     blocks = rows // mat_rows * ((mat_rows + 127) // 128) if mat_rows else rows // 128 + G
-    scales = torch.empty((cols + 127) // 128 * blocks, device=x.device)
+    scales = x.new_empty((cols + 127) // 128 * blocks)
     nat.call("fuma_split_blocks", ptr(x), x.stride(0), rows, cols, ptr(offsets), G, mat_rows, T, ptr(out),
              ptr(scales), stream_of(x))
     return out, scales
@@ -146,7 +146,7 @@ def _operand(x: torch.Tensor, offsets, G: int):
         return planes, _ceil8(cols), scales
     ld = x.stride(0)
     if ld % 8 or x.data_ptr() % 16:
-        out = torch.empty((rows, _ceil8(cols)), device=x.device, dtype=x.dtype)
+        out = x.new_empty((rows, _ceil8(cols)))
         nat.call("fuma_pad_rows", ptr(x), ld, rows, cols, ptr(out), _ceil8(cols), None, 0, 0, 0, stream_of(x))
         return out, _ceil8(cols), None
     return x, ld, None
@@ -162,7 +162,7 @@ def _weight_operand(w: torch.Tensor, offsets, T: int):
         planes, scales = _split(w.view(G * N, K), offsets, G, N, T)
         return planes, _ceil8(K), scales
     if K % 8 or w.data_ptr() % 16:
-        out = torch.empty((G, N, _ceil8(K)), device=w.device, dtype=w.dtype)
+        out = w.new_empty((G, N, _ceil8(K)))
         nat.call("fuma_pad_rows", ptr(w), K, G * N, K, ptr(out), _ceil8(K), ptr(offsets), G, N, T, stream_of(w))
         return out, _ceil8(K), None
     return w, K, None
@@ -175,7 +175,7 @@ class _GroupedLinearFn(torch.autograd.Function):
         the backward pass needs again (fp32: planes instead of the values), laid out once."""
         T = x.shape[0]
         G, N, K = weight.shape
-        y = torch.empty((T, N), device=x.device, dtype=x.dtype)
+        y = x.new_empty((T, N))
         a, w = (x, _ceil8(K), None), (weight, _ceil8(K), None)
         if T:
             bias_rows = 0
@@ -215,21 +215,21 @@ class _GroupedLinearFn(torch.autograd.Function):
         g = _unit_stride(g)
         a, lda, a_s = _operand(g, offsets, G) if T and (want_x or want_w) else (g, _ceil8(N), None)
         if want_x:
-            dx = torch.empty((T, K), device=dev, dtype=dt)
+            dx = g.new_empty((T, K))
             if T:
                 nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, ptr(a_s), ptr(w), ldw, ptr(w_s), ptr(offsets), G, T, N,
                          K, code, ptr(dx), err, s)
         if want_w:
-            dw = torch.empty((G, N, K), device=dev, dtype=dt)
+            dw = g.new_empty((G, N, K))
             nbytes = nat.load().fuma_grouped_wgrad_work_bytes(T, N, K, code)
-            work = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+            work = g.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
             nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, ptr(a_s), ptr(b), ldb, ptr(b_s), ptr(offsets), G, T, N, K,
                      code, ptr(dw), ptr(work), nbytes, err, s)
         if want_b:
             shared = len(bias_shape) == 1
-            db = torch.empty(bias_shape, device=dev, dtype=dt)
+            db = g.new_empty(bias_shape)
             nbytes = nat.load().fuma_grouped_bias_grad_work_bytes(T, N, 1 if shared else G)
-            work = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+            work = g.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
             nat.call("fuma_grouped_bias_grad", ptr(g), g.stride(0) if T else N, ptr(offsets), G, 1 if shared else 0, T, N,
                      code, ptr(db), ptr(work), nbytes, s)
         return dx, dw, None, db
@@ -292,7 +292,7 @@ class _MixFn(torch.autograd.Function):
     def compute(coeff, experts):
         S, E = coeff.shape
         x = _flat(experts)
-        out = torch.empty((S, *experts.shape[1:]), device=experts.device, dtype=experts.dtype)
+        out = experts.new_empty((S, *experts.shape[1:]))
         nat.call("fuma_mix_experts", ptr(coeff), coeff.stride(0), coeff.stride(1), ptr(x), S, E, x.numel() // E,
                  _DTYPES[experts.dtype], ptr(out), ptr(error_flag(experts.device)), stream_of(experts))
         return out
@@ -315,9 +315,9 @@ class _MixFn(torch.autograd.Function):
         dc = de = work = None
         nbytes = 0
         if want_c:
-            dc = torch.empty((S, E), device=dev)
+            dc = coeff.new_empty((S, E))
             nbytes = nat.load().fuma_mix_experts_work_bytes(S, E, P, code)
-            work = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            work = coeff.new_empty(nbytes, dtype=torch.uint8)
         if want_e:
             de = torch.empty_like(experts, memory_format=torch.contiguous_format)
         g, x = _flat(g), _flat(experts)
@@ -347,7 +347,8 @@ def mix_experts(coeff: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
     if experts.dim() < 1 or coeff.dim() != 2 or coeff.shape[1] != experts.shape[0] or experts.shape[0] < 1:
         raise ValueError(f"coeff must be [systems, experts] for experts [experts, ...] (got {tuple(coeff.shape)} and "
                          f"{tuple(experts.shape)})")
-    _same_device(experts.device, coeff=coeff)
+    if coeff.device != experts.device:
+        _same_device(experts.device, coeff=coeff)
     return _apply(_MixFn, guard_capture(coeff, experts), coeff, experts)
 
 

@@ -669,3 +669,26 @@ def test_two_threads_on_two_streams():
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_default_dtype_of_64_bits():
+    """The work arrays do not follow torch's default type."""
+    from flash_uma_b200.fp8 import Fp8Weight, fp8_linear
+    from flash_uma_b200.grouped import MoleLinear
+    g = torch.Generator(device=DEV).manual_seed(3)
+    off = torch.tensor([0, 130, 257], device=DEV)
+    layer = MoleLinear(torch.randn(4, 72, 130, device=DEV, generator=g))
+    x = torch.randn(257, 130, device=DEV, generator=g).requires_grad_(True)
+    c = torch.rand(2, 4, device=DEV, generator=g).requires_grad_(True)
+    w8 = torch.randn(72, 130, device=DEV, generator=g)
+
+    def run():
+        y = layer(x, c, off)
+        return (y.detach(), *torch.autograd.grad(y.sum(), [x, c, layer.experts]), fp8_linear(x, Fp8Weight(w8)).detach())
+    want = run()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = run()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(p.dtype == q.dtype and torch.equal(p, q) for p, q in zip(got, want))
