@@ -124,20 +124,21 @@ def _ceil8(n: int) -> int:
 
 
 def _split(x: torch.Tensor, offsets, G: int, mat_rows: int, T: int):
-    """The two fp16 planes [2, rows, cols rounded up to 8] of an fp32 operand [rows, cols] and their block scales
-    (``fuma_split_blocks``): of ragged rows, or (``mat_rows`` > 0) of matrices of that many rows, those of groups
-    with rows (of T)."""
+    """One array with the two fp16 planes [2, rows, cols rounded up to 8] of an fp32 operand [rows, cols] and, behind
+    them, their block scales (``fuma_split_blocks``), and the scales' address: of ragged rows, or (``mat_rows`` > 0) of
+    matrices of that many rows, those of groups with rows (of T)."""
     rows, cols = x.shape
-    out = x.new_empty((2, rows, _ceil8(cols)), dtype=torch.float16)
+    planes = rows * _ceil8(cols)   # two of 2 bytes: as many floats
     blocks = rows // mat_rows * ((mat_rows + 127) // 128) if mat_rows else rows // 128 + G
-    scales = x.new_empty((cols + 127) // 128 * blocks)
-    nat.call("fuma_split_blocks", ptr(x), x.stride(0), rows, cols, ptr(offsets), G, mat_rows, T, ptr(out),
-             ptr(scales), stream_of(x))
-    return out, scales
+    out = x.new_empty(planes + (cols + 127) // 128 * blocks)
+    at = out.data_ptr()
+    nat.call("fuma_split_blocks", ptr(x), x.stride(0), rows, cols, ptr(offsets), G, mat_rows, T, at, at + 4 * planes,
+             stream_of(x))
+    return out, at + 4 * planes
 
 
 def _operand(x: torch.Tensor, offsets, G: int):
-    """(tensor, leading dimension, scales) of a row operand for the C ABI: 16-bit rows a multiple of 16 bytes apart and
+    """(tensor, leading dimension, address of the scales) of a row operand for the C ABI: 16-bit rows a multiple of 16 bytes apart and
     aligned to that (a copy where they are not), fp32 as planes."""
     x = _unit_stride(x)
     rows, cols = x.shape
@@ -153,7 +154,7 @@ def _operand(x: torch.Tensor, offsets, G: int):
 
 
 def _weight_operand(w: torch.Tensor, offsets, T: int):
-    """(tensor, leading dimension, scales) of the matrices [G, N, K] for the C ABI, likewise; a copy leaves out the
+    """(tensor, leading dimension, address of the scales) of the matrices [G, N, K] for the C ABI, likewise; a copy leaves out the
     matrices of groups without rows."""
     if not w.is_contiguous():
         w = w.contiguous()
@@ -183,20 +184,20 @@ class _GroupedLinearFn(torch.autograd.Function):
                 bias_rows = 1 if bias.dim() == 1 else G
                 bias = bias.contiguous()
             a, w = _operand(x, offsets, G), _weight_operand(weight, offsets, T)
-            nat.call("fuma_grouped_linear", ptr(a[0]), a[1], ptr(a[2]), ptr(w[0]), w[1], ptr(w[2]), ptr(offsets), G,
+            nat.call("fuma_grouped_linear", ptr(a[0]), a[1], a[2], ptr(w[0]), w[1], w[2], ptr(offsets), G,
                      ptr(bias), bias_rows, T, N, K, _DTYPES[x.dtype], ptr(y), ptr(error_flag(x.device)), stream_of(x))
         if keep_x or keep_w:
-            return y, a if keep_x else (None, 0, None), w if keep_w else (None, 0, None)
+            return y, a if keep_x else (None, 0), w if keep_w else (None, 0)
         return y
 
     @staticmethod
     def forward(ctx, x, weight, offsets, bias):
         want_x, want_w, _, _ = ctx.needs_input_grad
-        a = w = (None, 0, None)
+        a = w = (None, 0)
         out = _GroupedLinearFn.compute(x, weight, offsets, bias, want_w, want_x)
         if want_w or want_x:
             out, a, w = out
-        ctx.save_for_backward(a[0], a[2], w[0], w[2], offsets)
+        ctx.save_for_backward(a[0], w[0], offsets)
         ctx.lds = a[1], w[1]
         ctx.shapes = x.shape[0], weight.shape, None if bias is None else bias.shape
         return out
@@ -204,7 +205,7 @@ class _GroupedLinearFn(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, g):
-        b, b_s, w, w_s, offsets = ctx.saved_tensors
+        b, w, offsets = ctx.saved_tensors
         ldb, ldw = ctx.lds
         T, (G, N, K), bias_shape = ctx.shapes
         dev, dt = g.device, g.dtype
@@ -217,14 +218,16 @@ class _GroupedLinearFn(torch.autograd.Function):
         if want_x:
             dx = g.new_empty((T, K))
             if T:
-                nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, ptr(a_s), ptr(w), ldw, ptr(w_s), ptr(offsets), G, T, N,
-                         K, code, ptr(dx), err, s)
+                w_s = w.data_ptr() + 4 * G * N * ldw if code == 0 else None
+                nat.call("fuma_grouped_linear_dgrad", ptr(a), lda, a_s, ptr(w), ldw, w_s, ptr(offsets), G, T, N, K, code,
+                         ptr(dx), err, s)
         if want_w:
             dw = g.new_empty((G, N, K))
             nbytes = nat.load().fuma_grouped_wgrad_work_bytes(T, N, K, code)
             work = g.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-            nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, ptr(a_s), ptr(b), ldb, ptr(b_s), ptr(offsets), G, T, N, K,
-                     code, ptr(dw), ptr(work), nbytes, err, s)
+            b_s = b.data_ptr() + 4 * T * ldb if code == 0 else None
+            nat.call("fuma_grouped_linear_wgrad", ptr(a), lda, a_s, ptr(b), ldb, b_s, ptr(offsets), G, T, N, K, code,
+                     ptr(dw), ptr(work), nbytes, err, s)
         if want_b:
             shared = len(bias_shape) == 1
             db = g.new_empty(bias_shape)
