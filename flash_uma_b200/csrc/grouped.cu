@@ -35,7 +35,7 @@
 // MMA; a pair moves 32 KB each way.
 //
 // Structure: 384 threads, one CTA per SM. Warp 0 loads operand tiles by TMA into a ring; warp 1
-// allocates TMEM, and its lane 0 issues the MMAs; warp 2 (weight gradient) clears the rows behind a group's end; warp 3
+// allocates TMEM and issues the MMAs from one elected lane; warp 2 (weight gradient) clears the rows behind a group's end; warp 3
 // works out the items ahead of time and hands them to the others through a ring (with every warp doing it, 64-bit
 // divisions and dependent loads took 1,000 cycles of each tile's epilogue); warps 4-11 are the epilogue. The MMA
 // thread's own instructions count: 512 cycles of MMA per stage leave no room for descriptors built from scratch
