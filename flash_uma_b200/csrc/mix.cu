@@ -217,6 +217,12 @@ __global__ void __launch_bounds__(256) mix_dcoeff_join_kernel(const float* __res
 // two warpgroups take turns). Warps 12-19 are the epilogue.
 constexpr int kMixTcThreads = 640;
 constexpr int kMixTcMax = 128;   // rows of A, of R and of X
+// Barriers of the operand ring: tile `it` of a CTA signals slot it % kMixSlots, whichever buffer (it % depth, depth <= kMixSlots) it
+// lies in. Two warpgroups take turns at filling, and a wait by parity is only good for one that has seen the barrier's phase
+// before: with as many slots as buffers, a warpgroup at a ring of one buffer would meet every second phase of its barrier and
+// pass at once. With an even number of slots each warpgroup waits for every phase of every slot that it ever waits for, in
+// order, and a slot's next phase cannot end before it has: that is a tile kMixSlots >= depth further on, behind its own.
+constexpr int kMixSlots = 4;
 constexpr int kMixCtrlRegs = 48, kMixLoadRegs = 88, kMixEpiRegs = 128;   // 640 x 96 at launch = 128 x (48 + 2 x 88 + 2 x 128)
 
 struct MixTcArgs {
@@ -344,8 +350,8 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
   uint8_t* smem_c = smem_a + kPA * kc * rm * 128;
   uint8_t* smem_raw_tile = smem_c + L::kStaging + 1024;    // behind the barriers
   uint64_t* bar_full = reinterpret_cast<uint64_t*>(smem_c + L::kStaging);
-  uint64_t* bar_empty = bar_full + 8;
-  uint64_t* bar_acc_full = bar_empty + 8;
+  uint64_t* bar_empty = bar_full + kMixSlots;
+  uint64_t* bar_acc_full = bar_empty + kMixSlots;
   uint64_t* bar_acc_empty = bar_acc_full + 2;
   uint64_t* bar_dc_empty = bar_acc_empty + 2;
   uint64_t* bar_dc_full = bar_dc_empty + 2;
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 8; ++s) {
+    for (int s = 0; s < kMixSlots; ++s) {
       mbar_init(&bar_full[s], !kF32 && p.tma ? 1 : 128);
       mbar_init(&bar_empty[s], 1);
     }
@@ -445,12 +451,12 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       const uint32_t plane_a = kc * rm * 8, plane_r = rk * 8, plane_x = rm * 8;
       const uint32_t tm = __shfl_sync(kFull, tmem, 0);
       const int ksteps = rk / 16;
-      int it = 0, s = 0, phase = 0;
+      int it = 0, s = 0;
       bool ok = true;
       for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++it) {
-        const int buf = it & 1;
+        const int buf = it & 1, slot = it % kMixSlots;
         ok = it < 2 || mbar_wait(&bar_acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, p.err, kErrWaitAccEmpty);
-        ok = ok && mbar_wait(&bar_full[s], phase, abort_flag, p.err, kErrWaitFull);
+        ok = ok && mbar_wait(&bar_full[slot], (it / kMixSlots) & 1, abort_flag, p.err, kErrWaitFull);
         ok = __all_sync(kFull, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -491,13 +497,10 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
             }
           }
         }
-        mix_commit(&bar_empty[s]);
+        mix_commit(&bar_empty[slot]);
         mix_commit(&bar_acc_full[buf]);
         if (kDc && (it % L::kDcTiles == L::kDcTiles - 1 || tile + gridDim.x >= tiles)) mix_commit(&bar_dc_full[it / L::kDcTiles & 1]);
-        if (++s == p.stages) {
-          s = 0;
-          phase ^= 1;
-        }
+        if (++s == p.stages) s = 0;
       }
       __syncwarp();
       mix_commit(bar_done);
@@ -510,30 +513,31 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       uint64_t* full = kF32 ? bar_raw_full : bar_full;
       uint64_t* empty = kF32 ? bar_raw_empty : bar_empty;
       const int depth = kF32 ? p.tma : p.stages, bytes = kF32 ? raw_bytes : stage_bytes;
+      const int slots = kF32 ? depth : kMixSlots;
       uint8_t* base = kF32 ? smem_raw_tile : smem;
       const int row_bytes = kF32 ? 256 : 128;
       int it = 0;
       bool ok = true;
       for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++it) {
-        const int s = it % depth;
-        ok = it < depth || mbar_wait(&empty[s], ((it / depth) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
+        const int s = it % depth, slot = it % slots, last = it - depth;   // the tile that was here before
+        ok = last < 0 || mbar_wait(&empty[last % slots], (last / slots) & 1, abort_flag, p.err, kErrWaitEmpty);
         ok = __all_sync(kFull, ok);
         if (!ok) break;
         if (lane == 0) {
-          mbar_expect_tx(&full[s], bytes);
+          mbar_expect_tx(&full[slot], bytes);
           uint8_t* st = base + s * bytes;
 #pragma unroll
           for (int c = 0; c < L::kChunks; ++c) {
-            tma_load_2d(st + c * rk * row_bytes, &tmR, (int)(tile * kBN) + c * 64, 0, &full[s]);
+            tma_load_2d(st + c * rk * row_bytes, &tmR, (int)(tile * kBN) + c * 64, 0, &full[slot]);
             if (kDc)
-              tma_load_2d(st + L::kChunks * rk * row_bytes + c * rm * row_bytes, &tmX, (int)(tile * kBN) + c * 64, 0, &full[s]);
+              tma_load_2d(st + L::kChunks * rk * row_bytes + c * rm * row_bytes, &tmX, (int)(tile * kBN) + c * 64, 0, &full[slot]);
           }
         }
         __syncwarp();
       }
       if (*abort_flag && lane == 0) {
         for (int j = it - 1; j >= 0 && j >= it - depth; --j) {
-          for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&full[j % depth], (j / depth) & 1); ++i) {
+          for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&full[j % slots], (j / slots) & 1); ++i) {
           }
         }
       }
@@ -601,7 +605,8 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
           // four tiles on: this warpgroup's too, nobody is there before another barrier, and everybody has left it
           *reinterpret_cast<uint4*>(tile_max + ((it + 4) & 7) * 4) = make_uint4(0u, 0u, 0u, 0u);
         }
-        const bool ok = it < p.stages || mbar_wait(&bar_empty[s], ((it / p.stages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
+        const int last = it - p.stages;   // the tile that was in this stage before
+        const bool ok = last < 0 || mbar_wait(&bar_empty[last % kMixSlots], (last / kMixSlots) & 1, abort_flag, p.err, kErrWaitEmpty);
         uint8_t* dst = smem + s * stage_bytes + row0 * 128 + ((((u >> 1) ^ row0) & 7) << 4) + (u & 1) * 8;
         if (ok) {
 #pragma unroll
@@ -627,7 +632,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&bar_full[s]);
+        mbar_arrive(&bar_full[it % kMixSlots]);
         if (p.tma) mbar_arrive(&bar_raw_empty[rb]);
       }
     } else if (!p.tma) {
@@ -660,7 +665,8 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
         }
       };
       fetch(0, v[0]);
-      if (it >= p.stages) ok = mbar_wait(&bar_empty[s], ((it / p.stages) - 1) & 1, abort_flag, p.err, kErrWaitEmpty);
+      const int last = it - p.stages;   // the tile that was in this stage before
+      if (last >= 0) ok = mbar_wait(&bar_empty[last % kMixSlots], (last / kMixSlots) & 1, abort_flag, p.err, kErrWaitEmpty);
       if (!ok) break;
       // this thread's 16 bytes in row row0 of a tile; rows 8 further on are 1024 bytes on and
       // have the same swizzle
@@ -684,7 +690,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(&bar_full[s]);
+      mbar_arrive(&bar_full[it % kMixSlots]);
     }
     }
   } else {
@@ -869,7 +875,7 @@ int tc_stages(int K, int M, bool dc, int raw) {
   const int tile = MixTc<T>::stage_bytes(K, m, dc);
   const int raw_bytes = sizeof(T) == 4 ? raw * (tile / MixTc<T>::kPlanesR / 2 * 4) : 0;
   const int n = (kSmemLimit - MixTc<T>::kFixed - MixTc<T>::coeff_bytes(K, m) - raw_bytes) / tile;
-  return n < 4 ? n : 4;
+  return n < kMixSlots ? n : kMixSlots;
 }
 
 int tc_grid(int64_t P, int bn) {

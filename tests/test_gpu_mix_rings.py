@@ -1,0 +1,57 @@
+"""Large expert mixes against fp64: 8 tiles and more for every thread block, so that each ring of the tensor-core kernel (operand
+stages, raw tiles, accumulators, tile scales, the drain of dc) goes round, at each depth that the shapes come to. The
+columns' magnitudes change from tile to tile, so that values or a scale of another tile show.
+
+Bounds, in units of 2^-24 of S = the sum of |products|: the tensor core truncates (2) up to three additions per 16
+products; two fp16 planes on each side leave 12 (fp32); a rounded addition is 1. Then half an eps of the result's type.
+dc: 16 steps of 16 columns stay in the tensor core's sum, one addition per such sum and thread block, a few in fp64."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+ALIGNED, ODD = 160000, 160003
+
+
+def _check(got, want, S, steps, what):
+    t = got.dtype
+    tol = torch.finfo(t).eps / 2 * want.abs() + steps * 2.0 ** -24 * S + torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), bad.nonzero()[0].tolist())
+
+
+def _compare(S, E, P, dt):
+    from flash_uma_b200 import linear
+    from flash_uma_b200.grouped import mix_experts
+    g = torch.Generator(device=DEV).manual_seed(S * 1000 + E)
+    tile = 64 if dt == torch.float32 else 128
+    steps_of = 12 if dt == torch.float32 else 0
+    n_tiles = -(-P // tile)
+
+    def matrices(n):
+        mag = 2.0 ** torch.randint(-6, 7, (n_tiles,), device=DEV, generator=g)
+        return (torch.randn(n, P, device=DEV, generator=g) * mag.repeat_interleave(tile)[:P]).to(dt)
+    c = torch.randn(S, E, device=DEV, generator=g).requires_grad_(True)
+    x, gw = matrices(E).requires_grad_(True), matrices(S)
+
+    def run():
+        w = mix_experts(c, x)
+        return (w.detach(), *torch.autograd.grad(w, [c, x], gw))
+    w, dc, dx = run()
+    linear.check_errors()
+    C, X, GW = c.detach().double(), x.detach().double(), gw.double()
+    _check(w, C @ X, C.abs() @ X.abs(), 6 * -(-E // 16) + steps_of + 2, "w")
+    _check(dx, C.T @ GW, C.T.abs() @ GW.abs(), 6 * -(-S // 16) + steps_of + 2, "dx")
+    sms = torch.cuda.get_device_properties(DEV).multi_processor_count
+    _check(dc, GW @ X.T, GW.abs() @ X.abs().T, 6 * 16 + -(-n_tiles // sms) + steps_of + 4, "dc")
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(run(), (w, dc, dx)))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("S,E,P", [(64, 32, ALIGNED), (64, 32, ODD), (70, 70, ALIGNED), (70, 70, ODD), (128, 64, ALIGNED),
+                                   (128, 64, ODD), (112, 97, ODD), (128, 128, ODD)])
+def test_stages_of_the_operand_ring(S, E, P, dt):
+    """One to four operand stages, filled by two warpgroups in turn."""
+    _compare(S, E, P, dt)
