@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(256) mix_dcoeff_join_kernel(const float* __res
 // two warpgroups take turns). Warps 12-19 are the epilogue.
 constexpr int kMixTcThreads = 640;
 constexpr int kMixTcMax = 128;   // rows of A, of R and of X
-// Barriers of the operand ring: tile `it` of a CTA signals slot it % kMixSlots, whichever buffer (it % depth, depth <= kMixSlots) it
-// lies in. Two warpgroups take turns at filling, and a wait by parity is only good for one that has seen the barrier's phase
+// Barriers of the operand ring and of the ring of raw tiles: tile `it` of a CTA signals slot it % kMixSlots, whichever buffer
+// (it % depth, depth <= kMixSlots) it lies in. Two warpgroups take turns, and a wait by parity is only good for one that has seen the barrier's phase
 // before: with as many slots as buffers, a warpgroup at a ring of one buffer would meet every second phase of its barrier and
 // pass at once. With an even number of slots each warpgroup waits for every phase of every slot that it ever waits for, in
 // order, and a slot's next phase cannot end before it has: that is a tile kMixSlots >= depth further on, behind its own.
@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
   uint64_t* bar_dc_empty = bar_acc_empty + 2;
   uint64_t* bar_dc_full = bar_dc_empty + 2;
   uint64_t* bar_raw_full = bar_dc_full + 2;
-  uint64_t* bar_raw_empty = bar_raw_full + 4;
-  uint64_t* bar_done = bar_raw_empty + 4;
+  uint64_t* bar_raw_empty = bar_raw_full + kMixSlots;
+  uint64_t* bar_done = bar_raw_empty + kMixSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* row_scale = reinterpret_cast<float*>(tmem_slot + 2);   // [128]
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       mbar_init(&bar_dc_full[b], 1);
 
     }
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < kMixSlots; ++b) {
       mbar_init(&bar_raw_full[b], 1);
       mbar_init(&bar_raw_empty[b], 128);
     }
@@ -513,14 +513,13 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       uint64_t* full = kF32 ? bar_raw_full : bar_full;
       uint64_t* empty = kF32 ? bar_raw_empty : bar_empty;
       const int depth = kF32 ? p.tma : p.stages, bytes = kF32 ? raw_bytes : stage_bytes;
-      const int slots = kF32 ? depth : kMixSlots;
       uint8_t* base = kF32 ? smem_raw_tile : smem;
       const int row_bytes = kF32 ? 256 : 128;
       int it = 0;
       bool ok = true;
       for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++it) {
-        const int s = it % depth, slot = it % slots, last = it - depth;   // the tile that was here before
-        ok = last < 0 || mbar_wait(&empty[last % slots], (last / slots) & 1, abort_flag, p.err, kErrWaitEmpty);
+        const int s = it % depth, slot = it % kMixSlots, last = it - depth;   // the tile that was here before
+        ok = last < 0 || mbar_wait(&empty[last % kMixSlots], (last / kMixSlots) & 1, abort_flag, p.err, kErrWaitEmpty);
         ok = __all_sync(kFull, ok);
         if (!ok) break;
         if (lane == 0) {
@@ -537,7 +536,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       }
       if (*abort_flag && lane == 0) {
         for (int j = it - 1; j >= 0 && j >= it - depth; --j) {
-          for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&full[j % slots], (j / slots) & 1); ++i) {
+          for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&full[j % kMixSlots], (j / kMixSlots) & 1); ++i) {
           }
         }
       }
@@ -572,7 +571,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
           return w;
         };
         // (no end of the loop after a failed wait: the other threads count on this one at the barriers below)
-        if (p.tma) mbar_wait(&bar_raw_full[rb], (it / p.tma) & 1, abort_flag, p.err, kErrWaitFull);
+        if (p.tma) mbar_wait(&bar_raw_full[it % kMixSlots], (it / kMixSlots) & 1, abort_flag, p.err, kErrWaitFull);
         // the tile's largest magnitudes, as bits: of R's rows and of X's. `all`: with values that are not finite, which is
         // what tells that there are any; a second round then leaves them out
         uint32_t* tm = tile_max + (it & 7) * 4;
@@ -633,7 +632,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(&bar_full[it % kMixSlots]);
-        if (p.tma) mbar_arrive(&bar_raw_empty[rb]);
+        if (p.tma) mbar_arrive(&bar_raw_empty[it % kMixSlots]);
       }
     } else if (!p.tma) {
     const int rounds_r = rk / 8, rounds = rounds_r + (kDc ? rm / 8 : 0);   // 8 rows a round, 16 units of 16 bytes per row

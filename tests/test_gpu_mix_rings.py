@@ -55,3 +55,10 @@ def _compare(S, E, P, dt):
 def test_stages_of_the_operand_ring(S, E, P, dt):
     """One to four operand stages, filled by two warpgroups in turn."""
     _compare(S, E, P, dt)
+
+
+@pytest.mark.parametrize("S,E", [(128, 80), (100, 96), (128, 96), (112, 97), (128, 128)])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_one_raw_tile(S, E, dt):
+    """Shapes at which fp32 has room for one raw tile beside one operand stage."""
+    _compare(S, E, ALIGNED, dt)

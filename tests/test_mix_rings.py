@@ -103,12 +103,12 @@ def run(stages, raw, slots, raw_slots, seed):
             del blocked[a]
 
 
-@pytest.mark.parametrize("raw", [0, 2, 4])
+@pytest.mark.parametrize("raw", [0, 1, 2, 4])
 @pytest.mark.parametrize("stages", [1, 2, 3, 4])
-def test_operand_ring(stages, raw):
-    """Four barriers for any number of stages."""
+def test_rings(stages, raw):
+    """Four barriers for any number of stages, and four for any number of raw buffers."""
     for seed in range(300):
-        run(stages, raw, 4, raw or 1, seed)
+        run(stages, raw, 4, 4, seed)
 
 
 @pytest.mark.parametrize("raw", [0, 2])
@@ -116,3 +116,10 @@ def test_the_model_finds_a_ring_of_one_stage_on_one_barrier(raw):
     with pytest.raises(Fault):
         for seed in range(300):
             run(1, raw, 1, raw or 1, seed)
+
+
+@pytest.mark.parametrize("stages", [1, 2, 4])
+def test_the_model_finds_one_raw_buffer_on_one_barrier(stages):
+    with pytest.raises(Fault):
+        for seed in range(300):
+            run(stages, 1, 4, 1, seed)
