@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       mbar_init(&bar_full[s], 1);
-      mbar_init(&bar_empty[s], 1);
+      mbar_init(&bar_empty[s], kMode == kModeDw ? 2 : 1);   // the MMAs' completion; the weight gradient's clearing warp
       mbar_init(&bar_clear[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -604,11 +604,14 @@ __global__ void __launch_bounds__(kGThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_item_empty[n % kRing]);
         if (t.kblocks < 0) break;
-        // every stage's barrier in order, also where nothing is to clear: a wait for a phase two ahead of the barrier's
-        // would return at once
-        for (int kt = 0; ok && kt < t.kblocks; ++kt)
-          ok = mbar_wait(&bar_full[(it + kt) % L::kStages], ((it + kt) / L::kStages) & 1, abort_flag, p.err, kErrWaitFull);
-        ok = __all_sync(kFull, ok);
+        // every stage's barrier in order, also where nothing is to clear, and no stage is loaded again before this warp has
+        // seen it full: a wait by parity means nothing to a warp that is two phases behind
+        for (int kt = 0; kt < t.kblocks; ++kt) {
+          const int s = (it + kt) % L::kStages;
+          ok = __all_sync(kFull, mbar_wait(&bar_full[s], ((it + kt) / L::kStages) & 1, abort_flag, p.err, kErrWaitFull));
+          if (!ok) break;
+          if (lane == 0 && (kt + 1 < t.kblocks || !t.tail)) mbar_arrive(&bar_empty[s]);
+        }
         if (!ok) break;
         if (t.tail) {
           const int s = (it + t.kblocks - 1) % L::kStages;
@@ -623,7 +626,10 @@ __global__ void __launch_bounds__(kGThreads, 1)
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_clear[s]);
+          if (lane == 0) {
+            mbar_arrive(&bar_clear[s]);
+            mbar_arrive(&bar_empty[s]);
+          }
         }
         it += t.kblocks;
       }
