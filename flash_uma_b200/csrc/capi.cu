@@ -952,7 +952,7 @@ int fuma_mix_experts_bwd(const void* grad, const float* coeff, int64_t stride_s,
   if (dexperts) REQUIRE_ALIGNED(dexperts, "dexperts");
   BIND(grad);
   return grouped_done("mix_experts_bwd", (int)launch_mix_bwd(coeff, stride_s, stride_e, grad, experts, S, E, P, dtype,
-                                                             dcoeff, dexperts, static_cast<float*>(work), err_flag,
+                                                             dcoeff, dexperts, static_cast<double*>(work), err_flag,
                                                              (cudaStream_t)stream));
 }
 

@@ -127,6 +127,6 @@ cudaError_t launch_mix(const float* c, int64_t cs, int64_t ce, const void* X, in
 int64_t mix_bwd_work_bytes(int S, int E, int64_t P, int dtype);
 // dc and dX (either may be null) from dW; part: mix_bwd_work_bytes when dc is asked for
 cudaError_t launch_mix_bwd(const float* c, int64_t cs, int64_t ce, const void* dW, const void* X, int S, int E, int64_t P,
-                           int dtype, float* dc, void* dX, float* part, int* err, cudaStream_t s);
+                           int dtype, float* dc, void* dX, double* part, int* err, cudaStream_t s);
 
 }  // namespace fuma

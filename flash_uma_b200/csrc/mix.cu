@@ -6,7 +6,7 @@
 //   dc[s, e]  = sum_p dW[s, p] X[e, p]
 //
 // Coefficients and their gradients are fp32, the matrices fp32, bf16 or fp16; sums are fp32, and the sum over
-// P is joined in fp64.
+// P is in fp32 over at most kDcFlush columns and in fp64 from there on.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -76,6 +76,7 @@ __device__ __forceinline__ void store4(T* row, int64_t p, int64_t P, float4 v) {
 
 constexpr int kMixCols = 256, kMixRows = 32, kMixE = 64;
 constexpr int kMixSmem = kMixE * (kMixCols + kMixRows) * 4;
+constexpr int kDcFlush = 4096;
 
 }  // namespace
 
@@ -126,19 +127,26 @@ __global__ void __launch_bounds__(256) mix_kernel(const float* __restrict__ c, i
   }
 }
 
-// dc partial sums: block (split, s-tile, e-tile) adds the products of its share of the columns; a thread has
+// dc partial sums [split][e][s]: block (split, s-tile, e-tile) adds the products of its share of the columns; a thread has
 // 4 x 4 of the 64 x 64 (s, e) pairs.
 constexpr int kDcCols = 64, kDcPad = kDcCols + 4;
 
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256) mix_dcoeff_kernel(const T* __restrict__ dW, const T* __restrict__ X, int S, int E,
-                                                         int64_t P, int64_t share, float* __restrict__ part) {
+                                                         int64_t P, int64_t share, double* __restrict__ part) {
   __shared__ float ds[64][kDcPad], xs[64][kDcPad];
   const int s0 = blockIdx.y * 64, e0 = blockIdx.z * 64;
   const int ts = threadIdx.x >> 4, te = threadIdx.x & 15;
   const int64_t pa = (int64_t)blockIdx.x * share, pb = min(P, pa + share);
   float acc[4][4] = {};
+  double sum[4][4] = {};
   for (int64_t p = pa; p < pb; p += kDcCols) {
+    if ((p - pa) % kDcFlush == 0)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sum[i >> 2][i & 3] += (double)acc[i >> 2][i & 3];
+        acc[i >> 2][i & 3] = 0.0f;
+      }
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * (kDcCols / 4); i += 256) {
       const int r = i / (kDcCols / 4), q = (i % (kDcCols / 4)) * 4;
@@ -164,26 +172,27 @@ __global__ void __launch_bounds__(256) mix_dcoeff_kernel(const T* __restrict__ d
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int s = s0 + ts + 16 * i, e = e0 + te + 16 * j;
-      if (s < S && e < E) part[((int64_t)blockIdx.x * S + s) * E + e] = acc[i][j];
+      if (s < S && e < E) part[((int64_t)blockIdx.x * E + e) * S + s] = sum[i][j] + (double)acc[i][j];
     }
 }
 
-// dc[i] = sum over the splits, in order, in fp64: one warp per entry.
-__global__ void __launch_bounds__(256) mix_dcoeff_join_kernel(const float* __restrict__ part, int splits, int64_t n,
+// dc[s, e] = sum over the splits [split][e][s], in a fixed order, in fp64: 8 warps for 32 entries.
+__global__ void __launch_bounds__(256) mix_dcoeff_join_kernel(const double* __restrict__ part, int splits, int S, int E,
                                                               float* __restrict__ out) {
+  const int64_t n = (int64_t)S * E;
   const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
   __shared__ double sm[8][32];
   const int w = threadIdx.x >> 5;
   double s = 0.0;
   if (i < n)
-    for (int k = w; k < splits; k += 8) s += (double)part[k * n + i];
+    for (int k = w; k < splits; k += 8) s += part[k * n + i];
   sm[w][threadIdx.x & 31] = s;
   __syncthreads();
   if (w == 0 && i < n) {
     double t = sm[0][threadIdx.x];
 #pragma unroll
     for (int k = 1; k < 8; ++k) t += sm[k][threadIdx.x];
-    out[i] = (float)t;
+    out[i % S * E + i / S] = (float)t;
   }
 }
 
@@ -205,7 +214,7 @@ __global__ void __launch_bounds__(256) mix_dcoeff_join_kernel(const float* __res
 // down to 2^-18 of the tile's largest, 2^-40 of that below). Three bf16 planes need no scale, but six products, and the
 // MMAs (N = 64 takes 60 cycles) were then what the backward pass waited for: 312 us at 128 x 64 x 524,288.
 // dc leaves TMEM for fp32 registers after every tile (fp32, with the tiles' scales) or every 256 columns, each addition
-// there rounded to nearest, and each CTA's sums go to a slot of their own.
+// there rounded to nearest, and from there, every kDcFlush columns, to fp64 sums in a slot of the CTA's own.
 //
 // A tile is a short piece of up to 256 rows that lie megabytes apart. Loads and stores of the threads' own ran at 1.7 TB/s on
 // it (8 warps, 256 bytes per row; a read of the same bytes), TMA at 6.5, so rows that TMA can address (16-byte multiples)
@@ -231,7 +240,7 @@ struct MixTcArgs {
   const void* R;
   const void* X;         // backward only
   void* out;
-  float* part;           // backward only: [gridDim.x][K][M]
+  double* part;          // backward only: [gridDim.x][M][K]
   int M, K;
   int64_t P;
   int stages;            // of operand tiles
@@ -320,6 +329,8 @@ struct MixTc {
   static constexpr int kChunks = kBN / 64;
   static constexpr int kUnit = kF32 ? 4 : 8;           // values per 16 bytes of global memory
   static constexpr int kDcTiles = kF32 ? 1 : 256 / kBN;   // tiles per drain of dc
+  static constexpr int kFlushTiles = kDcFlush / kBN;
+  static_assert(kFlushTiles % kDcTiles == 0, "a flush follows a drain");
   static int stage_bytes(int K, int M, bool dc) { return kPlanesR * kChunks * 128 * (ceil16(K) + (dc ? ceil16(M) : 0)); }
   static int coeff_bytes(int K, int M) { return kPlanesA * ((K + 63) / 64) * ceil16(M) * 128; }
   static constexpr int kStaging = 8 * 4096;
@@ -704,10 +715,37 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
 #pragma unroll
     for (int i = 0; i < (kDc ? 64 : 1); ++i) acc[i] = 0.0f;
     const float scale = kFp16 && q * 32 + lane < M ? row_scale[q * 32 + lane] : 1.0f;
+    // the register sums to the CTA's fp64 slot, which this thread alone adds to: dc row s = R's row, one per lane
+    auto add_dc = [&](bool first) {
+      const int s = q * 32 + lane, e0 = half * dc_half;
+      double* part = p.part + ((int64_t)blockIdx.x * M + e0) * K + s;
+      int n = s < K ? min(dc_half, M - e0) : 0;
+      asm volatile("" : "+r"(n));   // opaque, or 64 predicates are made before the loop over the tiles and kept
+      // conversion and access in one statement: left apart, the compiler carries fp64 sums through the loop over the tiles
+      // (64 x 32 x 491,520 bf16: 49 us, so 39)
+#define FUMA_ADD_DC(access)                                                                                              \
+  _Pragma("unroll") for (int i = 0; i < (kDc ? 64 : 1); ++i) {                                                           \
+    if (i < n)                                                                                                           \
+      asm volatile("{\n\t.reg .f64 d;\n\tcvt.f64.f32 d, %1;\n\t" access ".f64 [%0], d;\n\t}" ::"l"(part), "f"(acc[i]) \
+                   : "memory");                                                                                          \
+    part += K;                                                                                                           \
+    acc[i] = 0.0f;                                                                                                       \
+  }
+      if (first) {
+        FUMA_ADD_DC("st.global")
+      } else {
+        FUMA_ADD_DC("red.global.add")
+      }
+#undef FUMA_ADD_DC
+    };
     int it = 0;
-    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
+    bool ok = true;
+    int64_t tile = blockIdx.x;
+    do {   // backward: runs of kDcFlush columns
+    const int it_end = it + L::kFlushTiles;
+    for (; tile < tiles && (!kDc || it < it_end); tile += gridDim.x, ++it) {
       const int buf = it & 1;
-      bool ok = mbar_wait(&bar_acc_full[buf], (it >> 1) & 1, abort_flag, p.err, kErrWaitAcc);
+      ok = mbar_wait(&bar_acc_full[buf], (it >> 1) & 1, abort_flag, p.err, kErrWaitAcc);
       ok = __all_sync(kFull, ok && !*abort_flag);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -799,21 +837,16 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
         mbar_arrive(&bar_acc_empty[buf]);
       }
       if constexpr (kDc) {
-        if ((it % L::kDcTiles == L::kDcTiles - 1 || tile + gridDim.x >= tiles) && !drain_dc()) break;
-      }
-    }
-    if (p.tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the staging area outlives its reads
-    __syncwarp();
-    if constexpr (kDc) {
-      const int s = q * 32 + lane;   // dc row; its columns are the experts (rows of X)
-      if (s < K) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const int e = half * dc_half + i;
-          if (i < dc_half && e < M) p.part[((int64_t)blockIdx.x * K + s) * M + e] = acc[i];
+        if (it % L::kDcTiles == L::kDcTiles - 1 || tile + gridDim.x >= tiles) {
+          ok = drain_dc();
+          if (!ok) break;
         }
       }
     }
+    if constexpr (kDc) add_dc(it <= L::kFlushTiles);
+    } while (kDc && ok && tile < tiles);
+    if (p.tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the staging area outlives its reads
+    __syncwarp();
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -845,14 +878,14 @@ cudaError_t run_mix(const float* c, int64_t cs, int64_t ce, const void* X, int S
 // Column shares: about two blocks per SM over all (s, e) tiles, at least 512 columns each.
 int64_t dcoeff_share(int S, int E, int64_t P) {
   const int64_t tiles = (int64_t)((S + 63) / 64) * ((E + 63) / 64);
-  int64_t splits = (2 * 148 + tiles - 1) / tiles;
+  int64_t splits = (2 * sm_count() + tiles - 1) / tiles;
   int64_t share = (P + splits - 1) / splits;
   if (share < 512) share = 512;
   return (share + kDcCols - 1) / kDcCols * kDcCols;
 }
 
 template <typename T, bool kVec>
-cudaError_t run_dcoeff(const void* dW, const void* X, int S, int E, int64_t P, float* part, float* out,
+cudaError_t run_dcoeff(const void* dW, const void* X, int S, int E, int64_t P, double* part, float* out,
                        cudaStream_t s) {
   const int64_t share = dcoeff_share(S, E, P);
   const int splits = (int)((P + share - 1) / share);
@@ -860,8 +893,7 @@ cudaError_t run_dcoeff(const void* dW, const void* X, int S, int E, int64_t P, f
       static_cast<const T*>(dW), static_cast<const T*>(X), S, E, P, share, part);
   const cudaError_t st = cudaGetLastError();
   if (st != cudaSuccess) return st;
-  const int64_t n = (int64_t)S * E;
-  mix_dcoeff_join_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, splits, n, out);
+  mix_dcoeff_join_kernel<<<(unsigned)(((int64_t)S * E + 31) / 32), 256, 0, s>>>(part, splits, S, E, out);
   return cudaGetLastError();
 }
 
@@ -955,14 +987,13 @@ int64_t bwd_splits(int S, int E, int64_t P) {
 
 template <typename T>
 cudaError_t any_bwd(const float* c, int64_t cs, int64_t ce, const void* dW, const void* X, int S, int E, int64_t P,
-                    float* dc, void* dX, float* part, int* err, cudaStream_t s) {
+                    float* dc, void* dX, double* part, int* err, cudaStream_t s) {
   if (dc && dX && tc_fits<T>(S, E, true)) {
     MixTcArgs p{};
     p.c = c; p.cm = ce; p.ck = cs; p.R = dW; p.X = X; p.out = dX; p.part = part; p.M = E; p.K = S; p.P = P; p.err = err;
     const cudaError_t st = run_tc<T, true>(p, s);
     if (st != cudaSuccess) return st;
-    const int64_t n = (int64_t)S * E;
-    mix_dcoeff_join_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, tc_grid(P, MixTc<T>::kBN), n, dc);
+    mix_dcoeff_join_kernel<<<(unsigned)(((int64_t)S * E + 31) / 32), 256, 0, s>>>(part, tc_grid(P, MixTc<T>::kBN), S, E, dc);
     return cudaGetLastError();
   }
   if (dX) {
@@ -989,11 +1020,11 @@ int64_t mix_bwd_work_bytes(int S, int E, int64_t P, int dtype) {
   const int64_t tc = dtype == kDtypeF32 ? bwd_splits<float>(S, E, P)
                      : dtype == kDtypeBf16 ? bwd_splits<__nv_bfloat16>(S, E, P) : bwd_splits<__half>(S, E, P);
   if (tc > n) n = tc;
-  return n * S * E * 4;
+  return n * S * E * 8;
 }
 
 cudaError_t launch_mix_bwd(const float* c, int64_t cs, int64_t ce, const void* dW, const void* X, int S, int E, int64_t P,
-                           int dtype, float* dc, void* dX, float* part, int* err, cudaStream_t s) {
+                           int dtype, float* dc, void* dX, double* part, int* err, cudaStream_t s) {
   if (dtype == kDtypeF32) return any_bwd<float>(c, cs, ce, dW, X, S, E, P, dc, dX, part, err, s);
   if (dtype == kDtypeBf16) return any_bwd<__nv_bfloat16>(c, cs, ce, dW, X, S, E, P, dc, dX, part, err, s);
   return any_bwd<__half>(c, cs, ce, dW, X, S, E, P, dc, dX, part, err, s);

@@ -62,3 +62,19 @@ def test_stages_of_the_operand_ring(S, E, P, dt):
 def test_one_raw_tile(S, E, dt):
     """Shapes at which fp32 has room for one raw tile beside one operand stage."""
     _compare(S, E, ALIGNED, dt)
+
+
+@pytest.mark.parametrize("both", [True, False])
+def test_long_sums_of_one_sign(both):
+    """dc over 3 * 2^23 columns. Every product is a little more than 1, by an amount that an fp32 sum of a thread's whole share would
+    drop at each addition once it is large (460 and 3,600 units, by where the share ends). fp32 sums end after 4,096 columns: 64
+    sums of 64 columns from the tensor core (24 units inside each, 12 for the planes), or 1,024 sums of 4."""
+    from flash_uma_b200.grouped import mix_experts
+    P = 3 * 2 ** 23
+    step = 2.0 ** -13 if both else 2.0 ** -10
+    x = torch.full((1, P), 1.0 + step * (1.0 - 2.0 ** -6), device=DEV).requires_grad_(both)
+    c = torch.ones(1, 1, device=DEV, requires_grad=True)
+    dc = torch.autograd.grad(mix_experts(c, x), [c, x] if both else [c], torch.ones(1, P, device=DEV))[0]
+    want = float(x.detach()[0, 0].double()) * P
+    steps = 64 + 24 + 12 + 4 if both else 1024 + 4 + 2
+    assert abs(float(dc) - want) <= steps * 2.0 ** -24 * want
