@@ -15,7 +15,7 @@ import torch
 from . import _native as nat
 from ._native import ptr, stream_of
 from .grouped import (_DTYPES, MAX_GROUPS, _apply, _check_dtype, _once, _opaque, _same_device, _unit_stride, check_groups,
-                      guard_capture)
+                      guard_capture, refuse_fx_trace)
 from .linear import error_flag
 
 _BLOCK = 128
@@ -29,11 +29,18 @@ def _blocks(n: int) -> int:
     return (n + _BLOCK - 1) // _BLOCK
 
 
+def _refuse_trace() -> None:
+    refuse_fx_trace()
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("quantisation to fp8 cannot be traced: a traced graph would hold the empty codes alone")
+
+
 class Fp8Weight:
     """Frozen weights [N, K] or [G, N, K] (any floating type, on a GPU) as e4m3 codes and scales, and
     the same of the transposed matrices for the input gradient: two bytes per weight in all."""
 
     def __init__(self, weight: torch.Tensor):
+        _refuse_trace()
         nat.require_cuda(weight)
         if weight.dim() not in (2, 3):
             raise ValueError(f"weight must be [N, K] or [groups, N, K] (got {tuple(weight.shape)})")
@@ -65,6 +72,7 @@ class Fp8Weight:
 def quantize_rows(x: torch.Tensor):
     """x [T, K] -> (codes uint8 [T, K rounded up to 16], scales float32 [ceil(K / 128), T]): e4m3 in
     blocks of 128 along each row (``fuma_quantize_rows_fp8``)."""
+    _refuse_trace()
     nat.require_cuda(x)
     code = _check_dtype("x", x)
     if x.dim() != 2 or x.shape[1] < 1:

@@ -22,6 +22,7 @@ import weakref
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from ._native import ptr, stream_of
@@ -85,16 +86,26 @@ def guard_capture(*inputs) -> bool:
     return True
 
 
+def refuse_fx_trace() -> None:
+    """A graph traced by ``make_fx`` would hold the empty outputs and none of the kernels, which torch does not see."""
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("the expert-mixture calls cannot be traced by make_fx or torch.export (their kernels are not "
+                           "torch operators)")
+
+
 def _apply(fn, capturing: bool, *args):
-    """``fn.apply`` where a gradient may be asked for, else its forward alone."""
-    if torch.is_grad_enabled():
-        for t in args:
-            if isinstance(t, torch.Tensor) and t.requires_grad:
-                out = fn.apply(*args)
-                if not capturing:
-                    with _live_lock:
-                        _live_nodes.add(out.grad_fn)
-                return out
+    """``fn.apply`` where a gradient may be asked for, else its forward alone. Under torch's transformations always the
+    former: ``torch.jit.trace`` records it, and forward mode and ``torch.func`` find no rule and raise, where they would take
+    outputs of the bare forward for constants."""
+    refuse_fx_trace()
+    if (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+            or torch._C._are_functorch_transforms_active()
+            or torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args)):
+        out = fn.apply(*args)
+        if not capturing and out.grad_fn is not None:
+            with _live_lock:
+                _live_nodes.add(out.grad_fn)
+        return out
     return fn.compute(*args)
 
 
