@@ -170,6 +170,29 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
 }
 
+// This warp's lanes and `cols` columns of TMEM (rounded up to 16) times a factor per lane.
+__device__ __forceinline__ void tmem_scale(uint32_t taddr, int cols, float s) {
+#pragma unroll 1
+  for (int c = 0; c < cols; c += 16) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr + c)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * s);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr + c)
+        : "memory");
+  }
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
 // (x: contiguous, y: rows, z: matrix); all planes. Issued by one elected lane of a converged warp. kPair: `bar` is a
 // shared::cluster address, in either CTA of the pair.
 template <bool kPair>
@@ -756,15 +779,18 @@ __global__ void __launch_bounds__(kGThreads, 1)
         ok = __all_sync(kFull, ok && !*abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        // the product of two scales may leave the fp32 range where the result does not: kSplit multiplies by two powers
-        // of two with half the exponent each
+        // the product of two scales may leave the fp32 range where the result does not (and 0 x inf is NaN): then it is applied as
+        // two powers of two with half the exponent each. kSplit multiplies twice always, kFp8 takes the first factor to TMEM if a
+        // row of the warp needs it (a multiplication more, or a branch to one, in its drain: 8 to 17 us of 186 a pass)
         float s = 1.0f, s2 = 1.0f;
         if constexpr (kKind == kFp8) s = s_a * s_b;
-        if constexpr (kKind == kSplit) {
+        const bool wide = kKind == kFp8 && __any_sync(kFull, s == 0.0f || s > 3.402823466e38f);
+        if (kKind == kSplit || (wide && s == s)) {   // (a scale that is NaN makes the sums NaN)
           const int e = (int)(__float_as_uint(s_a) >> 23) + (int)(__float_as_uint(s_b) >> 23) - 254, h = e >> 1;
           s = __uint_as_float((uint32_t)(h + 127) << 23);
           s2 = __uint_as_float((uint32_t)(e - h + 127) << 23);
         }
+        if (wide) tmem_scale(tmem + (uint32_t)(buf * kMaxBN + col0) + ((uint32_t)(q * 32) << 16), ncols, s2);
         const uint32_t taddr = tmem + (uint32_t)(buf * kMaxBN + col0) + ((uint32_t)(q * 32) << 16);
 #pragma unroll
         for (int c = 0; c < 4; c += 2) {

@@ -255,3 +255,24 @@ def test_rows_past_32_bit_offsets():
     w8 = Fp8Weight(torch.randn(N, K, device=DEV, generator=g))
     y = fp8_linear(x, w8)
     assert torch.equal(y[-n:], fp8_linear(x[-n:].contiguous(), w8)) and not y[:-n].any()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_scales_whose_product_leaves_the_fp32_range(dt):
+    """Blocks of the largest magnitudes whose products are all zero add nothing; blocks of the smallest add what they hold."""
+    from flash_uma_b200.fp8 import Fp8Weight, fp8_linear
+    g = torch.Generator(device=DEV).manual_seed(8)
+    T, K, N = 40, 384, 72
+    x = torch.randn(T, K, device=DEV, generator=g).to(dt)
+    w = torch.randn(N, K, device=DEV, generator=g)
+    x[:, :128], w[:, :128] = 0.0, 0.0
+    want = fp8_linear(x, Fp8Weight(w))
+    x[::2, 0], w[:, 1] = torch.finfo(dt).max, 3e38    # scales 2^120 (fp16 2^8) and 2^120; every product is 0
+    assert torch.equal(fp8_linear(x, Fp8Weight(w)), want)
+    x[3, 200] = float("nan")
+    got = fp8_linear(x, Fp8Weight(w))
+    keep = torch.arange(T, device=DEV) != 3
+    assert torch.isnan(got[3]).all() and torch.equal(got[keep], want[keep])
+    if dt != torch.float16:                           # 2^-126 and 2^-24: 128 products of 2^-134
+        y = fp8_linear(torch.full((T, 128), 2.0 ** -118, device=DEV, dtype=dt), Fp8Weight(torch.full((N, 128), 2.0 ** -16, device=DEV)))
+        assert (y.double() == 2.0 ** -127).all()
