@@ -318,6 +318,13 @@ __device__ __forceinline__ float2 fp16_scale(uint32_t amax_bits) {
   return make_float2(__uint_as_float((uint32_t)(127 + e) << 23), __uint_as_float((uint32_t)(127 - e) << 23));
 }
 
+// a b as two powers of two with half the exponent each: the product of two scales may leave the fp32 range where the
+// result does not.
+__device__ __forceinline__ float2 half_exponents(float a, float b) {
+  const int e = (int)(__float_as_uint(a) >> 23) + (int)(__float_as_uint(b) >> 23) - 254, h = e >> 1;
+  return make_float2(__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(e - h + 127) << 23));
+}
+
 __host__ __device__ inline int ceil16(int n) { return (n + 15) / 16 * 16; }
 
 template <typename T>
@@ -757,9 +764,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
         full = __all_sync(kFull, full && !*abort_flag);
         if (!full) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        // (powers of two; their product may leave the fp32 range where the result does not)
-        const int e = (int)(__float_as_uint(ts.x) >> 23) + (int)(__float_as_uint(ts.y) >> 23) - 254, eh = e >> 1;
-        const float s1 = __uint_as_float((uint32_t)(eh + 127) << 23), s2 = __uint_as_float((uint32_t)(e - eh + 127) << 23);
+        const float2 sc = half_exponents(ts.x, ts.y);
         if (q * 32 < K) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -768,7 +773,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
               mix_tmem_ld16(dc_tmem + (dcn & 1) * 128 + half * dc_half + c * 16 + lanes, r);
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                if constexpr (kF32) acc[c * 16 + i] = fmaf(__uint_as_float(r[i]) * s1, s2, acc[c * 16 + i]);
+                if constexpr (kF32) acc[c * 16 + i] = fmaf(__uint_as_float(r[i]) * sc.x, sc.y, acc[c * 16 + i]);
                 else acc[c * 16 + i] += __uint_as_float(r[i]);
               }
             }
@@ -781,6 +786,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       if (q * 32 < M) {
         const uint32_t d1 = tmem + buf * kBN + half * kHalfCols + lanes;
         const int rows = min(32, M - q * 32);
+        const float2 so = kF32 ? half_exponents(scale, ts.x) : make_float2(scale, 1.0f);
         if (p.tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
 #pragma unroll
@@ -792,7 +798,7 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
             for (int j = 0; j < 8; ++j) {
               float o[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(r[4 * j + i]) * scale * ts.x;
+              for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(r[4 * j + i]) * so.x * so.y;
               *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(o[0], o[1], o[2], o[3]);
             }
           } else {

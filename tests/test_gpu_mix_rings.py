@@ -78,3 +78,21 @@ def test_long_sums_of_one_sign(both):
     want = float(x.detach()[0, 0].double()) * P
     steps = 64 + 24 + 12 + 4 if both else 1024 + 4 + 2
     assert abs(float(dc) - want) <= steps * 2.0 ** -24 * want
+
+
+@pytest.mark.parametrize("up,down", [(120, -100), (-100, 120)])
+def test_coefficients_and_matrices_at_the_ends_of_the_fp32_range(up, down):
+    """Coefficients about 2^up and matrices about 2^down: results about 2^20."""
+    from flash_uma_b200.grouped import mix_experts
+    S, E, P = 64, 32, 1000
+    g = torch.Generator(device=DEV).manual_seed(3)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)   # noqa: E731
+    c = (r(S, E) * 2.0 ** up).requires_grad_(True)
+    x, gw = (r(E, P) * 2.0 ** down).requires_grad_(True), r(S, P) * 2.0 ** down
+    w = mix_experts(c, x)
+    dx, = torch.autograd.grad(w, [x], gw, retain_graph=True)
+    both = torch.autograd.grad(w, [c, x], gw)[1]
+    C, X, GW = c.detach().double(), x.detach().double(), gw.double()
+    _check(w.detach(), C @ X, C.abs() @ X.abs(), 6 * 2 + 14, "w")
+    for got in (dx, both):
+        _check(got, C.T @ GW, C.T.abs() @ GW.abs(), 6 * 4 + 14, "dx")
