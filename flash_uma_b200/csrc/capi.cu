@@ -713,12 +713,15 @@ int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P, int32_t dty
 
 namespace {
 
+constexpr int32_t kMaxWidth = 1 << 30;   // sums with a tile's width stay in 32 bits
+
 int64_t ceil8(int64_t n) { return (n + 7) / 8 * 8; }
 
 int check_grouped(const char* what, int32_t G, int64_t T, int32_t N, int32_t K, int32_t dtype) {
   REQUIRE(G >= 1 && G <= kMaxGroups, "%s: G=%d must be from 1 to %d", what, G, kMaxGroups);
   REQUIRE(T >= 0 && T < (int64_t(1) << 31) - 256, "%s: T=%lld out of range", what, (long long)T);
   REQUIRE(N > 0 && K > 0, "%s: N=%d and K=%d must be positive", what, N, K);
+  REQUIRE(N <= kMaxWidth && K <= kMaxWidth, "%s: N=%d and K=%d must be at most %d", what, N, K, kMaxWidth);
   REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "%s: dtype=%d must be 0 (fp32), 1 (bf16) or 2 (fp16)", what, dtype);
   REQUIRE((int64_t)G * (N > K ? N : K) < (int64_t(1) << 31), "%s: G * max(N, K) too large", what);
   REQUIRE((T / 128 + G) * (int64_t)((N > K ? N : K) / 32 + 1) < (int64_t(1) << 31), "%s: too many output tiles", what);
@@ -817,6 +820,7 @@ int fuma_grouped_bias_grad(const void* dy, int64_t lddy, const int64_t* offsets,
                            int32_t N, int32_t dtype, void* db, void* work, int64_t work_bytes, void* stream) {
   CHECK(check_grouped("grouped_bias_grad", G, T, N, N, dtype));
   REQUIRE(lddy >= N, "grouped_bias_grad: lddy=%lld must be >= N", (long long)lddy);
+  REQUIRE(N <= 256 * 65535, "grouped_bias_grad: N=%d too large", N);
   REQUIRE(db && (T == 0 || dy), "grouped_bias_grad: null pointer");
   REQUIRE(offsets || G == 1, "grouped_bias_grad: offsets may be NULL for one group only");
   const int64_t need = T > 0 ? grouped_colsum_work_bytes(T, N, shared ? 1 : G) : 0;
@@ -863,7 +867,7 @@ int fuma_pad_rows(const void* x, int64_t ldx, int64_t rows, int32_t cols, void* 
 
 int fuma_quantize_rows_fp8(const void* x, int64_t ldx, int64_t T, int32_t K, int32_t dtype, void* codes, int64_t ldq,
                            float* scales, void* stream) {
-  REQUIRE(T >= 0 && T < (int64_t(1) << 31) && K > 0, "quantize_rows_fp8: bad shape T=%lld K=%d",
+  REQUIRE(T >= 0 && T < (int64_t(1) << 31) && K > 0 && K <= kMaxWidth, "quantize_rows_fp8: bad shape T=%lld K=%d",
           (long long)T, K);
   REQUIRE(dtype >= kDtypeF32 && dtype <= kDtypeF16, "quantize_rows_fp8: dtype=%d must be 0, 1 or 2", dtype);
   REQUIRE(ldx >= K, "quantize_rows_fp8: ldx=%lld must be >= K", (long long)ldx);

@@ -687,8 +687,8 @@ __global__ void __launch_bounds__(kGThreads, 1)
     if constexpr (kMode != kModeDw) {
       // rows before the first and behind the last group: zeros
       const int64_t head = group_at(p.offsets, 0, p.T), tail = group_at(p.offsets, p.G, p.T);
-      const int esize = p.out_dtype == kDtypeF32 ? 4 : 2, row_bytes = p.N * esize;
-      const int unit = p.N % 8 ? esize : 16, units_row = row_bytes / unit;
+      const int esize = p.out_dtype == kDtypeF32 ? 4 : 2, unit = p.N % 8 ? esize : 16;
+      const int64_t row_bytes = (int64_t)p.N * esize, units_row = row_bytes / unit;
       const int64_t dead = units || head == tail ? head + (p.T - tail) : 0, n = dead * units_row;
       for (int64_t i = (int64_t)blockIdx.x * (kEpiWarps * 32) + threadIdx.x - kEpiWarp0 * 32; i < n;
            i += (int64_t)gridDim.x * (kEpiWarps * 32)) {

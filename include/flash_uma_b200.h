@@ -332,7 +332,7 @@ int fuma_morton_reorder_noalloc(const float* pos, const int64_t* Z, const int64_
  * launch needs no host copy of it; empty groups are allowed, rows outside [offsets[0],
  * offsets[G]) are written as zeros, and offsets may be NULL for one group of all rows. Offsets that
  * decrease or leave [0, T] put 64 into err_flag (the results are then undefined, all accesses stay in
- * bounds). 1 <= G <= 4096; any N and K; leading dimensions (elements) of the operands multiples
+ * bounds). 1 <= G <= 4096; any N and K up to 2^30 (bias gradient: N up to 2^24 - 256); leading dimensions (elements) of the operands multiples
  * of 8 (fuma_pad_rows makes such a copy), arrays 16-byte aligned; outputs contiguous. Work space: see the *_work_bytes
  * functions (0: may be NULL); calls that overlap need one each.
  *

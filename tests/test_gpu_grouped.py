@@ -692,3 +692,14 @@ def test_default_dtype_of_64_bits():
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(p.dtype == q.dtype and torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_rows_of_2_31_bytes_outside_all_groups_are_zeros():
+    from flash_uma_b200.grouped import grouped_linear
+    T, N, K, dt = 3, 2 ** 30, 8, torch.bfloat16
+    w = torch.zeros(1, N, K, device=DEV, dtype=dt)
+    w[0, -5:] = 1.0
+    poison = torch.full((T, N), float("nan"), device=DEV, dtype=dt)   # the memory that the result is likely to get
+    del poison
+    y = grouped_linear(torch.ones(T, K, device=DEV, dtype=dt), w, torch.tensor([1, 2], device=DEV))
+    assert not y[0].any() and not y[2].any() and not y[1, :-5].any() and (y[1, -5:] == K).all()

@@ -114,3 +114,15 @@ def test_cpu_tensors_refused():
                  lambda: quantize_rows(x), lambda: Fp8Weight(x)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_widths_that_32_bit_sums_do_not_hold_are_refused(lib):
+    wide = 2 ** 30 + 8
+    f = lib
+    assert f.fuma_grouped_linear(P, 16, None, P, 16, None, P, 1, None, 0, 10, wide, 16, 1, P, None, None) == -1
+    assert b"at most" in f.fuma_last_error()
+    assert f.fuma_grouped_linear_dgrad(P, wide, None, P, 16, None, P, 1, 10, wide, 16, 1, P, None, None) == -1
+    assert f.fuma_grouped_linear(P, wide, None, P, wide, None, P, 1, None, 0, 10, 24, wide, 1, P, None, None) == -1
+    assert f.fuma_quantize_rows_fp8(P, wide, 4, wide, 1, P, wide, P, None) == -1
+    assert f.fuma_grouped_bias_grad(P, 2 ** 24, P, 1, 1, 10, 2 ** 24, 1, P, P, 1 << 40, None) == -1
+    assert b"too large" in f.fuma_last_error()
