@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import math
 import os
+import threading
 
 import torch
 import torch.nn as nn
@@ -32,6 +33,7 @@ from ._native import ptr, stream_of
 _MODES = ("f16x3", "tf32x3", "tf32", "f16")
 _F16_MODES = ("f16x3", "f16")   # fp16 tensor cores on the row-packed split operands
 _err_flags: dict[int, torch.Tensor] = {}
+_err_lock = threading.Lock()
 _err_host: dict[int, torch.Tensor] = {}     # pinned mirrors, filled asynchronously by snapshot_errors()
 
 _ERR_RANGE = 16
@@ -54,8 +56,13 @@ def error_flag(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _err_flags.get(idx)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _err_flags[idx] = t
+        with _err_lock:   # one flag for all threads
+            t = _err_flags.get(idx)
+            if t is None:
+                t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.current_stream(idx).synchronize()   # kernels and readers on any stream use it from here on
+                _err_flags[idx] = t
     return t
 
 

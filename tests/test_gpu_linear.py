@@ -199,3 +199,24 @@ def test_linear_f16_transposed_tiles(M, N, K, half, monkeypatch):
         err = (y[:, :N].cpu().double() - ref).abs()
         bound = tol(K) * ref.abs().max() + (2.0 ** -11 * ref.abs() if half else 0.0)
         assert bool((err <= bound).all())
+
+
+def test_error_flag_is_zero_on_every_stream_from_the_first_call_on():
+    """The device's flag is made on the stream of the first call, behind whatever that stream still has to do."""
+    from flash_uma_b200 import linear
+    held = dict(linear._err_flags)
+    linear._err_flags.clear()
+    side = torch.cuda.Stream()
+    try:
+        with torch.cuda.stream(side):
+            poison = torch.full((1,), 77, dtype=torch.int32, device=DEV)   # the memory that the flag is likely to get
+            torch.cuda.synchronize()
+            del poison
+            torch.cuda._sleep(200_000_000)                                  # 0.1 s
+            flag = linear.error_flag(torch.device("cuda", torch.cuda.current_device()))
+        assert int(flag) == 0
+        linear.check_errors()
+    finally:
+        torch.cuda.synchronize()
+        linear._err_flags.clear()
+        linear._err_flags.update(held)
