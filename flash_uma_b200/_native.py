@@ -66,7 +66,7 @@ _SIGS = {
     "fuma_morton_reorder_noalloc": [_P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P],
 }
 
-# scratch sizes (name -> argument types, return type int64)
+# scratch sizes and launch counts (name -> argument types, return type int64)
 _SIZE_SIGS = {
     "fuma_morton_scratch_bytes": [_I64],
     "fuma_neighbor_scratch_bytes": [_I64, _P],
@@ -74,6 +74,7 @@ _SIZE_SIGS = {
     "fuma_grouped_bias_grad_work_bytes": [_I64, _I32, _I32],
     "fuma_fp8_work_bytes": [_I64, _I32],
     "fuma_mix_experts_work_bytes": [_I32, _I32, _I64, _I32],
+    "fuma_mix_experts_bwd_launches": [_I32, _I32, _I32, _I32, _I32],
 }
 
 _lib = None
@@ -138,10 +139,10 @@ _SIGS["fuma_rotate_scatter_fwd_f16x3"] = _SIGS["fuma_rotate_scatter_fwd"][:-1] +
 
 KERNELS_PER_CALL = {name: 1 for name in _SIGS}
 KERNELS_PER_CALL["fuma_gather_bwd"] = 3
-KERNELS_PER_CALL["fuma_grouped_linear_wgrad"] = 2
+KERNELS_PER_CALL["fuma_grouped_linear_wgrad"] = 2   # with a group long enough to be cut (launches_of)
 KERNELS_PER_CALL["fuma_grouped_bias_grad"] = 2
 KERNELS_PER_CALL["fuma_grouped_linear_fp8"] = 2
-KERNELS_PER_CALL["fuma_mix_experts_bwd"] = 2
+KERNELS_PER_CALL["fuma_mix_experts_bwd"] = 2        # both gradients of up to 128 systems and experts (launches_of)
 KERNELS_PER_CALL["fuma_gather_fwd"] = 2
 KERNELS_PER_CALL["fuma_csr_permute"] = 2
 KERNELS_PER_CALL["fuma_neighbor_list"] = 4
@@ -159,6 +160,14 @@ def launches_of(name: str, args) -> int:
     """Kernel launches of one call of entry point ``name`` with arguments ``args``."""
     if name in ("fuma_morton_reorder", "fuma_morton_reorder_noalloc") and args[5] > 16384:
         return 28   # bounds, keys, 8 radix passes of 3 kernels, permutation, renumbering
+    if name == "fuma_grouped_linear_wgrad":   # no rows: a memset; long batches: the parts of cut groups are joined
+        T, N, K, dtype = args[8:12]
+        return 0 if T == 0 else 2 if load().fuma_grouped_wgrad_work_bytes(T, N, K, dtype) else 1
+    if name == "fuma_grouped_bias_grad" and args[5] == 0:
+        return 1
+    if name == "fuma_mix_experts_bwd":
+        S, E, _, dtype, dc, dx = args[5:11]
+        return load().fuma_mix_experts_bwd_launches(S, E, dtype, dc is not None, dx is not None)
     return KERNELS_PER_CALL.get(name, 1)
 
 

@@ -707,6 +707,10 @@ int64_t fuma_grouped_bias_grad_work_bytes(int64_t T, int32_t N, int32_t groups) 
   return T > 0 && N > 0 && groups > 0 ? grouped_colsum_work_bytes(T, N, groups) : 0;
 }
 
+int64_t fuma_mix_experts_bwd_launches(int32_t S, int32_t E, int32_t dtype, int32_t dcoeff, int32_t dexperts) {
+  return S > 0 && E > 0 ? mix_bwd_launches(S, E, dtype, dcoeff != 0, dexperts != 0) : 0;
+}
+
 int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P, int32_t dtype) {
   return S > 0 && E > 0 && P > 0 ? mix_bwd_work_bytes(S, E, P, dtype) : 0;
 }

@@ -124,6 +124,7 @@ void launch_quantize_weight(const float* w, int G, int N, int K, void* codes, in
 // out[s, p] = sum_e c[s * cs + e * ce] X[e, p]
 cudaError_t launch_mix(const float* c, int64_t cs, int64_t ce, const void* X, int S, int E, int64_t P, int dtype,
                        void* out, int* err, cudaStream_t s);
+int mix_bwd_launches(int S, int E, int dtype, bool dc, bool dX);   // kernels of a launch_mix_bwd
 int64_t mix_bwd_work_bytes(int S, int E, int64_t P, int dtype);
 // dc and dX (either may be null) from dW; part: mix_bwd_work_bytes when dc is asked for
 cudaError_t launch_mix_bwd(const float* c, int64_t cs, int64_t ce, const void* dW, const void* X, int S, int E, int64_t P,

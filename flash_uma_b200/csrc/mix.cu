@@ -1020,6 +1020,12 @@ cudaError_t launch_mix(const float* c, int64_t cs, int64_t ce, const void* X, in
   return any_mix<__half>(c, cs, ce, X, S, E, P, out, err, s);
 }
 
+int mix_bwd_launches(int S, int E, int dtype, bool dc, bool dX) {
+  const bool tc = dtype == kDtypeF32 ? tc_fits<float>(S, E, true)
+                  : dtype == kDtypeBf16 ? tc_fits<__nv_bfloat16>(S, E, true) : tc_fits<__half>(S, E, true);
+  return dc && dX && tc ? 2 : (dX ? 1 : 0) + (dc ? 2 : 0);   // any_bwd
+}
+
 int64_t mix_bwd_work_bytes(int S, int E, int64_t P, int dtype) {
   const int64_t share = dcoeff_share(S, E, P);
   int64_t n = (P + share - 1) / share;   // the coefficients' gradient alone

@@ -395,6 +395,8 @@ int fuma_mix_experts(const float* coeff, int64_t stride_s, int64_t stride_e, con
  * dexperts[e, p] = sum_s coeff[s, e] grad[s, p]; either may be NULL. Both together read grad and experts once.
  * work: fuma_mix_experts_work_bytes when dcoeff is asked for. */
 int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P, int32_t dtype);
+/* Kernels that such a call launches (dcoeff, dexperts: whether they are asked for). */
+int64_t fuma_mix_experts_bwd_launches(int32_t S, int32_t E, int32_t dtype, int32_t dcoeff, int32_t dexperts);
 int fuma_mix_experts_bwd(const void* grad, const float* coeff, int64_t stride_s, int64_t stride_e, const void* experts,
                          int32_t S, int32_t E, int64_t P, int32_t dtype, float* dcoeff, void* dexperts, void* work,
                          int64_t work_bytes, int* err_flag, void* stream);

@@ -703,3 +703,33 @@ def test_rows_of_2_31_bytes_outside_all_groups_are_zeros():
     del poison
     y = grouped_linear(torch.ones(T, K, device=DEV, dtype=dt), w, torch.tensor([1, 2], device=DEV))
     assert not y[0].any() and not y[2].any() and not y[1, :-5].any() and (y[1, -5:] == K).all()
+
+
+def test_launches_are_counted_as_they_happen():
+    from flash_uma_b200 import _native as nat
+    from flash_uma_b200.fp8 import Fp8Weight, fp8_linear
+    from flash_uma_b200.grouped import grouped_linear, mix_experts
+
+    def grouped(lens, dt):
+        x, w, off, b, gy = _make(lens, 72, 40, dt, "shared")
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+        return lambda: torch.autograd.grad(grouped_linear(x, w, off, b), leaves, gy)
+
+    def mix(S, E, grads):
+        c, x = torch.rand(S, E, device=DEV), torch.rand(E, 1000, device=DEV)
+        leaves = [t.requires_grad_(True) for t, g in zip((c, x), grads) if g]
+        return lambda: torch.autograd.grad(mix_experts(c, x), leaves, torch.ones(S, 1000, device=DEV))
+    x, w8 = torch.rand(40, 136, device=DEV), Fp8Weight(torch.rand(72, 136, device=DEV))
+    for f in (grouped([40, 3], torch.bfloat16), grouped([40, 3], torch.float32), grouped([2047, 9], torch.bfloat16),
+              mix(5, 4, (1, 1)), mix(5, 4, (1, 0)), mix(5, 4, (0, 1)), mix(129, 4, (1, 1)), lambda: fp8_linear(x, w8)):
+        f()
+        torch.cuda.synchronize()
+        probe = nat.LaunchProbe()
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+            nat.set_probe(probe)
+            try:
+                f()
+            finally:
+                nat.set_probe(None)
+            torch.cuda.synchronize()
+        assert probe.launches == sum("fuma::" in e.name for e in prof.events()), probe.counts

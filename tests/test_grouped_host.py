@@ -126,3 +126,18 @@ def test_widths_that_32_bit_sums_do_not_hold_are_refused(lib):
     assert f.fuma_quantize_rows_fp8(P, wide, 4, wide, 1, P, wide, P, None) == -1
     assert f.fuma_grouped_bias_grad(P, 2 ** 24, P, 1, 1, 10, 2 ** 24, 1, P, P, 1 << 40, None) == -1
     assert b"too large" in f.fuma_last_error()
+
+
+def test_launches_of_the_calls_that_vary(lib):
+    from flash_uma_b200 import _native as nat
+
+    def wgrad(T):
+        return nat.launches_of("fuma_grouped_linear_wgrad", (P, 64, P, P, 64, P, P, 1, T, 64, 64, 0, P, P, 0, None, None))
+
+    def mix(S, E, dtype, dc, dx):
+        return nat.launches_of("fuma_mix_experts_bwd", (P, P, E, 1, P, S, E, 1000, dtype, dc, dx, P, 0, None, None))
+    assert [wgrad(0), wgrad(2048), wgrad(2049)] == [0, 1, 2]
+    assert [nat.launches_of("fuma_grouped_bias_grad", (P, 8, P, 1, 0, T, 8, 0, P, P, 0, None)) for T in (0, 5)] == [1, 2]
+    assert [mix(128, 128, d, P, P) for d in (0, 1, 2)] == [2, 2, 2]
+    assert [mix(129, 2, 1, P, P), mix(2, 129, 1, P, P)] == [3, 3]
+    assert [mix(4, 4, 1, P, None), mix(4, 4, 1, None, P)] == [2, 1]
