@@ -86,9 +86,13 @@ def guard_capture(*inputs) -> bool:
     return True
 
 
+_dispatch_mode, _PROXY = torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+_tracing_state, _functorch_active = torch._C._get_tracing_state, torch._C._are_functorch_transforms_active
+
+
 def refuse_fx_trace() -> None:
     """A graph traced by ``make_fx`` would hold the empty outputs and none of the kernels, which torch does not see."""
-    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+    if _dispatch_mode(_PROXY) is not None:
         raise RuntimeError("the expert-mixture calls cannot be traced by make_fx or torch.export (their kernels are not "
                            "torch operators)")
 
@@ -98,9 +102,13 @@ def _apply(fn, capturing: bool, *args):
     former: ``torch.jit.trace`` records it, and forward mode and ``torch.func`` find no rule and raise, where they would take
     outputs of the bare forward for constants."""
     refuse_fx_trace()
-    if (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
-            or torch._C._are_functorch_transforms_active()
-            or torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args)):
+    recorded = forward_ad._current_level >= 0 or _tracing_state() is not None or _functorch_active()
+    if not recorded and torch.is_grad_enabled():
+        for t in args:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                recorded = True
+                break
+    if recorded:
         out = fn.apply(*args)
         if not capturing and out.grad_fn is not None:
             with _live_lock:
