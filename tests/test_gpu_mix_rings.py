@@ -96,3 +96,51 @@ def test_coefficients_and_matrices_at_the_ends_of_the_fp32_range(up, down):
     _check(w.detach(), C @ X, C.abs() @ X.abs(), 6 * 2 + 14, "w")
     for got in (dx, both):
         _check(got, C.T @ GW, C.T.abs() @ GW.abs(), 6 * 4 + 14, "dx")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("S,E,P", [(160, 96, 20000), (96, 160, 20003), (130, 129, 9000)])
+def test_more_than_128_systems_or_experts(S, E, P, dt):
+    """The vector kernels, in several rounds over systems and experts: n rounded additions for a contraction of n, for dc 1,024 of 4
+    products (5 units each way) before fp64."""
+    from flash_uma_b200.grouped import mix_experts
+    g = torch.Generator(device=DEV).manual_seed(5)
+    c = torch.randn(S, E, device=DEV, generator=g).requires_grad_(True)
+    x = torch.randn(E, P, device=DEV, generator=g).to(dt).requires_grad_(True)
+    gw = torch.randn(S, P, device=DEV, generator=g).to(dt)
+    w = mix_experts(c, x)
+    dc, dx = torch.autograd.grad(w, [c, x], gw, retain_graph=True)
+    C, X, GW = c.detach().double(), x.detach().double(), gw.double()
+    planes = 12 if dt == torch.float32 else 0   # the forward may take the tensor cores
+    _check(w.detach(), C @ X, C.abs() @ X.abs(), max(E, 6 * -(-E // 16) + planes) + 2, "w")
+    _check(dx, C.T @ GW, C.T.abs() @ GW.abs(), max(S, 6 * -(-S // 16) + planes) + 2, "dx")
+    _check(dc, GW @ X.T, GW.abs() @ X.abs().T, 1024 + 8, "dc")
+    assert torch.equal(torch.autograd.grad(w, [c], gw, retain_graph=True)[0], dc)
+    assert torch.equal(torch.autograd.grad(w, [x], gw)[0], dx)
+
+
+def test_systems_and_experts_of_unlike_magnitudes():
+    """fp32, systems and experts 2^-20 to 2^20 apart. A scale for a row of coefficients, and one for 64 columns of all matrices,
+    brings the largest magnitude M below 2^15, where a second plane's rounding is 2^-25: 2^-39 M (2^-40 of the largest at its
+    least, half a unit more for the division's power of two), or 2^-22 of the value. So each product may be off by
+    2^-39 (M_c |x| + |c| M_x) beside the planes' 12 2^-24 |c x|."""
+    from flash_uma_b200.grouped import mix_experts
+    S, E, P = 70, 40, 3000
+    g = torch.Generator(device=DEV).manual_seed(11)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)   # noqa: E731
+    mag = lambda n: 2.0 ** torch.randint(-20, 21, (n, 1), device=DEV, generator=g)   # noqa: E731
+    c = (r(S, E) * mag(S) * mag(E).T).requires_grad_(True)
+    x, gw = (r(E, P) * mag(E)).requires_grad_(True), r(S, P) * mag(S)
+    w = mix_experts(c, x)
+    dc, dx = torch.autograd.grad(w, [c, x], gw)
+    C, X, GW = c.detach().double(), x.detach().double(), gw.double()
+
+    def check(got, A, B, Ma, Mb, steps, what):
+        """got = A @ B; Ma, Mb: the magnitudes that the rows' scales of A and the columns' of B go by, broadcast."""
+        S_ = A.abs() @ B.abs()
+        extra = Ma * B.abs().sum(0)[None] + A.abs().sum(1)[:, None] * Mb
+        tol = steps * 2.0 ** -24 * S_ + 2.0 ** -39 * extra + 2.0 ** -24 * (A @ B).abs()
+        assert ((got.double() - A @ B).abs() <= tol).all(), what
+    check(w.detach(), C, X, C.abs().amax(1, keepdim=True), X.abs().max(), 6 * 3 + 14, "w")
+    check(dx, C.T, GW, C.abs().amax(0)[:, None], GW.abs().max(), 6 * 5 + 14, "dx")
+    check(dc, GW, X.T, GW.abs().max(), X.abs().max(), 6 * 4 + 1 + 16, "dc")
