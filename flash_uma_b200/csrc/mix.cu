@@ -127,6 +127,16 @@ __global__ void __launch_bounds__(256) mix_kernel(const float* __restrict__ c, i
   }
 }
 
+// An fp32 sum to an fp64 slot that no other thread adds to, stored or added. Conversion and access are one statement: left
+// apart, the compiler carries fp64 sums through the loops before, for want of registers (mix_tc_kernel, 64 x 32 x 491,520 bf16: 49
+// us, so 39; mix_dcoeff_kernel, 160 x 96: 1,416, so 1,095).
+__device__ __forceinline__ void store_f64(double* at, float v) {
+  asm volatile("{\n\t.reg .f64 d;\n\tcvt.f64.f32 d, %1;\n\tst.global.f64 [%0], d;\n\t}" ::"l"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ void add_f64(double* at, float v) {
+  asm volatile("{\n\t.reg .f64 d;\n\tcvt.f64.f32 d, %1;\n\tred.global.add.f64 [%0], d;\n\t}" ::"l"(at), "f"(v) : "memory");
+}
+
 // dc partial sums [split][e][s]: block (split, s-tile, e-tile) adds the products of its share of the columns; a thread has
 // 4 x 4 of the 64 x 64 (s, e) pairs.
 constexpr int kDcCols = 64, kDcPad = kDcCols + 4;
@@ -138,15 +148,10 @@ __global__ void __launch_bounds__(256) mix_dcoeff_kernel(const T* __restrict__ d
   const int s0 = blockIdx.y * 64, e0 = blockIdx.z * 64;
   const int ts = threadIdx.x >> 4, te = threadIdx.x & 15;
   const int64_t pa = (int64_t)blockIdx.x * share, pb = min(P, pa + share);
+  for (int64_t p0 = pa; p0 < pb; p0 += kDcFlush) {
   float acc[4][4] = {};
-  double sum[4][4] = {};
-  for (int64_t p = pa; p < pb; p += kDcCols) {
-    if ((p - pa) % kDcFlush == 0)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        sum[i >> 2][i & 3] += (double)acc[i >> 2][i & 3];
-        acc[i >> 2][i & 3] = 0.0f;
-      }
+  const int64_t p1 = min(pb, p0 + kDcFlush);
+  for (int64_t p = p0; p < p1; p += kDcCols) {
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * (kDcCols / 4); i += 256) {
       const int r = i / (kDcCols / 4), q = (i % (kDcCols / 4)) * 4;
@@ -172,8 +177,13 @@ __global__ void __launch_bounds__(256) mix_dcoeff_kernel(const T* __restrict__ d
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int s = s0 + ts + 16 * i, e = e0 + te + 16 * j;
-      if (s < S && e < E) part[((int64_t)blockIdx.x * E + e) * S + s] = sum[i][j] + (double)acc[i][j];
+      if (s < S && e < E) {
+        double* at = part + ((int64_t)blockIdx.x * E + e) * S + s;
+        if (p0 == pa) store_f64(at, acc[i][j]);
+        else add_f64(at, acc[i][j]);
+      }
     }
+  }
 }
 
 // dc[s, e] = sum over the splits [split][e][s], in a fixed order, in fp64: 8 warps for 32 entries.
@@ -728,22 +738,18 @@ __global__ void __launch_bounds__(kMixTcThreads, 1) mix_tc_kernel(const __grid_c
       double* part = p.part + ((int64_t)blockIdx.x * M + e0) * K + s;
       int n = s < K ? min(dc_half, M - e0) : 0;
       asm volatile("" : "+r"(n));   // opaque, or 64 predicates are made before the loop over the tiles and kept
-      // conversion and access in one statement: left apart, the compiler carries fp64 sums through the loop over the tiles
-      // (64 x 32 x 491,520 bf16: 49 us, so 39)
-#define FUMA_ADD_DC(access)                                                                                              \
-  _Pragma("unroll") for (int i = 0; i < (kDc ? 64 : 1); ++i) {                                                           \
-    if (i < n)                                                                                                           \
-      asm volatile("{\n\t.reg .f64 d;\n\tcvt.f64.f32 d, %1;\n\t" access ".f64 [%0], d;\n\t}" ::"l"(part), "f"(acc[i]) \
-                   : "memory");                                                                                          \
-    part += K;                                                                                                           \
-    acc[i] = 0.0f;                                                                                                       \
-  }
+      // one loop or the other: a choice for each entry cost 4 us of 39
       if (first) {
-        FUMA_ADD_DC("st.global")
+#pragma unroll
+        for (int i = 0; i < (kDc ? 64 : 1); ++i, part += K)
+          if (i < n) store_f64(part, acc[i]);
       } else {
-        FUMA_ADD_DC("red.global.add")
+#pragma unroll
+        for (int i = 0; i < (kDc ? 64 : 1); ++i, part += K)
+          if (i < n) add_f64(part, acc[i]);
       }
-#undef FUMA_ADD_DC
+#pragma unroll
+      for (int i = 0; i < (kDc ? 64 : 1); ++i) acc[i] = 0.0f;
     };
     int it = 0;
     bool ok = true;
