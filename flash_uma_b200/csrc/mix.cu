@@ -931,8 +931,9 @@ int tc_grid(int64_t P, int bn) {
 // latter more. us, vector and tensor cores, for matrices of 491,520 values (odd: 102,307):
 //   bf16  S E = 128  19.8, 17.6 (of 16,384 values 4.3, 5.1); 512  36.7, 19.2;  odd 1024  15.0, 21.7; 2048  25.1, 23.0
 //   fp32  S E = 512  38.2, 53.6; 1024  54.8, 54.6; 2048  90.6, 56.7;           odd 2048  23.5, 34.9
-// Both gradients at once always go to the tensor cores, which read the matrices once: bf16 S E = 8 28 + 4,
-// vector 10 + 127 + 4; fp32 84 + 4, vector 10 + 125 + 4.
+// Both gradients at once always go to the tensor cores, which read the matrices once: bf16 S E = 8 30 + 3,
+// vector 13 + 127 + 5; fp32 89 + 4, vector 13 + 125 + 5. (dc alone takes the vector kernel at every size: the one-pass kernel
+// has no form without dX.)
 template <typename T>
 bool use_tc(int S, int E, int64_t P) {
   const bool aligned = P * sizeof(T) % 16 == 0;

@@ -36,7 +36,7 @@ def _refuse_trace() -> None:
 
 
 class Fp8Weight:
-    """Frozen weights [N, K] or [G, N, K] (any floating type, on a GPU) as e4m3 codes and scales, and
+    """Frozen weights [N, K] or [G, N, K] (float32, bfloat16 or float16, on a GPU) as e4m3 codes and scales, and
     the same of the transposed matrices for the input gradient: two bytes per weight in all."""
 
     def __init__(self, weight: torch.Tensor):

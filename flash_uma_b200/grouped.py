@@ -357,7 +357,7 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
 def mix_experts(coeff: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
     """``W[s] = sum_e coeff[s, e] experts[e]``: coeff [S, E] float32 (any strides), experts [E, ...]
     float32, bfloat16 or float16 -> [S, ...] of the experts' type, summed in fp32. Differentiable
-    (once) in both; the gradient of coeff is float32, its sum over a matrix joined in fp64. Large fp32 mixes run
+    (once) in both; the gradient of coeff is float32, its sum over a matrix in fp64 after at most 4,096 values. Large fp32 mixes run
     on the tensor cores with the precision of :func:`grouped_linear`'s fp32 maps, a block being the same 64 values
     of all matrices; a value that is not finite makes the results that depend on it not finite."""
     if torch.compiler.is_compiling():

@@ -391,7 +391,7 @@ int fuma_grouped_linear_fp8(const void* x, int64_t ldx, const void* w_codes, con
 /* out[s, p] = sum_e coeff[s * stride_s + e * stride_e] experts[e, p], p < P; coeff fp32, any P. */
 int fuma_mix_experts(const float* coeff, int64_t stride_s, int64_t stride_e, const void* experts, int32_t S, int32_t E,
                      int64_t P, int32_t dtype, void* out, int* err_flag, void* stream);
-/* From grad [S, P]: dcoeff[s, e] = sum_p grad[s, p] experts[e, p], fp32 [S, E], joined in fp64 without atomics, and
+/* From grad [S, P]: dcoeff[s, e] = sum_p grad[s, p] experts[e, p], fp32 [S, E], in fp64 after at most 4,096 columns, in a fixed order, and
  * dexperts[e, p] = sum_s coeff[s, e] grad[s, p]; either may be NULL. Both together read grad and experts once.
  * work: fuma_mix_experts_work_bytes when dcoeff is asked for. */
 int64_t fuma_mix_experts_work_bytes(int32_t S, int32_t E, int64_t P, int32_t dtype);
