@@ -241,8 +241,6 @@ def call(name: str, *args) -> None:
 
 def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
+        if t is not None and not t.is_cuda:
             raise RuntimeError("flash_uma_b200 ops run on CUDA tensors only (no CPU fallback); "
                                f"got a tensor on {t.device}")

@@ -101,7 +101,8 @@ def _apply(fn, capturing: bool, *args):
     """``fn.apply`` where a gradient may be asked for, else its forward alone. Under torch's transformations always the
     former: ``torch.jit.trace`` records it, and forward mode and ``torch.func`` find no rule and raise, where they would take
     outputs of the bare forward for constants."""
-    refuse_fx_trace()
+    if _dispatch_mode(_PROXY) is not None:
+        refuse_fx_trace()
     recorded = forward_ad._current_level >= 0 or _tracing_state() is not None or _functorch_active()
     if not recorded and torch.is_grad_enabled():
         for t in args:
@@ -313,9 +314,10 @@ class _MixFn(torch.autograd.Function):
     @staticmethod
     def compute(coeff, experts):
         S, E = coeff.shape
+        stride_s, stride_e = coeff.stride()
         x = _flat(experts)
         out = experts.new_empty((S, *experts.shape[1:]))
-        nat.call("fuma_mix_experts", ptr(coeff), coeff.stride(0), coeff.stride(1), ptr(x), S, E, x.numel() // E,
+        nat.call("fuma_mix_experts", coeff.data_ptr(), stride_s, stride_e, x.data_ptr(), S, E, x.numel() // E,
                  _DTYPES[experts.dtype], ptr(out), ptr(error_flag(experts.device)), stream_of(experts))
         return out
 
@@ -366,9 +368,10 @@ def mix_experts(coeff: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
     _check_dtype("experts", experts)
     if coeff.dtype != torch.float32:
         raise TypeError(f"coeff must be float32 (got {coeff.dtype})")
-    if experts.dim() < 1 or coeff.dim() != 2 or coeff.shape[1] != experts.shape[0] or experts.shape[0] < 1:
-        raise ValueError(f"coeff must be [systems, experts] for experts [experts, ...] (got {tuple(coeff.shape)} and "
-                         f"{tuple(experts.shape)})")
+    c_shape, e_shape = coeff.shape, experts.shape
+    if not e_shape or len(c_shape) != 2 or c_shape[1] != e_shape[0] or e_shape[0] < 1:
+        raise ValueError(f"coeff must be [systems, experts] for experts [experts, ...] (got {tuple(c_shape)} and "
+                         f"{tuple(e_shape)})")
     if coeff.device != experts.device:
         _same_device(experts.device, coeff=coeff)
     return _apply(_MixFn, guard_capture(coeff, experts), coeff, experts)

@@ -53,7 +53,9 @@ def error_flag(device: torch.device) -> torch.Tensor:
     (codes 1-5), an f16x3 input is out of the fp16 range (code 16), the Morton reorder met an
     edge index outside [0, N) (code 32), or a grouped dense map got offsets that decrease or leave
     [0, T] (code 64)."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
+    idx = device.index
+    if idx is None:
+        idx = torch.cuda.current_device()
     t = _err_flags.get(idx)
     if t is None:
         with _err_lock:   # one flag for all threads
