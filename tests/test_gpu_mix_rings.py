@@ -144,3 +144,38 @@ def test_systems_and_experts_of_unlike_magnitudes():
     check(w.detach(), C, X, C.abs().amax(1, keepdim=True), X.abs().max(), 6 * 3 + 14, "w")
     check(dx, C.T, GW, C.abs().amax(0)[:, None], GW.abs().max(), 6 * 5 + 14, "dx")
     check(dc, GW, X.T, GW.abs().max(), X.abs().max(), 6 * 4 + 1 + 16, "dc")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_large_mixes_on_two_streams_and_replayed(dt):
+    """Two mixes of several tiles a thread block in flight at once, and a captured one on new data, give the eager calls' bits."""
+    from flash_uma_b200.grouped import mix_experts
+    g = torch.Generator(device=DEV).manual_seed(13)
+
+    def make(S, E, P):
+        c = torch.rand(S, E, device=DEV, generator=g).requires_grad_(True)
+        x = torch.randn(E, P, device=DEV, generator=g).to(dt).requires_grad_(True)
+        gw = torch.randn(S, P, device=DEV, generator=g).to(dt)
+
+        def run():
+            w = mix_experts(c, x)
+            return (w.detach(), *torch.autograd.grad(w, [c, x], gw))
+        return run, x
+    (a, xa), (b, _) = make(70, 70, ALIGNED), make(128, 96, ODD)
+    want = a(), b()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            got_b = b()
+        got_a = a()
+        torch.cuda.current_stream().wait_stream(side)
+        for got, w in ((got_a, want[0]), (got_b, want[1])):
+            assert all(torch.equal(p, q) for p, q in zip(got, w))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = a()
+    with torch.no_grad():
+        xa.mul_(-3.0)
+    graph.replay()
+    assert all(torch.equal(p, q) for p, q in zip(out, a()))
